@@ -21,17 +21,19 @@ LIB_PATH = os.path.join(HERE, "libfastgguf_hip.so")
 OK, ERR, ERR_ARG, SKIP_TYPE, SKIP_MEM, ERR_DEVICE = 0, -1, -2, -3, -4, -5
 ORDER_AUTO, ORDER_ROW, ORDER_REPACKED = -1, 0, 1
 ACT_Q8, ACT_Q8K = 1, 2
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 
 #: every symbol include/fastgguf_hip.h declares
 EXPORTS = (
     "fgh_open", "fgh_close", "fgh_info", "fgh_last_error", "fgh_upload", "fgh_tensor_free",
     "fgh_matvec", "fgh_matvec_multi", "fgh_matmul", "fgh_moe_ffn", "fgh_attention",
     "fgh_matvec_dev", "fgh_matvec_multi_dev", "fgh_matvec_silu_dev", "fgh_matvec_gate_up_silu_dev", "fgh_ffn_dev", "fgh_matmul_dev", "fgh_matmul_dev_noalloc", "fgh_moe_ffn_dev",
-    "fgh_attention_dev", "fgh_kvq_store_dev", "fgh_kvq_attention_dev",
+    "fgh_attention_dev", "fgh_kvq_store_dev", "fgh_kvq_attention_dev", "fgh_paged_store_dev", "fgh_paged_attention_dev",
     "fgh_graph_begin", "fgh_graph_end", "fgh_graph_launch", "fgh_graph_destroy",
     "fgh_dev_alloc", "fgh_dev_free", "fgh_copy_h2d", "fgh_copy_d2h", "fgh_copy_d2d", "fgh_checksum_dev", "fgh_memcpy_dev", "fgh_mfma_peak_dev", "fgh_sync",
     "fgh_event_create", "fgh_event_record", "fgh_event_elapsed_ms", "fgh_event_destroy",
     "fgh_quantize", "fgh_block_ints", "fgh_gemm_block_ints", "fgh_moe_block_ints", "fgh_expf", "fgh_fp16_to_f32", "fgh_matvec_shape", "fgh_matmul_path",
+    "fgh_paged_slot", "fgh_paged_check",
     "fgh_gguf_open", "fgh_gguf_close", "fgh_gguf_summary", "fgh_gguf_tensor", "fgh_gguf_find",
     "fgh_gguf_kv_num", "fgh_gguf_kv_str", "fgh_gguf_data", "fgh_upload_gguf",
 )
@@ -52,6 +54,69 @@ class InfoT(C.Structure):
     _fields_ = [("vram", C.c_uint64), ("budget", C.c_uint64), ("used", C.c_uint64),
                 ("n_offloaded", C.c_int32), ("n_skip_type", C.c_int32), ("n_skip_mem", C.c_int32),
                 ("device", C.c_int32), ("name", C.c_char * 96)]
+
+
+class PagedCache(C.Structure):
+    """fgh_paged_cache: device pointers to the K pages [n_head_kv][page][hd], the V pages
+    [n_head_kv][hd][page] and the tables int32 [n_seq][table_stride]."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("page_stride", C.c_int64), ("type", C.c_uint32),
+                ("n_pages", C.c_int32), ("page", C.c_int32), ("table_stride", C.c_int32), ("n_head_kv", C.c_int32),
+                ("hd", C.c_int32)]
+
+    def __init__(self, type_: int, k_dev: int, v_dev: int, table_dev: int, *, n_pages: int, page: int, table_stride: int,
+                 n_head_kv: int, hd: int, page_stride: int = 0):
+        super().__init__(k_dev, v_dev, table_dev, page_stride, type_, n_pages, page, table_stride, n_head_kv, hd)
+
+
+class PagedBatch(C.Structure):
+    """fgh_paged_batch: device pointers to tok int32 [n_seq + 1] and len int32 [n_seq]."""
+    _fields_ = [("tok", C.c_void_p), ("len", C.c_void_p), ("n_seq", C.c_int32), ("n_tok", C.c_int32), ("max_tok", C.c_int32),
+                ("max_len", C.c_int32)]
+
+    def __init__(self, tok_dev: int, len_dev: int, *, n_seq: int, n_tok: int, max_tok: int, max_len: int):
+        super().__init__(tok_dev, len_dev, n_seq, n_tok, max_tok, max_len)
+
+
+class PagedRope(C.Structure):
+    """fgh_paged_rope: the head norms (device pointers to their weights, 0: none) and the rotation
+    of n_rot values (0: none), in halves or in pairs."""
+    _fields_ = [("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq_factors", C.c_void_p), ("eps", C.c_float),
+                ("freq_base", C.c_float), ("freq_scale", C.c_float), ("n_rot", C.c_int32), ("rope", C.c_int32)]
+
+    def __init__(self, *, n_rot: int = 0, halves: bool = False, freq_base: float = 10000.0, freq_scale: float = 1.0,
+                 freq_factors: int = 0, q_norm: int = 0, k_norm: int = 0, eps: float = 1e-5):
+        super().__init__(q_norm, k_norm, freq_factors, eps, freq_base, freq_scale, n_rot, ROPE_HALVES if halves else ROPE_PAIRS)
+
+
+class PagedMask(C.Structure):
+    """fgh_paged_mask: scale, score cap (0: none), window (0: none), ALiBi slopes and prefixes
+    (device pointers, 0: none)."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int32), ("slopes", C.c_void_p),
+                ("prefix", C.c_void_p)]
+
+    def __init__(self, scale: float, *, softcap: float = 0.0, window: int = 0, slopes: int = 0, prefix: int = 0):
+        super().__init__(scale, softcap, window, slopes, prefix)
+
+
+def paged_check(cache: PagedCache, batch: PagedBatch, n_head: int, *, rope: PagedRope | None = None,
+                mask: PagedMask | None = None, ldq: int | None = None, ldkv: int | None = None, ldo: int | None = None) -> str:
+    """What the paged calls would refuse about these descriptors and strides, or "" (no device needed)."""
+    err = C.create_string_buffer(256)
+    rows = n_head * cache.hd
+    rc = load_library().fgh_paged_check(C.byref(cache), C.byref(batch), C.byref(rope) if rope else None,
+                                        C.byref(mask) if mask else None, n_head, rows if ldq is None else ldq,
+                                        cache.n_head_kv * cache.hd if ldkv is None else ldkv, rows if ldo is None else ldo, err,
+                                        len(err))
+    return "" if rc == OK else err.value.decode()
+
+
+def paged_slot(cache: PagedCache, table: np.ndarray, seq: int, pos: int, head: int, d: int, v: bool = False) -> int:
+    """The offset in values at which the paged kernels find value d of a head of a position in the K (or
+    V) pages, or -1 where they read and write nothing; table: host int32 [n_seq][table_stride] (no device needed)."""
+    t = np.ascontiguousarray(table, np.int32)
+    if t.shape != (t.shape[0], cache.table_stride) or not 0 <= seq < t.shape[0]:
+        raise ValueError("paged_slot: table is [n_seq][table_stride]")
+    return load_library().fgh_paged_slot(C.byref(cache), _p(t), seq, pos, head, d, int(v))
 
 
 _LIB = None
@@ -90,6 +155,13 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "fgh_kvq_store_dev": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, i32, vp]),
         "fgh_kvq_attention_dev": (i32, [vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, i32,
                                         C.c_float]),
+        "fgh_paged_store_dev": (i32, [vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedRope), i32, vp, i64,
+                                      vp, vp, i64, vp, i64]),
+        "fgh_paged_attention_dev": (i32, [vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedMask), i32, vp,
+                                          i64, vp, i64]),
+        "fgh_paged_slot": (i64, [C.POINTER(PagedCache), vp, i32, i32, i32, i32, i32]),
+        "fgh_paged_check": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedRope), C.POINTER(PagedMask), i32,
+                                  i64, i64, i64, C.c_char_p, C.c_size_t]),
         "fgh_graph_begin": (i32, [vp]),
         "fgh_graph_end": (i32, [vp, C.POINTER(vp)]),
         "fgh_graph_launch": (i32, [vp, vp]),
@@ -560,6 +632,15 @@ class Backend:
         self._check(self.lib.fgh_kvq_attention_dev(self.ctx, n_tok, n_head, n_head_kv, hd, kbits, vbits, q_dev,
                                                    o_dev, kq_dev, vq_dev, cap, st_dev, en_dev, max_len, scale))
 
+    def paged_store_dev(self, cache: PagedCache, batch: PagedBatch, rope: PagedRope, n_head: int, q_dev: int, ldq: int,
+                        k_dev: int, v_dev: int, ldkv: int, q_out_dev: int, ldo: int):
+        self._check(self.lib.fgh_paged_store_dev(self.ctx, cache, batch, rope, n_head, q_dev, ldq, k_dev, v_dev, ldkv,
+                                                 q_out_dev, ldo))
+
+    def paged_attention_dev(self, cache: PagedCache, batch: PagedBatch, mask: PagedMask, n_head: int, q_dev: int, ldq: int,
+                            o_dev: int, ldo: int):
+        self._check(self.lib.fgh_paged_attention_dev(self.ctx, cache, batch, mask, n_head, q_dev, ldq, o_dev, ldo))
+
     def kvq_store(self, k, v, pos, kq, vq, kbits: int, vbits: int):
         """Writes rows k / v ([n_tok][n_head_kv][hd]) at positions pos into host copies of the
         quantized caches kq / vq ([cap][slot bytes]), on the device; returns the new caches."""
@@ -606,5 +687,5 @@ class Backend:
                 self.dev_free(b)
 
 
-__all__ = ["Backend", "BackendError", "Gguf", "Tensor", "load_library", "EXPORTS", "T_Q4_K", "T_Q5_0", "T_Q5_K", "T_Q6_K", "T_Q8_0",
+__all__ = ["Backend", "BackendError", "Gguf", "PagedBatch", "PagedCache", "PagedMask", "PagedRope", "Tensor", "load_library", "EXPORTS", "T_Q4_K", "T_Q5_0", "T_Q5_K", "T_Q6_K", "T_Q8_0",
            "ORDER_AUTO", "ORDER_ROW", "ORDER_REPACKED"]

@@ -4,6 +4,8 @@
 // own CPU kernels).
 #include <hip/hip_runtime.h>
 
+#include <float.h>
+#include <math.h>
 #include <stdarg.h>
 #include <stdlib.h>
 #include <stdio.h>
@@ -16,6 +18,7 @@
 
 #include "../../include/fastgguf_hip.h"
 #include "fgh_internal.h"
+#include "fgh_paged.h"
 
 static const int FG_BATCH = 64;  // prompt batch limit (fastgguf.c:2139)
 
@@ -979,6 +982,106 @@ static bool kvq_shape_ok(int hd, int kbits, int vbits) {
            (vbits == 2 || vbits == 4 || vbits == 8);
 }
 
+// the paged calls' arguments: null, or what is wrong with them. Pointers' values are checked by the calls.
+static const char *paged_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_rope *r,
+                               const fgh_paged_mask *m, int n_head, int64_t ldq, int64_t ldkv, int64_t ldo) {
+    if (!c || !b || (!r && !m)) return "null descriptor";
+    if (c->type != FGH_T_F32 && c->type != FGH_T_F16 && c->type != FGH_T_BF16) return "the cache's type is not F32, F16 or BF16";
+    if (c->hd != 64 && c->hd != 80 && c->hd != 96 && c->hd != 128 && c->hd != 256) return "hd is not 64, 80, 96, 128 or 256";
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return "page is not a power of 2 from 16 to 256";
+    if (c->n_pages < 1 || c->table_stride < 1 || c->n_head_kv < 1 || c->n_head_kv > 4096) return "bad n_pages, table_stride or n_head_kv";
+    if (c->page_stride != 0 && (c->page_stride < (int64_t)c->n_head_kv * c->page * c->hd || c->page_stride % 8 != 0 || c->page_stride > (int64_t)1 << 40))
+        return "page_stride is smaller than a page or no multiple of 8";
+    if (b->n_seq < 1 || b->n_seq > 65535 || b->n_tok < 1 || b->max_tok < 1 || b->max_len < 1) return "bad n_seq, n_tok, max_tok or max_len";
+    if (n_head < (m ? 1 : 0) || n_head > 65535 / 4) return "bad n_head";
+    if ((n_head > 0 && (ldq < (int64_t)n_head * c->hd || ldo < (int64_t)n_head * c->hd)) || ldq % 4 != 0 || ldo % 4 != 0)
+        return "ldq or ldo is smaller than a row or no multiple of 4";
+    if (ldq > (int64_t)1 << 31 || ldo > (int64_t)1 << 31 || ldkv > (int64_t)1 << 31) return "a stride is too large";
+    if (r) {
+        if (ldkv < (int64_t)c->n_head_kv * c->hd || ldkv % 4 != 0) return "ldkv is smaller than a row or no multiple of 4";
+        if (r->n_rot < 0 || r->n_rot > c->hd || r->n_rot % 2 != 0) return "n_rot is odd or not 0 .. hd";
+        if (r->rope != FGH_ROPE_PAIRS && r->rope != FGH_ROPE_HALVES) return "unknown rope";
+        if (r->n_rot > 0 && !(r->freq_base > 0.0f && r->freq_base <= FLT_MAX && r->freq_scale > 0.0f && r->freq_scale <= FLT_MAX))
+            return "freq_base and freq_scale are not positive and finite";
+        if ((r->q_norm || r->k_norm) && !(r->eps >= 0.0f && r->eps <= FLT_MAX)) return "eps is negative or not finite";
+    }
+    if (m) {
+        if (n_head % c->n_head_kv != 0) return "n_head is no multiple of n_head_kv";
+        if (!(fabsf(m->scale) <= FLT_MAX) || !(m->softcap >= 0.0f && m->softcap <= FLT_MAX) || m->window < 0)
+            return "scale, softcap or window is negative or not finite";
+        if ((int64_t)b->n_tok * (n_head / c->n_head_kv) > INT32_MAX / 2) return "too many rows";
+    }
+    return nullptr;
+}
+static fgh::Paged paged_args(const fgh_paged_cache *c, const fgh_paged_batch *b) {
+    fgh::Paged p{};
+    p.k = (uint8_t *)c->k, p.v = (uint8_t *)c->v, p.table = c->table, p.tok = b->tok, p.len = b->len;
+    p.page_stride = c->page_stride ? c->page_stride : (int64_t)c->n_head_kv * c->page * c->hd;
+    p.type = (int)c->type, p.n_pages = c->n_pages, p.shift = __builtin_ctz((unsigned)c->page), p.table_stride = c->table_stride;
+    p.n_head_kv = c->n_head_kv, p.hd = c->hd, p.n_seq = b->n_seq, p.n_tok = b->n_tok, p.max_tok = std::min(b->max_tok, b->n_tok);
+    p.max_len = (int)std::min<int64_t>(b->max_len, std::min<int64_t>((int64_t)c->table_stride * c->page, INT32_MAX / 2));
+    return p;
+}
+int fgh_paged_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_rope *r, const fgh_paged_mask *m,
+                    int n_head, int64_t ldq, int64_t ldkv, int64_t ldo, char *err, size_t err_len) {
+    const char *why = paged_check(c, b, r, m, n_head, ldq, ldkv, ldo);
+    if (why && err && err_len) snprintf(err, err_len, "%s", why);
+    return why ? FGH_ERR_ARG : FGH_OK;
+}
+int64_t fgh_paged_slot(const fgh_paged_cache *c, const int32_t *table, int s, int pos, int kvh, int d, int is_v) {
+    if (!c || !table || c->page < 16 || s < 0 || pos < 0 || pos >= (int64_t)c->table_stride * c->page || kvh < 0 || kvh >= c->n_head_kv || d < 0 || d >= c->hd) return -1;
+    const fgh_paged_batch b{};
+    const fgh::Paged p = paged_args(c, &b);
+    const int page = table[(int64_t)s * p.table_stride + (pos >> p.shift)], in = pos & ((1 << p.shift) - 1);
+    if (!fgh::paged_ok(p, page)) return -1;
+    return fgh::paged_head(p, page, kvh) + (is_v ? ((int64_t)d << p.shift) + in : (int64_t)in * p.hd + d);
+}
+int fgh_paged_store_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_rope *rope,
+                        int n_head, const float *q, int64_t ldq, const float *k, const float *v, int64_t ldkv, float *qo,
+                        int64_t ldo) {
+    if (!c) return FGH_ERR_ARG;
+    if (!rope) return fail(c, FGH_ERR_ARG, "paged_store: null descriptor");
+    if (const char *why = paged_check(cache, batch, rope, nullptr, n_head, ldq, ldkv, ldo))
+        return fail(c, FGH_ERR_ARG, "paged_store: %s", why);
+    if (!cache->k || !cache->v || !cache->table || !batch->tok || !batch->len || !k || !v || (n_head > 0 && (!q || !qo)))
+        return fail(c, FGH_ERR_ARG, "paged_store: null pointer");
+    if (((uintptr_t)cache->table | (uintptr_t)batch->tok | (uintptr_t)batch->len | (uintptr_t)rope->q_norm | (uintptr_t)rope->k_norm | (uintptr_t)rope->freq_factors) % 4 != 0)
+        return fail(c, FGH_ERR_ARG, "paged_store: pointers must be 4-byte aligned");
+    if (((uintptr_t)cache->k | (uintptr_t)cache->v | (uintptr_t)k | (uintptr_t)v | (n_head > 0 ? (uintptr_t)q | (uintptr_t)qo : 0)) % 16 != 0)
+        return fail(c, FGH_ERR_ARG, "paged_store: the cache, q, k, v and q_out must be 16-byte aligned");
+    if (n_head > 0 && q == qo && ldq != ldo) return fail(c, FGH_ERR_ARG, "paged_store: q_out is q, with another stride");
+    INJECT(c);
+    HIP_TRY(c, hipSetDevice(c->device));
+    fgh::PagedStoreArgs a{};
+    a.p = paged_args(cache, batch);
+    a.r = fgh::PagedRopeArgs{rope->q_norm, rope->k_norm, rope->n_rot ? rope->freq_factors : nullptr, rope->eps,
+                             rope->n_rot ? log2((double)rope->freq_base) : 0.0, rope->freq_scale / 6.283185307179586476925,
+                             rope->n_rot, rope->rope == FGH_ROPE_HALVES};
+    a.q = q, a.k = k, a.v = v, a.qo = qo, a.ldq = ldq, a.ldkv = ldkv, a.ldo = ldo, a.n_head = n_head;
+    HIP_TRY(c, fgh::launch_paged_store(a, c->stream));
+    return FGH_OK;
+}
+int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_mask *mask,
+                            int n_head, const float *q, int64_t ldq, float *o, int64_t ldo) {
+    if (!c) return FGH_ERR_ARG;
+    if (!mask) return fail(c, FGH_ERR_ARG, "paged_attention: null descriptor");
+    if (const char *why = paged_check(cache, batch, nullptr, mask, n_head, ldq, 0, ldo))
+        return fail(c, FGH_ERR_ARG, "paged_attention: %s", why);
+    if (!cache->k || !cache->v || !cache->table || !batch->tok || !batch->len || !q || !o)
+        return fail(c, FGH_ERR_ARG, "paged_attention: null pointer");
+    if (((uintptr_t)cache->table | (uintptr_t)batch->tok | (uintptr_t)batch->len | (uintptr_t)mask->slopes | (uintptr_t)mask->prefix) % 4 != 0)
+        return fail(c, FGH_ERR_ARG, "paged_attention: pointers must be 4-byte aligned");
+    if (((uintptr_t)cache->k | (uintptr_t)cache->v | (uintptr_t)q | (uintptr_t)o) % 16 != 0)
+        return fail(c, FGH_ERR_ARG, "paged_attention: the cache, q and o must be 16-byte aligned");
+    INJECT(c);
+    HIP_TRY(c, hipSetDevice(c->device));
+    fgh::PagedAttnArgs a{};
+    a.p = paged_args(cache, batch);
+    a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo, a.n_head = n_head, a.window = mask->window, a.scale = mask->scale;
+    a.softcap = mask->softcap, a.slopes = mask->slopes, a.prefix = mask->prefix;
+    HIP_TRY(c, fgh::launch_paged_attention(a, c->stream));
+    return FGH_OK;
+}
 int fgh_kvq_store_dev(fgh_ctx *c, int n_tok, int n_head_kv, int hd, int kbits, int vbits, const float *k,
                       const float *v, int stride, uint8_t *kq, uint8_t *vq, int cap, const int32_t *pos) {
     if (!c) return FGH_ERR_ARG;

@@ -1,0 +1,81 @@
+// fgh_paged.h - the paged KV cache's addressing and batch description, shared by its append
+// (fgh_paged.hip) and its attention (fgh_pattn.hip). Internal.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fgh {
+
+// fgh_paged_cache and fgh_paged_batch as the kernels take them
+struct Paged {
+    uint8_t *k, *v;
+    const int32_t *table, *tok, *len;
+    int64_t page_stride;  // values between pages
+    int type, n_pages, shift, table_stride, n_head_kv, hd;  // 1 << shift positions a page
+    int n_seq, n_tok, max_tok, max_len;  // max_len: at most the table's positions
+};
+
+// offset in values of a head's block within k or v, for a page that is known to be in range
+__host__ __device__ inline int64_t paged_head(const Paged &a, int page, int kvh) {
+    return page * a.page_stride + ((int64_t)kvh * a.hd << a.shift);
+}
+__host__ __device__ inline bool paged_ok(const Paged &a, int page) { return (uint32_t)page < (uint32_t)a.n_pages; }
+
+// A sequence's rows t0 .. t0 + n - 1 and its positions. ok: within the batch's bounds; otherwise its
+// rows (clamped to the buffers) are NaN and nothing is appended.
+struct PagedSeq {
+    int t0, n, len;
+    bool ok;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const Paged &a, int s) {
+    const int b = a.tok[s], e = a.tok[s + 1], len = a.len[s];
+    PagedSeq q;
+    q.t0 = min(max(b, 0), a.n_tok);
+    q.n = max(min(e, a.n_tok) - q.t0, 0);
+    q.len = len;
+    q.ok = b >= 0 && e <= a.n_tok && q.n <= a.max_tok && len >= q.n && len <= a.max_len;
+    return q;
+}
+// the sequence of row t, or -1: the last s with tok[s] <= t, if t < tok[s + 1]. Every wavefront finds
+// it for itself, 64 starts a load.
+__device__ __forceinline__ int paged_find(const Paged &a, int t) {
+    const int lane = threadIdx.x & 63;
+    int s = -1;
+    for (int b = 0; b <= a.n_seq; b += 64) {  // starts tok[0] .. tok[n_seq]: the last one ends the batch
+        const int i = b + lane;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(i <= a.n_seq && a.tok[min(i, a.n_seq)] <= t);
+        s += __builtin_popcountll(m);
+        if (m != ~0ull) break;
+    }
+    return s >= a.n_seq ? -1 : s;
+}
+
+struct PagedRopeArgs {
+    const float *qw, *kw, *factors;
+    float eps;
+    double log2_base, scale_turns;  // log2(freq_base), freq_scale / (2 pi)
+    int n_rot, halves;
+};
+struct PagedStoreArgs {
+    Paged p;
+    PagedRopeArgs r;
+    const float *q, *k, *v;
+    float *qo;
+    int64_t ldq, ldkv, ldo;
+    int n_head;
+};
+hipError_t launch_paged_store(const PagedStoreArgs &a, hipStream_t s);
+
+struct PagedAttnArgs {
+    Paged p;
+    const float *q, *slopes;
+    float *o;
+    const int32_t *prefix;
+    int64_t ldq, ldo;
+    int n_head, window;
+    float scale, softcap;
+};
+hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
+
+}  // namespace fgh

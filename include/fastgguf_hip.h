@@ -276,6 +276,82 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
                           const float *q_dev, float *o_dev, const uint8_t *kq_dev, const uint8_t *vq_dev,
                           int cap, const int32_t *st_dev, const int32_t *en_dev, int max_len, float scale);
 
+/* ---- paged KV cache: several sequences, each with a table of pages. No counterpart in the
+ * reference, whose caches are rings of one sequence: for callers that serve many. The two calls below
+ * stand between the QKV and the O projection of a layer: the append of a batch's keys and values
+ * with the head norms and the position rotation (the reference's rope, for GGUF's rope types), and
+ * the attention over the pages. Activations are fp32, as everywhere here; results agree with the
+ * formulas to within 1e-5 relative per output vector. Both calls are asynchronous on the context's
+ * stream and can be captured (the attention's scratch must have its size from an eager call with the same
+ * descriptors, or larger ones, before).
+ *
+ * The cache: n_pages pages for `page` positions of n_head_kv heads of hd values of `type` (FGH_T_F32,
+ * FGH_T_F16 or FGH_T_BF16). K page: [n_head_kv][page][hd]; V page, transposed: [n_head_kv][hd][page].
+ * Pages start page_stride values apart in k and in v (0: n_head_kv * page * hd). Position j of
+ * sequence s is in page table[s * table_stride + j / page], place j % page.
+ * Requires hd 64, 80, 96, 128 or 256; page a power of 2 from 16 to 256; k and v 16-byte aligned,
+ * page_stride a multiple of 8. Offsets are 64-bit. */
+typedef struct {
+    void *k, *v;            /* device */
+    const int32_t *table;   /* device, [n_seq][table_stride] */
+    int64_t page_stride;
+    uint32_t type;
+    int32_t n_pages, page, table_stride, n_head_kv, hd;
+} fgh_paged_cache;
+/* The batch: sequence s's new tokens are rows tok[s] .. tok[s + 1] - 1 of the activations (any
+ * number, none included), and len[s] is its number of positions with them, so token i of n has
+ * position len[s] - n + i. n_tok is the number of rows in the buffers; rows before tok[0] and from
+ * tok[n_seq] on belong to no sequence and are left as they were. max_tok and max_len bound every
+ * sequence's new tokens and length. As these stay on the device, a sequence that breaks a bound
+ * (more than max_tok tokens, len above max_len or the table's positions or below its
+ * number of tokens, rows outside 0 .. n_tok) is no error: its rows are NaN and nothing is appended.
+ * tok is read as non-decreasing. */
+typedef struct {
+    const int32_t *tok;     /* device, [n_seq + 1] */
+    const int32_t *len;     /* device, [n_seq] */
+    int32_t n_seq, n_tok, max_tok, max_len;
+} fgh_paged_batch;
+/* What happens to the heads of q and k on the way. RMS norm, where q_norm / k_norm (device, [hd]) is
+ * not NULL: x * w / sqrt(mean(x^2) + eps). Rotation of the first n_rot values (even, 0: none) of each
+ * head by the angles p * freq_scale * freq_base^(-2i / n_rot) / freq_factors[i] (device, [n_rot / 2],
+ * or NULL for 1) of position p, formed in 64 bits; pairs (2i, 2i + 1) with FGH_ROPE_PAIRS, (i, i + n_rot / 2)
+ * with FGH_ROPE_HALVES. */
+#define FGH_ROPE_PAIRS 0
+#define FGH_ROPE_HALVES 1
+typedef struct {
+    const float *q_norm, *k_norm, *freq_factors;
+    float eps, freq_base, freq_scale;
+    int32_t n_rot, rope;
+} fgh_paged_rope;
+/* q: [n_tok][ldq], k and v: [n_tok][ldkv], head h at h * hd (ldq == ldkv and three pointers into one
+ * row: a fused QKV projection). q_out: [n_tok][ldo], may be q itself with ldo == ldq. k' and v go to the pages
+ * rounded to nearest even (F16: beyond 65504 to infinity). n_head 0: keys and values only, q and q_out unused.
+ * A token whose page is not 0 .. n_pages - 1 appends nothing. No two tokens of a call may share a
+ * slot (tables that share a page at positions being written). Pointers 16-byte aligned, strides multiples of 4. */
+FGH_API int fgh_paged_store_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, const fgh_paged_batch *batch,
+                        const fgh_paged_rope *rope, int n_head, const float *q_dev, int64_t ldq, const float *k_dev,
+                        const float *v_dev, int64_t ldkv, float *q_out_dev, int64_t ldo);
+/* o = softmax(s) v of every row (token, head), head h reading K / V head h / (n_head / n_head_kv):
+ *   s_j = scale q . k_j; softcap > 0: s = softcap tanh(s / softcap); slopes (device, [n_head], or NULL):
+ *   s -= slopes[h] |p - j|
+ * over the positions j that position p sees: j <= p or j < prefix[s] (device, [n_seq], or NULL: a prefix
+ * that all tokens see), j < len, and p - j < window (window > 0). Sequences do not see each other, so
+ * packed documents are sequences. Pages without a visible position are not read (their table entries may
+ * be anything); a row that sees a position whose page is not 0 .. n_pages - 1 is NaN. Values in
+ * positions that no row of a sequence sees do not matter, NaN included; a q or k that is not finite
+ * makes the rows that see it NaN or finite, a v that is not finite makes them not finite, and other
+ * rows stay as they are. len[s] counts the new tokens: append them first.
+ * q: [n_tok][ldq], o: [n_tok][ldo], not overlapping. Pointers 16-byte aligned, strides multiples of 4. */
+typedef struct {
+    float scale, softcap;
+    int32_t window;
+    const float *slopes;
+    const int32_t *prefix;
+} fgh_paged_mask;
+FGH_API int fgh_paged_attention_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, const fgh_paged_batch *batch,
+                            const fgh_paged_mask *mask, int n_head, const float *q_dev, int64_t ldq, float *o_dev,
+                            int64_t ldo);
+
 /* ---- HIP graphs of device-resident calls (launch-bound decode loops) ----
  * fgh_graph_begin starts capturing the context stream; the *_dev calls that follow are recorded,
  * not run; fgh_graph_end instantiates them as one executable graph that fgh_graph_launch replays
@@ -345,7 +421,13 @@ FGH_API int fgh_event_destroy(fgh_ctx *ctx, void *ev);
  * fgh_matmul_path: the kernels that fgh_matmul of ntok tokens (X rows cols apart) runs on a device of
  * num_cu compute units for n_mats matrices of rows x cols (order as fgh_upload resolved it):
  * FGH_MATMUL_DECODE the decode launches per token, FGH_MATMUL_GEMM the prompt GEMM, FGH_MATMUL_TOKENS
- * the kernels that share a matrix's weights between tokens. Needs no device. */
+ * the kernels that share a matrix's weights between tokens. Needs no device.
+ * fgh_paged_slot: where the paged kernels find value d of head kvh of position pos of sequence s in k (is_v 0) or v
+ * (is_v 1), as an offset in values, or -1 where they read and write nothing; `table` is host memory here
+ * (cache->table is not used). Needs no device.
+ * fgh_paged_check: the argument checks of fgh_paged_store_dev (rope not NULL) and fgh_paged_attention_dev
+ * (mask not NULL) on descriptors and strides, without pointers being read: FGH_OK, or FGH_ERR_ARG with a message in
+ * err. Needs no device. */
 #define FGH_MATMUL_DECODE 0
 #define FGH_MATMUL_GEMM 1
 #define FGH_MATMUL_TOKENS 2
@@ -366,6 +448,10 @@ FGH_API int fgh_fp16_to_f32(fgh_ctx *ctx, const uint16_t *h, int n, float *out);
 FGH_API int fgh_matvec_shape(fgh_ctx *ctx, uint32_t type, int order, int64_t cols, int64_t row_tiles, int ntok,
                              int32_t *shape);
 FGH_API int fgh_matmul_path(uint32_t type, int order, int64_t cols, int64_t rows, int64_t n_mats, int ntok, int num_cu);
+FGH_API int64_t fgh_paged_slot(const fgh_paged_cache *cache, const int32_t *table, int s, int pos, int kvh, int d, int is_v);
+FGH_API int fgh_paged_check(const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_rope *rope,
+                    const fgh_paged_mask *mask, int n_head, int64_t ldq, int64_t ldkv, int64_t ldo, char *err,
+                    size_t err_len);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,604 @@
+"""The paged KV cache on the device against float64 (tests/paged_ref.py): the append with head norms and rotation, and
+the attention over the pages, at the sizes, masks and damaged inputs where they can go wrong.
+
+Tolerances are per value, from the inputs: half a step of the cache's type for what is stored, and the
+bounds that paged_ref derives for the fp32 arithmetic."""
+import numpy as np
+import pytest
+from paged_ref import HALF_STEP, T_BF16, T_F16, T_F32, Batch, attention, decode, encode, store
+
+from fastgguf_amd.backend import ERR_ARG, BackendError, PagedBatch, PagedCache, PagedMask, PagedRope
+
+pytestmark = pytest.mark.gpu
+
+
+class Dev:
+    """Device copies of host arrays, freed together."""
+
+    def __init__(self, backend):
+        self.be, self.at, self.ptr = backend, [], {}
+
+    def put(self, a):
+        a = np.ascontiguousarray(a)
+        p = self.be.dev_alloc(max(16, a.nbytes))
+        self.at.append(p)
+        self.be.h2d(p, a)
+        return p
+
+    def get(self, p, like):
+        out = np.empty_like(like)
+        self.be.d2h(out, p)
+        return out
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        for p in self.at:
+            self.be.dev_free(p)
+
+
+def put_batch(d, b, max_len=None, max_tok=None):
+    """The cache and batch descriptors of b, its arrays on the device."""
+    cache = PagedCache(b.type, d.put(b.k), d.put(b.v), d.put(b.table), n_pages=b.n_pages, page=b.page, table_stride=b.stride,
+                       n_head_kv=b.n_kv, hd=b.hd, page_stride=b.page_stride)
+    batch = PagedBatch(d.put(b.tok), d.put(b.len), n_seq=len(b.news), n_tok=b.n_tok, max_tok=max_tok or max(b.news + [1]),
+                       max_len=max_len or max(b.lens + [1]))
+    return cache, batch
+
+
+def run_attention(be, b, q=None, scale=None, max_len=None, max_tok=None, slopes=None, prefix=None, extra=0, **kw):
+    """o [n_tok][n_head][hd] from rows `extra` values apart; o's rows are 777 before the call."""
+    q = b.q if q is None else q
+    scale = b.hd**-0.5 if scale is None else scale
+    row = b.n_head * b.hd
+    with Dev(be) as d:
+        cache, batch = put_batch(d, b, max_len, max_tok)
+        wide = np.full((b.n_tok, row + extra), 777.0, np.float32)
+        wide[:, :row] = q.reshape(b.n_tok, row)
+        qd, od = d.put(wide), d.put(np.full_like(wide, 777.0))
+        mask = PagedMask(scale, slopes=d.put(slopes) if slopes is not None else 0,
+                         prefix=d.put(np.asarray(prefix, np.int32)) if prefix is not None else 0, **kw)
+        be.paged_attention_dev(cache, batch, mask, b.n_head, qd, row + extra, od, row + extra)
+        o = d.get(od, wide)
+    assert (o[:, row:] == 777.0).all()
+    return o[:, :row].reshape(b.n_tok, b.n_head, b.hd)
+
+
+def check_attention(be, b, scale=None, max_len=None, max_tok=None, extra=0, **kw):
+    scale = b.hd**-0.5 if scale is None else scale
+    scale = float(np.float32(scale))
+    o = run_attention(be, b, scale=scale, max_len=max_len, max_tok=max_tok, extra=extra, **kw)
+    want, tol, mine = attention(b, b.q, scale, **kw)
+    assert (o[~mine] == 777.0).all()  # rows of no sequence
+    off = np.abs(o[mine] - want[mine])
+    assert (off <= tol[mine]).all(), (float((off / tol[mine]).max()), np.argwhere(~(off <= tol[mine]))[:4])
+    return o
+
+
+# ---- the append ----
+
+STORES = [  # type, hd, heads, K / V heads, page, news, lens, norms, n_rot, halves
+    (T_F16, 128, 8, 2, 16, [1], [1], False, 128, False),
+    (T_F16, 128, 8, 2, 16, [1], [4096], True, 128, True),
+    (T_BF16, 64, 4, 4, 32, [1, 1, 0, 1], [17, 64, 0, 100], True, 64, True),
+    (T_F16, 80, 5, 1, 64, [70, 0, 3], [70, 5, 131], True, 20, True),
+    (T_F32, 96, 4, 2, 16, [33, 16, 1], [40, 16, 300], False, 96, False),
+    (T_BF16, 256, 4, 2, 128, [129, 2], [129, 260], True, 256, True),
+    (T_F32, 256, 2, 1, 256, [3], [300], True, 64, False),
+    (T_F16, 64, 4, 1, 64, [200, 7], [451, 7], False, 0, False),
+    (T_F16, 128, 32, 8, 16, [5], [70], False, 126, True),
+    (T_BF16, 80, 3, 3, 16, [64], [64], True, 80, False),
+]
+
+
+@pytest.mark.parametrize("i", range(len(STORES)))
+@pytest.mark.parametrize("form", ["fused", "apart", "in place"])
+def test_store(backend, i, form):
+    t, hd, nh, nkv, page, news, lens, normed, n_rot, halves = STORES[i]
+    b = Batch(100 + i, t, hd, nh, nkv, page, news, lens, pad=(i % 3, 2 * (i % 2)), gap=8 * (i % 4))
+    r = b.rng
+    qkv = (r.standard_normal((b.n_tok, nh + 2 * nkv, hd)) * np.exp(r.uniform(-3, 3, (1, nh + 2 * nkv, 1)))).astype(np.float32)
+    norm = [(1 + 0.3 * r.standard_normal(hd)).astype(np.float32) for _ in range(2)] if normed else None
+    factors = np.exp(r.uniform(0, 2, max(1, n_rot // 2))).astype(np.float32) if i % 2 else None
+    base, scale = (500000.0, 0.25) if i % 3 == 0 else (10000.0, 1.0)
+    q, k, v, eq, ek = store(b, qkv, norm, n_rot, halves, base, scale, factors)
+    row = (nh + 2 * nkv) * hd
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        rope = PagedRope(n_rot=n_rot, halves=halves, freq_base=base, freq_scale=scale,
+                         freq_factors=d.put(factors) if factors is not None else 0, q_norm=d.put(norm[0]) if norm else 0,
+                         k_norm=d.put(norm[1]) if norm else 0)
+        if form == "apart":
+            qd, ldq = d.put(qkv[:, :nh]), nh * hd
+            wide = np.full((2, b.n_tok, nkv * hd + 12), 3.0, np.float32)
+            wide[0, :, :nkv * hd] = qkv[:, nh:nh + nkv].reshape(b.n_tok, -1)
+            wide[1, :, :nkv * hd] = qkv[:, nh + nkv:].reshape(b.n_tok, -1)
+            kd, vd, ldkv = d.put(wide[0]), d.put(wide[1]), nkv * hd + 12
+        else:
+            qd, ldq = d.put(qkv), row
+            kd, vd, ldkv = qd + 4 * nh * hd, qd + 4 * (nh + nkv) * hd, row
+        before = np.full((b.n_tok, nh * hd + 4), 777.0, np.float32)
+        od, ldo = (qd, row) if form == "in place" else (d.put(before), nh * hd + 4)
+        backend.paged_store_dev(cache, batch, rope, nh, qd, ldq, kd, vd, ldkv, od, ldo)
+        if form == "in place":
+            got = d.get(od, qkv)
+            assert np.array_equal(got[:, nh:], qkv[:, nh:])
+            got, before = got[:, :nh], qkv[:, :nh]
+        else:
+            got = d.get(od, before)
+            assert (got[:, nh * hd:] == 777.0).all()
+            got, before = got[:, :nh * hd].reshape(b.n_tok, nh, hd), before[:, :nh * hd].reshape(b.n_tok, nh, hd)
+        kc, vc = d.get(cache.k, b.k), d.get(cache.v, b.v)
+    touched = {False: np.zeros(b.k.shape, bool), True: np.zeros(b.k.shape, bool)}
+    mine = np.zeros(b.n_tok, bool)
+    for tok, s, pos in b.tokens():
+        mine[tok] = True
+        assert (np.abs(got[tok] - q[tok]) <= eq[tok] + 1e-30).all()
+        for h in range(nkv):
+            for is_v, code, want, err in ((False, kc, k[tok, h], ek[tok, h]), (True, vc, v[tok, h], 0.0)):
+                at = b.at(s, pos, h, is_v)
+                touched[is_v][at] = True
+                step = HALF_STEP[t] if t != T_F32 or is_v else 0.0
+                # half a step of the stored value, itself off by err (F16 below 2^-14: half of 2^-24)
+                assert (np.abs(decode(code[at], t) - want) <= step * (np.abs(want) + err) + err + 2.0**-25 * (t == T_F16)).all()
+                if is_v:
+                    assert np.array_equal(code[at], encode(v[tok, h].astype(np.float32), t))
+    assert np.array_equal(got[~mine], before[~mine])
+    for is_v, code, old in ((False, kc, b.k), (True, vc, b.v)):  # nothing else changes
+        assert np.array_equal(code[~touched[is_v]], old[~touched[is_v]])
+
+
+def test_store_far_positions(backend):
+    """Angles at positions where 32 bits would hold no fraction of a turn."""
+    b = Batch(7, T_F16, 64, 2, 1, 256, [3], [3])
+    far = 1 << 20
+    b.lens, b.len, b.stride = [far], np.array([far], np.int32), far // 256
+    b.table = np.full((1, b.stride), -1, np.int32)
+    b.table[0, -1] = 0
+    qkv = b.rng.standard_normal((3, 4, 64)).astype(np.float32)
+    q, k, _, eq, ek = store(b, qkv, None, 64, True, 5e6)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        qd, od = d.put(qkv), d.put(np.zeros((3, 2, 64), np.float32))
+        backend.paged_store_dev(cache, batch, PagedRope(n_rot=64, halves=True, freq_base=5e6), 2, qd, 256, qd + 512, qd + 768, 256, od, 128)
+        got, kc = d.get(od, np.zeros((3, 2, 64), np.float32)), d.get(cache.k, b.k)
+    assert (np.abs(got - q) <= eq).all()
+    for i in range(3):
+        at = b.at(0, far - 3 + i, 0, False)
+        assert (np.abs(decode(kc[at], T_F16) - k[i, 0]) <= 2.0**-11 * (np.abs(k[i, 0]) + ek[i, 0]) + ek[i, 0] + 2.0**-25).all()
+
+
+def test_store_without_queries(backend):
+    b = Batch(8, T_BF16, 64, 2, 2, 16, [5], [20])
+    kv = b.rng.standard_normal((2, 5, 2, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        backend.paged_store_dev(cache, batch, PagedRope(), 0, 0, 0, d.put(kv[0]), d.put(kv[1]), 128, 0, 0)
+        kc, vc = d.get(cache.k, b.k), d.get(cache.v, b.v)
+    for tok, s, pos in b.tokens():
+        for h in range(2):
+            assert np.array_equal(kc[b.at(s, pos, h, False)], encode(kv[0, tok, h], T_BF16))
+            assert np.array_equal(vc[b.at(s, pos, h, True)], encode(kv[1, tok, h], T_BF16))
+
+
+def test_store_overflow_and_specials(backend):
+    """F16 rounds to nearest even, past 65504 to infinity; NaN stays NaN."""
+    b = Batch(9, T_F16, 64, 1, 1, 16, [1], [1])
+    kv = np.zeros((2, 1, 1, 64), np.float32)
+    kv[:, 0, 0, :10] = [65504, 65519.9, 65520, -1e30, np.inf, np.nan, 2.0**-24, 2.0**-25, 1 + 2.0**-11, 1 + 3 * 2.0**-11]
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        backend.paged_store_dev(cache, batch, PagedRope(), 0, 0, 0, d.put(kv[0]), d.put(kv[1]), 64, 0, 0)
+        kc, vc = d.get(cache.k, b.k), d.get(cache.v, b.v)
+    with np.errstate(over="ignore"):
+        want = kv[0, 0, 0].astype(np.float16)
+    for c in (kc[b.at(0, 0, 0, False)], vc[b.at(0, 0, 0, True)]):
+        assert np.array_equal(c.view(np.float16), want, equal_nan=True)
+
+
+# ---- damaged batches: in-bounds, named by NaN, nothing appended ----
+
+def damaged(b, how):
+    """Makes sequence 1 of 3 break a bound; (max_len, max_tok) of the call."""
+    if how == "longer than max_len":
+        return max(b.lens[0], b.lens[2]), None
+    if how == "more than max_tok":
+        return None, max(b.news[0], b.news[2])
+    if how == "shorter than its tokens":
+        b.len[1] = b.news[1] - 1
+    if how == "longer than the table":
+        b.len[1] = b.stride * b.page + 1
+        return b.stride * b.page * 4, None
+    if how == "negative":
+        b.len[1] = -5
+    return None, None
+
+
+HOWS = ["longer than max_len", "more than max_tok", "shorter than its tokens", "longer than the table", "negative"]
+
+
+@pytest.mark.parametrize("how", HOWS)
+@pytest.mark.parametrize("news", [[2, 3, 1], [40, 70, 30]])
+def test_damaged_sequences(backend, how, news):
+    b = Batch(20, T_F16, 64, 4, 2, 16, news, [news[0] + 9, news[1] + 100, news[2]])
+    max_len, max_tok = damaged(b, how)
+    o = run_attention(backend, b, max_len=max_len, max_tok=max_tok)
+    want, tol, _ = attention(b, b.q, float(np.float32(0.125)))
+    bad = np.arange(b.tok[1], b.tok[2])
+    assert np.isnan(o[bad]).all()
+    fine = np.setdiff1d(np.arange(b.n_tok), bad)
+    assert (np.abs(o[fine] - want[fine]) <= tol[fine]).all()
+    qkv = b.rng.standard_normal((b.n_tok, 8, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b, max_len, max_tok)
+        qd, od = d.put(qkv), d.put(np.zeros((b.n_tok, 4, 64), np.float32))
+        backend.paged_store_dev(cache, batch, PagedRope(n_rot=64), 4, qd, 512, qd + 1024, qd + 1536, 512, od, 256)
+        got, kc, vc = d.get(od, np.zeros((b.n_tok, 4, 64), np.float32)), d.get(cache.k, b.k), d.get(cache.v, b.v)
+    assert np.isnan(got[bad]).all() and np.isfinite(got[fine]).all()
+    changed = np.zeros(b.k.shape, bool)
+    for s in (0, 2):
+        for pos in range(b.lens[s] - b.news[s], b.lens[s]):
+            for h in range(2):
+                changed[b.at(s, pos, h, False)] = True
+    assert np.array_equal(kc != b.k, changed & (kc != b.k)) and (kc != b.k).sum() > 0.9 * changed.sum()
+    assert (vc != b.v).sum() <= changed.sum()
+
+
+@pytest.mark.parametrize("page_no", [-1, 0x7FFFFFFF, -0x80000000, "n_pages"])
+@pytest.mark.parametrize("news", [[1, 1], [40, 5]])
+def test_bad_pages(backend, page_no, news):
+    """A page that does not exist: the rows that see one of its positions are NaN, the others as they are; an append into it
+    writes nothing."""
+    b = Batch(21, T_BF16, 64, 4, 2, 16, news, [news[0] + 70, 60])
+    b_good = Batch(21, T_BF16, 64, 4, 2, 16, news, [news[0] + 70, 60])
+    bad_pos = (b.lens[0] - 10) // 16 * 16  # page of the last positions: early new tokens do not see it
+    b.table[0, bad_pos // 16] = b.n_pages if page_no == "n_pages" else page_no
+    want, tol, _ = attention(b_good, b.q, 0.125)
+    o = run_attention(backend, b)
+    for t, s, p in b.tokens():
+        if s == 0 and p >= bad_pos:
+            assert np.isnan(o[t]).all()
+        else:
+            assert (np.abs(o[t] - want[t]) <= tol[t]).all()
+    kv = b.rng.standard_normal((b.n_tok, 2, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        kd = d.put(kv)
+        backend.paged_store_dev(cache, batch, PagedRope(), 0, 0, 0, kd, kd, 128, 0, 0)
+        kc = d.get(cache.k, b.k)
+    changed = np.zeros(b.k.shape, bool)
+    for t, s, p in b.tokens():
+        if not (s == 0 and b.table[0, p // 16] != b_good.table[0, p // 16]):
+            for h in range(2):
+                changed[b.at(s, p, h, False)] = True
+    assert not (kc != b.k)[~changed].any()
+
+
+# ---- attention ----
+
+SHAPES = [  # type, hd, heads, K / V heads, page, news, lens
+    (T_F16, 128, 8, 2, 16, [1], [1]),
+    (T_F16, 128, 8, 2, 16, [1, 1, 1], [2, 15, 16]),
+    (T_F16, 128, 32, 8, 64, [1, 1, 0, 1], [1000, 33, 0, 257]),
+    (T_BF16, 128, 4, 4, 32, [1, 1], [700, 31]),
+    (T_F32, 128, 8, 1, 16, [1, 1], [129, 515]),
+    (T_F16, 64, 16, 1, 128, [1], [2049]),
+    (T_F16, 64, 17, 1, 16, [1, 1], [100, 63]),  # 17 rows a K / V head
+    (T_BF16, 80, 5, 5, 16, [1, 3, 2], [200, 65, 2]),
+    (T_F32, 80, 4, 2, 256, [2], [700]),
+    (T_F16, 96, 6, 3, 32, [1, 2, 5], [64, 128, 300]),
+    (T_F32, 96, 2, 1, 16, [3], [50]),
+    (T_BF16, 256, 4, 2, 32, [1, 1], [300, 64]),
+    (T_F16, 256, 8, 4, 16, [2], [600]),
+    (T_F32, 256, 2, 2, 64, [1], [130]),
+    (T_F16, 128, 8, 2, 16, [17, 33, 4], [17, 50, 400]),
+    (T_F16, 128, 4, 1, 64, [200], [200]),
+    (T_F16, 128, 3, 1, 16, [64, 1, 0, 130], [700, 90, 40, 131]),
+    (T_BF16, 128, 2, 2, 32, [150], [333]),
+    (T_F32, 128, 2, 1, 16, [70, 40], [70, 300]),
+    (T_BF16, 64, 4, 4, 16, [100, 65, 64], [100, 65, 64]),
+    (T_F16, 80, 2, 1, 64, [90], [190]),
+    (T_F32, 80, 2, 2, 16, [65], [80]),
+    (T_BF16, 96, 4, 2, 128, [129], [400]),
+    (T_BF16, 256, 4, 2, 16, [70], [150]),
+    (T_F16, 256, 2, 1, 32, [100, 30], [100, 200]),
+    (T_F32, 256, 1, 1, 16, [40], [100]),
+]
+
+
+def shape(i, seed=0, **kw):
+    t, hd, nh, nkv, page, news, lens = SHAPES[i]
+    return Batch(300 + i + 1000 * seed, t, hd, nh, nkv, page, news, lens, **kw)
+
+
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_attention(backend, i):
+    check_attention(backend, shape(i, pad=(i % 2, i % 3), gap=16 * (i % 3)), extra=4 * (i % 4))
+
+
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+@pytest.mark.parametrize("how", ["cap", "bias", "window", "prefix", "all"])
+def test_attention_forms(backend, i, how):
+    b = shape(i, seed=1)
+    kw = {}
+    if how in ("cap", "all"):
+        kw["softcap"] = 5.0
+        b.q *= 4
+    if how in ("bias", "all"):
+        kw["slopes"] = np.exp2(-np.linspace(0.3, 8, b.n_head)).astype(np.float32)
+    if how in ("window", "all"):
+        kw["window"] = [1, 7, 16, 40, 64, 129, 1000][i % 7]
+    if how in ("prefix", "all"):
+        kw["prefix"] = np.array([[0, m, m // 2, -3, 1, m + 100][(i + s) % 6] for s, m in enumerate(b.lens)], np.int32)
+    check_attention(backend, b, **kw)
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("news", [1, 4, 40])
+def test_attention_sharp_scores(backend, t, news):
+    """Scores of up to some hundreds, large maxima late in the range, and a scale that is not hd^-0.5."""
+    b = Batch(40, t, 64, 4, 2, 16, [news], [400], sigma=3.0)
+    b.q *= 20
+    check_attention(backend, b, scale=0.31)
+    check_attention(backend, b, scale=-0.31)
+    check_attention(backend, b, scale=0.0)
+
+
+@pytest.mark.parametrize("t,tiny,huge", [(T_F16, 2.0**-12, 3e4), (T_BF16, 1e-25, 1e25), (T_F32, 1e-25, 1e25)])
+@pytest.mark.parametrize("news", [1, 40])
+def test_attention_ranges(backend, t, tiny, huge, news):
+    """Queries far outside 16-bit range, and values of the cache at the ends of its type's."""
+    for k_size, q_size, v_size in ((1.0, 1e6, 1.0), (1.0, 1e-9, huge), (tiny, 1.0 / tiny, tiny)):
+        b = Batch(41, t, 128, 4, 2, 16, [news], [100])
+        b.k, b.v = encode(decode(b.k, t) * k_size, t), encode(decode(b.v, t) * v_size / 8, t)
+        b.q = (b.q * q_size).astype(np.float32)
+        scale = 0.088 / (k_size * q_size)
+        o = run_attention(backend, b, scale=scale)
+        want, tol, _ = attention(b, b.q, float(np.float32(scale)))
+        assert (np.abs(o - want) <= tol).all()
+
+
+@pytest.mark.parametrize("lens", [[5000], [3, 5000, 1200, 64]])
+@pytest.mark.parametrize("news", [1, 4])
+def test_attention_long_split(backend, lens, news):
+    """Ranges that are split over workgroups, lengths far apart, a bound far above them."""
+    b = Batch(42, T_F16, 64, 4, 1, 16, [min(news, m) for m in lens], lens)
+    check_attention(backend, b)
+    b.stride += 2000  # a table for 32000 positions more
+    b.table = np.concatenate([b.table, np.full((len(lens), 2000), -1, np.int32)], 1)
+    check_attention(backend, b, max_len=b.stride * 16)
+
+
+@pytest.mark.parametrize("news", [1, 3, 50, 200])
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+def test_attention_stale_positions(backend, t, news):
+    """What positions behind a sequence's end, behind its window and in free pages hold does not matter."""
+    b = Batch(43, t, 128, 4, 2, 64, [news, 1], [news + 90, 30])
+    for kw in ({}, {"window": 20}):
+        for s, m in enumerate(b.lens):
+            first = max(0, m - b.news[s] - (20 if kw else 10**6) + 1)
+            for pos in list(range(m, -(-m // 64) * 64)) + list(range(first)):
+                for h in range(2):
+                    for is_v, buf in ((False, b.k), (True, b.v)):
+                        at = b.at(s, pos, h, is_v)
+                        buf[at] = encode(np.where(np.arange(128) % 2, np.nan, np.inf), t)
+        with np.errstate(invalid="ignore"):
+            o = run_attention(backend, b, scale=0.0884, **kw)
+        clean = Batch(43, t, 128, 4, 2, 64, [news, 1], [news + 90, 30])
+        want, tol, _ = attention(clean, clean.q, float(np.float32(0.0884)), **kw)
+        assert (np.abs(o - want) <= tol).all()
+    b.table[0, :max(0, b.lens[0] - news - 20 + 1) // 64] = -7  # pages that the window has left
+    o = run_attention(backend, b, scale=0.0884, window=20)
+    assert (np.abs(o - want) <= tol).all()
+
+
+@pytest.mark.parametrize("what", ["k", "v", "q"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("news", [4, 90])
+def test_attention_non_finite(backend, what, value, news):
+    """A new token's value that is not finite: the tokens before it do not see it, whatever tile they share."""
+    t, hd = T_F16, 128
+    b, clean = [Batch(44, t, hd, 4, 2, 16, [news], [news + 20]) for _ in range(2)]
+    at = news // 2  # of the new tokens
+    if what == "q":
+        b.q[at, 1, 5] = value
+    else:
+        (b.k if what == "k" else b.v)[b.at(0, 20 + at, 1, what == "v")[7]] = encode(np.float32([value]), t)[0]
+    with np.errstate(invalid="ignore"):
+        o = run_attention(backend, b, scale=0.0884)
+    want, tol, _ = attention(clean, clean.q, float(np.float32(0.0884)))
+    for r in range(news):
+        for h in range(4):
+            hit = (r == at and h == 1) if what == "q" else (r >= at and h // 2 == 1)
+            if not hit:
+                assert (np.abs(o[r, h] - want[r, h]) <= tol[r, h]).all(), (r, h)
+            elif what == "v":  # value 7 of the head is not finite, the others as they were
+                assert not np.isfinite(o[r, h, 7])
+                rest = np.arange(hd) != 7
+                assert (np.abs(o[r, h] - want[r, h]) <= tol[r, h])[rest].all()
+            elif np.isnan(value):
+                assert np.isnan(o[r, h]).all()
+
+
+def test_attention_64_bit_offsets(backend):
+    """Pages past 2^32 bytes from the start of the cache."""
+    b = Batch(45, T_F16, 64, 4, 2, 16, [2], [40])
+    stride, n = (1 << 30) + 64, 4
+    with Dev(backend) as d:
+        big = [backend.dev_alloc(2 * n * stride) for _ in range(2)]
+        try:
+            pages = [3, 1, 2]
+            for j in range(3):
+                old = int(b.table[0, j]) * b.page_stride
+                for p, src in zip(big, (b.k, b.v)):
+                    backend.h2d(p + 2 * pages[j] * stride, src[old:old + b.page_values])
+            cache = PagedCache(T_F16, big[0], big[1], d.put(np.array([pages], np.int32)), n_pages=n, page=16, table_stride=3,
+                               n_head_kv=2, hd=64, page_stride=stride)
+            batch = PagedBatch(d.put(b.tok), d.put(b.len), n_seq=1, n_tok=2, max_tok=2, max_len=48)
+            od = d.put(np.zeros((2, 4, 64), np.float32))
+            backend.paged_attention_dev(cache, batch, PagedMask(0.125), 4, d.put(b.q), 256, od, 256)
+            o = d.get(od, np.zeros((2, 4, 64), np.float32))
+            kv = b.rng.standard_normal((2, 2, 64)).astype(np.float32)
+            kd = d.put(kv)
+            backend.paged_store_dev(cache, batch, PagedRope(), 0, 0, 0, kd, kd, 128, 0, 0)
+            k2, v2 = np.empty(b.page_values, np.uint16), np.empty(b.page_values, np.uint16)
+            backend.d2h(k2, big[0] + 2 * 2 * stride)
+            backend.d2h(v2, big[1] + 2 * 2 * stride)
+        finally:
+            for p in big:
+                backend.dev_free(p)
+    want, tol, _ = attention(b, b.q, 0.125)
+    assert (np.abs(o - want) <= tol).all()
+    for t, pos in ((0, 38), (1, 39)):
+        for h in range(2):
+            at = h * 64 * 16
+            assert np.array_equal(k2[at + pos % 16 * 64:][:64], encode(kv[t, h], T_F16))
+            assert np.array_equal(v2[at + pos % 16:at + 64 * 16:16], encode(kv[t, h], T_F16))
+
+
+def test_attention_many_sequences(backend):
+    """More sequences than a wavefront has lanes, empty ones among them."""
+    rng = np.random.default_rng(5)
+    news = [int(v) for v in rng.choice([0, 1, 1, 1, 2], 150)]
+    lens = [n + int(v) for n, v in zip(news, rng.integers(0, 40, 150))]
+    check_attention(backend, Batch(46, T_F16, 64, 2, 1, 16, news, lens))
+    news = [int(v) for v in rng.choice([0, 1, 9, 20], 150)]
+    lens = [n + int(v) for n, v in zip(news, rng.integers(0, 40, 150))]
+    check_attention(backend, Batch(47, T_F16, 64, 2, 1, 16, news, lens))
+
+
+def test_same_results_twice(backend):
+    """No order of arrival in the results."""
+    for i in (2, 5, 16):
+        b = shape(i, seed=2)
+        first = run_attention(backend, b)
+        for _ in range(3):
+            assert np.array_equal(first.view(np.uint32), run_attention(backend, b).view(np.uint32))
+
+
+# ---- together ----
+
+@pytest.mark.parametrize("t", [T_F32, T_F16])
+def test_prompt_then_decode(backend, t):
+    """Two sequences: their prompts appended and read in a batch, then tokens one by one from a recorded graph whose
+    lengths move on, against float64 over everything appended."""
+    hd, nh, nkv, page, steps = 64, 4, 2, 16, 6
+    prompts = [37, 5]
+    b = Batch(60, t, hd, nh, nkv, page, prompts, [p + steps for p in prompts])
+    b.lens, b.len = prompts, np.array(prompts, np.int32)
+    row = (nh + 2 * nkv) * hd
+    kw = dict(n_rot=hd, halves=True)
+    r = np.random.default_rng(61)
+    norm = [(1 + 0.2 * r.standard_normal(hd)).astype(np.float32) for _ in range(2)]
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b, max_len=b.stride * page)
+        rope = PagedRope(q_norm=d.put(norm[0]), k_norm=d.put(norm[1]), **kw)
+        mask = PagedMask(hd**-0.5)
+
+        def step(be, x, q, o):
+            be.paged_store_dev(cache, batch, rope, nh, x, row, x + 4 * nh * hd, x + 4 * (nh + nkv) * hd, row, q, nh * hd)
+            be.paged_attention_dev(cache, batch, mask, nh, q, nh * hd, o, nh * hd)
+
+        def check(qkv, o, k_codes):
+            q, _, _, eq, _ = store(b, qkv, norm, **kw)
+            b.k, b.v = k_codes
+            want, tol, mine = attention(b, q.astype(np.float32), float(np.float32(hd**-0.5)))
+            # q' is off by eq: scores by eq |k| / 8
+            k = np.abs(decode(b.k, t)).max()
+            tol = tol + 4 * eq.sum(-1).max() * k * hd**-0.5 * np.abs(decode(b.v, t)).max()
+            assert (np.abs(o - want)[mine] <= tol[mine]).all()
+
+        def codes():
+            return d.get(cache.k, b.k), d.get(cache.v, b.v)
+
+        n = sum(prompts)
+        qkv = r.standard_normal((n, nh + 2 * nkv, hd)).astype(np.float32)
+        like = np.zeros((n, nh, hd), np.float32)
+        x, q, o = d.put(qkv), d.put(like), d.put(like)
+        step(backend, x, q, o)
+        check(qkv, d.get(o, like), codes())
+
+        # decode: the same descriptors' arrays, new contents, one graph
+        b.news, b.tok, b.n_tok = [1, 1], np.array([0, 1, 2], np.int32), 2
+        batch.n_tok, batch.max_tok = 2, 1
+        backend.h2d(batch.tok, b.tok)
+        like = np.zeros((2, nh, hd), np.float32)
+
+        def next_token(i):
+            b.lens = [p + i + 1 for p in prompts]
+            b.len = np.array(b.lens, np.int32)
+            backend.h2d(batch.len, b.len)
+            qkv = r.standard_normal((2, nh + 2 * nkv, hd)).astype(np.float32)
+            backend.h2d(x, qkv)
+            return qkv
+
+        qkv = next_token(0)
+        step(backend, x, q, o)  # sizes the scratch
+        check(qkv, d.get(o, like), codes())
+        backend.graph_begin()
+        step(backend, x, q, o)
+        g = backend.graph_end()
+        try:
+            for i in range(1, steps):
+                qkv = next_token(i)
+                backend.graph_launch(g)
+                check(qkv, d.get(o, like), codes())
+                replay = d.get(o, like)
+                step(backend, x, q, o)  # the eager calls, on the same inputs
+                assert np.array_equal(replay, d.get(o, like))
+        finally:
+            backend.graph_destroy(g)
+
+
+def test_agrees_with_ring_attention(backend):
+    """An fp32 paged cache against fgh_attention over the same positions in its ring."""
+    b = Batch(62, T_F32, 128, 8, 2, 16, [5], [300])
+    ring = [np.stack([np.concatenate([b.rows(0, h, is_v)[p] for h in range(2)]) for p in range(300)]).astype(np.float32)
+            for is_v in (False, True)]
+    en = np.arange(295, 300)
+    want = backend.attention(b.q, ring[0], ring[1], np.zeros(5), en, 2, 128**-0.5)
+    o = run_attention(backend, b)
+    _, tol, _ = attention(b, b.q, 128**-0.5)
+    assert (np.abs(o - want) <= 2 * tol).all()
+
+
+def test_refusals(backend):
+    b = Batch(63, T_F16, 64, 4, 2, 16, [1], [5])
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        p = d.put(np.zeros(1024, np.float32))
+        rope, mask = PagedRope(n_rot=64), PagedMask(0.125)
+
+        def refused(call, word):
+            with pytest.raises(BackendError) as e:
+                call()
+            assert e.value.status == ERR_ARG and word in str(e.value)
+
+        st = lambda q=p, k=p + 1024, v=p + 1536, o=p + 2048, rope=rope, ldq=256, ldo=256, n=4: backend.paged_store_dev(  # noqa: E731
+            cache, batch, rope, n, q, ldq, k, v, 128, o, ldo)
+        at = lambda q=p, o=p + 2048, mask=mask, n=4, ldq=256, ldo=256: backend.paged_attention_dev(  # noqa: E731
+            cache, batch, mask, n, q, ldq, o, ldo)
+        st()
+        at()
+        refused(lambda: st(q=0), "null")
+        refused(lambda: st(k=0), "null")
+        refused(lambda: st(k=p + 4), "aligned")
+        refused(lambda: st(o=p + 8), "aligned")
+        refused(lambda: st(ldq=255), "ldq")
+        refused(lambda: st(q=p, o=p, ldo=260), "stride")
+        refused(lambda: st(rope=PagedRope(n_rot=3)), "n_rot")
+        refused(lambda: st(rope=PagedRope(q_norm=p + 2)), "aligned")
+        refused(lambda: at(q=0), "null")
+        refused(lambda: at(o=p + 4), "aligned")
+        refused(lambda: at(n=3), "n_head")
+        refused(lambda: at(mask=PagedMask(float("nan"))), "scale")
+        refused(lambda: at(mask=PagedMask(1.0, prefix=p + 1)), "aligned")
+        for field, value, word in (("type", 8, "type"), ("hd", 72, "hd"), ("page", 24, "page"), ("k", 0, "null"), ("v", cache.v + 2, "aligned"),
+                                   ("table", 0, "null"), ("page_stride", 8, "page_stride")):
+            old = getattr(cache, field)
+            setattr(cache, field, value)
+            refused(at, word)
+            refused(st, word)
+            setattr(cache, field, old)
+        at()
