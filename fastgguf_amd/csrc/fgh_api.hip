@@ -38,6 +38,7 @@ struct fgh_ctx {
     DevBuf x, y, aqs, ad, abs;
     DevBuf gq;          // prompt-GEMM activation records (launch_gemm_quant layout)
     DevBuf as;          // attention scores / weights
+    DevBuf pa;          // paged attention: sums of split ranges
     DevBuf kqr, kor;    // TurboQuant attention: rotated queries, rotated outputs
     DevBuf msel, mw, mg, mu, md, mlog;  // MoE: selection, weights, gate / up / down outputs
     DevBuf mseg, mslot, mimx, mimh;         // MoE: per-expert slot counts and buckets, Q8_K images of x and h
@@ -519,7 +520,7 @@ void fgh_close(fgh_ctx *c) {
     (void)hipSetDevice(c->device);
     (void)hipStreamSynchronize(c->stream);
     for (DevBuf *b : {&c->x, &c->y, &c->aqs, &c->ad, &c->abs, &c->gq, &c->msel, &c->mw, &c->mg,
-                      &c->mu, &c->md, &c->mlog, &c->mseg, &c->mslot, &c->mimx, &c->mimh, &c->ck, &c->as, &c->kqr,
+                      &c->mu, &c->md, &c->mlog, &c->mseg, &c->mslot, &c->mimx, &c->mimh, &c->ck, &c->as, &c->pa, &c->kqr,
                       &c->kor, &c->h})
         if (b->p) (void)hipFree(b->p);
     free_retired(c);
@@ -1079,6 +1080,12 @@ int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_
     a.p = paged_args(cache, batch);
     a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo, a.n_head = n_head, a.window = mask->window, a.scale = mask->scale;
     a.softcap = mask->softcap, a.slopes = mask->slopes, a.prefix = mask->prefix;
+    const size_t slots = fgh::paged_attention_plan(a, c->num_cu);
+    if (slots) {
+        if (int rc = grow(c, c->pa, slots * (a.p.hd + 2) * 4)) return rc;
+        a.part = (float *)c->pa.p;
+        a.stat = a.part + slots * a.p.hd;
+    }
     HIP_TRY(c, fgh::launch_paged_attention(a, c->stream));
     return FGH_OK;
 }

@@ -75,7 +75,15 @@ struct PagedAttnArgs {
     int64_t ldq, ldo;
     int n_head, window;
     float scale, softcap;
+    // Sequences of few rows per K / V head (new tokens x query heads of the head) go to the decode kernel, the others
+    // to the prompt kernel; each kernel's ranges of positions are split over up to ds / ps workgroups, 0: not
+    // launched. Split ranges leave their sums in part [split][slot][hd] and stat [split][slot][2]. Decode slots: (sequence,
+    // K / V head, one of drows rows).
+    int ds, ps, drows;
+    float *part, *stat;
 };
+// the plan (ds, ps, drows) for a device of num_cu compute units; returns the slots x splits of part, then stat
+size_t paged_attention_plan(PagedAttnArgs &a, int num_cu);
 hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
 
 }  // namespace fgh

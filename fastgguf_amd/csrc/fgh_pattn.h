@@ -1,0 +1,188 @@
+// fgh_pattn.h - what the paged attention's kernels share (fgh_pdecode.hip, fgh_pprompt.hip, fgh_pattn.hip). Internal.
+//
+// fp32 results from 16-bit matrix instructions: every operand is a sum of 16-bit parts, and the products of parts are
+// summed in the fp32 accumulators.
+//   F16 cache   q and the weights as 2 halves (22 bits); K and V as they are: 2 products
+//   BF16 cache  q and the weights as 3 bf16, cut so that they hold all 24 bits; 3 products
+//   F32 cache   K and V too as 3 bf16; the 6 products down to 2^-16 of the largest (the 3 left out are below 2^-24)
+// Halves have 5 bits of exponent, so q rows are brought to [1, 2) by a power of two (the scores take it
+// back with the scale), and the weights, 0 .. 1 beside the largest, are carried times 2^10 (PBIAS): down to 2^-24 of the
+// largest both of a weight's halves are then normal numbers.
+#pragma once
+
+#include "fgh_internal.h"
+#include "fgh_paged.h"
+
+namespace fgh {
+
+typedef uint32_t pu4 __attribute__((ext_vector_type(4)));
+typedef float pf2 __attribute__((ext_vector_type(2)));
+typedef float pf4 __attribute__((ext_vector_type(4)));
+typedef float pf16 __attribute__((ext_vector_type(16)));
+typedef _Float16 ph2 __attribute__((ext_vector_type(2)));
+typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pb8 __attribute__((ext_vector_type(8)));
+
+template <int TYPE>
+struct PagedType {
+    static constexpr int ES = TYPE == T_F32 ? 4 : 2;  // bytes a cached value
+    static constexpr int NQ = TYPE == T_F16 ? 2 : 3;  // parts of q and of the weights
+    static constexpr int NK = TYPE == T_F32 ? 3 : 1;  // parts of K and V
+};
+
+// D += A B, 16 x 16 with 32 products a sum, or 32 x 32 with 16. A: lane l holds row l % 16 (32), values 8 (l / 16 (32)) .. + 7; B: column
+// l % 16 (32), the same values. D: column l % 16 (32); register r is row 4 (l / 16) + r, or 8 (r / 4) + 4 (l / 32) + r % 4.
+template <int TYPE>
+__device__ __forceinline__ void mma16(pf4 &d, pu4 x, pu4 y) {
+    if constexpr (TYPE == T_F16) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, x), __builtin_bit_cast(ph8, y), d, 0, 0, 0);
+    else d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pb8, x), __builtin_bit_cast(pb8, y), d, 0, 0, 0);
+}
+template <int TYPE>
+__device__ __forceinline__ void mma32(pf16 &d, pu4 x, pu4 y) {
+    if constexpr (TYPE == T_F16) d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ph8, x), __builtin_bit_cast(ph8, y), d, 0, 0, 0);
+    else d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pb8, x), __builtin_bit_cast(pb8, y), d, 0, 0, 0);
+}
+
+// 8 fp32 values as NP vectors of 8 16-bit parts
+template <int TYPE, int NP>
+__device__ __forceinline__ void parts8(const float *x, pu4 (&out)[NP]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const pf2 v = {x[2 * i], x[2 * i + 1]};
+        if constexpr (TYPE == T_F16) {  // to nearest, then what is left to nearest
+            const ph2 h = __builtin_convertvector(v, ph2);
+            out[0][i] = __builtin_bit_cast(uint32_t, h);
+            out[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v - __builtin_convertvector(h, pf2), ph2));
+        } else {  // the upper halves of the words, cut: what is left is exact, and 8 + 8 + 8 bits hold it all
+            pf2 r = v;
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                const uint32_t a = __float_as_uint(r.x), b = __float_as_uint(r.y);
+                out[k][i] = __builtin_amdgcn_perm(b, a, 0x07060302);
+                r.x -= __uint_as_float(a & 0xffff0000u);
+                r.y -= __uint_as_float(b & 0xffff0000u);
+            }
+        }
+    }
+}
+// 8 cached values (16 or 32 bytes) as parts
+template <int TYPE>
+__device__ __forceinline__ void cache8(const pu4 *raw, pu4 (&out)[PagedType<TYPE>::NK]) {
+    if constexpr (TYPE == T_F32) {
+        const float x[8] = {__uint_as_float(raw[0].x), __uint_as_float(raw[0].y), __uint_as_float(raw[0].z), __uint_as_float(raw[0].w),
+                            __uint_as_float(raw[1].x), __uint_as_float(raw[1].y), __uint_as_float(raw[1].z), __uint_as_float(raw[1].w)};
+        parts8<TYPE, 3>(x, out);
+    } else
+        out[0] = raw[0];
+}
+
+// cached value e of 8 in raw: whether it is not finite
+template <int TYPE>
+__device__ __forceinline__ bool raw_bad(const pu4 *raw, int e) {
+    if constexpr (TYPE == T_F32) return (raw[e / 4][e % 4] & 0x7f800000u) == 0x7f800000u;
+    const uint32_t h = raw[0][e / 2] >> (16 * (e & 1));
+    return TYPE == T_F16 ? (h & 0x7c00u) == 0x7c00u : (h & 0x7f80u) == 0x7f80u;
+}
+template <int TYPE>
+__device__ __forceinline__ void raw_zero(pu4 *raw, int e) {
+    if constexpr (TYPE == T_F32) raw[e / 4][e % 4] = 0;
+    else raw[0][e / 2] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+}
+template <int TYPE>
+__device__ __forceinline__ float cached(const uint8_t *base, int64_t i) {
+    if constexpr (TYPE == T_F32) return ((const float *)base)[i];
+    else if constexpr (TYPE == T_F16) return (float)((const _Float16 *)base)[i];
+    else return __uint_as_float((uint32_t)((const uint16_t *)base)[i] << 16);
+}
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float PBIAS = 10.0f;  // weights are 2^(PBIAS + s - m): s in powers of two, m a running reference of the row
+constexpr float PTOP = 15.0f;   // m follows a larger s where the exponent would pass this: a half's largest is 2^16
+
+// tanh: y + y^3 g(y^2) below 0.65 (g fitted at Chebyshev nodes), 1 - 2 / (e^(2 y) + 1) above: within 3 roundings
+__device__ __forceinline__ float tanh_near(float y) {
+    const float z = y * y;
+    float g = -0.005932980682700872f;
+    g = __builtin_fmaf(g, z, 0.020881319418549538f);
+    g = __builtin_fmaf(g, z, -0.053825847804546356f);
+    g = __builtin_fmaf(g, z, 0.13332600891590118f);
+    g = __builtin_fmaf(g, z, -0.333333283662796f);
+    const float small = __builtin_fmaf(y * z, g, y);
+    const float e = __builtin_amdgcn_exp2f(fabsf(y) * (2.0f * LOG2E));
+    const float big = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), y);
+    return fabsf(y) < 0.65f ? small : big;
+}
+
+// What turns a row's products into scores in powers of two, s = v mul (v the products, unless a form has changed them)
+struct PagedScore {
+    float mul;             // |scale| log2(e), times the power of two that q was divided by; above 0, so that -inf v
+                           // are -inf scores (q takes the scale's sign, and a scale of 0 is 2^-126 here)
+    float cap_in, cap_out; // |scale| / softcap (with that power), softcap log2(e); cap_out 0: none
+    float slope;           // slopes[h] log2(e)
+    bool bias;
+    // NE products of positions j0 .. j0 + NE - 1 of a row at position p
+    template <int NE>
+    __device__ __forceinline__ float apply(float (&v)[NE], int j0, int p) const {
+        if (cap_out > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] = cap_out * tanh_near(v[e] * cap_in);
+            if (!bias) return 1.0f;
+        } else if (bias) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) v[e] *= mul;
+        } else
+            return mul;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) v[e] = __builtin_fmaf(-slope, fabsf((float)(p - j0 - e)), v[e]);
+        return 1.0f;
+    }
+};
+__device__ __forceinline__ PagedScore paged_score(const PagedAttnArgs &a, int head, float q_size) {
+    PagedScore c;
+    c.mul = fmaxf(fabsf(a.scale) * LOG2E * q_size, __FLT_MIN__);
+    c.cap_in = a.softcap > 0.0f ? fabsf(a.scale) / a.softcap * q_size : 0.0f;
+    c.cap_out = a.softcap * LOG2E;
+    c.bias = a.slopes != nullptr;
+    c.slope = c.bias ? a.slopes[head] * LOG2E : 0.0f;
+    return c;
+}
+
+// the power of two that brings a row's largest magnitude to [1, 2), as the factor that undoes it (amax 0 or
+// not finite: 1)
+__device__ __forceinline__ float row_size(float amax) {
+    const uint32_t e = __float_as_uint(amax) >> 23;
+    return e >= 1 && e <= 252 ? __uint_as_float(e << 23) : 1.0f;
+}
+
+// positions lo .. hi that the new tokens i0 .. i1 of a sequence see, and those that all of them see
+struct PagedSpan {
+    int lo, hi, in_lo, in_hi;
+};
+__device__ __forceinline__ int row_lo(const PagedAttnArgs &a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs &a, const PagedSeq &q, int prefix, int i0, int i1) {
+    const int p0 = q.len - q.n + i0, p1 = q.len - q.n + i1;
+    return PagedSpan{row_lo(a, p0), max(p1, prefix - 1), row_lo(a, p1), max(p0, prefix - 1)};
+}
+__device__ __forceinline__ int paged_prefix(const PagedAttnArgs &a, int s, const PagedSeq &q) {
+    return a.prefix ? min(a.prefix[s], q.len) : 0;
+}
+// a range of n units over at most `splits` workgroups, `least` units or more each: the units of one, and how many
+// workgroups have any
+struct PagedChunk {
+    int per, used;
+};
+__device__ __forceinline__ PagedChunk paged_chunk(int n, int splits, int least) {
+    const int per = ((n + splits - 1) / splits + least - 1) / least * least;
+    return PagedChunk{per, (n + per - 1) / per};
+}
+
+constexpr int DEC_ROWS = 16;                // rows of the decode kernel
+constexpr int DEC_STEP = 32, DEC_LEAST = 4; // positions a step of a wavefront, least steps of a workgroup
+// the decode kernel's steps of a range
+__device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
+
+hipError_t launch_paged_decode(const PagedAttnArgs &a, hipStream_t s);
+hipError_t launch_paged_prompt(const PagedAttnArgs &a, hipStream_t s);
+
+}  // namespace fgh

@@ -1,10 +1,9 @@
 // fgh_pattn.hip - attention over the paged KV cache on gfx950.
-#include "fgh_paged.h"
+#include <hip/hip_runtime.h>
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+#include <algorithm>
 
-#include "fgh_internal.h"
+#include "fgh_pattn.h"
 
 namespace fgh {
 
@@ -25,6 +24,7 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnArgs a) {
     if (s < 0) return;
     float *o = a.o + t * a.ldo + (int64_t)h * hd;
     const PagedSeq sq = paged_seq(a.p, s);
+    if (a.ds > 0 && (int64_t)sq.n * (a.n_head / a.p.n_head_kv) <= DEC_ROWS) return;
     if (!sq.ok) {
         for (int i = lane; i < hd; i += 64) o[i] = __builtin_nanf("");
         return;
@@ -69,11 +69,74 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnArgs a) {
         if (lane + 64 * e < hd) o[lane + 64 * e] = acc[e] / l;
 }
 
+// Sums of split ranges joined: grid (sequence x K / V head, fours of rows), a wavefront per row. Lane groups of hd / 4 lanes take
+// splits in turn, 16 bytes a lane; always the same order.
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+    const int nkv = a.p.n_head_kv, G = a.n_head / nkv, s = blockIdx.x / nkv, kvh = blockIdx.x - s * nkv;
+    const int r = __builtin_amdgcn_readfirstlane((int)blockIdx.y * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63, hd = a.p.hd;
+    const PagedSeq q = paged_seq(a.p, s);
+    if (!q.ok || (int64_t)q.n * G > DEC_ROWS || r >= q.n * G) return;
+    const int used = paged_chunk(dec_steps(paged_span(a, q, paged_prefix(a, s, q), 0, q.n - 1)), a.ds, DEC_LEAST).used;
+    if (used == 1) return;
+    const int64_t t = q.t0 + r / G, row = (int64_t)blockIdx.x * a.drows + r, all = (int64_t)gridDim.x * a.drows;
+    const int h = kvh * G + r % G;
+    // at most 64 splits: lane i has split i's
+    float c = __FLT_MAX__, l = 0.0f;
+    if (lane < used) {
+        c = a.stat[2 * (lane * all + row)];
+        l = a.stat[2 * (lane * all + row) + 1];
+    }
+    float cm = c;
+    for (int o = 1; o < 64; o <<= 1) cm = fminf(cm, __shfl_xor(cm, o, 64));
+    const float f = __builtin_amdgcn_exp2f(cm - c);
+    l *= f;
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+    const int per = hd / 4, groups = 64 / per, g = lane / per, d = 4 * (lane - g * per);
+    pf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b = 0; b < used; b += groups) {  // uniform
+        const int i = b + g;
+        const float w = __shfl(f, min(i, 63), 64);
+        if (g < groups && i < used) o += w * *(const pf4 *)(a.part + (i * all + row) * hd + d);
+    }
+    for (int k = 1; k < groups; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float z = __shfl(o[e], (lane + k * per) & 63, 64);
+            if (g == 0) o[e] += z;
+        }
+    if (g == 0) *(pf4 *)(a.o + t * a.ldo + (int64_t)h * hd + d) = o / l;
+}
+
 }  // namespace
 
+// Splits: workgroups for every compute unit eight times over (sequences' lengths differ, and the bounds may be far above
+// them: the kernels split what is there), at most 64 (a lane each in the join), at least 128 positions each.
+size_t paged_attention_plan(PagedAttnArgs &a, int num_cu) {
+    const int G = a.n_head / a.p.n_head_kv;
+    const int64_t most = (int64_t)a.p.max_tok * G;  // rows of a sequence and K / V head
+    const int64_t heads = (int64_t)a.p.n_seq * a.p.n_head_kv;
+    a.ps = most > DEC_ROWS ? 1 : 0;
+    a.ds = 0;
+    a.drows = (int)std::min<int64_t>(most, DEC_ROWS);
+    if (a.ps == 0 || a.p.n_seq > 1) {
+        const int64_t want = std::max<int64_t>(1, 8 * (int64_t)num_cu / heads);
+        a.ds = (int)std::min<int64_t>({64, want, (a.p.max_len + DEC_STEP * DEC_LEAST - 1) / (DEC_STEP * DEC_LEAST)});
+    }
+    return a.ds > 1 ? (size_t)a.ds * heads * a.drows : 0;
+}
+
 hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
-    paged_attn_kernel<<<dim3((unsigned)a.p.n_tok, (unsigned)a.n_head), 64, 0, s>>>(a);
-    return hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (a.ds > 0 && (e = launch_paged_decode(a, s)) != hipSuccess) return e;
+    if (a.ds > 1) {
+        paged_join_kernel<<<dim3((unsigned)a.p.n_seq * (unsigned)a.p.n_head_kv, (unsigned)(a.drows + 3) / 4), 256, 0, s>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (a.ps > 0) {
+        paged_attn_kernel<<<dim3((unsigned)a.p.n_tok, (unsigned)a.n_head), 64, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace fgh
