@@ -182,6 +182,51 @@ constexpr int DEC_STEP = 32, DEC_LEAST = 4; // positions a step of a wavefront, 
 // the decode kernel's steps of a range
 __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
 
+constexpr int PRO_ROWS = 128;               // rows of a workgroup of the prompt kernel
+constexpr int PRO_UNIT = 64, PRO_LEAST = 1; // positions are split in units of 64
+__device__ __forceinline__ int pro_units(const PagedSpan &r) { return (r.hi - (r.lo & ~(PRO_UNIT - 1))) / PRO_UNIT + 1; }
+// at most as many tiles of PRO_ROWS rows as a batch's sequences can have, per K / V head
+inline int64_t paged_tiles(const PagedAttnArgs &a) {
+    return (int64_t)a.p.n_tok * (a.n_head / a.p.n_head_kv) / PRO_ROWS + a.p.n_seq;
+}
+// Tile `index` of the batch: the sequences' tiles in order (of those that are the prompt kernel's). s = -1: there are fewer.
+struct PagedTile {
+    int s, r0, index;
+    PagedSeq q;
+};
+__device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int index) {
+    const int lane = threadIdx.x & 63, G = a.n_head / a.p.n_head_kv;
+    int64_t before = 0;  // tiles of the sequences before the 64 looked at
+    PagedTile t;
+    t.s = -1, t.r0 = 0, t.index = index, t.q = PagedSeq{};
+    for (int b = 0; b < a.p.n_seq; b += 64) {
+        const int s = b + lane;
+        int64_t own = 0;
+        if (s < a.p.n_seq) {
+            const PagedSeq q = paged_seq(a.p, s);
+            const int64_t rows = (int64_t)q.n * G;
+            own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (rows + PRO_ROWS - 1) / PRO_ROWS;
+        }
+        int64_t upto = own;  // with this lane's
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t z = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += z;
+        }
+        const uint64_t m = __builtin_amdgcn_ballot_w64(before + upto > index);
+        if (m) {
+            const int at = __builtin_ctzll(m);
+            t.s = b + at;
+            t.r0 = (int)(index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
+            t.s = __builtin_amdgcn_readfirstlane(t.s);
+            t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
+            t.q = paged_seq(a.p, t.s);
+            return t;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return t;
+}
+
 hipError_t launch_paged_decode(const PagedAttnArgs &a, hipStream_t s);
 hipError_t launch_paged_prompt(const PagedAttnArgs &a, hipStream_t s);
 

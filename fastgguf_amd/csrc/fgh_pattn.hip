@@ -9,82 +9,15 @@ namespace fgh {
 
 namespace {
 
-__device__ __forceinline__ float paged_get(const uint8_t *base, int64_t i, int type) {
-    if (type == T_F32) return ((const float *)base)[i];
-    if (type == T_F16) return (float)((const _Float16 *)base)[i];
-    return (float)((const __bf16 *)base)[i];
-}
-
-// one wavefront per (token, head): 64 positions at a time, a lane each for the scores, a lane per value of the head for
-// the sums, with the softmax's running maximum and sum
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnArgs a) {
-    __shared__ float q[256];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = a.p.hd, kvh = h / (a.n_head / a.p.n_head_kv);
-    const int s = paged_find(a.p, t);
-    if (s < 0) return;
-    float *o = a.o + t * a.ldo + (int64_t)h * hd;
-    const PagedSeq sq = paged_seq(a.p, s);
-    if (a.ds > 0 && (int64_t)sq.n * (a.n_head / a.p.n_head_kv) <= DEC_ROWS) return;
-    if (!sq.ok) {
-        for (int i = lane; i < hd; i += 64) o[i] = __builtin_nanf("");
-        return;
-    }
-    const int pos = sq.len - sq.n + (t - sq.t0);
-    const int hi = max(pos, a.prefix ? min(a.prefix[s], sq.len) - 1 : 0);
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    for (int i = lane; i < hd; i += 64) q[i] = a.q[t * a.ldq + (int64_t)h * hd + i];
-    __syncthreads();
-    const float slope = a.slopes ? a.slopes[h] : 0.0f;
-    float m = -__builtin_inff(), l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t j0 = lo; j0 <= hi; j0 += 64) {
-        const int j = (int)min(j0 + lane, (int64_t)hi);
-        const int page = a.p.table[(int64_t)s * a.p.table_stride + (j >> a.p.shift)], in = j & ((1 << a.p.shift) - 1);
-        const bool ok = paged_ok(a.p, page);
-        const int64_t at = paged_head(a.p, ok ? page : 0, kvh);
-        float x = 0.0f;
-        for (int i = 0; i < hd; ++i) x = __builtin_fmaf(q[i], paged_get(a.p.k, at + (int64_t)in * hd + i, a.p.type), x);
-        x *= a.scale;
-        if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-        if (a.slopes) x -= slope * fabsf((float)(pos - j));
-        if (!ok) x = __builtin_nanf("");
-        if (j0 + lane > hi) x = -__builtin_inff();
-        float mx = x;
-        bool bad = x != x;
-        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-        const float mn = fmaxf(m, mx), scale = expf(m - mn), p = j0 + lane > hi ? 0.0f : bad ? x : expf(x - mn);
-        float sum = p;
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        l = l * scale + sum;
-        m = mn;
-        for (int e = 0; e < 4; ++e) acc[e] *= scale;
-        for (int u = 0; u < 64 && j0 + u <= hi; ++u) {
-            const float pu = __shfl(p, u, 64);
-            const int64_t au = __shfl(at, u, 64) + __shfl(in, u, 64);
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < hd)
-                    acc[e] = __builtin_fmaf(pu, paged_get(a.p.v, au + ((int64_t)(lane + 64 * e) << a.p.shift), a.p.type), acc[e]);
-        }
-    }
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < hd) o[lane + 64 * e] = acc[e] / l;
-}
-
-// Sums of split ranges joined: grid (sequence x K / V head, fours of rows), a wavefront per row. Lane groups of hd / 4 lanes take
-// splits in turn, 16 bytes a lane; always the same order.
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-    const int nkv = a.p.n_head_kv, G = a.n_head / nkv, s = blockIdx.x / nkv, kvh = blockIdx.x - s * nkv;
-    const int r = __builtin_amdgcn_readfirstlane((int)blockIdx.y * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63, hd = a.p.hd;
-    const PagedSeq q = paged_seq(a.p, s);
-    if (!q.ok || (int64_t)q.n * G > DEC_ROWS || r >= q.n * G) return;
-    const int used = paged_chunk(dec_steps(paged_span(a, q, paged_prefix(a, s, q), 0, q.n - 1)), a.ds, DEC_LEAST).used;
-    if (used == 1) return;
-    const int64_t t = q.t0 + r / G, row = (int64_t)blockIdx.x * a.drows + r, all = (int64_t)gridDim.x * a.drows;
-    const int h = kvh * G + r % G;
+// Sums of split ranges joined: a wavefront per row. Lane groups of hd / 4 lanes take splits in turn, 16 bytes a lane; always the
+// same order. Slot `slot` of `slots`, used of its splits written; row to o.
+__device__ __forceinline__ void join_row(const PagedAttnArgs &a, int64_t slot, int64_t slots, int used, float *out) {
+    const int lane = threadIdx.x & 63, hd = a.p.hd;
     // at most 64 splits: lane i has split i's
     float c = __FLT_MAX__, l = 0.0f;
     if (lane < used) {
-        c = a.stat[2 * (lane * all + row)];
-        l = a.stat[2 * (lane * all + row) + 1];
+        c = a.stat[2 * (lane * slots + slot)];
+        l = a.stat[2 * (lane * slots + slot) + 1];
     }
     float cm = c;
     for (int o = 1; o < 64; o <<= 1) cm = fminf(cm, __shfl_xor(cm, o, 64));
@@ -96,7 +29,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     for (int b = 0; b < used; b += groups) {  // uniform
         const int i = b + g;
         const float w = __shfl(f, min(i, 63), 64);
-        if (g < groups && i < used) o += w * *(const pf4 *)(a.part + (i * all + row) * hd + d);
+        if (g < groups && i < used) o += w * *(const pf4 *)(a.part + (i * slots + slot) * hd + d);
     }
     for (int k = 1; k < groups; ++k)
 #pragma unroll
@@ -104,7 +37,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
             const float z = __shfl(o[e], (lane + k * per) & 63, 64);
             if (g == 0) o[e] += z;
         }
-    if (g == 0) *(pf4 *)(a.o + t * a.ldo + (int64_t)h * hd + d) = o / l;
+    if (g == 0) *(pf4 *)(out + d) = o / l;
+}
+
+// grid (sequence x K / V head, fours of rows)
+__global__ __launch_bounds__(256) void paged_join_decode_kernel(PagedAttnArgs a) {
+    const int nkv = a.p.n_head_kv, G = a.n_head / nkv, s = blockIdx.x / nkv, kvh = blockIdx.x - s * nkv;
+    const int r = __builtin_amdgcn_readfirstlane((int)blockIdx.y * 4 + (threadIdx.x >> 6));
+    const PagedSeq q = paged_seq(a.p, s);
+    if (!q.ok || (int64_t)q.n * G > DEC_ROWS || r >= q.n * G) return;
+    const int used = paged_chunk(dec_steps(paged_span(a, q, paged_prefix(a, s, q), 0, q.n - 1)), a.ds, DEC_LEAST).used;
+    if (used == 1) return;
+    join_row(a, (int64_t)blockIdx.x * a.drows + r, (int64_t)gridDim.x * a.drows, used,
+             a.o + (q.t0 + r / G) * a.ldo + (int64_t)(kvh * G + r % G) * a.p.hd);
+}
+// grid (tile x K / V head, eights of rows): each wavefront two rows
+__global__ __launch_bounds__(256) void paged_join_prompt_kernel(PagedAttnArgs a) {
+    const int nkv = a.p.n_head_kv, G = a.n_head / nkv, kvh = blockIdx.x % nkv;
+    const PagedTile t = paged_tile(a, blockIdx.x / nkv);
+    if (t.s < 0 || !t.q.ok) return;
+    const int R = min(PRO_ROWS, t.q.n * G - t.r0);
+    const int used = paged_chunk(pro_units(paged_span(a, t.q, paged_prefix(a, t.s, t.q), t.r0 / G, (t.r0 + R - 1) / G)), a.ps, PRO_LEAST).used;
+    if (used == 1) return;
+    for (int k = 0; k < 2; ++k) {
+        const int r = __builtin_amdgcn_readfirstlane((int)blockIdx.y * 8 + k * 4 + (threadIdx.x >> 6));
+        if (r >= R) return;
+        const int row = t.r0 + r;
+        join_row(a, (int64_t)blockIdx.x * PRO_ROWS + r, (int64_t)gridDim.x * PRO_ROWS, used,
+                 a.o + (t.q.t0 + row / G) * a.ldo + (int64_t)(kvh * G + row % G) * a.p.hd);
+    }
 }
 
 }  // namespace
@@ -115,25 +76,35 @@ size_t paged_attention_plan(PagedAttnArgs &a, int num_cu) {
     const int G = a.n_head / a.p.n_head_kv;
     const int64_t most = (int64_t)a.p.max_tok * G;  // rows of a sequence and K / V head
     const int64_t heads = (int64_t)a.p.n_seq * a.p.n_head_kv;
-    a.ps = most > DEC_ROWS ? 1 : 0;
+    a.ps = 0;
     a.ds = 0;
     a.drows = (int)std::min<int64_t>(most, DEC_ROWS);
+    const int units = (a.p.max_len + PRO_UNIT - 1) / PRO_UNIT;
+    size_t slots = 0;
+    if (most > DEC_ROWS) {
+        const int64_t wgs = paged_tiles(a) * a.p.n_head_kv;
+        a.ps = (int)std::min<int64_t>({64, std::max<int64_t>(1, 2 * (int64_t)num_cu / wgs), units});
+        if (a.ps > 1) slots = (size_t)a.ps * wgs * PRO_ROWS;
+    }
     if (a.ps == 0 || a.p.n_seq > 1) {
         const int64_t want = std::max<int64_t>(1, 8 * (int64_t)num_cu / heads);
         a.ds = (int)std::min<int64_t>({64, want, (a.p.max_len + DEC_STEP * DEC_LEAST - 1) / (DEC_STEP * DEC_LEAST)});
+        if (a.ds > 1) slots = std::max(slots, (size_t)a.ds * heads * a.drows);
     }
-    return a.ds > 1 ? (size_t)a.ds * heads * a.drows : 0;
+    return slots;
 }
 
+// the decode kernel's sums are joined before the prompt kernel's take their place
 hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
     hipError_t e = hipSuccess;
     if (a.ds > 0 && (e = launch_paged_decode(a, s)) != hipSuccess) return e;
     if (a.ds > 1) {
-        paged_join_kernel<<<dim3((unsigned)a.p.n_seq * (unsigned)a.p.n_head_kv, (unsigned)(a.drows + 3) / 4), 256, 0, s>>>(a);
+        paged_join_decode_kernel<<<dim3((unsigned)a.p.n_seq * (unsigned)a.p.n_head_kv, (unsigned)(a.drows + 3) / 4), 256, 0, s>>>(a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (a.ps > 0) {
-        paged_attn_kernel<<<dim3((unsigned)a.p.n_tok, (unsigned)a.n_head), 64, 0, s>>>(a);
+    if (a.ps > 0 && (e = launch_paged_prompt(a, s)) != hipSuccess) return e;
+    if (a.ps > 1) {
+        paged_join_prompt_kernel<<<dim3((unsigned)(paged_tiles(a) * a.p.n_head_kv), PRO_ROWS / 8), 256, 0, s>>>(a);
         e = hipGetLastError();
     }
     return e;

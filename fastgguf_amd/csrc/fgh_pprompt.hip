@@ -1,0 +1,359 @@
+// fgh_pprompt.hip - paged attention of many rows per K / V head: prompts.
+//
+// A workgroup takes 128 rows of a sequence and K / V head (row = new token x the head's query heads + query head, so the
+// heads that share K and V share its tiles), 32 a wavefront, and goes over their positions in tiles of KT. K and V^T
+// tiles come into LDS by direct loads (16 bytes a lane), two tiles deep: the next one is on its way while this one is used.
+//   S^T = K q^T: 32 x 32 x 16 products, A = 32 K rows out of LDS, B = q in registers. LDS row m of a 16-position block holds position
+//         (m & 3) | (m & 8) >> 1 | (m & 4) << 1, so that a lane's 16 scores of 32 positions are two runs of 8 positions,
+//   O^T += V^T P^T: which are what it has to give as B. Neither scores nor weights leave their lane; a row's maximum takes
+//         one exchange with the lane 32 away, and only where the row's reference has to follow it.
+// 16-byte words are kept in LDS at (word ^ row) (word + row / 4 or / 8 mod words where their number is no power of 2), so that
+// lanes that read the same word of neighbouring rows meet in no bank.
+#include <hip/hip_runtime.h>
+
+#include "fgh_pattn.h"
+
+namespace fgh {
+
+namespace {
+
+template <int TYPE, int HD>
+struct Pro {
+    static constexpr int ES = PagedType<TYPE>::ES, NQ = PagedType<TYPE>::NQ, NK = PagedType<TYPE>::NK;
+    static constexpr int W = ES / 2;           // 16-byte words of 8 values
+    static constexpr int KT = HD * ES > 256 ? 32 : 64;
+    static constexpr int KS = HD / 16;         // steps of 16 along the head
+    static constexpr int VB = (HD + 31) / 32;  // blocks of 32 of V's values
+    static constexpr int KW = HD * ES / 16;    // words of a K row
+    static constexpr int VW = KT * ES / 16;    // words of a V^T row
+    static constexpr int KBYTES = KT * HD * ES;
+    static constexpr int VROWS = VB * 32;      // with the rows behind hd 80, never loaded, their sums never stored
+    static constexpr int VBYTES = VROWS * KT * ES;
+    static constexpr int BYTES = KBYTES + VBYTES;
+    static constexpr int OCC = HD > 128 || (TYPE == T_F32 && HD > 64) ? 1 : 2;
+    static constexpr int KL = KBYTES / 4 / 1024 + (KBYTES / 4 % 1024 != 0);  // direct loads of a wavefront: its KT / 4 K rows
+    static constexpr int VL = HD * KT * ES / 4 / 1024 + (HD * KT * ES / 4 % 1024 != 0);  // and its HD / 4 V rows
+};
+
+// where word w of row r is kept, in words from the row's start
+template <int NW>
+__device__ __forceinline__ int word_at(int r, int w) {
+    if constexpr (NW == 4) return w ^ (r >> 1 & 3);
+    else if constexpr ((NW & (NW - 1)) == 0) return w ^ (r & (NW < 16 ? NW - 1 : 15));
+    else return (w + r / (NW % 16 == 10 ? 8 : NW % 16 == 12 || NW % 16 == 4 ? 4 : 2)) % NW;
+}
+// the word that is kept there
+template <int NW>
+__device__ __forceinline__ int word_of(int r, int at) {
+    if constexpr ((NW & (NW - 1)) == 0) return word_at<NW>(r, at);
+    else return (at + 4 * NW - r / (NW % 16 == 10 ? 8 : NW % 16 == 12 || NW % 16 == 4 ? 4 : 2)) % NW;
+}
+// LDS row of a 16-position block <-> position
+__device__ __forceinline__ int swap_rows(int m) { return (m & ~12) | (m & 8) >> 1 | (m & 4) << 1; }
+
+__device__ __forceinline__ void lds_load16(const uint8_t *src, uint8_t *dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
+template <int TYPE, int HD>
+__global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel(PagedAttnArgs a) {
+    using P = Pro<TYPE, HD>;
+    constexpr int KT = P::KT, ES = P::ES, W = P::W;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ uint32_t odd_l[2];  // positions of the tile with a V value that is not finite and that only some rows see
+    const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
+    const int kvh = blockIdx.x % nkv, split = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // tiles in reverse: those late in a sequence have the most positions and start first
+    const PagedTile tl = paged_tile(a, (int)(gridDim.x / nkv) - 1 - (int)(blockIdx.x / nkv));
+    if (tl.s < 0) return;
+    const PagedSeq q = tl.q;
+    const int s = tl.s, r0 = tl.r0, R = min(PRO_ROWS, q.n * G - r0);
+    if (!q.ok) {
+        if (split == 0)
+            for (int64_t i = tid; i < (int64_t)R * HD; i += 256) {
+                const int r = r0 + (int)(i / HD), x = (int)(i % HD);
+                a.o[(q.t0 + r / G) * a.ldo + (int64_t)(kvh * G + r % G) * HD + x] = __builtin_nanf("");
+            }
+        return;
+    }
+    const int prefix = paged_prefix(a, s, q);
+    const PagedSpan sp = paged_span(a, q, prefix, r0 / G, (r0 + R - 1) / G);
+    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, PRO_LEAST);
+    if (split >= ch.used) return;
+    const int ubase = sp.lo & ~(PRO_UNIT - 1);  // the split's positions k0 .. k1, whole units but for the range's ends
+    const int k0 = max(sp.lo & ~(KT - 1), ubase + split * ch.per * PRO_UNIT), k1 = min(sp.hi, ubase + (split + 1) * ch.per * PRO_UNIT - 1);
+
+    // this lane's row: column lane % 32 of the wavefront's products
+    const int half = lane >> 5, wr = wave * 32 + (lane & 31);
+    const bool mine = wr < R;
+    const int row = r0 + (mine ? wr : 0), tok = row / G, head = kvh * G + row - tok * G;
+    const int pos = q.len - q.n + tok;
+    const int lo = mine ? row_lo(a, pos) : 0x7fffffff, hi = mine ? max(pos, prefix - 1) : -1;
+
+    const int mask = (1 << a.p.shift) - 1;
+    const int32_t *table = a.p.table + (int64_t)s * a.p.table_stride;
+    // the pages of a tile: one entry for 16 positions, past the range its last
+    constexpr int NE = KT / 16;
+    int ent[NE];
+    auto pages = [&](int kb) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) ent[e] = table[min(kb + 16 * e, sp.hi) >> a.p.shift];
+    };
+    const int64_t hsize = (int64_t)kvh * HD << a.p.shift;
+    auto load = [&](int kb, uint8_t *buf) {
+        int64_t hb[NE];  // the entries' K / V head blocks
+#pragma unroll
+        for (int e = 0; e < NE; ++e) hb[e] = (paged_ok(a.p, ent[e]) ? ent[e] : 0) * a.p.page_stride + hsize;
+        // K: this wavefront's KT / 4 LDS rows, positions of one 16-block
+        const int kr0 = wave * (KT / 4), kblk = kr0 & ~15;
+        int64_t hk = hb[0];
+#pragma unroll
+        for (int e = 1; e < NE; ++e) hk = kblk == 16 * e ? hb[e] : hk;
+        const uint8_t *kp = a.p.k + (hk + (int64_t)((kb + kblk) & mask) * HD) * ES;
+#pragma unroll
+        for (int i = 0; i < P::KL; ++i) {
+            const int x = i * 64 + lane;  // of the wavefront's words
+            if (KT / 4 * P::KW % 64 == 0 || x < KT / 4 * P::KW) {
+                const int r = kr0 + x / P::KW, w = word_of<P::KW>(r, x % P::KW);
+                lds_load16(kp + (int64_t)swap_rows(r & 15) * HD * ES + w * 16, buf + kr0 * HD * ES + i * 1024);
+            }
+        }
+        // V^T: this wavefront's HD / 4 rows
+        const int vr0 = wave * (HD / 4);
+#pragma unroll
+        for (int i = 0; i < P::VL; ++i) {
+            const int x = i * 64 + lane;
+            if (HD / 4 * P::VW % 64 == 0 || x < HD / 4 * P::VW) {
+                const int r = vr0 + x / P::VW, w = word_of<P::VW>(r, x % P::VW), j = w * (16 / ES);
+                int64_t hv = hb[0];
+#pragma unroll
+                for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
+                lds_load16(a.p.v + (hv + ((int64_t)r << a.p.shift) + ((kb + j) & mask)) * ES, buf + P::KBYTES + vr0 * KT * ES + i * 1024);
+            }
+        }
+    };
+    // of the loaded tile: 16-position blocks whose page does not exist
+    auto missing = [&]() {
+        uint32_t b = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) b |= paged_ok(a.p, ent[e]) ? 0u : 1u << e;
+        return b;
+    };
+
+    int kb = k0;
+    pages(kb);
+    load(kb, lds);
+    uint32_t gone = missing(), gone_next = 0;
+    if (kb + KT <= k1) pages(kb + KT);
+
+    pu4 qp[P::KS][P::NQ];
+    PagedScore score;
+    {
+        float amax = 0.0f;
+        const float *src = a.q + (q.t0 + tok) * a.ldq + (int64_t)head * HD + half * 8;
+        float x[P::KS][8];
+#pragma unroll
+        for (int ks = 0; ks < P::KS; ++ks) {
+            const pf4 u = *(const pf4 *)(src + ks * 16), v = *(const pf4 *)(src + ks * 16 + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[ks][e] = mine ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.0f;
+                amax = fmaxf(amax, fabsf(x[ks][e]));
+            }
+        }
+        float size = 1.0f;
+        if constexpr (TYPE == T_F16) size = row_size(fmaxf(amax, __shfl_xor(amax, 32, 64)));
+        const float inv = (a.scale < 0.0f ? -1.0f : 1.0f) / size;
+#pragma unroll
+        for (int ks = 0; ks < P::KS; ++ks) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[ks][e] *= inv;
+            parts8<TYPE, P::NQ>(x[ks], qp[ks]);
+        }
+        score = paged_score(a, head, size);
+    }
+
+    pf16 acc[P::VB];
+#pragma unroll
+    for (int b = 0; b < P::VB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
+    float c = __FLT_MAX__, l = 0.0f;
+
+    for (int n = 0; kb <= k1; kb += KT, n ^= 1) {
+        uint8_t *buf = lds + n * P::BYTES;
+        __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt 0: this wavefront's part of the tile is in LDS
+        __syncthreads();                    // everyone's is, and the other buffer has been read
+        if (kb + KT <= k1) {
+            load(kb + KT, lds + (n ^ 1) * P::BYTES);
+            gone_next = missing();
+            if (kb + 2 * KT <= k1) pages(kb + 2 * KT);
+        }
+        // positions of the tile that count here: first .. last; whole: all of them, for every row
+        const int first = max(sp.lo, k0), last = min(sp.hi, k1);
+        const bool whole = kb >= max(sp.in_lo, k0) && kb + KT - 1 <= min(sp.in_hi, k1) && gone == 0;
+        uint64_t odd = 0;
+        if (!whole) {
+            // V values at positions that no row sees become zeros, and so do those that are not finite (see below)
+            if (tid < 2) odd_l[tid] = 0;
+            __syncthreads();
+            for (int x = tid; x < HD * P::VW; x += 256) {
+                const int r = x / P::VW, at = x % P::VW, j = word_of<P::VW>(r, at) * (16 / ES);
+                pu4 *word = (pu4 *)(buf + P::KBYTES + (r * P::VW + at) * 16);
+                pu4 v[W];
+                v[0] = *word;
+                uint32_t bad = 0;
+#pragma unroll
+                for (int e = 0; e < 16 / ES; ++e) {
+                    const bool none = (gone >> ((j + e) / 16) & 1) || kb + j + e < first || kb + j + e > last;
+                    const bool inf = raw_bad<TYPE>(v, e);
+                    if (none || inf) raw_zero<TYPE>(v, e);
+                    if (inf && !none) bad |= 1u << e;
+                }
+                *word = v[0];
+                if (bad) atomicOr(&odd_l[j / 32], bad << (j & 31));
+            }
+            __syncthreads();
+            odd = odd_l[0] | (uint64_t)odd_l[1] << 32;
+        }
+#pragma unroll
+        for (int h = 0; h < KT / 32; ++h) {
+            pf16 sc;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+            const int kr = h * 32 + (lane & 31);
+#pragma unroll
+            for (int ks = 0; ks < P::KS; ++ks) {
+                pu4 raw[W], kp[P::NK];
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    raw[w] = *(const pu4 *)(buf + kr * HD * ES + word_at<P::KW>(kr, (2 * ks + half) * W + w) * 16);
+                cache8<TYPE>(raw, kp);
+#pragma unroll
+                for (int x = P::NQ - 1; x >= 0; --x)
+#pragma unroll
+                    for (int y = P::NK - 1; y >= 0; --y)
+                        if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const int j0 = kb + h * 32 + kk * 16 + half * 8;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = sc[8 * kk + e];
+                const float mul = score.apply(v, j0, pos);
+                if (!whole) {
+                    const bool no = gone >> (2 * h + kk) & 1;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (no) v[e] = __builtin_nanf("");
+                        if (j0 + e < max(lo, first) || j0 + e > min(hi, last)) v[e] = -__builtin_inff();
+                    }
+                }
+                float top = v[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) top = fmaxf(top, v[e]);
+                top *= mul;
+                if (__builtin_amdgcn_ballot_w64(top + c > PTOP)) {
+                    const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
+                    if (mx + c > PTOP) {
+                        const float cn = PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
+                        c = cn;
+                        l *= f;
+#pragma unroll
+                        for (int b = 0; b < P::VB; ++b) acc[b] *= f;
+                    }
+                }
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], mul, c));
+                    l += p[e];
+                }
+                pu4 pp[P::NQ];
+                parts8<TYPE, P::NQ>(p, pp);
+#pragma unroll
+                for (int b = 0; b < P::VB; ++b) {
+                    const int vr = b * 32 + (lane & 31);
+                    pu4 raw[W], vp[P::NK];
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        raw[w] = *(const pu4 *)(buf + P::KBYTES + vr * KT * ES + word_at<P::VW>(vr, ((2 * h + kk) * 2 + half) * W + w) * 16);
+                    cache8<TYPE>(raw, vp);
+#pragma unroll
+                    for (int x = P::NQ - 1; x >= 0; --x)
+#pragma unroll
+                        for (int y = P::NK - 1; y >= 0; --y)
+                            if (x + y < 3) mma32<TYPE>(acc[b], vp[y], pp[x]);
+                }
+            }
+        }
+        while (odd) {  // values that are not finite, left out above: added to the rows that see them
+            const int j = kb + __builtin_ctzll(odd);
+            odd &= odd - 1;
+            const int64_t at = paged_head(a.p, table[j >> a.p.shift], kvh) + (j & mask);
+            if (j >= lo && j <= hi)
+#pragma unroll
+                for (int b = 0; b < P::VB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int d = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                        if (HD % 32 == 0 || d < HD) {
+                            const float z = cached<TYPE>(a.p.v, at + ((int64_t)d << a.p.shift));
+                            if (not_finite(z)) acc[b][r] += z;
+                        }
+                    }
+        }
+        gone = gone_next;
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!mine) return;
+    const int64_t slot = (((int64_t)split * (gridDim.x / nkv) + tl.index) * nkv + kvh) * PRO_ROWS + wr;
+    float *out = ch.used == 1 ? a.o + (q.t0 + tok) * a.ldo + (int64_t)head * HD : a.part + slot * HD;
+#pragma unroll
+    for (int b = 0; b < P::VB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * b + 8 * i + 4 * half;
+            if (HD % 32 == 0 || d < HD) {
+                pf4 o = {acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+                *(pf4 *)(out + d) = ch.used == 1 ? o / l : o;
+            }
+        }
+    if (ch.used > 1 && half == 0) {
+        a.stat[2 * slot] = c;
+        a.stat[2 * slot + 1] = l;
+    }
+}
+
+template <int TYPE, int HD>
+hipError_t launch_one(const PagedAttnArgs &a, hipStream_t s) {
+    constexpr int bytes = 2 * Pro<TYPE, HD>::BYTES;
+    paged_prompt_kernel<TYPE, HD><<<dim3((unsigned)(paged_tiles(a) * a.p.n_head_kv), (unsigned)a.ps), 256, bytes, s>>>(a);
+    return hipGetLastError();
+}
+template <int TYPE>
+hipError_t launch_type(const PagedAttnArgs &a, hipStream_t s) {
+    switch (a.p.hd) {
+    case 64: return launch_one<TYPE, 64>(a, s);
+    case 80: return launch_one<TYPE, 80>(a, s);
+    case 96: return launch_one<TYPE, 96>(a, s);
+    case 128: return launch_one<TYPE, 128>(a, s);
+    case 256: return launch_one<TYPE, 256>(a, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_paged_prompt(const PagedAttnArgs &a, hipStream_t s) {
+    switch (a.p.type) {
+    case T_F32: return launch_type<T_F32>(a, s);
+    case T_F16: return launch_type<T_F16>(a, s);
+    case T_BF16: return launch_type<T_BF16>(a, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace fgh
