@@ -37,6 +37,15 @@ __device__ __forceinline__ PagedSeq paged_seq(const Paged &a, int s) {
     q.ok = b >= 0 && e <= a.n_tok && q.n <= a.max_tok && len >= q.n && len <= a.max_len;
     return q;
 }
+// the same of a uniform s, in scalar registers (the loads' results would stay in vector registers)
+__device__ __forceinline__ PagedSeq paged_useq(const Paged &a, int s) {
+    PagedSeq q = paged_seq(a, s);
+    q.t0 = __builtin_amdgcn_readfirstlane(q.t0);
+    q.n = __builtin_amdgcn_readfirstlane(q.n);
+    q.len = __builtin_amdgcn_readfirstlane(q.len);
+    q.ok = __builtin_amdgcn_readfirstlane(q.ok);
+    return q;
+}
 // the sequence of row t, or -1: the last s with tok[s] <= t, if t < tok[s + 1]. Every wavefront finds
 // it for itself, 64 starts a load.
 __device__ __forceinline__ int paged_find(const Paged &a, int t) {

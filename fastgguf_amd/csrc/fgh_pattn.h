@@ -165,7 +165,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs &a, const Pa
     return PagedSpan{row_lo(a, p0), max(p1, prefix - 1), row_lo(a, p1), max(p0, prefix - 1)};
 }
 __device__ __forceinline__ int paged_prefix(const PagedAttnArgs &a, int s, const PagedSeq &q) {
-    return a.prefix ? min(a.prefix[s], q.len) : 0;
+    return a.prefix ? min(__builtin_amdgcn_readfirstlane(a.prefix[s]), q.len) : 0;  // s: uniform
 }
 // a range of n units over at most `splits` workgroups, `least` units or more each: the units of one, and how many
 // workgroups have any
@@ -219,7 +219,7 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int inde
             t.r0 = (int)(index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
             t.s = __builtin_amdgcn_readfirstlane(t.s);
             t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
-            t.q = paged_seq(a.p, t.s);
+            t.q = paged_useq(a.p, t.s);
             return t;
         }
         before += __shfl(upto, 63, 64);

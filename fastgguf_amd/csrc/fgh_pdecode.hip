@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
     const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
     const int kvh = blockIdx.x % nkv, split = blockIdx.x / nkv % a.ds, s = blockIdx.x / nkv / a.ds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const PagedSeq q = paged_seq(a.p, s);
+    const PagedSeq q = paged_useq(a.p, s);
     if (q.n == 0 || (a.ps > 0 && (int64_t)q.n * G > DEC_ROWS)) return;  // the prompt kernel's
     const int64_t rows = (int64_t)q.n * G;
     if (!q.ok) {
@@ -236,13 +236,16 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
                 if (j < sp.lo || j > sp.hi) continue;
                 const int page = entry(j);
                 if (!paged_ok(a.p, page)) continue;
-                const int64_t at = paged_head(a.p, page, kvh) + (j & mask);
+                int shift = a.p.shift;
+                asm volatile("" : "+s"(shift));  // this rare path must not cost registers: no addresses formed ahead,
+                const int64_t at = paged_head(a.p, page, kvh) + (j & mask) + ((int64_t)(quad * 4) << shift);
 #pragma unroll
                 for (int b = 0; b < D::VB; ++b)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float z = cached<TYPE>(a.p.v, at + ((int64_t)(16 * b + quad * 4 + r) << a.p.shift));
+                        const float z = cached<TYPE>(a.p.v, at + ((int64_t)(16 * b + r) << shift));
                         if (not_finite(z) && j >= lo && j <= hi) acc[b][r] += z;
+                        asm volatile("" : "+s"(shift)::"memory");  // and one value at a time
                     }
             }
         }

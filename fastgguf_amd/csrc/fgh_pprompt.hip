@@ -7,8 +7,8 @@
 //         (m & 3) | (m & 8) >> 1 | (m & 4) << 1, so that a lane's 16 scores of 32 positions are two runs of 8 positions,
 //   O^T += V^T P^T: which are what it has to give as B. Neither scores nor weights leave their lane; a row's maximum takes
 //         one exchange with the lane 32 away, and only where the row's reference has to follow it.
-// 16-byte words are kept in LDS at (word ^ row) (word + row / 4 or / 8 mod words where their number is no power of 2), so that
-// lanes that read the same word of neighbouring rows meet in no bank.
+// 16-byte words of a row are kept in LDS at (word ^ row), so that lanes that read the same word of neighbouring rows
+// meet in no bank.
 #include <hip/hip_runtime.h>
 
 #include "fgh_pattn.h"
@@ -24,29 +24,22 @@ struct Pro {
     static constexpr int KT = HD * ES > 256 ? 32 : 64;
     static constexpr int KS = HD / 16;         // steps of 16 along the head
     static constexpr int VB = (HD + 31) / 32;  // blocks of 32 of V's values
-    static constexpr int KW = HD * ES / 16;    // words of a K row
+    static constexpr int KD = HD * ES / 16;    // words of a K row
+    static constexpr int KW = KD <= 8 ? 8 : KD <= 16 ? 16 : KD <= 32 ? 32 : 64;  // and their places in LDS
     static constexpr int VW = KT * ES / 16;    // words of a V^T row
-    static constexpr int KBYTES = KT * HD * ES;
+    static constexpr int KBYTES = KT * KW * 16;
     static constexpr int VROWS = VB * 32;      // with the rows behind hd 80, never loaded, their sums never stored
     static constexpr int VBYTES = VROWS * KT * ES;
     static constexpr int BYTES = KBYTES + VBYTES;
     static constexpr int OCC = HD > 128 || (TYPE == T_F32 && HD > 64) ? 1 : 2;
-    static constexpr int KL = KBYTES / 4 / 1024 + (KBYTES / 4 % 1024 != 0);  // direct loads of a wavefront: its KT / 4 K rows
-    static constexpr int VL = HD * KT * ES / 4 / 1024 + (HD * KT * ES / 4 % 1024 != 0);  // and its HD / 4 V rows
+    static constexpr int KL = KT / 4 * KW / 64;           // direct loads of a wavefront for its KT / 4 K rows
+    static constexpr int VL = HD * VW / 64;               // and of all four for V
 };
 
-// where word w of row r is kept, in words from the row's start
+// what a row's words are kept at: word w of row r at w ^ turn(r)
 template <int NW>
-__device__ __forceinline__ int word_at(int r, int w) {
-    if constexpr (NW == 4) return w ^ (r >> 1 & 3);
-    else if constexpr ((NW & (NW - 1)) == 0) return w ^ (r & (NW < 16 ? NW - 1 : 15));
-    else return (w + r / (NW % 16 == 10 ? 8 : NW % 16 == 12 || NW % 16 == 4 ? 4 : 2)) % NW;
-}
-// the word that is kept there
-template <int NW>
-__device__ __forceinline__ int word_of(int r, int at) {
-    if constexpr ((NW & (NW - 1)) == 0) return word_at<NW>(r, at);
-    else return (at + 4 * NW - r / (NW % 16 == 10 ? 8 : NW % 16 == 12 || NW % 16 == 4 ? 4 : 2)) % NW;
+__device__ __forceinline__ int turn(int r) {
+    return NW == 4 ? r >> 1 & 3 : r & (NW < 16 ? NW - 1 : 15);
 }
 // LDS row of a 16-position block <-> position
 __device__ __forceinline__ int swap_rows(int m) { return (m & ~12) | (m & 8) >> 1 | (m & 4) << 1; }
@@ -93,18 +86,22 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
 
     const int mask = (1 << a.p.shift) - 1;
     const int32_t *table = a.p.table + (int64_t)s * a.p.table_stride;
-    // the pages of a tile: one entry for 16 positions, past the range its last
+    // a tile's pages, one entry for 16 positions (past the range its last): lane e asks for entry e, one tile ahead
     constexpr int NE = KT / 16;
-    int ent[NE];
-    auto pages = [&](int kb) {
-#pragma unroll
-        for (int e = 0; e < NE; ++e) ent[e] = table[min(kb + 16 * e, sp.hi) >> a.p.shift];
-    };
+    int ent = 0;
+    auto pages = [&](int kb) { ent = table[min(kb + 16 * min(lane, NE - 1), sp.hi) >> a.p.shift]; };
     const int64_t hsize = (int64_t)kvh * HD << a.p.shift;
+    uint32_t gone_next = 0;
     auto load = [&](int kb, uint8_t *buf) {
         int64_t hb[NE];  // the entries' K / V head blocks
+        gone_next = 0;   // 16-position blocks whose page does not exist
 #pragma unroll
-        for (int e = 0; e < NE; ++e) hb[e] = (paged_ok(a.p, ent[e]) ? ent[e] : 0) * a.p.page_stride + hsize;
+        for (int e = 0; e < NE; ++e) {
+            const int page = __builtin_amdgcn_readlane(ent, e);
+            const bool ok = paged_ok(a.p, page);
+            hb[e] = (ok ? page : 0) * a.p.page_stride + hsize;
+            gone_next |= ok ? 0u : 1u << e;
+        }
         // K: this wavefront's KT / 4 LDS rows, positions of one 16-block
         const int kr0 = wave * (KT / 4), kblk = kr0 & ~15;
         int64_t hk = hb[0];
@@ -113,38 +110,26 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
         const uint8_t *kp = a.p.k + (hk + (int64_t)((kb + kblk) & mask) * HD) * ES;
 #pragma unroll
         for (int i = 0; i < P::KL; ++i) {
-            const int x = i * 64 + lane;  // of the wavefront's words
-            if (KT / 4 * P::KW % 64 == 0 || x < KT / 4 * P::KW) {
-                const int r = kr0 + x / P::KW, w = word_of<P::KW>(r, x % P::KW);
-                lds_load16(kp + (int64_t)swap_rows(r & 15) * HD * ES + w * 16, buf + kr0 * HD * ES + i * 1024);
-            }
+            const int r = kr0 + i * (64 / P::KW) + lane / P::KW, w = lane % P::KW ^ turn<P::KW>(r);
+            if (P::KD == P::KW || w < P::KD)
+                lds_load16(kp + (uint32_t)(swap_rows(r & 15) * HD * ES + w * 16), buf + kr0 * P::KW * 16 + i * 1024);
         }
-        // V^T: this wavefront's HD / 4 rows
-        const int vr0 = wave * (HD / 4);
+        // V^T: loads wave, wave + 4, ..
+        constexpr int VR = 64 / P::VW;  // rows a load
+        const int vr = wave * VR + lane / P::VW, j = (lane % P::VW ^ turn<P::VW>(vr)) * (16 / ES);
+        int64_t hv = hb[0];
 #pragma unroll
-        for (int i = 0; i < P::VL; ++i) {
-            const int x = i * 64 + lane;
-            if (HD / 4 * P::VW % 64 == 0 || x < HD / 4 * P::VW) {
-                const int r = vr0 + x / P::VW, w = word_of<P::VW>(r, x % P::VW), j = w * (16 / ES);
-                int64_t hv = hb[0];
+        for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
+        const uint8_t *vp = a.p.v + (hv + ((int64_t)vr << a.p.shift) + ((kb + j) & mask)) * ES;
 #pragma unroll
-                for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
-                lds_load16(a.p.v + (hv + ((int64_t)r << a.p.shift) + ((kb + j) & mask)) * ES, buf + P::KBYTES + vr0 * KT * ES + i * 1024);
-            }
-        }
+        for (int i = 0; i < (P::VL + 3) / 4; ++i)  // 4 VR rows on: the same turn
+            if (P::VL % 4 == 0 || wave + 4 * i < P::VL)
+                lds_load16(vp + (((uint32_t)(4 * VR * i) << a.p.shift) * ES), buf + P::KBYTES + (wave + 4 * i) * 1024);
     };
-    // of the loaded tile: 16-position blocks whose page does not exist
-    auto missing = [&]() {
-        uint32_t b = 0;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) b |= paged_ok(a.p, ent[e]) ? 0u : 1u << e;
-        return b;
-    };
-
     int kb = k0;
     pages(kb);
     load(kb, lds);
-    uint32_t gone = missing(), gone_next = 0;
+    uint32_t gone = gone_next;
     if (kb + KT <= k1) pages(kb + KT);
 
     pu4 qp[P::KS][P::NQ];
@@ -181,13 +166,15 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
         for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
     float c = __FLT_MAX__, l = 0.0f;
 
+    // where this lane's words are: the K row it gives, and the V^T row; word w of either at (place ^ 16 w)
+    const uint32_t k_at = (lane & 31) * P::KW * 16 + ((half * W) ^ turn<P::KW>(lane & 31)) * 16;
+    const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31)) * 16;
     for (int n = 0; kb <= k1; kb += KT, n ^= 1) {
         uint8_t *buf = lds + n * P::BYTES;
         __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt 0: this wavefront's part of the tile is in LDS
         __syncthreads();                    // everyone's is, and the other buffer has been read
         if (kb + KT <= k1) {
             load(kb + KT, lds + (n ^ 1) * P::BYTES);
-            gone_next = missing();
             if (kb + 2 * KT <= k1) pages(kb + 2 * KT);
         }
         // positions of the tile that count here: first .. last; whole: all of them, for every row
@@ -199,7 +186,7 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
             if (tid < 2) odd_l[tid] = 0;
             __syncthreads();
             for (int x = tid; x < HD * P::VW; x += 256) {
-                const int r = x / P::VW, at = x % P::VW, j = word_of<P::VW>(r, at) * (16 / ES);
+                const int r = x / P::VW, at = x % P::VW, j = (at ^ turn<P::VW>(r)) * (16 / ES);
                 pu4 *word = (pu4 *)(buf + P::KBYTES + (r * P::VW + at) * 16);
                 pu4 v[W];
                 v[0] = *word;
@@ -222,13 +209,12 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
             pf16 sc;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-            const int kr = h * 32 + (lane & 31);
 #pragma unroll
             for (int ks = 0; ks < P::KS; ++ks) {
                 pu4 raw[W], kp[P::NK];
 #pragma unroll
                 for (int w = 0; w < W; ++w)
-                    raw[w] = *(const pu4 *)(buf + kr * HD * ES + word_at<P::KW>(kr, (2 * ks + half) * W + w) * 16);
+                    raw[w] = *(const pu4 *)(buf + (k_at ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
                 cache8<TYPE>(raw, kp);
 #pragma unroll
                 for (int x = P::NQ - 1; x >= 0; --x)
@@ -275,11 +261,10 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
                 parts8<TYPE, P::NQ>(p, pp);
 #pragma unroll
                 for (int b = 0; b < P::VB; ++b) {
-                    const int vr = b * 32 + (lane & 31);
                     pu4 raw[W], vp[P::NK];
 #pragma unroll
                     for (int w = 0; w < W; ++w)
-                        raw[w] = *(const pu4 *)(buf + P::KBYTES + vr * KT * ES + word_at<P::VW>(vr, ((2 * h + kk) * 2 + half) * W + w) * 16);
+                        raw[w] = *(const pu4 *)(buf + (v_at ^ ((2 * h + kk) * 2 * W + w) * 16) + b * 32 * P::VW * 16);
                     cache8<TYPE>(raw, vp);
 #pragma unroll
                     for (int x = P::NQ - 1; x >= 0; --x)
@@ -292,7 +277,9 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
         while (odd) {  // values that are not finite, left out above: added to the rows that see them
             const int j = kb + __builtin_ctzll(odd);
             odd &= odd - 1;
-            const int64_t at = paged_head(a.p, table[j >> a.p.shift], kvh) + (j & mask);
+            int shift = a.p.shift;
+            asm volatile("" : "+s"(shift));  // this rare path must not cost registers: no addresses formed ahead,
+            const int64_t at = paged_head(a.p, table[j >> shift], kvh) + (j & mask) + ((int64_t)(4 * half) << shift);
             if (j >= lo && j <= hi)
 #pragma unroll
                 for (int b = 0; b < P::VB; ++b)
@@ -300,8 +287,9 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
                     for (int r = 0; r < 16; ++r) {
                         const int d = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
                         if (HD % 32 == 0 || d < HD) {
-                            const float z = cached<TYPE>(a.p.v, at + ((int64_t)d << a.p.shift));
+                            const float z = cached<TYPE>(a.p.v, at + ((int64_t)(d - 4 * half) << shift));
                             if (not_finite(z)) acc[b][r] += z;
+                            asm volatile("" : "+s"(shift)::"memory");  // and one value at a time
                         }
                     }
         }
