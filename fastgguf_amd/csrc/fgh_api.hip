@@ -1080,11 +1080,12 @@ int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_
     a.p = paged_args(cache, batch);
     a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo, a.n_head = n_head, a.window = mask->window, a.scale = mask->scale;
     a.softcap = mask->softcap, a.slopes = mask->slopes, a.prefix = mask->prefix;
-    const size_t slots = fgh::paged_attention_plan(a, c->num_cu);
-    if (slots) {
-        if (int rc = grow(c, c->pa, slots * (a.p.hd + 2) * 4)) return rc;
-        a.part = (float *)c->pa.p;
-        a.stat = a.part + slots * a.p.hd;
+    const fgh::PagedScratch need = fgh::paged_attention_plan(a, c->num_cu);
+    if (need.part) {
+        if (int rc = grow(c, c->pa, need.info * sizeof(fgh::PagedSlot) + (need.part + need.stat) * 4)) return rc;
+        a.info = (fgh::PagedSlot *)c->pa.p;
+        a.part = (float *)(a.info + need.info);
+        a.stat = a.part + need.part;
     }
     HIP_TRY(c, fgh::launch_paged_attention(a, c->stream));
     return FGH_OK;

@@ -76,6 +76,10 @@ struct PagedStoreArgs {
 };
 hipError_t launch_paged_store(const PagedStoreArgs &a, hipStream_t s);
 
+// a slot: how many splits of its range were used (0, 1: nothing to join), its rows and where they are in the batch
+struct PagedSlot {
+    int32_t used, rows, t0, r0;
+};
 struct PagedAttnArgs {
     Paged p;
     const float *q, *slopes;
@@ -85,14 +89,18 @@ struct PagedAttnArgs {
     int n_head, window;
     float scale, softcap;
     // Sequences of few rows per K / V head (new tokens x query heads of the head) go to the decode kernel, the others
-    // to the prompt kernel; each kernel's ranges of positions are split over up to ds / ps workgroups, 0: not
-    // launched. Split ranges leave their sums in part [split][slot][hd] and stat [split][slot][2]. Decode slots: (sequence,
-    // K / V head, one of drows rows).
-    int ds, ps, drows;
+    // to the prompt kernel; each kernel's ranges of positions are split over up to ds / ps workgroups (0: not
+    // launched) of at least dleast steps / pleast units each. Split ranges leave their sums in part and stat, by slot (a workgroup's
+    // rows) and split, and what the join has to know of a slot in info.
+    int ds, ps, drows, dleast, pleast;
     float *part, *stat;
+    PagedSlot *info;
 };
-// the plan (ds, ps, drows) for a device of num_cu compute units; returns the slots x splits of part, then stat
-size_t paged_attention_plan(PagedAttnArgs &a, int num_cu);
+struct PagedScratch {
+    size_t part, stat, info;  // floats, floats, slots
+};
+// the plan for a device of num_cu compute units, and the scratch it needs
+PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu);
 hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
 
 }  // namespace fgh

@@ -83,6 +83,21 @@ __device__ __forceinline__ bool raw_bad(const pu4 *raw, int e) {
     const uint32_t h = raw[0][e / 2] >> (16 * (e & 1));
     return TYPE == T_F16 ? (h & 0x7c00u) == 0x7c00u : (h & 0x7f80u) == 0x7f80u;
 }
+// a word of cached values: not 0 where one is not finite
+template <int TYPE>
+__device__ __forceinline__ uint32_t infinite(uint32_t w) {
+    if constexpr (TYPE == T_F32) return ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+    else if constexpr (TYPE == T_F16) return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    else return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+// the word with zeros in the place of what is not finite
+template <int TYPE>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+    const uint32_t f = infinite<TYPE>(w);
+    if constexpr (TYPE == T_F32) return f ? 0u : w;
+    const uint32_t ones = f >> 15;  // 1 in each half that is not finite
+    return w & ~((ones << 16) - ones);
+}
 template <int TYPE>
 __device__ __forceinline__ void raw_zero(pu4 *raw, int e) {
     if constexpr (TYPE == T_F32) raw[e / 4][e % 4] = 0;
@@ -126,7 +141,10 @@ struct PagedScore {
     __device__ __forceinline__ float apply(float (&v)[NE], int j0, int p) const {
         if (cap_out > 0.0f) {
 #pragma unroll
-            for (int e = 0; e < NE; ++e) v[e] = cap_out * tanh_near(v[e] * cap_in);
+            for (int e = 0; e < NE; ++e) {
+                v[e] = cap_out * tanh_near(v[e] * cap_in);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once would cost registers
+            }
             if (!bias) return 1.0f;
         } else if (bias) {
 #pragma unroll
@@ -178,12 +196,12 @@ __device__ __forceinline__ PagedChunk paged_chunk(int n, int splits, int least) 
 }
 
 constexpr int DEC_ROWS = 16;                // rows of the decode kernel
-constexpr int DEC_STEP = 32, DEC_LEAST = 4; // positions a step of a wavefront, least steps of a workgroup
+constexpr int DEC_STEP = 32;                // positions a step of a wavefront
 // the decode kernel's steps of a range
 __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
 
 constexpr int PRO_ROWS = 128;               // rows of a workgroup of the prompt kernel
-constexpr int PRO_UNIT = 64, PRO_LEAST = 1; // positions are split in units of 64
+constexpr int PRO_UNIT = 64;                // positions are split in units of 64
 __device__ __forceinline__ int pro_units(const PagedSpan &r) { return (r.hi - (r.lo & ~(PRO_UNIT - 1))) / PRO_UNIT + 1; }
 // at most as many tiles of PRO_ROWS rows as a batch's sequences can have, per K / V head
 inline int64_t paged_tiles(const PagedAttnArgs &a) {
@@ -196,27 +214,27 @@ struct PagedTile {
 };
 __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int index) {
     const int lane = threadIdx.x & 63, G = a.n_head / a.p.n_head_kv;
-    int64_t before = 0;  // tiles of the sequences before the 64 looked at
+    int before = 0;  // tiles of the sequences before the 64 looked at
     PagedTile t;
     t.s = -1, t.r0 = 0, t.index = index, t.q = PagedSeq{};
     for (int b = 0; b < a.p.n_seq; b += 64) {
         const int s = b + lane;
-        int64_t own = 0;
+        int own = 0;
         if (s < a.p.n_seq) {
             const PagedSeq q = paged_seq(a.p, s);
             const int64_t rows = (int64_t)q.n * G;
-            own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (rows + PRO_ROWS - 1) / PRO_ROWS;
+            own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (int)((rows + PRO_ROWS - 1) / PRO_ROWS);
         }
-        int64_t upto = own;  // with this lane's
+        int upto = own;  // with this lane's
         for (int o = 1; o < 64; o <<= 1) {
-            const int64_t z = __shfl_up(upto, o, 64);
+            const int z = __shfl_up(upto, o, 64);
             if (lane >= o) upto += z;
         }
         const uint64_t m = __builtin_amdgcn_ballot_w64(before + upto > index);
         if (m) {
             const int at = __builtin_ctzll(m);
             t.s = b + at;
-            t.r0 = (int)(index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
+            t.r0 = (index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
             t.s = __builtin_amdgcn_readfirstlane(t.s);
             t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
             t.q = paged_useq(a.p, t.s);

@@ -36,8 +36,10 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
     const int kvh = blockIdx.x % nkv, split = blockIdx.x / nkv % a.ds, s = blockIdx.x / nkv / a.ds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedSeq q = paged_useq(a.p, s);
-    if (q.n == 0 || (a.ps > 0 && (int64_t)q.n * G > DEC_ROWS)) return;  // the prompt kernel's
     const int64_t rows = (int64_t)q.n * G;
+    const bool none = q.n == 0 || (a.ps > 0 && rows > DEC_ROWS);  // the prompt kernel's
+    if (a.ds > 1 && split == 0 && tid == 0 && (none || !q.ok)) a.info[s * nkv + kvh].used = 0;
+    if (none) return;
     if (!q.ok) {
         if (split == 0)
             for (int64_t i = tid; i < rows * HD; i += 256) {
@@ -49,8 +51,9 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
     const int prefix = paged_prefix(a, s, q);
     const PagedSpan sp = paged_span(a, q, prefix, 0, q.n - 1);
     const int base = sp.lo & ~(DEC_STEP - 1), steps = dec_steps(sp);
-    const PagedChunk ch = paged_chunk(steps, a.ds, DEC_LEAST);
+    const PagedChunk ch = paged_chunk(steps, a.ds, a.dleast);
     if (split >= ch.used) return;
+    if (a.ds > 1 && split == 0 && tid == 0) a.info[s * nkv + kvh] = PagedSlot{ch.used, (int)rows, q.t0, 0};
     const int end = min(steps, (split + 1) * ch.per);
 
     // this lane's row: column m of the products
@@ -95,8 +98,17 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
             for (int w = 0; w < D::W; ++w) vr[b][w] = *(const pu4 *)(vp + ((int64_t)(16 * b) << a.p.shift) * D::ES + 16 * w);
     };
     int st = split * ch.per + wave;
+    if (st < end) pages(st);
+    float x[D::KS][8];  // q, asked for ahead of K and V: loads return in order
+#pragma unroll
+    for (int ks = 0; ks < D::KS; ++ks) {
+        const bool in = mine && ks * 32 + quad * 8 < HD;
+        const pf4 *src = (const pf4 *)(a.q + (q.t0 + i) * a.ldq + (int64_t)head * HD + (in ? ks * 32 + quad * 8 : 0));
+        const pf4 u = src[0], v = src[1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[ks][e] = in ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.0f;
+    }
     if (st < end) {
-        pages(st);
         load_k(st);
         load_v(st);
         if (st + 4 < end) pages(st + 4);
@@ -105,18 +117,11 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
     pu4 qp[D::KS][D::NQ];
     PagedScore score;
     {
-        float x[D::KS][8], amax = 0.0f;
+        float amax = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < D::KS; ++ks) {
-            const bool in = mine && ks * 32 + quad * 8 < HD;
-            const pf4 *src = (const pf4 *)(a.q + (q.t0 + i) * a.ldq + (int64_t)head * HD + (in ? ks * 32 + quad * 8 : 0));
-            const pf4 u = src[0], v = src[1];
+        for (int ks = 0; ks < D::KS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[ks][e] = in ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.0f;
-                amax = fmaxf(amax, fabsf(x[ks][e]));
-            }
-        }
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
         float size = 1.0f;
         if constexpr (TYPE == T_F16) {
             amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
@@ -181,7 +186,9 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
 #pragma unroll
                 for (int b = 0; b < D::VB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) odd |= raw_bad<TYPE>(vr[b], e);
+                    for (int w = 0; w < D::W; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) odd |= infinite<TYPE>(vr[b][w][i]) != 0;
                 odd = __builtin_amdgcn_ballot_w64(odd) != 0;
                 if (odd) {
 #pragma unroll
@@ -261,6 +268,8 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
 #pragma unroll
     for (int b = 0; b < D::VB; ++b) *(pf4 *)&acc_l[wave][m][16 * b + quad * 4] = acc[b];
     __syncthreads();
+    const int64_t at = ((int64_t)s * nkv + kvh) * a.ds + split;
+    float *part = a.part + at * a.drows * HD, *stat = a.stat + at * a.drows * 2;
     for (int x = tid; x < R * (HD / 4); x += 256) {
         const int r = x / (HD / 4), d = 4 * (x - r * (HD / 4));
         const float cm = fminf(fminf(c_l[0][r], c_l[1][r]), fminf(c_l[2][r], c_l[3][r]));
@@ -274,14 +283,10 @@ __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel
         }
         const int64_t t = q.t0 + r / G;
         const int h = kvh * G + r % G;
-        if (ch.used == 1) *(pf4 *)(a.o + t * a.ldo + (int64_t)h * HD + d) = o / lr;
+        if (ch.used == 1) *(pf4 *)(a.o + t * a.ldo + (int64_t)h * HD + d) = o * (1.0f / lr);
         else {
-            const int64_t at = (((int64_t)split * a.p.n_seq + s) * nkv + kvh) * a.drows + r;
-            *(pf4 *)(a.part + at * HD + d) = o;
-            if (d == 0) {
-                a.stat[2 * at] = cm;
-                a.stat[2 * at + 1] = lr;
-            }
+            *(pf4 *)(part + r * HD + d) = o;
+            if (d == 0) *(pf2 *)(stat + 2 * r) = pf2{cm, lr};
         }
     }
 }

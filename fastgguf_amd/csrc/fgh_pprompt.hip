@@ -41,6 +41,8 @@ template <int NW>
 __device__ __forceinline__ int turn(int r) {
     return NW == 4 ? r >> 1 & 3 : r & (NW < 16 ? NW - 1 : 15);
 }
+constexpr int SCHED_ALU = 6;  // what may move across these scheduling barriers: vector and scalar ALU, not products or LDS reads
+
 // LDS row of a 16-position block <-> position
 __device__ __forceinline__ int swap_rows(int m) { return (m & ~12) | (m & 8) >> 1 | (m & 4) << 1; }
 
@@ -53,14 +55,16 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     using P = Pro<TYPE, HD>;
     constexpr int KT = P::KT, ES = P::ES, W = P::W;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ uint32_t odd_l[2];  // positions of the tile with a V value that is not finite and that only some rows see
+    __shared__ uint32_t odd_l[2];  // positions of the tile with a V value that is not finite
     const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
     const int kvh = blockIdx.x % nkv, split = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // tiles in reverse: those late in a sequence have the most positions and start first
     const PagedTile tl = paged_tile(a, (int)(gridDim.x / nkv) - 1 - (int)(blockIdx.x / nkv));
-    if (tl.s < 0) return;
+    const int64_t slot = (int64_t)tl.index * nkv + kvh;
     const PagedSeq q = tl.q;
+    if (a.ps > 1 && split == 0 && tid == 0 && (tl.s < 0 || !q.ok)) a.info[slot].used = 0;
+    if (tl.s < 0) return;
     const int s = tl.s, r0 = tl.r0, R = min(PRO_ROWS, q.n * G - r0);
     if (!q.ok) {
         if (split == 0)
@@ -72,8 +76,9 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     }
     const int prefix = paged_prefix(a, s, q);
     const PagedSpan sp = paged_span(a, q, prefix, r0 / G, (r0 + R - 1) / G);
-    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, PRO_LEAST);
+    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, a.pleast);
     if (split >= ch.used) return;
+    if (a.ps > 1 && split == 0 && tid == 0) a.info[slot] = PagedSlot{ch.used, R, q.t0, r0};
     const int ubase = sp.lo & ~(PRO_UNIT - 1);  // the split's positions k0 .. k1, whole units but for the range's ends
     const int k0 = max(sp.lo & ~(KT - 1), ubase + split * ch.per * PRO_UNIT), k1 = min(sp.hi, ubase + (split + 1) * ch.per * PRO_UNIT - 1);
 
@@ -93,6 +98,8 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     const int64_t hsize = (int64_t)kvh * HD << a.p.shift;
     uint32_t gone_next = 0;
     auto load = [&](int kb, uint8_t *buf) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // the lanes' offsets are formed for every tile, not kept
         int64_t hb[NE];  // the entries' K / V head blocks
         gone_next = 0;   // 16-position blocks whose page does not exist
 #pragma unroll
@@ -110,13 +117,13 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
         const uint8_t *kp = a.p.k + (hk + (int64_t)((kb + kblk) & mask) * HD) * ES;
 #pragma unroll
         for (int i = 0; i < P::KL; ++i) {
-            const int r = kr0 + i * (64 / P::KW) + lane / P::KW, w = lane % P::KW ^ turn<P::KW>(r);
+            const int r = kr0 + i * (64 / P::KW) + ln / P::KW, w = ln % P::KW ^ turn<P::KW>(r);
             if (P::KD == P::KW || w < P::KD)
                 lds_load16(kp + (uint32_t)(swap_rows(r & 15) * HD * ES + w * 16), buf + kr0 * P::KW * 16 + i * 1024);
         }
         // V^T: loads wave, wave + 4, ..
         constexpr int VR = 64 / P::VW;  // rows a load
-        const int vr = wave * VR + lane / P::VW, j = (lane % P::VW ^ turn<P::VW>(vr)) * (16 / ES);
+        const int vr = wave * VR + ln / P::VW, j = (ln % P::VW ^ turn<P::VW>(vr)) * (16 / ES);
         int64_t hv = hb[0];
 #pragma unroll
         for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
@@ -128,6 +135,27 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     };
     int kb = k0;
     pages(kb);
+    // q rows come in pieces of 32 values, 8 lanes a row, and change places in this wavefront's 4 KB of the second
+    // buffer; so do the outputs. (A lane's own row straight from memory, 16 bytes of 32 rows a load, took 64 cycles a load.)
+    uint8_t *own = lds + wave * 4096 + (2 * P::BYTES - 16384);
+    struct Place {
+        int64_t tok;
+        uint32_t head;
+    };
+    auto place = [&](int r) {  // row r of this wavefront in q and o (past the last: the last)
+        const int z = r0 + min(wave * 32 + r, R - 1), t = z / G;
+        return Place{q.t0 + t, (uint32_t)((kvh * G + z - t * G) * HD)};
+    };
+    constexpr int QP = (HD + 31) / 32;
+    pf4 qv[QP][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int rr = lane >> 3, rw = lane & 7;
+        const Place at = place(8 * u + rr);
+        const float *src = a.q + at.tok * a.ldq + at.head + 4 * rw;
+#pragma unroll
+        for (int g = 0; g < QP; ++g) qv[g][u] = *(const pf4 *)(src + (HD % 32 != 0 && g == QP - 1 && rw >= HD % 32 / 4 ? 0 : 32 * g));
+    }
     load(kb, lds);
     uint32_t gone = gone_next;
     if (kb + KT <= k1) pages(kb + KT);
@@ -135,26 +163,38 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     pu4 qp[P::KS][P::NQ];
     PagedScore score;
     {
-        float amax = 0.0f;
-        const float *src = a.q + (q.t0 + tok) * a.ldq + (int64_t)head * HD + half * 8;
-        float x[P::KS][8];
-#pragma unroll
-        for (int ks = 0; ks < P::KS; ++ks) {
-            const pf4 u = *(const pf4 *)(src + ks * 16), v = *(const pf4 *)(src + ks * 16 + 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[ks][e] = mine ? (e < 4 ? u[e & 3] : v[e & 3]) : 0.0f;
-                amax = fmaxf(amax, fabsf(x[ks][e]));
-            }
-        }
         float size = 1.0f;
-        if constexpr (TYPE == T_F16) size = row_size(fmaxf(amax, __shfl_xor(amax, 32, 64)));
+        if constexpr (TYPE == T_F16) {  // the rows' largest magnitudes
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float m = 0.0f;
+#pragma unroll
+                for (int g = 0; g < QP; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(qv[g][u][e]));
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+                ((float *)own)[8 * u + (lane >> 3)] = m;
+            }
+            size = row_size(((const float *)own)[lane & 31]);
+        }
         const float inv = (a.scale < 0.0f ? -1.0f : 1.0f) / size;
 #pragma unroll
-        for (int ks = 0; ks < P::KS; ++ks) {
+        for (int g = 0; g < QP; ++g) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[ks][e] *= inv;
-            parts8<TYPE, P::NQ>(x[ks], qp[ks]);
+            for (int u = 0; u < 4; ++u) *(pf4 *)(own + (8 * u + (lane >> 3)) * 128 + ((lane ^ lane >> 3) & 7) * 16) = qv[g][u];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (2 * g + k < P::KS) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const pf4 z = *(const pf4 *)(own + (lane & 31) * 128 + ((4 * k + 2 * half + e) ^ (lane & 7)) * 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[4 * e + i] = mine ? z[i] * inv : 0.0f;
+                    }
+                    parts8<TYPE, P::NQ>(x, qp[2 * g + k]);
+                }
         }
         score = paged_score(a, head, size);
     }
@@ -169,6 +209,103 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     // where this lane's words are: the K row it gives, and the V^T row; word w of either at (place ^ 16 w)
     const uint32_t k_at = (lane & 31) * P::KW * 16 + ((half * W) ^ turn<P::KW>(lane & 31)) * 16;
     const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31)) * 16;
+    const int first = max(sp.lo, k0), last = min(sp.hi, k1);  // the positions that count here
+
+    // Positions h * 32 .. of a tile. plain: seen by every row, scores without cap or bias. Straight-line code but for the scores'
+    // forms and the rows' references, so that LDS reads run ahead of the products.
+    auto part32 = [&](const uint8_t *buf, int kb, int h, bool whole, bool plain) {
+        uint32_t k_lane = k_at, v_lane = v_at;
+        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the words' places are formed where they are read, not kept
+        constexpr int AHEAD = 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
+        pu4 raw[SLOTS][W];
+        auto read_k = [&](int ks) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) raw[ks % SLOTS][w] = *(const pu4 *)(buf + (k_lane ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
+        };
+        auto read_v = [&](int x) {
+            const int kk = x / P::VB, b = x % P::VB;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ ((2 * h + kk) * 2 * W + w) * 16) + b * 32 * P::VW * 16);
+        };
+        pf16 sc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < AHEAD; ++ks) read_k(ks);
+#pragma unroll
+        for (int ks = 0; ks < P::KS; ++ks) {
+            if (ks + AHEAD < P::KS) read_k(ks + AHEAD);
+            pu4 kp[P::NK];
+            cache8<TYPE>(raw[ks % SLOTS], kp);
+#pragma unroll
+            for (int x = P::NQ - 1; x >= 0; --x)
+#pragma unroll
+                for (int y = P::NK - 1; y >= 0; --y)
+                    if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
+            __builtin_amdgcn_sched_barrier(SCHED_ALU);
+        }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) read_v(x);
+        float v[2][8], mul = score.mul;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = sc[e];
+        if (!plain) {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const int j0 = kb + h * 32 + kk * 16 + half * 8;
+                mul = score.apply(v[kk], j0, pos);
+                const bool no = gone >> (2 * h + kk) & 1;
+                const int l0 = max(lo, first) - j0, h0 = min(hi, last) - j0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (no) v[kk][e] = __builtin_nanf("");
+                    if (!whole && (e < l0 || e > h0)) v[kk][e] = -__builtin_inff();
+                }
+            }
+        }
+        float top = v[0][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, v[e / 8][e % 8]);
+        top *= mul;
+        if (__builtin_amdgcn_ballot_w64(top + c > PTOP)) {
+            const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
+            if (mx + c > PTOP) {
+                const float cn = PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
+                c = cn;
+                l *= f;
+#pragma unroll
+                for (int b = 0; b < P::VB; ++b) acc[b] *= f;
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[kk][e], mul, c));
+                l += p[e];
+            }
+            pu4 pp[P::NQ];
+            parts8<TYPE, P::NQ>(p, pp);
+#pragma unroll
+            for (int b = 0; b < P::VB; ++b) {
+                constexpr int N = 2 * P::VB;
+                const int x = kk * P::VB + b;
+                if (x + AHEAD < N) read_v(x + AHEAD);
+                pu4 vp[P::NK];
+                pu4 (&word)[W] = raw[x % SLOTS];
+                cache8<TYPE>(word, vp);
+#pragma unroll
+                for (int x = P::NQ - 1; x >= 0; --x)
+#pragma unroll
+                    for (int y = P::NK - 1; y >= 0; --y)
+                        if (x + y < 3) mma32<TYPE>(acc[b], vp[y], pp[x]);
+                __builtin_amdgcn_sched_barrier(SCHED_ALU);
+            }
+        }
+    };
+
     for (int n = 0; kb <= k1; kb += KT, n ^= 1) {
         uint8_t *buf = lds + n * P::BYTES;
         __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt 0: this wavefront's part of the tile is in LDS
@@ -177,141 +314,96 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
             load(kb + KT, lds + (n ^ 1) * P::BYTES);
             if (kb + 2 * KT <= k1) pages(kb + 2 * KT);
         }
-        // positions of the tile that count here: first .. last; whole: all of them, for every row
-        const int first = max(sp.lo, k0), last = min(sp.hi, k1);
-        const bool whole = kb >= max(sp.in_lo, k0) && kb + KT - 1 <= min(sp.in_hi, k1) && gone == 0;
+        const bool whole = kb >= max(sp.in_lo, k0) && kb + KT - 1 <= min(sp.in_hi, k1) && gone == 0;  // seen by every row
         uint64_t odd = 0;
         if (!whole) {
-            // V values at positions that no row sees become zeros, and so do those that are not finite (see below)
+            // V values at positions that no row sees become zeros, and so do those that are not finite: what only some of
+            // the rows see must not reach the others by way of 0 x NaN. The rows that see them get them below.
             if (tid < 2) odd_l[tid] = 0;
             __syncthreads();
             for (int x = tid; x < HD * P::VW; x += 256) {
                 const int r = x / P::VW, at = x % P::VW, j = (at ^ turn<P::VW>(r)) * (16 / ES);
                 pu4 *word = (pu4 *)(buf + P::KBYTES + (r * P::VW + at) * 16);
-                pu4 v[W];
-                v[0] = *word;
-                uint32_t bad = 0;
+                // of the word's values (all in one page): from .. to - 1 are seen by some row
+                constexpr int N = 16 / ES;
+                const bool none = gone >> (j / 16) & 1;
+                const int from = none ? N : min(max(first - kb - j, 0), N), to = min(max(last + 1 - kb - j, 0), N);
+                pu4 v = *word;
+                uint32_t inf = 0;
 #pragma unroll
-                for (int e = 0; e < 16 / ES; ++e) {
-                    const bool none = (gone >> ((j + e) / 16) & 1) || kb + j + e < first || kb + j + e > last;
-                    const bool inf = raw_bad<TYPE>(v, e);
-                    if (none || inf) raw_zero<TYPE>(v, e);
-                    if (inf && !none) bad |= 1u << e;
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (ES == 4) v[i] = i >= from && i < to ? v[i] : 0u;
+                    else v[i] &= (2 * i >= from && 2 * i < to ? 0x0000ffffu : 0u) | (2 * i + 1 >= from && 2 * i + 1 < to ? 0xffff0000u : 0u);
+                    inf |= infinite<TYPE>(v[i]);
                 }
-                *word = v[0];
-                if (bad) atomicOr(&odd_l[j / 32], bad << (j & 31));
+                if (inf) {  // rare
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) bad |= raw_bad<TYPE>(&v, e) ? 1u << e : 0u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = finite_only<TYPE>(v[i]);
+                    atomicOr(&odd_l[j / 32], bad << (j & 31));
+                }
+                if (inf || from > 0 || to < N) *word = v;
             }
             __syncthreads();
-            odd = odd_l[0] | (uint64_t)odd_l[1] << 32;
+            odd = (uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[0]) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[1]) << 32;
         }
+        const bool plain = whole && !(score.cap_out > 0.0f) && !score.bias;
 #pragma unroll
-        for (int h = 0; h < KT / 32; ++h) {
-            pf16 sc;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < P::KS; ++ks) {
-                pu4 raw[W], kp[P::NK];
-#pragma unroll
-                for (int w = 0; w < W; ++w)
-                    raw[w] = *(const pu4 *)(buf + (k_at ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
-                cache8<TYPE>(raw, kp);
-#pragma unroll
-                for (int x = P::NQ - 1; x >= 0; --x)
-#pragma unroll
-                    for (int y = P::NK - 1; y >= 0; --y)
-                        if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
-            }
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const int j0 = kb + h * 32 + kk * 16 + half * 8;
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = sc[8 * kk + e];
-                const float mul = score.apply(v, j0, pos);
-                if (!whole) {
-                    const bool no = gone >> (2 * h + kk) & 1;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (no) v[e] = __builtin_nanf("");
-                        if (j0 + e < max(lo, first) || j0 + e > min(hi, last)) v[e] = -__builtin_inff();
-                    }
-                }
-                float top = v[0];
-#pragma unroll
-                for (int e = 1; e < 8; ++e) top = fmaxf(top, v[e]);
-                top *= mul;
-                if (__builtin_amdgcn_ballot_w64(top + c > PTOP)) {
-                    const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
-                    if (mx + c > PTOP) {
-                        const float cn = PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
-                        c = cn;
-                        l *= f;
-#pragma unroll
-                        for (int b = 0; b < P::VB; ++b) acc[b] *= f;
-                    }
-                }
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], mul, c));
-                    l += p[e];
-                }
-                pu4 pp[P::NQ];
-                parts8<TYPE, P::NQ>(p, pp);
-#pragma unroll
-                for (int b = 0; b < P::VB; ++b) {
-                    pu4 raw[W], vp[P::NK];
-#pragma unroll
-                    for (int w = 0; w < W; ++w)
-                        raw[w] = *(const pu4 *)(buf + (v_at ^ ((2 * h + kk) * 2 * W + w) * 16) + b * 32 * P::VW * 16);
-                    cache8<TYPE>(raw, vp);
-#pragma unroll
-                    for (int x = P::NQ - 1; x >= 0; --x)
-#pragma unroll
-                        for (int y = P::NK - 1; y >= 0; --y)
-                            if (x + y < 3) mma32<TYPE>(acc[b], vp[y], pp[x]);
-                }
-            }
-        }
-        while (odd) {  // values that are not finite, left out above: added to the rows that see them
+        for (int h = 0; h < KT / 32; ++h) part32(buf, kb, h, whole, plain);
+        while (odd) {
             const int j = kb + __builtin_ctzll(odd);
             odd &= odd - 1;
             int shift = a.p.shift;
             asm volatile("" : "+s"(shift));  // this rare path must not cost registers: no addresses formed ahead,
             const int64_t at = paged_head(a.p, table[j >> shift], kvh) + (j & mask) + ((int64_t)(4 * half) << shift);
-            if (j >= lo && j <= hi)
 #pragma unroll
-                for (int b = 0; b < P::VB; ++b)
+            for (int b = 0; b < P::VB; ++b)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int d = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                        if (HD % 32 == 0 || d < HD) {
-                            const float z = cached<TYPE>(a.p.v, at + ((int64_t)(d - 4 * half) << shift));
-                            if (not_finite(z)) acc[b][r] += z;
-                            asm volatile("" : "+s"(shift)::"memory");  // and one value at a time
-                        }
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * b + 8 * (r / 4) + r % 4;
+                    if (HD % 32 == 0 || d + 4 * half < HD) {
+                        const float z = cached<TYPE>(a.p.v, at + ((int64_t)d << shift));
+                        if (not_finite(z) && j >= lo && j <= hi) acc[b][r] += z;
+                        asm volatile("" : "+s"(shift)::"memory");  // and one value at a time
                     }
+                }
         }
         gone = gone_next;
     }
     l += __shfl_xor(l, 32, 64);
-    if (!mine) return;
-    const int64_t slot = (((int64_t)split * (gridDim.x / nkv) + tl.index) * nkv + kvh) * PRO_ROWS + wr;
-    float *out = ch.used == 1 ? a.o + (q.t0 + tok) * a.ldo + (int64_t)head * HD : a.part + slot * HD;
+    if (ch.used > 1) {  // sums as the lanes hold them
+        if (wave * 32 >= R) return;
+        pf4 *part = (pf4 *)a.part + ((slot * a.ps + split) * 4 + wave) * (P::VB * 4 * 64) + lane;
 #pragma unroll
-    for (int b = 0; b < P::VB; ++b)
+        for (int b = 0; b < P::VB; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 32 * b + 8 * i + 4 * half;
-            if (HD % 32 == 0 || d < HD) {
-                pf4 o = {acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-                *(pf4 *)(out + d) = ch.used == 1 ? o / l : o;
-            }
+            for (int i = 0; i < 4; ++i)
+                part[(4 * b + i) * 64] = pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+        if (half == 0) *(pf2 *)(a.stat + ((slot * a.ps + split) * PRO_ROWS + wr) * 2) = pf2{c, l};
+        return;
+    }
+    __syncthreads();  // the buffers have been read
+    const float inv = 1.0f / l;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // the rows' places are formed again rather than kept
+    const int rr = ln >> 3, rw = ln & 7;
+    Place at[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at[u] = place(8 * u + rr);
+#pragma unroll
+    for (int b = 0; b < P::VB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *(pf4 *)(own + (lane & 31) * 128 + ((2 * i + half) ^ (lane & 7)) * 16) =
+                pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]} * inv;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const pf4 z = *(const pf4 *)(own + (8 * u + rr) * 128 + (rw ^ rr) * 16);
+            if (wave * 32 + 8 * u + rr < R && (HD % 32 == 0 || 32 * b + 4 * rw < HD))
+                *(pf4 *)(a.o + at[u].tok * a.ldo + at[u].head + 32 * b + 4 * rw) = z;
         }
-    if (ch.used > 1 && half == 0) {
-        a.stat[2 * slot] = c;
-        a.stat[2 * slot + 1] = l;
     }
 }
 
