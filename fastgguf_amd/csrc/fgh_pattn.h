@@ -65,6 +65,18 @@ __device__ __forceinline__ void parts8(const float *x, pu4 (&out)[NP]) {
         }
     }
 }
+// 8 16-bit parts times a power of two of at most 1
+template <int TYPE>
+__device__ __forceinline__ void scale8(pu4 &x, float f) {
+    if constexpr (TYPE == T_F16) {  // in two steps: a half goes down to 2^-24
+        const float r = f < 0x1p-20f ? 0x1p-20f : f;
+        const _Float16 a = (_Float16)r, b = (_Float16)(f / r);
+        x = __builtin_bit_cast(pu4, __builtin_bit_cast(ph8, x) * a * b);
+    } else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = __builtin_amdgcn_perm(__float_as_uint(__uint_as_float(x[i] & 0xffff0000u) * f), __float_as_uint(__uint_as_float(x[i] << 16) * f), 0x07060302);
+}
 // 8 cached values (16 or 32 bytes) as parts
 template <int TYPE>
 __device__ __forceinline__ void cache8(const pu4 *raw, pu4 (&out)[PagedType<TYPE>::NK]) {

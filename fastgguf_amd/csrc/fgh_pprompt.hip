@@ -21,7 +21,7 @@ template <int TYPE, int HD>
 struct Pro {
     static constexpr int ES = PagedType<TYPE>::ES, NQ = PagedType<TYPE>::NQ, NK = PagedType<TYPE>::NK;
     static constexpr int W = ES / 2;           // 16-byte words of 8 values
-    static constexpr int KT = HD * ES > 256 ? 32 : 64;
+    static constexpr int KT = HD * ES > 512 ? 32 : 64;
     static constexpr int KS = HD / 16;         // steps of 16 along the head
     static constexpr int VB = (HD + 31) / 32;  // blocks of 32 of V's values
     static constexpr int KD = HD * ES / 16;    // words of a K row
@@ -41,8 +41,6 @@ template <int NW>
 __device__ __forceinline__ int turn(int r) {
     return NW == 4 ? r >> 1 & 3 : r & (NW < 16 ? NW - 1 : 15);
 }
-constexpr int SCHED_ALU = 6;  // what may move across these scheduling barriers: vector and scalar ALU, not products or LDS reads
-
 // LDS row of a 16-position block <-> position
 __device__ __forceinline__ int swap_rows(int m) { return (m & ~12) | (m & 8) >> 1 | (m & 4) << 1; }
 
@@ -211,98 +209,139 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
     const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31)) * 16;
     const int first = max(sp.lo, k0), last = min(sp.hi, k1);  // the positions that count here
 
-    // Positions h * 32 .. of a tile. plain: seen by every row, scores without cap or bias. Straight-line code but for the scores'
-    // forms and the rows' references, so that LDS reads run ahead of the products.
-    auto part32 = [&](const uint8_t *buf, int kb, int h, bool whole, bool plain) {
-        uint32_t k_lane = k_at, v_lane = v_at;
-        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the words' places are formed where they are read, not kept
-        constexpr int AHEAD = 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
-        pu4 raw[SLOTS][W];
-        auto read_k = [&](int ks) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) raw[ks % SLOTS][w] = *(const pu4 *)(buf + (k_lane ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
-        };
-        auto read_v = [&](int x) {
-            const int kk = x / P::VB, b = x % P::VB;
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-                raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ ((2 * h + kk) * 2 * W + w) * 16) + b * 32 * P::VW * 16);
-        };
-        pf16 sc;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < AHEAD; ++ks) read_k(ks);
-#pragma unroll
-        for (int ks = 0; ks < P::KS; ++ks) {
-            if (ks + AHEAD < P::KS) read_k(ks + AHEAD);
-            pu4 kp[P::NK];
-            cache8<TYPE>(raw[ks % SLOTS], kp);
-#pragma unroll
-            for (int x = P::NQ - 1; x >= 0; --x)
-#pragma unroll
-                for (int y = P::NK - 1; y >= 0; --y)
-                    if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
-            __builtin_amdgcn_sched_barrier(SCHED_ALU);
-        }
-#pragma unroll
-        for (int x = 0; x < AHEAD; ++x) read_v(x);
-        float v[2][8], mul = score.mul;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = sc[e];
+    // A tile in blocks of 32 positions, h: scores S(h), weights W(h), sums. The products of S(1) are issued among the
+    // vector instructions of W(0), and those of the sums over block 0 among W(1)'s: a product takes the matrix pipe for 32 cycles, in which
+    // the wavefront can issue 8 vector instructions.
+    constexpr int NH = KT / 32, AHEAD = 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
+    struct Weights {
+        float v[2][8];  // scores, then weights, of this lane's positions 16 kk + 8 half + e of the block
+        float mul;
+        pu4 pp[2][P::NQ];
+    };
+    // weight e; the eighth of a run completes its parts
+    auto weigh = [&](Weights &w, int e) {
+        float &v = w.v[e / 8][e % 8];
+        v = __builtin_amdgcn_exp2f(__builtin_fmaf(v, w.mul, c));
+        l += v;
+        if (e % 8 == 7) parts8<TYPE, P::NQ>(w.v[e / 8], w.pp[e / 8]);
+    };
+    // the scores' forms, and what of them is not seen; the row's reference follows them. False: it does not have to.
+    auto forms = [&](Weights &w, int j, bool whole, bool plain) {
+        w.mul = score.mul;
         if (!plain) {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const int j0 = kb + h * 32 + kk * 16 + half * 8;
-                mul = score.apply(v[kk], j0, pos);
-                const bool no = gone >> (2 * h + kk) & 1;
+                const int j0 = j + kk * 16 + half * 8;
+                w.mul = score.apply(w.v[kk], j0, pos);
+                const bool no = gone >> ((j0 - kb) >> 4) & 1;
                 const int l0 = max(lo, first) - j0, h0 = min(hi, last) - j0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (no) v[kk][e] = __builtin_nanf("");
-                    if (!whole && (e < l0 || e > h0)) v[kk][e] = -__builtin_inff();
+                    if (no) w.v[kk][e] = __builtin_nanf("");
+                    if (!whole && (e < l0 || e > h0)) w.v[kk][e] = -__builtin_inff();
                 }
             }
         }
-        float top = v[0][0];
+        float top = w.v[0][0];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, v[e / 8][e % 8]);
-        top *= mul;
-        if (__builtin_amdgcn_ballot_w64(top + c > PTOP)) {
-            const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (mx + c > PTOP) {
-                const float cn = PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
-                c = cn;
-                l *= f;
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, w.v[e / 8][e % 8]);
+        return top * w.mul;
+    };
+    // the row's reference follows a larger score, in whole powers of two; the factor of what was formed before
+    auto follow = [&](float top) {
+        const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
+        float f = 1.0f;
+        if (mx + c > PTOP) {
+            const float cn = PBIAS - ceilf(mx);
+            f = __builtin_amdgcn_exp2f(cn - c);
+            c = cn;
+            l *= f;
 #pragma unroll
-                for (int b = 0; b < P::VB; ++b) acc[b] *= f;
-            }
+            for (int b = 0; b < P::VB; ++b) acc[b] *= f;
         }
+        return f;
+    };
+    auto tile = [&](const uint8_t *buf, bool whole, bool plain) {
+        uint32_t k_lane = k_at, v_lane = v_at;
+        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the words' places are formed where they are read, not kept
+        pu4 raw[SLOTS][W];
+        auto read_k = [&](int h, int ks) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            float p[8];
+            for (int w = 0; w < W; ++w) raw[ks % SLOTS][w] = *(const pu4 *)(buf + (k_lane ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
+        };
+        auto read_v = [&](int x) {  // x: 16-position run, then block of values
+            const int k = x / P::VB, b = x % P::VB;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[kk][e], mul, c));
-                l += p[e];
-            }
-            pu4 pp[P::NQ];
-            parts8<TYPE, P::NQ>(p, pp);
+            for (int w = 0; w < W; ++w) raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ (2 * k * W + w) * 16) + b * 32 * P::VW * 16);
+        };
+        auto scores = [&](int h, Weights &out, auto side) {
+            pf16 sc;
 #pragma unroll
-            for (int b = 0; b < P::VB; ++b) {
-                constexpr int N = 2 * P::VB;
-                const int x = kk * P::VB + b;
-                if (x + AHEAD < N) read_v(x + AHEAD);
-                pu4 vp[P::NK];
-                pu4 (&word)[W] = raw[x % SLOTS];
-                cache8<TYPE>(word, vp);
+            for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < AHEAD; ++ks) read_k(h, ks);
+#pragma unroll
+            for (int ks = 0; ks < P::KS; ++ks) {
+                if (ks + AHEAD < P::KS) read_k(h, ks + AHEAD);
+                pu4 kp[P::NK];
+                cache8<TYPE>(raw[ks % SLOTS], kp);
 #pragma unroll
                 for (int x = P::NQ - 1; x >= 0; --x)
 #pragma unroll
                     for (int y = P::NK - 1; y >= 0; --y)
-                        if (x + y < 3) mma32<TYPE>(acc[b], vp[y], pp[x]);
-                __builtin_amdgcn_sched_barrier(SCHED_ALU);
+                        if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
+#pragma unroll
+                for (int e = ks * 16 / P::KS; e < (ks + 1) * 16 / P::KS; ++e) side(e);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = sc[e];
+        };
+        constexpr int NX = 2 * P::VB;  // V words of a block
+        auto sums = [&](int h, const Weights &w, auto side) {
+#pragma unroll
+            for (int x = 0; x < NX; ++x) {
+                if (h * NX + x + AHEAD < NH * NX) read_v(h * NX + x + AHEAD);
+                pu4 vp[P::NK];
+                cache8<TYPE>(raw[(h * NX + x) % SLOTS], vp);
+#pragma unroll
+                for (int i = P::NQ - 1; i >= 0; --i)
+#pragma unroll
+                    for (int y = P::NK - 1; y >= 0; --y)
+                        if (i + y < 3) mma32<TYPE>(acc[x % P::VB], vp[y], w.pp[x / P::VB][i]);
+#pragma unroll
+                for (int e = x * 16 / NX; e < (x + 1) * 16 / NX; ++e) side(e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto first_v = [&]() {
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) read_v(x);
+        };
+        Weights w0;
+        auto alone = [](int) {};
+        scores(0, w0, alone);
+        if constexpr (NH == 1) first_v();
+        const float top0 = forms(w0, kb, whole, plain);
+        if (__builtin_amdgcn_ballot_w64(top0 + c > PTOP)) follow(top0);
+        if constexpr (NH == 1) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) weigh(w0, e);
+            sums(0, w0, alone);
+        } else {
+            Weights w1;
+            scores(1, w1, [&](int e) { weigh(w0, e); });
+            first_v();
+            const float top1 = forms(w1, kb + 32, whole, plain);
+            if (__builtin_amdgcn_ballot_w64(top1 + c > PTOP)) {  // block 0's weights wait for their sums
+                const float f = follow(top1);
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int i = 0; i < P::NQ; ++i) scale8<TYPE>(w0.pp[kk][i], f);
+            }
+            sums(0, w0, [&](int e) { weigh(w1, e); });
+            sums(1, w1, alone);
         }
     };
 
@@ -350,8 +389,7 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
             odd = (uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[0]) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[1]) << 32;
         }
         const bool plain = whole && !(score.cap_out > 0.0f) && !score.bias;
-#pragma unroll
-        for (int h = 0; h < KT / 32; ++h) part32(buf, kb, h, whole, plain);
+        tile(buf, whole, plain);
         while (odd) {
             const int j = kb + __builtin_ctzll(odd);
             odd &= odd - 1;
