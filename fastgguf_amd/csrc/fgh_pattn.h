@@ -28,6 +28,7 @@ struct PagedType {
     static constexpr int ES = TYPE == T_F32 ? 4 : 2;  // bytes a cached value
     static constexpr int NQ = TYPE == T_F16 ? 2 : 3;  // parts of q and of the weights
     static constexpr int NK = TYPE == T_F32 ? 3 : 1;  // parts of K and V
+    static constexpr int NPROD = TYPE == T_F16 ? 2 : TYPE == T_F32 ? 6 : 3;  // products of parts
 };
 
 // D += A B, 16 x 16 with 32 products a sum, or 32 x 32 with 16. A: lane l holds row l % 16 (32), values 8 (l / 16 (32)) .. + 7; B: column
@@ -43,27 +44,29 @@ __device__ __forceinline__ void mma32(pf16 &d, pu4 x, pu4 y) {
     else d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pb8, x), __builtin_bit_cast(pb8, y), d, 0, 0, 0);
 }
 
+// values 2 i and 2 i + 1 of 8 as NP vectors of 16-bit parts
+template <int TYPE, int NP>
+__device__ __forceinline__ void parts2(float a, float b, int i, pu4 (&out)[NP]) {
+    if constexpr (TYPE == T_F16) {  // to nearest, then what is left to nearest
+        const pf2 v = {a, b};
+        const ph2 h = __builtin_convertvector(v, ph2);
+        out[0][i] = __builtin_bit_cast(uint32_t, h);
+        out[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v - __builtin_convertvector(h, pf2), ph2));
+    } else {  // the upper halves of the words, cut: what is left is exact, and 8 + 8 + 8 bits hold it all
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
+            out[k][i] = __builtin_amdgcn_perm(v, u, 0x07060302);
+            a -= __uint_as_float(u & 0xffff0000u);
+            b -= __uint_as_float(v & 0xffff0000u);
+        }
+    }
+}
 // 8 fp32 values as NP vectors of 8 16-bit parts
 template <int TYPE, int NP>
 __device__ __forceinline__ void parts8(const float *x, pu4 (&out)[NP]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const pf2 v = {x[2 * i], x[2 * i + 1]};
-        if constexpr (TYPE == T_F16) {  // to nearest, then what is left to nearest
-            const ph2 h = __builtin_convertvector(v, ph2);
-            out[0][i] = __builtin_bit_cast(uint32_t, h);
-            out[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v - __builtin_convertvector(h, pf2), ph2));
-        } else {  // the upper halves of the words, cut: what is left is exact, and 8 + 8 + 8 bits hold it all
-            pf2 r = v;
-#pragma unroll
-            for (int k = 0; k < NP; ++k) {
-                const uint32_t a = __float_as_uint(r.x), b = __float_as_uint(r.y);
-                out[k][i] = __builtin_amdgcn_perm(b, a, 0x07060302);
-                r.x -= __uint_as_float(a & 0xffff0000u);
-                r.y -= __uint_as_float(b & 0xffff0000u);
-            }
-        }
-    }
+    for (int i = 0; i < 4; ++i) parts2<TYPE, NP>(x[2 * i], x[2 * i + 1], i, out);
 }
 // 8 16-bit parts times a power of two of at most 1
 template <int TYPE>

@@ -218,12 +218,21 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
         float mul;
         pu4 pp[2][P::NQ];
     };
-    // weight e; the eighth of a run completes its parts
+    // weight e, and the parts of two
     auto weigh = [&](Weights &w, int e) {
         float &v = w.v[e / 8][e % 8];
         v = __builtin_amdgcn_exp2f(__builtin_fmaf(v, w.mul, c));
         l += v;
-        if (e % 8 == 7) parts8<TYPE, P::NQ>(w.v[e / 8], w.pp[e / 8]);
+        asm volatile("" : "+v"(v), "+v"(l));  // here, not where they are used
+        if (e % 2 == 1) {
+            parts2<TYPE, P::NQ>(w.v[e / 8][e % 8 - 1], v, e % 8 / 2, w.pp[e / 8]);
+#pragma unroll
+            for (int i = 0; i < P::NQ; ++i) {
+                uint32_t z = w.pp[e / 8][i][e % 8 / 2];
+                asm volatile("" : "+v"(z));
+                w.pp[e / 8][i][e % 8 / 2] = z;
+            }
+        }
     };
     // the scores' forms, and what of them is not seen; the row's reference follows them. False: it does not have to.
     auto forms = [&](Weights &w, int j, bool whole, bool plain) {
@@ -274,7 +283,15 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
 #pragma unroll
             for (int w = 0; w < W; ++w) raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ (2 * k * W + w) * 16) + b * 32 * P::VW * 16);
         };
+        constexpr int NPROD = PagedType<TYPE>::NPROD;
+        auto beside = [&](int m, int of, auto side) {  // product m of `of`: its share of the 16 weights beside it
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (e >= m * 16 / of && e < (m + 1) * 16 / of) side(e);
+            __builtin_amdgcn_sched_barrier(0);
+        };
         auto scores = [&](int h, Weights &out, auto side) {
+            int m = 0;
             pf16 sc;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
@@ -289,16 +306,17 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
                 for (int x = P::NQ - 1; x >= 0; --x)
 #pragma unroll
                     for (int y = P::NK - 1; y >= 0; --y)
-                        if (x + y < 3) mma32<TYPE>(sc, kp[y], qp[ks][x]);
-#pragma unroll
-                for (int e = ks * 16 / P::KS; e < (ks + 1) * 16 / P::KS; ++e) side(e);
-                __builtin_amdgcn_sched_barrier(0);
+                        if (x + y < 3) {
+                            mma32<TYPE>(sc, kp[y], qp[ks][x]);
+                            beside(m++, P::KS * NPROD, side);
+                        }
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = sc[e];
         };
         constexpr int NX = 2 * P::VB;  // V words of a block
         auto sums = [&](int h, const Weights &w, auto side) {
+            int m = 0;
 #pragma unroll
             for (int x = 0; x < NX; ++x) {
                 if (h * NX + x + AHEAD < NH * NX) read_v(h * NX + x + AHEAD);
@@ -308,10 +326,10 @@ __global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel
                 for (int i = P::NQ - 1; i >= 0; --i)
 #pragma unroll
                     for (int y = P::NK - 1; y >= 0; --y)
-                        if (i + y < 3) mma32<TYPE>(acc[x % P::VB], vp[y], w.pp[x / P::VB][i]);
-#pragma unroll
-                for (int e = x * 16 / NX; e < (x + 1) * 16 / NX; ++e) side(e);
-                __builtin_amdgcn_sched_barrier(0);
+                        if (i + y < 3) {
+                            mma32<TYPE>(acc[x % P::VB], vp[y], w.pp[x / P::VB][i]);
+                            beside(m++, NX * NPROD, side);
+                        }
             }
         };
         auto first_v = [&]() {
