@@ -1059,7 +1059,7 @@ int fgh_paged_store_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_page
                              rope->n_rot ? log2((double)rope->freq_base) : 0.0, rope->freq_scale / 6.283185307179586476925,
                              rope->n_rot, rope->rope == FGH_ROPE_HALVES};
     a.q = q, a.k = k, a.v = v, a.qo = qo, a.ldq = ldq, a.ldkv = ldkv, a.ldo = ldo, a.n_head = n_head;
-    HIP_TRY(c, fgh::launch_paged_store(a, c->stream));
+    HIP_TRY(c, fgh::launch_paged_store(a, c->num_cu, c->stream));
     return FGH_OK;
 }
 int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_mask *mask,

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace fgh {
 
 // fgh_paged_cache and fgh_paged_batch as the kernels take them
@@ -60,6 +62,43 @@ __device__ __forceinline__ int paged_find(const Paged &a, int t) {
     return s >= a.n_seq ? -1 : s;
 }
 
+// A sequence's part of the batch in 64 positions from `base`, a multiple of 64: tile `index` of the sequences' tiles in
+// order. s = -1: there are fewer.
+struct PagedVTile {
+    int s, base;
+    PagedSeq q;
+};
+__device__ __forceinline__ PagedVTile paged_vtile(const Paged &a, int index) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    PagedVTile t;
+    t.s = -1, t.base = 0, t.q = PagedSeq{};
+    for (int b = 0; b < a.n_seq; b += 64) {
+        const int s = b + lane;
+        int own = 0, first = 0;
+        if (s < a.n_seq) {
+            const PagedSeq q = paged_seq(a, s);
+            first = (q.len - q.n) / 64;
+            own = q.n > 0 && q.ok ? (q.len - 1) / 64 - first + 1 : 0;
+        }
+        int upto = own;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int z = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += z;
+        }
+        const uint64_t m = __builtin_amdgcn_ballot_w64(before + upto > index);
+        if (m) {
+            const int at = __builtin_ctzll(m);
+            t.s = __builtin_amdgcn_readfirstlane(b + at);
+            t.base = __builtin_amdgcn_readfirstlane((__shfl(first, at, 64) + index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * 64);
+            t.q = paged_useq(a, t.s);
+            return t;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return t;
+}
+
 struct PagedRopeArgs {
     const float *qw, *kw, *factors;
     float eps;
@@ -73,8 +112,10 @@ struct PagedStoreArgs {
     float *qo;
     int64_t ldq, ldkv, ldo;
     int n_head;
+    // set by the launch: a token's heads over `parts` workgroups of heads_part, at most v_tiles tiles of V
+    int parts, heads_part, v_tiles;
 };
-hipError_t launch_paged_store(const PagedStoreArgs &a, hipStream_t s);
+hipError_t launch_paged_store(PagedStoreArgs &a, int num_cu, hipStream_t s);
 
 // a slot: how many splits of its range were used (0, 1: nothing to join), its rows and where they are in the batch
 struct PagedSlot {
