@@ -1081,11 +1081,14 @@ int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_
     a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo, a.n_head = n_head, a.window = mask->window, a.scale = mask->scale;
     a.softcap = mask->softcap, a.slopes = mask->slopes, a.prefix = mask->prefix;
     const fgh::PagedScratch need = fgh::paged_attention_plan(a, c->num_cu);
-    if (need.part) {
-        if (int rc = grow(c, c->pa, need.info * sizeof(fgh::PagedSlot) + (need.part + need.stat) * 4)) return rc;
-        a.info = (fgh::PagedSlot *)c->pa.p;
-        a.part = (float *)(a.info + need.info);
-        a.stat = a.part + need.part;
+    if (const size_t bytes = need.bytes()) {
+        if (int rc = grow(c, c->pa, bytes)) return rc;
+        a.dsum.info = (fgh::PagedSlot *)c->pa.p;
+        a.psum.info = a.dsum.info + need.dslot;
+        a.dsum.part = (float *)(a.psum.info + need.pslot);
+        a.psum.part = a.dsum.part + need.dpart;
+        a.dsum.stat = a.psum.part + need.ppart;
+        a.psum.stat = a.dsum.stat + need.drow * 2;
     }
     HIP_TRY(c, fgh::launch_paged_attention(a, c->stream));
     return FGH_OK;

@@ -121,6 +121,10 @@ hipError_t launch_paged_store(PagedStoreArgs &a, int num_cu, hipStream_t s);
 struct PagedSlot {
     int32_t used, rows, t0, r0;
 };
+struct PagedSums {
+    float *part, *stat;
+    PagedSlot *info;
+};
 struct PagedAttnArgs {
     Paged p;
     const float *q, *slopes;
@@ -134,11 +138,11 @@ struct PagedAttnArgs {
     // launched) of at least dleast steps / pleast units each. Split ranges leave their sums in part and stat, by slot (a workgroup's
     // rows) and split, and what the join has to know of a slot in info.
     int ds, ps, drows, dleast, pleast;
-    float *part, *stat;
-    PagedSlot *info;
+    PagedSums dsum, psum;
 };
 struct PagedScratch {
-    size_t part, stat, info;  // floats, floats, slots
+    size_t dpart, ppart, drow, prow, dslot, pslot;  // floats of part, rows of stat, slots of info
+    size_t bytes() const { return (dslot + pslot) * sizeof(PagedSlot) + (drow + prow) * 8 + (dpart + ppart) * 4; }
 };
 // the plan for a device of num_cu compute units, and the scratch it needs
 PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu);

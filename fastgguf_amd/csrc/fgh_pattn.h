@@ -1,4 +1,4 @@
-// fgh_pattn.h - what the paged attention's kernels share (fgh_pdecode.hip, fgh_pprompt.hip, fgh_pattn.hip). Internal.
+// fgh_pattn.h - what the paged attention's kernels share (fgh_pdecode.h, fgh_pprompt.h, fgh_pattn.hip). Internal.
 //
 // fp32 results from 16-bit matrix instructions: every operand is a sum of 16-bit parts, and the products of parts are
 // summed in the fp32 accumulators.
@@ -130,35 +130,48 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float PBIAS = 10.0f;  // weights are 2^(PBIAS + s - m): s in powers of two, m a running reference of the row
 constexpr float PTOP = 15.0f;   // m follows a larger s where the exponent would pass this: a half's largest is 2^16
 
-// tanh: y + y^3 g(y^2) below 0.65 (g fitted at Chebyshev nodes), 1 - 2 / (e^(2 y) + 1) above: within 3 roundings
-__device__ __forceinline__ float tanh_near(float y) {
+// tanh within 3 roundings: y + y^3 g(y^2) below 0.65 (g fitted at Chebyshev nodes), 1 - 2 / (e^(2 y) + 1) above
+__device__ __forceinline__ float tanh_below(float y) {
     const float z = y * y;
     float g = -0.005932980682700872f;
     g = __builtin_fmaf(g, z, 0.020881319418549538f);
     g = __builtin_fmaf(g, z, -0.053825847804546356f);
     g = __builtin_fmaf(g, z, 0.13332600891590118f);
     g = __builtin_fmaf(g, z, -0.333333283662796f);
-    const float small = __builtin_fmaf(y * z, g, y);
-    const float e = __builtin_amdgcn_exp2f(fabsf(y) * (2.0f * LOG2E));
-    const float big = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), y);
-    return fabsf(y) < 0.65f ? small : big;
+    return __builtin_fmaf(y * z, g, y);
 }
+__device__ __forceinline__ float tanh_above(float y) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(y) * (2.0f * LOG2E));
+    return copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), y);
+}
+constexpr float TANH_SPLIT = 0.65f;
 
 // What turns a row's products into scores in powers of two, s = v mul (v the products, unless a form has changed them)
 struct PagedScore {
     float mul;             // |scale| log2(e), times the power of two that q was divided by; above 0, so that -inf v
                            // are -inf scores (q takes the scale's sign, and a scale of 0 is 2^-126 here)
     float cap_in, cap_out; // |scale| / softcap (with that power), softcap log2(e); cap_out 0: none
-    float slope;           // slopes[h] log2(e)
+    float slope, down;     // |slopes[h]| log2(e), and -1 or 1 with the slope's sign turned around
     bool bias;
     // NE products of positions j0 .. j0 + NE - 1 of a row at position p
     template <int NE>
     __device__ __forceinline__ float apply(float (&v)[NE], int j0, int p) const {
         if (cap_out > 0.0f) {
+            float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-                v[e] = cap_out * tanh_near(v[e] * cap_in);
-                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once would cost registers
+                v[e] *= cap_in;
+                top = fmaxf(top, fabsf(v[e]));
+            }
+            if (__builtin_amdgcn_ballot_w64(!(top < TANH_SPLIT))) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    v[e] = cap_out * (fabsf(v[e]) < TANH_SPLIT ? tanh_below(v[e]) : tanh_above(v[e]));
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once would cost registers
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) v[e] = cap_out * tanh_below(v[e]);
             }
             if (!bias) return 1.0f;
         } else if (bias) {
@@ -166,8 +179,9 @@ struct PagedScore {
             for (int e = 0; e < NE; ++e) v[e] *= mul;
         } else
             return mul;
+        const float base = slope * (float)(p - j0);  // slope |p - j0 - e| = |slope (p - j0) - slope e|
 #pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = __builtin_fmaf(-slope, fabsf((float)(p - j0 - e)), v[e]);
+        for (int e = 0; e < NE; ++e) v[e] = __builtin_fmaf(down, fabsf(__builtin_fmaf((float)-e, slope, base)), v[e]);
         return 1.0f;
     }
 };
@@ -177,7 +191,9 @@ __device__ __forceinline__ PagedScore paged_score(const PagedAttnArgs &a, int he
     c.cap_in = a.softcap > 0.0f ? fabsf(a.scale) / a.softcap * q_size : 0.0f;
     c.cap_out = a.softcap * LOG2E;
     c.bias = a.slopes != nullptr;
-    c.slope = c.bias ? a.slopes[head] * LOG2E : 0.0f;
+    const float slope = c.bias ? a.slopes[head] : 0.0f;
+    c.slope = fabsf(slope) * LOG2E;
+    c.down = slope < 0.0f ? 1.0f : -1.0f;
     return c;
 }
 

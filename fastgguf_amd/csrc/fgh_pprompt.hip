@@ -1,472 +1,28 @@
-// fgh_pprompt.hip - paged attention of many rows per K / V head: prompts.
-//
-// A workgroup takes 128 rows of a sequence and K / V head (row = new token x the head's query heads + query head, so the
-// heads that share K and V share its tiles), 32 a wavefront, and goes over their positions in tiles of KT. K and V^T
-// tiles come into LDS by direct loads (16 bytes a lane), two tiles deep: the next one is on its way while this one is used.
-//   S^T = K q^T: 32 x 32 x 16 products, A = 32 K rows out of LDS, B = q in registers. LDS row m of a 16-position block holds position
-//         (m & 3) | (m & 8) >> 1 | (m & 4) << 1, so that a lane's 16 scores of 32 positions are two runs of 8 positions,
-//   O^T += V^T P^T: which are what it has to give as B. Neither scores nor weights leave their lane; a row's maximum takes
-//         one exchange with the lane 32 away, and only where the row's reference has to follow it.
-// 16-byte words of a row are kept in LDS at (word ^ row), so that lanes that read the same word of neighbouring rows
-// meet in no bank.
+// fgh_pprompt.hip - paged attention of batches with prompts: the prompt kernel's workgroups, then those of the decode kernel for the
+// sequences with few rows, in one launch.
 #include <hip/hip_runtime.h>
 
-#include "fgh_pattn.h"
+#include "fgh_pdecode.h"
+#include "fgh_pprompt.h"
 
 namespace fgh {
 
 namespace {
 
 template <int TYPE, int HD>
-struct Pro {
-    static constexpr int ES = PagedType<TYPE>::ES, NQ = PagedType<TYPE>::NQ, NK = PagedType<TYPE>::NK;
-    static constexpr int W = ES / 2;           // 16-byte words of 8 values
-    static constexpr int KT = HD * ES > 512 ? 32 : 64;
-    static constexpr int KS = HD / 16;         // steps of 16 along the head
-    static constexpr int VB = (HD + 31) / 32;  // blocks of 32 of V's values
-    static constexpr int KD = HD * ES / 16;    // words of a K row
-    static constexpr int KW = KD <= 8 ? 8 : KD <= 16 ? 16 : KD <= 32 ? 32 : 64;  // and their places in LDS
-    static constexpr int VW = KT * ES / 16;    // words of a V^T row
-    static constexpr int KBYTES = KT * KW * 16;
-    static constexpr int VROWS = VB * 32;      // with the rows behind hd 80, never loaded, their sums never stored
-    static constexpr int VBYTES = VROWS * KT * ES;
-    static constexpr int BYTES = KBYTES + VBYTES;
-    static constexpr int OCC = HD > 128 || (TYPE == T_F32 && HD > 64) ? 1 : 2;
-    static constexpr int KL = KT / 4 * KW / 64;           // direct loads of a wavefront for its KT / 4 K rows
-    static constexpr int VL = HD * VW / 64;               // and of all four for V
-};
-
-// what a row's words are kept at: word w of row r at w ^ turn(r)
-template <int NW>
-__device__ __forceinline__ int turn(int r) {
-    return NW == 4 ? r >> 1 & 3 : r & (NW < 16 ? NW - 1 : 15);
-}
-// LDS row of a 16-position block <-> position
-__device__ __forceinline__ int swap_rows(int m) { return (m & ~12) | (m & 8) >> 1 | (m & 4) << 1; }
-
-__device__ __forceinline__ void lds_load16(const uint8_t *src, uint8_t *dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
-}
-
-template <int TYPE, int HD>
-__global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel(PagedAttnArgs a) {
-    using P = Pro<TYPE, HD>;
-    constexpr int KT = P::KT, ES = P::ES, W = P::W;
+__global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel(PagedAttnArgs a, int nd) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ uint32_t odd_l[2];  // positions of the tile with a V value that is not finite
-    const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
-    const int kvh = blockIdx.x % nkv, split = blockIdx.y;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // tiles in reverse: those late in a sequence have the most positions and start first
-    const PagedTile tl = paged_tile(a, (int)(gridDim.x / nkv) - 1 - (int)(blockIdx.x / nkv));
-    const int64_t slot = (int64_t)tl.index * nkv + kvh;
-    const PagedSeq q = tl.q;
-    if (a.ps > 1 && split == 0 && tid == 0 && (tl.s < 0 || !q.ok)) a.info[slot].used = 0;
-    if (tl.s < 0) return;
-    const int s = tl.s, r0 = tl.r0, R = min(PRO_ROWS, q.n * G - r0);
-    if (!q.ok) {
-        if (split == 0)
-            for (int64_t i = tid; i < (int64_t)R * HD; i += 256) {
-                const int r = r0 + (int)(i / HD), x = (int)(i % HD);
-                a.o[(q.t0 + r / G) * a.ldo + (int64_t)(kvh * G + r % G) * HD + x] = __builtin_nanf("");
-            }
-        return;
-    }
-    const int prefix = paged_prefix(a, s, q);
-    const PagedSpan sp = paged_span(a, q, prefix, r0 / G, (r0 + R - 1) / G);
-    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, a.pleast);
-    if (split >= ch.used) return;
-    if (a.ps > 1 && split == 0 && tid == 0) a.info[slot] = PagedSlot{ch.used, R, q.t0, r0};
-    const int ubase = sp.lo & ~(PRO_UNIT - 1);  // the split's positions k0 .. k1, whole units but for the range's ends
-    const int k0 = max(sp.lo & ~(KT - 1), ubase + split * ch.per * PRO_UNIT), k1 = min(sp.hi, ubase + (split + 1) * ch.per * PRO_UNIT - 1);
-
-    // this lane's row: column lane % 32 of the wavefront's products
-    const int half = lane >> 5, wr = wave * 32 + (lane & 31);
-    const bool mine = wr < R;
-    const int row = r0 + (mine ? wr : 0), tok = row / G, head = kvh * G + row - tok * G;
-    const int pos = q.len - q.n + tok;
-    const int lo = mine ? row_lo(a, pos) : 0x7fffffff, hi = mine ? max(pos, prefix - 1) : -1;
-
-    const int mask = (1 << a.p.shift) - 1;
-    const int32_t *table = a.p.table + (int64_t)s * a.p.table_stride;
-    // a tile's pages, one entry for 16 positions (past the range its last): lane e asks for entry e, one tile ahead
-    constexpr int NE = KT / 16;
-    int ent = 0;
-    auto pages = [&](int kb) { ent = table[min(kb + 16 * min(lane, NE - 1), sp.hi) >> a.p.shift]; };
-    const int64_t hsize = (int64_t)kvh * HD << a.p.shift;
-    uint32_t gone_next = 0;
-    auto load = [&](int kb, uint8_t *buf) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));  // the lanes' offsets are formed for every tile, not kept
-        int64_t hb[NE];  // the entries' K / V head blocks
-        gone_next = 0;   // 16-position blocks whose page does not exist
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            const int page = __builtin_amdgcn_readlane(ent, e);
-            const bool ok = paged_ok(a.p, page);
-            hb[e] = (ok ? page : 0) * a.p.page_stride + hsize;
-            gone_next |= ok ? 0u : 1u << e;
-        }
-        // K: this wavefront's KT / 4 LDS rows, positions of one 16-block
-        const int kr0 = wave * (KT / 4), kblk = kr0 & ~15;
-        int64_t hk = hb[0];
-#pragma unroll
-        for (int e = 1; e < NE; ++e) hk = kblk == 16 * e ? hb[e] : hk;
-        const uint8_t *kp = a.p.k + (hk + (int64_t)((kb + kblk) & mask) * HD) * ES;
-#pragma unroll
-        for (int i = 0; i < P::KL; ++i) {
-            const int r = kr0 + i * (64 / P::KW) + ln / P::KW, w = ln % P::KW ^ turn<P::KW>(r);
-            if (P::KD == P::KW || w < P::KD)
-                lds_load16(kp + (uint32_t)(swap_rows(r & 15) * HD * ES + w * 16), buf + kr0 * P::KW * 16 + i * 1024);
-        }
-        // V^T: loads wave, wave + 4, ..
-        constexpr int VR = 64 / P::VW;  // rows a load
-        const int vr = wave * VR + ln / P::VW, j = (ln % P::VW ^ turn<P::VW>(vr)) * (16 / ES);
-        int64_t hv = hb[0];
-#pragma unroll
-        for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
-        const uint8_t *vp = a.p.v + (hv + ((int64_t)vr << a.p.shift) + ((kb + j) & mask)) * ES;
-#pragma unroll
-        for (int i = 0; i < (P::VL + 3) / 4; ++i)  // 4 VR rows on: the same turn
-            if (P::VL % 4 == 0 || wave + 4 * i < P::VL)
-                lds_load16(vp + (((uint32_t)(4 * VR * i) << a.p.shift) * ES), buf + P::KBYTES + (wave + 4 * i) * 1024);
-    };
-    int kb = k0;
-    pages(kb);
-    // q rows come in pieces of 32 values, 8 lanes a row, and change places in this wavefront's 4 KB of the second
-    // buffer; so do the outputs. (A lane's own row straight from memory, 16 bytes of 32 rows a load, took 64 cycles a load.)
-    uint8_t *own = lds + wave * 4096 + (2 * P::BYTES - 16384);
-    struct Place {
-        int64_t tok;
-        uint32_t head;
-    };
-    auto place = [&](int r) {  // row r of this wavefront in q and o (past the last: the last)
-        const int z = r0 + min(wave * 32 + r, R - 1), t = z / G;
-        return Place{q.t0 + t, (uint32_t)((kvh * G + z - t * G) * HD)};
-    };
-    constexpr int QP = (HD + 31) / 32;
-    pf4 qv[QP][4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int rr = lane >> 3, rw = lane & 7;
-        const Place at = place(8 * u + rr);
-        const float *src = a.q + at.tok * a.ldq + at.head + 4 * rw;
-#pragma unroll
-        for (int g = 0; g < QP; ++g) qv[g][u] = *(const pf4 *)(src + (HD % 32 != 0 && g == QP - 1 && rw >= HD % 32 / 4 ? 0 : 32 * g));
-    }
-    load(kb, lds);
-    uint32_t gone = gone_next;
-    if (kb + KT <= k1) pages(kb + KT);
-
-    pu4 qp[P::KS][P::NQ];
-    PagedScore score;
-    {
-        float size = 1.0f;
-        if constexpr (TYPE == T_F16) {  // the rows' largest magnitudes
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float m = 0.0f;
-#pragma unroll
-                for (int g = 0; g < QP; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(qv[g][u][e]));
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-                ((float *)own)[8 * u + (lane >> 3)] = m;
-            }
-            size = row_size(((const float *)own)[lane & 31]);
-        }
-        const float inv = (a.scale < 0.0f ? -1.0f : 1.0f) / size;
-#pragma unroll
-        for (int g = 0; g < QP; ++g) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) *(pf4 *)(own + (8 * u + (lane >> 3)) * 128 + ((lane ^ lane >> 3) & 7) * 16) = qv[g][u];
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (2 * g + k < P::KS) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const pf4 z = *(const pf4 *)(own + (lane & 31) * 128 + ((4 * k + 2 * half + e) ^ (lane & 7)) * 16);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[4 * e + i] = mine ? z[i] * inv : 0.0f;
-                    }
-                    parts8<TYPE, P::NQ>(x, qp[2 * g + k]);
-                }
-        }
-        score = paged_score(a, head, size);
-    }
-
-    pf16 acc[P::VB];
-#pragma unroll
-    for (int b = 0; b < P::VB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
-    float c = __FLT_MAX__, l = 0.0f;
-
-    // where this lane's words are: the K row it gives, and the V^T row; word w of either at (place ^ 16 w)
-    const uint32_t k_at = (lane & 31) * P::KW * 16 + ((half * W) ^ turn<P::KW>(lane & 31)) * 16;
-    const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31)) * 16;
-    const int first = max(sp.lo, k0), last = min(sp.hi, k1);  // the positions that count here
-
-    // A tile in blocks of 32 positions, h: scores S(h), weights W(h), sums. The products of S(1) are issued among the
-    // vector instructions of W(0), and those of the sums over block 0 among W(1)'s: a product takes the matrix pipe for 32 cycles, in which
-    // the wavefront can issue 8 vector instructions.
-    constexpr int NH = KT / 32, AHEAD = 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
-    struct Weights {
-        float v[2][8];  // scores, then weights, of this lane's positions 16 kk + 8 half + e of the block
-        float mul;
-        pu4 pp[2][P::NQ];
-    };
-    // weight e, and the parts of two
-    auto weigh = [&](Weights &w, int e) {
-        float &v = w.v[e / 8][e % 8];
-        v = __builtin_amdgcn_exp2f(__builtin_fmaf(v, w.mul, c));
-        l += v;
-        asm volatile("" : "+v"(v), "+v"(l));  // here, not where they are used
-        if (e % 2 == 1) {
-            parts2<TYPE, P::NQ>(w.v[e / 8][e % 8 - 1], v, e % 8 / 2, w.pp[e / 8]);
-#pragma unroll
-            for (int i = 0; i < P::NQ; ++i) {
-                uint32_t z = w.pp[e / 8][i][e % 8 / 2];
-                asm volatile("" : "+v"(z));
-                w.pp[e / 8][i][e % 8 / 2] = z;
-            }
-        }
-    };
-    // the scores' forms, and what of them is not seen; the row's reference follows them. False: it does not have to.
-    auto forms = [&](Weights &w, int j, bool whole, bool plain) {
-        w.mul = score.mul;
-        if (!plain) {
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                const int j0 = j + kk * 16 + half * 8;
-                w.mul = score.apply(w.v[kk], j0, pos);
-                const bool no = gone >> ((j0 - kb) >> 4) & 1;
-                const int l0 = max(lo, first) - j0, h0 = min(hi, last) - j0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (no) w.v[kk][e] = __builtin_nanf("");
-                    if (!whole && (e < l0 || e > h0)) w.v[kk][e] = -__builtin_inff();
-                }
-            }
-        }
-        float top = w.v[0][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, w.v[e / 8][e % 8]);
-        return top * w.mul;
-    };
-    // the row's reference follows a larger score, in whole powers of two; the factor of what was formed before
-    auto follow = [&](float top) {
-        const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
-        float f = 1.0f;
-        if (mx + c > PTOP) {
-            const float cn = PBIAS - ceilf(mx);
-            f = __builtin_amdgcn_exp2f(cn - c);
-            c = cn;
-            l *= f;
-#pragma unroll
-            for (int b = 0; b < P::VB; ++b) acc[b] *= f;
-        }
-        return f;
-    };
-    auto tile = [&](const uint8_t *buf, bool whole, bool plain) {
-        uint32_t k_lane = k_at, v_lane = v_at;
-        asm volatile("" : "+v"(k_lane), "+v"(v_lane));  // the words' places are formed where they are read, not kept
-        pu4 raw[SLOTS][W];
-        auto read_k = [&](int h, int ks) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) raw[ks % SLOTS][w] = *(const pu4 *)(buf + (k_lane ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
-        };
-        auto read_v = [&](int x) {  // x: 16-position run, then block of values
-            const int k = x / P::VB, b = x % P::VB;
-#pragma unroll
-            for (int w = 0; w < W; ++w) raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ (2 * k * W + w) * 16) + b * 32 * P::VW * 16);
-        };
-        constexpr int NPROD = PagedType<TYPE>::NPROD;
-        auto beside = [&](int m, int of, auto side) {  // product m of `of`: its share of the 16 weights beside it
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (e >= m * 16 / of && e < (m + 1) * 16 / of) side(e);
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        auto scores = [&](int h, Weights &out, auto side) {
-            int m = 0;
-            pf16 sc;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < AHEAD; ++ks) read_k(h, ks);
-#pragma unroll
-            for (int ks = 0; ks < P::KS; ++ks) {
-                if (ks + AHEAD < P::KS) read_k(h, ks + AHEAD);
-                pu4 kp[P::NK];
-                cache8<TYPE>(raw[ks % SLOTS], kp);
-#pragma unroll
-                for (int x = P::NQ - 1; x >= 0; --x)
-#pragma unroll
-                    for (int y = P::NK - 1; y >= 0; --y)
-                        if (x + y < 3) {
-                            mma32<TYPE>(sc, kp[y], qp[ks][x]);
-                            beside(m++, P::KS * NPROD, side);
-                        }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = sc[e];
-        };
-        constexpr int NX = 2 * P::VB;  // V words of a block
-        auto sums = [&](int h, const Weights &w, auto side) {
-            int m = 0;
-#pragma unroll
-            for (int x = 0; x < NX; ++x) {
-                if (h * NX + x + AHEAD < NH * NX) read_v(h * NX + x + AHEAD);
-                pu4 vp[P::NK];
-                cache8<TYPE>(raw[(h * NX + x) % SLOTS], vp);
-#pragma unroll
-                for (int i = P::NQ - 1; i >= 0; --i)
-#pragma unroll
-                    for (int y = P::NK - 1; y >= 0; --y)
-                        if (i + y < 3) {
-                            mma32<TYPE>(acc[x % P::VB], vp[y], w.pp[x / P::VB][i]);
-                            beside(m++, NX * NPROD, side);
-                        }
-            }
-        };
-        auto first_v = [&]() {
-#pragma unroll
-            for (int x = 0; x < AHEAD; ++x) read_v(x);
-        };
-        Weights w0;
-        auto alone = [](int) {};
-        scores(0, w0, alone);
-        if constexpr (NH == 1) first_v();
-        const float top0 = forms(w0, kb, whole, plain);
-        if (__builtin_amdgcn_ballot_w64(top0 + c > PTOP)) follow(top0);
-        if constexpr (NH == 1) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) weigh(w0, e);
-            sums(0, w0, alone);
-        } else {
-            Weights w1;
-            scores(1, w1, [&](int e) { weigh(w0, e); });
-            first_v();
-            const float top1 = forms(w1, kb + 32, whole, plain);
-            if (__builtin_amdgcn_ballot_w64(top1 + c > PTOP)) {  // block 0's weights wait for their sums
-                const float f = follow(top1);
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                    for (int i = 0; i < P::NQ; ++i) scale8<TYPE>(w0.pp[kk][i], f);
-            }
-            sums(0, w0, [&](int e) { weigh(w1, e); });
-            sums(1, w1, alone);
-        }
-    };
-
-    for (int n = 0; kb <= k1; kb += KT, n ^= 1) {
-        uint8_t *buf = lds + n * P::BYTES;
-        __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt 0: this wavefront's part of the tile is in LDS
-        __syncthreads();                    // everyone's is, and the other buffer has been read
-        if (kb + KT <= k1) {
-            load(kb + KT, lds + (n ^ 1) * P::BYTES);
-            if (kb + 2 * KT <= k1) pages(kb + 2 * KT);
-        }
-        const bool whole = kb >= max(sp.in_lo, k0) && kb + KT - 1 <= min(sp.in_hi, k1) && gone == 0;  // seen by every row
-        uint64_t odd = 0;
-        if (!whole) {
-            // V values at positions that no row sees become zeros, and so do those that are not finite: what only some of
-            // the rows see must not reach the others by way of 0 x NaN. The rows that see them get them below.
-            if (tid < 2) odd_l[tid] = 0;
-            __syncthreads();
-            for (int x = tid; x < HD * P::VW; x += 256) {
-                const int r = x / P::VW, at = x % P::VW, j = (at ^ turn<P::VW>(r)) * (16 / ES);
-                pu4 *word = (pu4 *)(buf + P::KBYTES + (r * P::VW + at) * 16);
-                // of the word's values (all in one page): from .. to - 1 are seen by some row
-                constexpr int N = 16 / ES;
-                const bool none = gone >> (j / 16) & 1;
-                const int from = none ? N : min(max(first - kb - j, 0), N), to = min(max(last + 1 - kb - j, 0), N);
-                pu4 v = *word;
-                uint32_t inf = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (ES == 4) v[i] = i >= from && i < to ? v[i] : 0u;
-                    else v[i] &= (2 * i >= from && 2 * i < to ? 0x0000ffffu : 0u) | (2 * i + 1 >= from && 2 * i + 1 < to ? 0xffff0000u : 0u);
-                    inf |= infinite<TYPE>(v[i]);
-                }
-                if (inf) {  // rare
-                    uint32_t bad = 0;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) bad |= raw_bad<TYPE>(&v, e) ? 1u << e : 0u;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = finite_only<TYPE>(v[i]);
-                    atomicOr(&odd_l[j / 32], bad << (j & 31));
-                }
-                if (inf || from > 0 || to < N) *word = v;
-            }
-            __syncthreads();
-            odd = (uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[0]) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)odd_l[1]) << 32;
-        }
-        const bool plain = whole && !(score.cap_out > 0.0f) && !score.bias;
-        tile(buf, whole, plain);
-        while (odd) {
-            const int j = kb + __builtin_ctzll(odd);
-            odd &= odd - 1;
-            int shift = a.p.shift;
-            asm volatile("" : "+s"(shift));  // this rare path must not cost registers: no addresses formed ahead,
-            const int64_t at = paged_head(a.p, table[j >> shift], kvh) + (j & mask) + ((int64_t)(4 * half) << shift);
-#pragma unroll
-            for (int b = 0; b < P::VB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * b + 8 * (r / 4) + r % 4;
-                    if (HD % 32 == 0 || d + 4 * half < HD) {
-                        const float z = cached<TYPE>(a.p.v, at + ((int64_t)d << shift));
-                        if (not_finite(z) && j >= lo && j <= hi) acc[b][r] += z;
-                        asm volatile("" : "+s"(shift)::"memory");  // and one value at a time
-                    }
-                }
-        }
-        gone = gone_next;
-    }
-    l += __shfl_xor(l, 32, 64);
-    if (ch.used > 1) {  // sums as the lanes hold them
-        if (wave * 32 >= R) return;
-        pf4 *part = (pf4 *)a.part + ((slot * a.ps + split) * 4 + wave) * (P::VB * 4 * 64) + lane;
-#pragma unroll
-        for (int b = 0; b < P::VB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                part[(4 * b + i) * 64] = pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-        if (half == 0) *(pf2 *)(a.stat + ((slot * a.ps + split) * PRO_ROWS + wr) * 2) = pf2{c, l};
-        return;
-    }
-    __syncthreads();  // the buffers have been read
-    const float inv = 1.0f / l;
-    int ln = lane;
-    asm volatile("" : "+v"(ln));  // the rows' places are formed again rather than kept
-    const int rr = ln >> 3, rw = ln & 7;
-    Place at[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) at[u] = place(8 * u + rr);
-#pragma unroll
-    for (int b = 0; b < P::VB; ++b) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *(pf4 *)(own + (lane & 31) * 128 + ((2 * i + half) ^ (lane & 7)) * 16) =
-                pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]} * inv;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const pf4 z = *(const pf4 *)(own + (8 * u + rr) * 128 + (rw ^ rr) * 16);
-            if (wave * 32 + 8 * u + rr < R && (HD % 32 == 0 || 32 * b + 4 * rw < HD))
-                *(pf4 *)(a.o + at[u].tok * a.ldo + at[u].head + 32 * b + 4 * rw) = z;
-        }
-    }
+    // grid (tiles x K / V heads, prompt splits and what the decode workgroups need)
+    const int block = blockIdx.x, y = blockIdx.y, d = (y - a.ps) * (int)gridDim.x + block;
+    if (y < a.ps) paged_prompt_block<TYPE, HD>(a, block, gridDim.x, y, lds);
+    else if (d < nd) paged_decode_block<TYPE, HD>(a, d, lds);
 }
 
 template <int TYPE, int HD>
 hipError_t launch_one(const PagedAttnArgs &a, hipStream_t s) {
-    constexpr int bytes = 2 * Pro<TYPE, HD>::BYTES;
-    paged_prompt_kernel<TYPE, HD><<<dim3((unsigned)(paged_tiles(a) * a.p.n_head_kv), (unsigned)a.ps), 256, bytes, s>>>(a);
+    constexpr int pro = 2 * Pro<TYPE, HD>::BYTES + 16, bytes = pro > dec_lds(HD) ? pro : dec_lds(HD);
+    const int x = (int)paged_tiles(a) * a.p.n_head_kv, nd = a.p.n_seq * a.ds * a.p.n_head_kv;
+    paged_prompt_kernel<TYPE, HD><<<dim3((unsigned)x, (unsigned)(a.ps + (nd + x - 1) / x)), 256, bytes, s>>>(a, nd);
     return hipGetLastError();
 }
 template <int TYPE>
