@@ -32,8 +32,9 @@ SOURCES = ["fgh_api.hip", "fgh_kernels.hip", "fgh_matvec.hip", "fgh_q4k.hip", "f
            "fgh_gemm32n.hip", "fgh_gemm6.hip", "fgh_moe.hip", "fgh_gguf.hip", "fgh_attn.hip", "fgh_kvq.hip",
            "fgh_kq.hip", "fgh_float.hip", "fgh_rowg.hip", "fgh_paged.hip", "fgh_pattn.hip", "fgh_pdecode.hip", "fgh_pprompt.hip"]
 # per-source additions: the nibble-type GEMM converts every MFMA result with a VALU instruction, so
-# its results go to VGPRs (without the flag the compiler writes them to AGPRs and copies each out)
-FILE_FLAGS = {"fgh_gemm32n.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "fgh_moemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# its results go to VGPRs (without the flag the compiler writes them to AGPRs and copies each out);
+# so do the paged attention's scores, and at hd 256 its q parts then fit without spills
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for f in ("fgh_gemm32n.hip", "fgh_moemm.hip", "fgh_pdecode.hip", "fgh_pprompt.hip")}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 
