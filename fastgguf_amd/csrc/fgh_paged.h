@@ -76,8 +76,9 @@ __device__ __forceinline__ PagedVTile paged_vtile(const Paged &a, int index) {
     for (int b = 0; b < a.n_seq; b += 64) {
         const int s = b + lane;
         int own = 0, first = 0;
+        PagedSeq q{};
         if (s < a.n_seq) {
-            const PagedSeq q = paged_seq(a, s);
+            q = paged_seq(a, s);
             first = (q.len - q.n) / 64;
             own = q.n > 0 && q.ok ? (q.len - 1) / 64 - first + 1 : 0;
         }
@@ -91,7 +92,8 @@ __device__ __forceinline__ PagedVTile paged_vtile(const Paged &a, int index) {
             const int at = __builtin_ctzll(m);
             t.s = __builtin_amdgcn_readfirstlane(b + at);
             t.base = __builtin_amdgcn_readfirstlane((__shfl(first, at, 64) + index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * 64);
-            t.q = paged_useq(a, t.s);
+            t.q.t0 = __builtin_amdgcn_readlane(q.t0, at), t.q.n = __builtin_amdgcn_readlane(q.n, at);
+            t.q.len = __builtin_amdgcn_readlane(q.len, at), t.q.ok = true;
             return t;
         }
         before += __shfl(upto, 63, 64);

@@ -228,6 +228,8 @@ __device__ __forceinline__ PagedChunk paged_chunk(int n, int splits, int least) 
 
 constexpr int DEC_ROWS = 16;                // rows of the decode kernel
 constexpr int DEC_STEP = 32;                // positions a step of a wavefront
+// workgroups of the decode kernel that a compute unit holds, by its registers
+constexpr int dec_resident(int type, int hd) { return hd > 128 || (type == T_F32 && hd > 96) ? 1 : 2; }
 // the decode kernel's steps of a range
 __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
 
@@ -251,8 +253,9 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int inde
     for (int b = 0; b < a.p.n_seq; b += 64) {
         const int s = b + lane;
         int own = 0;
+        PagedSeq q{};
         if (s < a.p.n_seq) {
-            const PagedSeq q = paged_seq(a.p, s);
+            q = paged_seq(a.p, s);
             const int64_t rows = (int64_t)q.n * G;
             own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (int)((rows + PRO_ROWS - 1) / PRO_ROWS);
         }
@@ -268,7 +271,8 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int inde
             t.r0 = (index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
             t.s = __builtin_amdgcn_readfirstlane(t.s);
             t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
-            t.q = paged_useq(a.p, t.s);
+            t.q.t0 = __builtin_amdgcn_readlane(q.t0, at), t.q.n = __builtin_amdgcn_readlane(q.n, at);
+            t.q.len = __builtin_amdgcn_readlane(q.len, at), t.q.ok = __builtin_amdgcn_readlane(q.ok, at);
             return t;
         }
         before += __shfl(upto, 63, 64);

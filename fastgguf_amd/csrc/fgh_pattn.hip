@@ -110,8 +110,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int np
 // where they are that many, and its join costs 5 to 20 us (2032 tokens behind 7168, 512 tiles: 600 us whole, 600 + 20 in two
 // splits; seven documents of up to 900 tokens, 252 tiles: 48.7 us whole, 33 + 5 in three). At least 4 units of 64 positions each (256 positions
 // of a tile take about 10 us, the join of a few splits 5), at most 8 splits: 64 tokens over 4096 positions take 28 + 5 us in 8, 27 + 7 in 16.
-// Decode: the same twice over, of 4 steps and more, a step for every wavefront; up to eight times over where that leaves 16 steps
-// each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take 137 us in 2 splits, 110 in 8, and 32 of 1024
+// Decode: what fits at once too, of 4 steps and more, a step for every wavefront (4 sequences of 3000 positions at hd 256, of which one workgroup
+// fits a compute unit: 21.5 us in 256 workgroups, 28.8 in 512); up to eight for every compute unit where that leaves 16 steps each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take 137 us in 2 splits, 110 in 8, and 32 of 1024
 // 27 in 2, 35 in 8. At most 64, which is what the join holds. The bounds may be far above the lengths: the kernels split what is there.
 PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
     const int G = a.n_head / a.p.n_head_kv;
@@ -130,7 +130,7 @@ PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
     }
     if (a.ps == 0 || a.p.n_seq > 1) {
         const int64_t steps = seen / DEC_STEP + 1;
-        const int64_t even = std::min<int64_t>(2 * (int64_t)num_cu / heads, (steps + 3) / 4), more = std::min<int64_t>(8 * (int64_t)num_cu / heads, steps / 16);
+        const int64_t even = std::min<int64_t>(dec_resident(a.p.type, a.p.hd) * (int64_t)num_cu / heads, (steps + 3) / 4), more = std::min<int64_t>(8 * (int64_t)num_cu / heads, steps / 16);
         a.ds = (int)std::min<int64_t>(64, std::max<int64_t>({1, even, more}));
         if (a.ds > 1) n.dslot = (size_t)heads, n.drow = n.dslot * a.ds * a.drows, n.dpart = n.drow * a.p.hd;
     }

@@ -21,7 +21,7 @@ struct Dec {
     static constexpr int W = ES / 2;             // 16-byte words of 8 values
     static constexpr int KS = (HD + 31) / 32;    // steps of 32 along the head
     static constexpr int VB = HD / 16;           // blocks of 16 of V's values
-    static constexpr int OCC = TYPE == T_F32 || HD > 128 ? 1 : 2;
+    static constexpr int OCC = dec_resident(TYPE, HD);
 };
 
 constexpr int dec_lds(int hd) { return (4 * DEC_ROWS * (hd + 4) + 8 * DEC_ROWS) * 4; }

@@ -209,7 +209,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     // A tile in blocks of 32 positions, h: scores S(h), weights W(h), sums. The products of S(1) are issued among the
     // vector instructions of W(0), and those of the sums over block 0 among W(1)'s: a product takes the matrix pipe for 32 cycles, in which
     // the wavefront can issue 8 vector instructions.
-    constexpr int NH = KT / 32, AHEAD = 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
+    constexpr int NH = KT / 32, AHEAD = P::NQ > 2 ? 2 : 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
     struct Weights {
         float v[2][8];  // scores, then weights, of this lane's positions 16 kk + 8 half + e of the block
         float mul;
