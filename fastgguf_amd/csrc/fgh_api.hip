@@ -991,15 +991,20 @@ static const char *paged_check(const fgh_paged_cache *c, const fgh_paged_batch *
     if (c->hd != 64 && c->hd != 80 && c->hd != 96 && c->hd != 128 && c->hd != 256) return "hd is not 64, 80, 96, 128 or 256";
     if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return "page is not a power of 2 from 16 to 256";
     if (c->n_pages < 1 || c->table_stride < 1 || c->n_head_kv < 1 || c->n_head_kv > 4096) return "bad n_pages, table_stride or n_head_kv";
-    if (c->page_stride != 0 && (c->page_stride < (int64_t)c->n_head_kv * c->page * c->hd || c->page_stride % 8 != 0 || c->page_stride > (int64_t)1 << 40))
-        return "page_stride is smaller than a page or no multiple of 8";
+    if (c->page_stride != 0 && (c->page_stride < (int64_t)c->n_head_kv * c->page * c->hd || c->page_stride % 8 != 0 || c->page_stride > ((int64_t)1 << 48) / c->n_pages))
+        return "page_stride is smaller than a page, no multiple of 8 or too large";
     if (b->n_seq < 1 || b->n_seq > 65535 || b->n_tok < 1 || b->max_tok < 1 || b->max_len < 1) return "bad n_seq, n_tok, max_tok or max_len";
     if (n_head < (m ? 1 : 0) || n_head > 65535 / 4) return "bad n_head";
-    if ((n_head > 0 && (ldq < (int64_t)n_head * c->hd || ldo < (int64_t)n_head * c->hd)) || ldq % 4 != 0 || ldo % 4 != 0)
-        return "ldq or ldo is smaller than a row or no multiple of 4";
-    if (ldq > (int64_t)1 << 31 || ldo > (int64_t)1 << 31 || ldkv > (int64_t)1 << 31) return "a stride is too large";
+    if (n_head > 0) {
+        if (ldq < (int64_t)n_head * c->hd || ldo < (int64_t)n_head * c->hd || ldq % 4 != 0 || ldo % 4 != 0)
+            return "ldq or ldo is smaller than a row or no multiple of 4";
+        if (ldq > (int64_t)1 << 31 || ldo > (int64_t)1 << 31) return "ldq or ldo is too large";
+    }
     if (r) {
-        if (ldkv < (int64_t)c->n_head_kv * c->hd || ldkv % 4 != 0) return "ldkv is smaller than a row or no multiple of 4";
+        if (ldkv < (int64_t)c->n_head_kv * c->hd || ldkv % 4 != 0 || ldkv > (int64_t)1 << 31)
+            return "ldkv is smaller than a row, no multiple of 4 or too large";
+        if (fgh::paged_vtiles(b->n_tok, b->n_seq) * c->n_head_kv + (int64_t)b->n_tok + 65536 > fgh::PAGED_GRID)  // a few for every compute unit besides
+            return "too many rows, sequences or K / V heads";
         if (r->n_rot < 0 || r->n_rot > c->hd || r->n_rot % 2 != 0) return "n_rot is odd or not 0 .. hd";
         if (r->rope != FGH_ROPE_PAIRS && r->rope != FGH_ROPE_HALVES) return "unknown rope";
         if (r->n_rot > 0 && !(r->freq_base > 0.0f && r->freq_base <= FLT_MAX && r->freq_scale > 0.0f && r->freq_scale <= FLT_MAX))
@@ -1008,9 +1013,12 @@ static const char *paged_check(const fgh_paged_cache *c, const fgh_paged_batch *
     }
     if (m) {
         if (n_head % c->n_head_kv != 0) return "n_head is no multiple of n_head_kv";
-        if (!(fabsf(m->scale) <= FLT_MAX) || !(m->softcap >= 0.0f && m->softcap <= FLT_MAX) || m->window < 0)
-            return "scale, softcap or window is negative or not finite";
-        if ((int64_t)b->n_tok * (n_head / c->n_head_kv) > INT32_MAX / 2) return "too many rows";
+        if (!(fabsf(m->scale) <= 1e15f)) return "scale is not -1e15 .. 1e15";
+        if (m->softcap != 0.0f && !(m->softcap >= 1e-15f && m->softcap <= 1e15f)) return "softcap is not 0 or 1e-15 .. 1e15";
+        if (m->window < 0) return "window is negative";
+        const int G = n_head / c->n_head_kv;
+        if ((int64_t)b->n_tok * G > INT32_MAX / 2) return "too many rows";
+        if (fgh::paged_tiles(b->n_tok, b->n_seq, G) * c->n_head_kv > fgh::PAGED_GRID) return "too many rows, sequences or K / V heads";
     }
     return nullptr;
 }
@@ -1030,7 +1038,7 @@ int fgh_paged_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fg
     return why ? FGH_ERR_ARG : FGH_OK;
 }
 int64_t fgh_paged_slot(const fgh_paged_cache *c, const int32_t *table, int s, int pos, int kvh, int d, int is_v) {
-    if (!c || !table || c->page < 16 || s < 0 || pos < 0 || pos >= (int64_t)c->table_stride * c->page || kvh < 0 || kvh >= c->n_head_kv || d < 0 || d >= c->hd) return -1;
+    if (!c || !table || c->page < 16 || (c->page & (c->page - 1)) || s < 0 || pos < 0 || pos >= (int64_t)c->table_stride * c->page || kvh < 0 || kvh >= c->n_head_kv || d < 0 || d >= c->hd) return -1;
     const fgh_paged_batch b{};
     const fgh::Paged p = paged_args(c, &b);
     const int page = table[(int64_t)s * p.table_stride + (pos >> p.shift)], in = pos & ((1 << p.shift) - 1);

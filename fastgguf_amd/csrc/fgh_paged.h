@@ -62,6 +62,10 @@ __device__ __forceinline__ int paged_find(const Paged &a, int t) {
     return s >= a.n_seq ? -1 : s;
 }
 
+// a launch's workgroups of 256: HIP takes up to 2^32 - 1 threads
+constexpr int64_t PAGED_GRID = (1 << 24) - 1;
+// at most as many tiles as sequences' new tokens can have: of n, n / 64 whole ones and two ends
+inline int64_t paged_vtiles(int64_t n_tok, int64_t n_seq) { return n_tok / 64 + 2 * std::min(n_seq, n_tok); }
 // A sequence's part of the batch in 64 positions from `base`, a multiple of 64: tile `index` of the sequences' tiles in
 // order. s = -1: there are fewer.
 struct PagedVTile {
@@ -142,6 +146,9 @@ struct PagedAttnArgs {
     int ds, ps, drows, dleast, pleast;
     PagedSums dsum, psum;
 };
+constexpr int PRO_ROWS = 128;  // rows of a workgroup of the prompt kernel
+// at most as many tiles of that many rows as a batch's sequences can have, per K / V head (G rows a token)
+inline int64_t paged_tiles(int64_t n_tok, int64_t n_seq, int G) { return n_tok * G / PRO_ROWS + n_seq; }
 struct PagedScratch {
     size_t dpart, ppart, drow, prow, dslot, pslot;  // floats of part, rows of stat, slots of info
     size_t bytes() const { return (dslot + pslot) * sizeof(PagedSlot) + (drow + prow) * 8 + (dpart + ppart) * 4; }

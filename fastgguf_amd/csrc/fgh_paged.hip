@@ -55,6 +55,7 @@ __device__ __forceinline__ void store_heads(const PagedStoreArgs &a, int t, int 
     const int s = paged_find(a.p, t);
     if (s < 0) return;
     const PagedSeq sq = paged_useq(a.p, s);
+    if ((uint32_t)(t - sq.t0) >= (uint32_t)sq.n) return;  // starts that decrease
     const int pos = sq.len - sq.n + (t - sq.t0);
     if (!sq.ok) {
         for (; in && h < min(end, a.n_head); h += step)
@@ -89,8 +90,10 @@ __device__ __forceinline__ void store_heads(const PagedStoreArgs &a, int t, int 
             } else {
                 float *sum = (float *)rows;
                 sum[lane] = ss;
+                __builtin_amdgcn_wave_barrier();  // LDS serves a wavefront in order: only the compiler must keep it
                 ss = 0.0f;
                 for (int i = 0; i < lanes; ++i) ss += sum[in ? mine * lanes + i : 0];
+                __builtin_amdgcn_wave_barrier();
             }
             const float r = 1.0f / sqrtf(ss / (float)hd + a.r.eps);
             if (norm) y = y * r * (isq ? wq : wk);
@@ -99,10 +102,12 @@ __device__ __forceinline__ void store_heads(const PagedStoreArgs &a, int t, int 
             sf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
             if (a.r.halves) {
                 rows[lane] = y;
+                __builtin_amdgcn_wave_barrier();
                 const float *row = (const float *)(rows + mine * lanes);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (in && x + e < a.r.n_rot) o[e] = row[x + e < half ? x + e + half : x + e - half];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (x + e < a.r.n_rot) {
@@ -198,10 +203,8 @@ hipError_t launch_paged_store(PagedStoreArgs &a, int num_cu, hipStream_t s) {
     a.parts = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * (int64_t)num_cu / a.p.n_tok));
     a.heads_part = ((heads + a.parts - 1) / a.parts + at_once - 1) / at_once * at_once;
     a.parts = (heads + a.heads_part - 1) / a.heads_part;
-    // at most as many tiles as the sequences can have: each n tokens, n / 64 whole ones and two ends
-    a.v_tiles = a.p.n_tok / STORE_V_POS + 2 * std::min(a.p.n_seq, a.p.n_tok);
+    a.v_tiles = (int)paged_vtiles(a.p.n_tok, a.p.n_seq);
     const int64_t grid = (int64_t)a.v_tiles * a.p.n_head_kv + (int64_t)a.p.n_tok * a.parts;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
     switch (a.p.type) {
     case T_F32: return launch_type<T_F32>(a, (unsigned)grid, s);
     case T_F16: return launch_type<T_F16>(a, (unsigned)grid, s);

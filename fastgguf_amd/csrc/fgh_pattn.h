@@ -5,8 +5,8 @@
 //   F16 cache   q and the weights as 2 halves (22 bits); K and V as they are: 2 products
 //   BF16 cache  q and the weights as 3 bf16, cut so that they hold all 24 bits; 3 products
 //   F32 cache   K and V too as 3 bf16; the 6 products down to 2^-16 of the largest (the 3 left out are below 2^-24)
-// Halves have 5 bits of exponent, so q rows are brought to [1, 2) by a power of two (the scores take it
-// back with the scale), and the weights, 0 .. 1 beside the largest, are carried times 2^10 (PBIAS): down to 2^-24 of the
+// Halves have 5 bits of exponent, so a q row's largest value is brought to [2^14, 2^15) by a power of two (the scores take it
+// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the weights, 0 .. 1 beside the largest, are carried times 2^10 (PBIAS): down to 2^-24 of the
 // largest both of a weight's halves are then normal numbers.
 #pragma once
 
@@ -197,11 +197,11 @@ __device__ __forceinline__ PagedScore paged_score(const PagedAttnArgs &a, int he
     return c;
 }
 
-// the power of two that brings a row's largest magnitude to [1, 2), as the factor that undoes it (amax 0 or
-// not finite: 1)
+// the power of two that brings a row's largest magnitude to [2^14, 2^15), or as near as 2^126 does, as the factor that undoes
+// it (amax not finite: 1)
 __device__ __forceinline__ float row_size(float amax) {
     const uint32_t e = __float_as_uint(amax) >> 23;
-    return e >= 1 && e <= 252 ? __uint_as_float(e << 23) : 1.0f;
+    return e == 255 ? 1.0f : __uint_as_float((e > 15 ? e - 14 : 1u) << 23);
 }
 
 // positions lo .. hi that the new tokens i0 .. i1 of a sequence see, and those that all of them see
@@ -214,7 +214,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs &a, const Pa
     return PagedSpan{row_lo(a, p0), max(p1, prefix - 1), row_lo(a, p1), max(p0, prefix - 1)};
 }
 __device__ __forceinline__ int paged_prefix(const PagedAttnArgs &a, int s, const PagedSeq &q) {
-    return a.prefix ? min(__builtin_amdgcn_readfirstlane(a.prefix[s]), q.len) : 0;  // s: uniform
+    return a.prefix ? min(max(__builtin_amdgcn_readfirstlane(a.prefix[s]), 0), q.len) : 0;  // s: uniform
 }
 // a range of n units over at most `splits` workgroups, `least` units or more each: the units of one, and how many
 // workgroups have any
@@ -233,13 +233,9 @@ constexpr int dec_resident(int type, int hd) { return hd > 128 || (type == T_F32
 // the decode kernel's steps of a range
 __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
 
-constexpr int PRO_ROWS = 128;               // rows of a workgroup of the prompt kernel
 constexpr int PRO_UNIT = 64;                // positions are split in units of 64
 __device__ __forceinline__ int pro_units(const PagedSpan &r) { return (r.hi - (r.lo & ~(PRO_UNIT - 1))) / PRO_UNIT + 1; }
-// at most as many tiles of PRO_ROWS rows as a batch's sequences can have, per K / V head
-inline int64_t paged_tiles(const PagedAttnArgs &a) {
-    return (int64_t)a.p.n_tok * (a.n_head / a.p.n_head_kv) / PRO_ROWS + a.p.n_seq;
-}
+inline int64_t paged_tiles(const PagedAttnArgs &a) { return paged_tiles(a.p.n_tok, a.p.n_seq, a.n_head / a.p.n_head_kv); }
 // Tile `index` of the batch: the sequences' tiles in order (of those that are the prompt kernel's). s = -1: there are fewer.
 struct PagedTile {
     int s, r0, index;

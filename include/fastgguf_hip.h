@@ -281,7 +281,8 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * stand between the QKV and the O projection of a layer: the append of a batch's keys and values
  * with the head norms and the position rotation (the reference's rope, for GGUF's rope types), and
  * the attention over the pages. Activations are fp32, as everywhere here; results agree with the
- * formulas to within 1e-5 relative per output vector. Both calls are asynchronous on the context's
+ * formulas to within 1e-5 relative per output vector, as long as fp32 scores do (a weight is off by its score's
+ * rounding: scores of hundreds cost as many 2^-24). Both calls are asynchronous on the context's
  * stream and can be captured (the attention's scratch must have its size from an eager call with the same
  * descriptors, or larger ones, before).
  *
@@ -290,7 +291,9 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * Pages start page_stride values apart in k and in v (0: n_head_kv * page * hd). Position j of
  * sequence s is in page table[s * table_stride + j / page], place j % page.
  * Requires hd 64, 80, 96, 128 or 256; page a power of 2 from 16 to 256; k and v 16-byte aligned,
- * page_stride a multiple of 8. Offsets are 64-bit. */
+ * page_stride a multiple of 8. Offsets are 64-bit. At most 16383 heads, 4096 K / V heads, 65535 sequences,
+ * and 2^24 - 1 workgroups a call (append: n_tok + (n_tok / 64 + 2 n_seq) n_head_kv + 65536, attention:
+ * (n_tok n_head / n_head_kv / 128 + n_seq) n_head_kv); more is refused. */
 typedef struct {
     void *k, *v;            /* device */
     const int32_t *table;   /* device, [n_seq][table_stride] */
@@ -305,7 +308,7 @@ typedef struct {
  * sequence's new tokens and length. As these stay on the device, a sequence that breaks a bound
  * (more than max_tok tokens, len above max_len or the table's positions or below its
  * number of tokens, rows outside 0 .. n_tok) is no error: its rows are NaN and nothing is appended.
- * tok is read as non-decreasing. */
+ * tok is read as non-decreasing: rows in two sequences of one that is not hold anything. */
 typedef struct {
     const int32_t *tok;     /* device, [n_seq + 1] */
     const int32_t *len;     /* device, [n_seq] */
@@ -324,7 +327,7 @@ typedef struct {
     int32_t n_rot, rope;
 } fgh_paged_rope;
 /* q: [n_tok][ldq], k and v: [n_tok][ldkv], head h at h * hd (ldq == ldkv and three pointers into one
- * row: a fused QKV projection). q_out: [n_tok][ldo], may be q itself with ldo == ldq. k' and v go to the pages
+ * row: a fused QKV projection). q_out: [n_tok][ldo], may be q itself with ldo == ldq, and else overlaps no input. k' and v go to the pages
  * rounded to nearest even (F16: beyond 65504 to infinity). n_head 0: keys and values only, q and q_out unused.
  * A token whose page is not 0 .. n_pages - 1 appends nothing. No two tokens of a call may share a
  * slot (tables that share a page at positions being written). Pointers 16-byte aligned, strides multiples of 4. */
@@ -338,9 +341,10 @@ FGH_API int fgh_paged_store_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, cons
  * that all tokens see), j < len, and p - j < window (window > 0). Sequences do not see each other, so
  * packed documents are sequences. Pages without a visible position are not read (their table entries may
  * be anything); a row that sees a position whose page is not 0 .. n_pages - 1 is NaN. Values in
- * positions that no row of a sequence sees do not matter, NaN included; a q or k that is not finite
- * makes the rows that see it NaN or finite, a v that is not finite makes them not finite, and other
- * rows stay as they are. len[s] counts the new tokens: append them first.
+ * positions that no row of a sequence sees do not matter, NaN included; with a q or k that is not finite
+ * the rows that see it hold anything, NaN where it is NaN; with a v that is not finite that value of theirs is not finite
+ * either; other rows and values stay as they are. scale: -1e15 .. 1e15; softcap: 0 or 1e-15
+ * .. 1e15. len[s] counts the new tokens: append them first.
  * q: [n_tok][ldq], o: [n_tok][ldo], not overlapping. Pointers 16-byte aligned, strides multiples of 4. */
 typedef struct {
     float scale, softcap;

@@ -182,6 +182,22 @@ def test_store_without_queries(backend):
             assert np.array_equal(vc[b.at(s, pos, h, True)], encode(kv[1, tok, h], T_BF16))
 
 
+def test_store_decreasing_starts(backend):
+    """Starts that decrease: rows of one sequence are appended, rows of two may not be read or written out of range."""
+    b = Batch(10, T_F16, 64, 2, 1, 16, [5, 0, 5], [5, 0, 9])
+    b.tok, b.n_tok = np.array([0, 5, 3, 8], np.int32), 8
+    qkv = b.rng.standard_normal((8, 4, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b, max_tok=5)
+        qd, od = d.put(qkv), d.put(np.full((8, 2, 64), 777.0, np.float32))
+        backend.paged_store_dev(cache, batch, PagedRope(), 2, qd, 256, qd + 512, qd + 768, 256, od, 128)
+        got, kc = d.get(od, np.zeros((8, 2, 64), np.float32)), d.get(cache.k, b.k)
+    for t in (0, 1, 2, 5, 6, 7):
+        assert np.array_equal(got[t], qkv[t, :2])
+        s, pos = (0, t) if t < 3 else (2, 9 - 5 + t - 3)
+        assert np.array_equal(kc[b.at(s, pos, 0, False)], encode(qkv[t, 2], T_F16))
+
+
 def test_store_overflow_and_specials(backend):
     """F16 rounds to nearest even, past 65504 to infinity; NaN stays NaN."""
     b = Batch(9, T_F16, 64, 1, 1, 16, [1], [1])
@@ -357,6 +373,40 @@ def test_attention_ranges(backend, t, tiny, huge, news):
         o = run_attention(backend, b, scale=scale)
         want, tol, _ = attention(b, b.q, float(np.float32(scale)))
         assert (np.abs(o - want) <= tol).all()
+
+
+@pytest.mark.parametrize("news", [1, 40])
+def test_attention_outlier_channels(backend, news):
+    """A channel whose K is large and whose q is small beside the row's others: it counts as much as they do."""
+    b = Batch(48, T_F16, 64, 4, 2, 16, [news], [100])
+    size = np.ones(64)
+    size[7] = 2.0**13
+    for s, m in enumerate(b.lens):
+        for pos in range(m):
+            for h in range(2):
+                at = b.at(s, pos, h, False)
+                b.k[at] = encode(decode(b.k[at], T_F16) * size / 8, T_F16)
+    b.q = (b.q / size).astype(np.float32)
+    check_attention(backend, b)
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [40, 1, 2]])
+def test_attention_prefix_limits(backend, news):
+    """A prefix is taken as 0 .. len, whatever it holds."""
+    b = Batch(49, T_F16, 64, 4, 2, 16, news, [n + 30 for n in news])
+    check_attention(backend, b, prefix=np.array([-2**31, 2**31 - 1, -1], np.int32))
+
+
+SPLITS = [(T_BF16, 80, 4), (T_F32, 96, 2), (T_F16, 256, 2), (T_F32, 256, 1), (T_BF16, 128, 4), (T_F32, 80, 2), (T_F16, 96, 3)]
+
+
+@pytest.mark.parametrize("t,hd,nh", SPLITS)
+@pytest.mark.parametrize("news,lens", [([1], [2500]), ([3, 1], [2500, 700]), ([40], [2500]), ([40, 1, 0, 3], [2100, 1500, 9, 3])])
+def test_attention_splits(backend, t, hd, nh, news, lens):
+    """Both kernels' split ranges and their joins, one launch with both included, for each way a head's values are laid out."""
+    b = Batch(50, t, hd, nh, 1, 32, news, lens, pad=(1, 2))
+    check_attention(backend, b)
+    check_attention(backend, b, window=1000, softcap=9.0)
 
 
 @pytest.mark.parametrize("lens", [[5000], [3, 5000, 1200, 64]])
@@ -549,6 +599,47 @@ def test_prompt_then_decode(backend, t):
                 assert np.array_equal(replay, d.get(o, like))
         finally:
             backend.graph_destroy(g)
+
+
+def test_graphs_share_scratch(backend):
+    """Recorded calls with split ranges, of generation, of a prompt and of both, replayed in turn with eager calls
+    between them: each gives the eager call's values for the queries that are there then."""
+    shapes = [([1, 1], [3000, 2000]), ([40], [2500]), ([40, 1, 3], [1000, 2500, 700])]
+    r = np.random.default_rng(64)
+    with Dev(backend) as d:
+        runs = []
+        for i, (news, lens) in enumerate(shapes):
+            b = Batch(65 + i, T_F16, 128, 8, 2, 64, news, lens)
+            cache, batch = put_batch(d, b)
+            q, o = d.put(b.q), d.put(b.q)
+
+            def call(cache=cache, batch=batch, q=q, o=o):
+                backend.paged_attention_dev(cache, batch, PagedMask(128**-0.5), 8, q, 1024, o, 1024)
+
+            runs.append([b, q, o, call, None])
+        for x in runs:  # sizes the scratch
+            x[3]()
+        backend.sync()
+        for x in runs:
+            backend.graph_begin()
+            x[3]()
+            x[4] = backend.graph_end()
+        try:
+            for turn in range(4):
+                for b, q, o, call, g in runs[turn % 3:] + runs[:turn % 3]:
+                    b.q = r.standard_normal(b.q.shape).astype(np.float32)
+                    backend.h2d(q, b.q)
+                    backend.h2d(o, np.zeros_like(b.q))
+                    backend.graph_launch(g)
+                    got = d.get(o, b.q)
+                    call()
+                    assert np.array_equal(got.view(np.uint32), d.get(o, b.q).view(np.uint32))
+                    if turn == 3:
+                        want, tol, _ = attention(b, b.q, float(np.float32(128**-0.5)))
+                        assert (np.abs(got - want) <= tol).all()
+        finally:
+            for x in runs:
+                backend.graph_destroy(x[4])
 
 
 def test_agrees_with_ring_attention(backend):

@@ -64,6 +64,26 @@ def test_refused_mask():
     assert B.paged_check(c, b, 4, mask=B.PagedMask(1.0)) == "too many rows"
 
 
+def test_refused_sizes():
+    """More workgroups than a launch takes, offsets past 64 bits, scales at which fp32 scores would not be finite."""
+    mask = B.PagedMask(0.125)
+    c, b = descriptors(n_head_kv=4096, n_seq=65535)
+    assert "too many" in B.paged_check(c, b, 4096, mask=mask)
+    c, b = descriptors(n_head_kv=4096, n_seq=65535, n_tok=65535)
+    assert "too many" in B.paged_check(c, b, 0, rope=B.PagedRope())
+    c, b = descriptors(n_tok=1 << 24)
+    assert "too many" in B.paged_check(c, b, 4, rope=B.PagedRope())
+    c, b = descriptors(n_head_kv=255, n_seq=65535, n_tok=1 << 15)
+    assert B.paged_check(c, b, 255, mask=mask) == "" and B.paged_check(c, b, 255, rope=B.PagedRope()) == "too many rows, sequences or K / V heads"
+    c, b = descriptors(n_pages=1 << 20, page_stride=1 << 30)
+    assert "page_stride" in B.paged_check(c, b, 4, mask=mask)
+    c, b = descriptors(n_pages=1 << 20, page_stride=1 << 28)
+    assert B.paged_check(c, b, 4, mask=mask) == ""
+    for kw in (dict(scale=1e20), dict(scale=-1e20), dict(scale=1.0, softcap=1e-30), dict(scale=1.0, softcap=1e30)):
+        assert B.paged_check(c, b, 4, mask=B.PagedMask(**kw)) != "", kw
+    assert B.paged_check(c, b, 0, rope=B.PagedRope(), ldq=3, ldo=-1) == ""  # not used without queries
+
+
 @pytest.mark.parametrize("page,hd,gap", [(16, 64, 0), (64, 80, 8), (256, 128, 24)])
 def test_slots(page, hd, gap):
     """Every value of every position has a place of its own, inside its page."""
@@ -91,6 +111,12 @@ def test_slots_of_bad_pages():
         for is_v in (False, True):
             got = B.paged_slot(c, table, s, pos, 1, 5, is_v)
             assert (got >= 0) == there and got < 8 * 2 * 16 * 64
+
+
+def test_slots_of_bad_caches():
+    for page in (0, 8, 24, 48):
+        c, _ = descriptors(page=page)
+        assert B.paged_slot(c, np.zeros((1, 4), np.int32), 0, 1, 0, 0) == -1
 
 
 def test_slots_are_64_bit():
