@@ -143,12 +143,13 @@ struct PagedAttnArgs {
     // to the prompt kernel; each kernel's ranges of positions are split over up to ds / ps workgroups (0: not
     // launched) of at least dleast steps / pleast units each. Split ranges leave their sums in part and stat, by slot (a workgroup's
     // rows) and split, and what the join has to know of a slot in info.
-    int ds, ps, drows, dleast, pleast;
+    int ds, ps, drows, prows;
+    bool alone;
     PagedSums dsum, psum;
 };
-constexpr int PRO_ROWS = 128;  // rows of a workgroup of the prompt kernel
+constexpr int PRO_ROWS = 128;  // rows of a workgroup of the prompt kernel, at most
 // at most as many tiles of that many rows as a batch's sequences can have, per K / V head (G rows a token)
-inline int64_t paged_tiles(int64_t n_tok, int64_t n_seq, int G) { return n_tok * G / PRO_ROWS + n_seq; }
+inline int64_t paged_tiles(int64_t n_tok, int64_t n_seq, int G, int rows) { return (n_tok * G + (rows - 1) * n_seq) / rows; }
 struct PagedScratch {
     size_t dpart, ppart, drow, prow, dslot, pslot;  // floats of part, rows of stat, slots of info
     size_t bytes() const { return (dslot + pslot) * sizeof(PagedSlot) + (drow + prow) * 8 + (dpart + ppart) * 4; }

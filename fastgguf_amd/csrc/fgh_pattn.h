@@ -221,8 +221,8 @@ __device__ __forceinline__ int paged_prefix(const PagedAttnArgs &a, int s, const
 struct PagedChunk {
     int per, used;
 };
-__device__ __forceinline__ PagedChunk paged_chunk(int n, int splits, int least) {
-    const int per = ((n + splits - 1) / splits + least - 1) / least * least;
+__device__ __forceinline__ PagedChunk paged_chunk(int n, int splits, int least, int whole) {
+    const int per = max(((n + splits - 1) / splits + whole - 1) / whole * whole, least);
     return PagedChunk{per, (n + per - 1) / per};
 }
 
@@ -233,15 +233,18 @@ constexpr int dec_resident(int type, int hd) { return hd > 128 || (type == T_F32
 // the decode kernel's steps of a range
 __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r.lo & ~(DEC_STEP - 1))) / DEC_STEP + 1; }
 
-constexpr int PRO_UNIT = 64;                // positions are split in units of 64
+constexpr int PRO_UNIT = 64;                // positions are split in units of 64,
+constexpr int PRO_LEAST = 4;                // that many and more each
 __device__ __forceinline__ int pro_units(const PagedSpan &r) { return (r.hi - (r.lo & ~(PRO_UNIT - 1))) / PRO_UNIT + 1; }
-inline int64_t paged_tiles(const PagedAttnArgs &a) { return paged_tiles(a.p.n_tok, a.p.n_seq, a.n_head / a.p.n_head_kv); }
+inline int64_t paged_tiles(const PagedAttnArgs &a) { return paged_tiles(a.p.n_tok, a.p.n_seq, a.n_head / a.p.n_head_kv, a.prows); }
+// whether there is a form of the prompt kernel with half the rows (not where its tiles are of 32 positions)
+constexpr bool pro_half(int type, int hd) { return !(type == T_F32 && hd > 128); }
 // Tile `index` of the batch: the sequences' tiles in order (of those that are the prompt kernel's). s = -1: there are fewer.
 struct PagedTile {
     int s, r0, index;
     PagedSeq q;
 };
-__device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int index) {
+__device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int tile_rows, int index) {
     const int lane = threadIdx.x & 63, G = a.n_head / a.p.n_head_kv;
     int before = 0;  // tiles of the sequences before the 64 looked at
     PagedTile t;
@@ -253,7 +256,7 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int inde
         if (s < a.p.n_seq) {
             q = paged_seq(a.p, s);
             const int64_t rows = (int64_t)q.n * G;
-            own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (int)((rows + PRO_ROWS - 1) / PRO_ROWS);
+            own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (int)((rows + tile_rows - 1) / tile_rows);
         }
         int upto = own;  // with this lane's
         for (int o = 1; o < 64; o <<= 1) {
@@ -264,7 +267,7 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int inde
         if (m) {
             const int at = __builtin_ctzll(m);
             t.s = b + at;
-            t.r0 = (index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * PRO_ROWS;
+            t.r0 = (index - before - (__shfl(upto, at, 64) - __shfl(own, at, 64))) * tile_rows;
             t.s = __builtin_amdgcn_readfirstlane(t.s);
             t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
             t.q.t0 = __builtin_amdgcn_readlane(q.t0, at), t.q.n = __builtin_amdgcn_readlane(q.n, at);

@@ -87,8 +87,8 @@ __device__ __forceinline__ void join_prompt(const PagedAttnArgs &a, int slot, in
     pf4 o[4];
     for (int i = 0; i < 4; ++i) o[i] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
     float cm = __FLT_MAX__, lr = 0.0f;
-    join_splits<4, 4>((const pf4 *)a.psum.part + ((int64_t)slot * a.ps * 4 + wave) * (vb * 4 * 64) + b * 4 * 64 + lane, (int64_t)vb * 4 * 64 * 4, 64,
-                      (const pf2 *)a.psum.stat + (int64_t)slot * a.ps * PRO_ROWS + r, PRO_ROWS, 0, 1, in.used, o, cm, lr);
+    join_splits<4, 4>((const pf4 *)a.psum.part + ((int64_t)slot * a.ps * (a.prows / 32) + wave) * (vb * 4 * 64) + b * 4 * 64 + lane, (int64_t)vb * 4 * 64 * (a.prows / 32), 64,
+                      (const pf2 *)a.psum.stat + (int64_t)slot * a.ps * a.prows + r, a.prows, 0, 1, in.used, o, cm, lr);
     const int row = in.r0 + r;
     float *out = a.o + (in.t0 + row / G) * a.ldo + (int64_t)(kvh * G + row % G) * hd;
     const float inv = 1.0f / lr;
@@ -120,13 +120,17 @@ PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
     // positions that a sequence's rows see
     const int64_t seen = a.window > 0 && !a.prefix ? std::min<int64_t>(a.p.max_len, (int64_t)a.window + a.p.max_tok - 1) : a.p.max_len;
     PagedScratch n{0, 0, 0, 0, 0, 0};
-    a.ps = a.ds = 0;
-    a.dleast = 4, a.pleast = 4;
+    a.ps = a.ds = 0, a.alone = false;
+    a.prows = PRO_ROWS;
     a.drows = (int)std::min<int64_t>(most, DEC_ROWS);
     if (most > DEC_ROWS) {
-        const int64_t wgs = paged_tiles(a) * a.p.n_head_kv, units = (seen + PRO_UNIT - 1) / PRO_UNIT + 1;
-        a.ps = (int)std::min<int64_t>({8, std::max<int64_t>(1, (2 * (int64_t)num_cu + wgs / 2) / wgs), (units + a.pleast - 1) / a.pleast});
-        if (a.ps > 1) n.pslot = (size_t)wgs, n.prow = n.pslot * a.ps * PRO_ROWS, n.ppart = n.prow * ((a.p.hd + 31) / 32 * 32);
+        const int64_t units = (seen + PRO_UNIT - 1) / PRO_UNIT + 1, splits = std::min<int64_t>(8, (units + PRO_LEAST - 1) / PRO_LEAST);
+        int64_t wgs = paged_tiles(a) * a.p.n_head_kv;
+        if (wgs * splits <= num_cu && pro_half(a.p.type, a.p.hd)) a.prows = PRO_ROWS / 2, wgs = paged_tiles(a) * a.p.n_head_kv;
+        a.ps = (int)std::min<int64_t>(splits, std::max<int64_t>(1, (2 * (int64_t)num_cu + wgs / 2) / wgs));
+        // workgroups with rows, a sequence's last tile counted half: it may be there or not
+        a.alone = (paged_tiles(a) - a.p.n_seq / 2) * a.p.n_head_kv * a.ps * 4 <= (int64_t)num_cu * 5;
+        if (a.ps > 1) n.pslot = (size_t)wgs, n.prow = n.pslot * a.ps * a.prows, n.ppart = n.prow * ((a.p.hd + 31) / 32 * 32);
     }
     if (a.ps == 0 || a.p.n_seq > 1) {
         const int64_t steps = seen / DEC_STEP + 1;

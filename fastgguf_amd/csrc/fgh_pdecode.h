@@ -51,7 +51,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
     const int prefix = paged_prefix(a, s, q);
     const PagedSpan sp = paged_span(a, q, prefix, 0, q.n - 1);
     const int base = sp.lo & ~(DEC_STEP - 1), steps = dec_steps(sp);
-    const PagedChunk ch = paged_chunk(steps, a.ds, a.dleast);
+    const PagedChunk ch = paged_chunk(steps, a.ds, 4, 4);
     if (split >= ch.used) return;
     if (a.ds > 1 && split == 0 && tid == 0) a.dsum.info[s * nkv + kvh] = PagedSlot{ch.used, (int)rows, q.t0, 0};
     const int end = min(steps, (split + 1) * ch.per);

@@ -15,10 +15,12 @@
 
 namespace fgh {
 
-template <int TYPE, int HD>
+// RW: wavefronts along the rows, 4, or 2 with the four in pairs that take half a tile's positions each
+template <int TYPE, int HD, int RW>
 struct Pro {
     static constexpr int ES = PagedType<TYPE>::ES, NQ = PagedType<TYPE>::NQ, NK = PagedType<TYPE>::NK;
     static constexpr int W = ES / 2;           // 16-byte words of 8 values
+    static constexpr int ROWS = 32 * RW, PW = 4 / RW;
     static constexpr int KT = HD * ES > 512 ? 32 : 64;
     static constexpr int KS = HD / 16;         // steps of 16 along the head
     static constexpr int VB = (HD + 31) / 32;  // blocks of 32 of V's values
@@ -29,7 +31,12 @@ struct Pro {
     static constexpr int VROWS = VB * 32;      // with the rows behind hd 80, never loaded, their sums never stored
     static constexpr int VBYTES = VROWS * KT * ES;
     static constexpr int BYTES = KBYTES + VBYTES;
+    static constexpr int LDS = 2 * BYTES + 16 + (PW > 1 ? RW * 512 : 0);
+    static_assert(PW == 1 || (KT == 64 && RW * VB * 4096 <= 2 * BYTES - 16384), "a block for every wavefront, its sums beside the rows' staging");
     static constexpr int OCC = HD > 128 || (TYPE == T_F32 && HD > 64) ? 1 : 2;
+    // The loads' places kept in registers, where there are any left: 8192 tokens, f16, hd 128 take 1035 us so and 1075 otherwise;
+    // 1008 tokens behind 7168, bf16, 342 with spills and 320.
+    static constexpr bool KEEP = !(NQ > 2 && HD == 128 && RW == 4);
     static constexpr int KL = KT / 4 * KW / 64;           // direct loads of a wavefront for its KT / 4 K rows
     static constexpr int VL = HD * VW / 64;               // and of all four for V
 };
@@ -46,21 +53,21 @@ __device__ __forceinline__ void lds_load16(const uint8_t *src, uint8_t *dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
 
-template <int TYPE, int HD>
+template <int TYPE, int HD, int RW>
 __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int block, int blocks, int split, uint8_t *lds) {
-    using P = Pro<TYPE, HD>;
+    using P = Pro<TYPE, HD, RW>;
     constexpr int KT = P::KT, ES = P::ES, W = P::W;
     uint32_t *odd_l = (uint32_t *)(lds + 2 * P::BYTES);  // positions of the tile with a V value that is not finite
     const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
     const int kvh = block % nkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // tiles in reverse: those late in a sequence have the most positions and start first
-    const PagedTile tl = paged_tile(a, (blocks - 1 - block) / nkv);
+    const PagedTile tl = paged_tile(a, P::ROWS, (blocks - 1 - block) / nkv);
     const int64_t slot = (int64_t)tl.index * nkv + kvh;
     const PagedSeq q = tl.q;
     if (a.ps > 1 && split == 0 && tid == 0 && (tl.s < 0 || !q.ok)) a.psum.info[slot].used = 0;
     if (tl.s < 0) return;
-    const int s = tl.s, r0 = tl.r0, R = min(PRO_ROWS, q.n * G - r0);
+    const int s = tl.s, r0 = tl.r0, R = min(P::ROWS, q.n * G - r0);
     if (!q.ok) {
         if (split == 0)
             for (int64_t i = tid; i < (int64_t)R * HD; i += 256) {
@@ -71,14 +78,14 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     }
     const int prefix = paged_prefix(a, s, q);
     const PagedSpan sp = paged_span(a, q, prefix, r0 / G, (r0 + R - 1) / G);
-    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, a.pleast);
+    const PagedChunk ch = paged_chunk(pro_units(sp), a.ps, PRO_LEAST, 1);
     if (split >= ch.used) return;
     if (a.ps > 1 && split == 0 && tid == 0) a.psum.info[slot] = PagedSlot{ch.used, R, q.t0, r0};
     const int ubase = sp.lo & ~(PRO_UNIT - 1);  // the split's positions k0 .. k1, whole units but for the range's ends
     const int k0 = max(sp.lo & ~(KT - 1), ubase + split * ch.per * PRO_UNIT), k1 = min(sp.hi, ubase + (split + 1) * ch.per * PRO_UNIT - 1);
 
     // this lane's row: column lane % 32 of the wavefront's products
-    const int half = lane >> 5, wr = wave * 32 + (lane & 31);
+    const int half = lane >> 5, rg = wave % RW, pg = wave / RW, wr = rg * 32 + (lane & 31);
     const bool mine = wr < R;
     const int row = r0 + (mine ? wr : 0), tok = row / G, head = kvh * G + row - tok * G;
     const int pos = q.len - q.n + tok;
@@ -86,43 +93,40 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 
     const int mask = (1 << a.p.shift) - 1;
     const int32_t *table = a.p.table + (int64_t)s * a.p.table_stride;
-    // a tile's pages, one entry for 16 positions (past the range its last): lane e asks for entry e, one tile ahead
-    constexpr int NE = KT / 16;
+    // Direct loads: V^T's are loads wave, wave + 4, .. of VR rows, a lane's word at the same positions (v_pos) in all of them; K's are of
+    // this wavefront's KT / 4 LDS rows, positions of one 16-block. A lane asks for the page of its V positions one tile ahead; the
+    // K rows' page is that of lane k_from.
+    constexpr int NE = KT / 16, VR = 64 / P::VW, KR = 64 / P::KW;
+    const int kr0 = wave * (KT / 4), kblk = kr0 & ~15;
+    const int k_from = (kblk * ES / 16) ^ turn<P::VW>(wave * VR);
+    auto lane_now = [&]() {  // what follows from it is kept, or formed for every tile
+        int ln = lane;
+        if (!P::KEEP) asm volatile("" : "+v"(ln));
+        return ln;
+    };
+    auto v_row = [&](int ln) { return wave * VR + ln / P::VW; };
+    auto v_pos = [&](int ln) { return (ln % P::VW ^ turn<P::VW>(v_row(ln))) * (16 / ES); };
     int ent = 0;
-    auto pages = [&](int kb) { ent = table[min(kb + 16 * min(lane, NE - 1), sp.hi) >> a.p.shift]; };
+    auto pages = [&](int kb) { ent = table[min(kb + v_pos(lane_now()), sp.hi) >> a.p.shift]; };
     const int64_t hsize = (int64_t)kvh * HD << a.p.shift;
     uint32_t gone_next = 0;  // 16-position blocks of the next tile whose page does not exist
     auto load = [&](int kb, uint8_t *buf) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));  // the lanes' offsets are formed for every tile, not kept
-        int64_t hb[NE];               // the entries' K / V head blocks
+        const int ln = lane_now(), vj = v_pos(ln);
+        const int kq = (kr0 & 15) | ln / P::KW, kw = (ln % P::KW) ^ turn<P::KW>(kq), krow = swap_rows(kq) * HD * ES;
+        const bool ok = paged_ok(a.p, ent);
+        const int page = ok ? ent : 0;
         gone_next = 0;
+        if (__builtin_amdgcn_ballot_w64(!ok) != 0)
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            const int page = __builtin_amdgcn_readlane(ent, e);
-            const bool ok = paged_ok(a.p, page);
-            hb[e] = (ok ? page : 0) * a.p.page_stride + hsize;
-            gone_next |= ok ? 0u : 1u << e;
-        }
-        // K: this wavefront's KT / 4 LDS rows, positions of one 16-block
-        const int kr0 = wave * (KT / 4), kblk = kr0 & ~15;
-        int64_t hk = hb[0];
+            for (int e = 0; e < NE; ++e) gone_next |= __builtin_amdgcn_ballot_w64(!ok && vj / 16 == e) ? 1u << e : 0u;
+        const uint8_t *kp = a.p.k + (__builtin_amdgcn_readlane(page, k_from) * a.p.page_stride + hsize + (int64_t)((kb + kblk) & mask) * HD) * ES;
 #pragma unroll
-        for (int e = 1; e < NE; ++e) hk = kblk == 16 * e ? hb[e] : hk;
-        const uint8_t *kp = a.p.k + (hk + (int64_t)((kb + kblk) & mask) * HD) * ES;
-#pragma unroll
-        for (int i = 0; i < P::KL; ++i) {
-            const int r = kr0 + i * (64 / P::KW) + ln / P::KW, w = ln % P::KW ^ turn<P::KW>(r);
+        for (int i = 0; i < P::KL; ++i) {  // KR rows on: other bits of the row, so of its turn and its place
+            const int w = kw ^ turn<P::KW>(i * KR);
             if (P::KD == P::KW || w < P::KD)
-                lds_load16(kp + (uint32_t)(swap_rows(r & 15) * HD * ES + w * 16), buf + kr0 * P::KW * 16 + i * 1024);
+                lds_load16(kp + (uint32_t)(krow + w * 16) + swap_rows(i * KR) * HD * ES, buf + kr0 * P::KW * 16 + i * 1024);
         }
-        // V^T: loads wave, wave + 4, ..
-        constexpr int VR = 64 / P::VW;  // rows a load
-        const int vr = wave * VR + ln / P::VW, j = (ln % P::VW ^ turn<P::VW>(vr)) * (16 / ES);
-        int64_t hv = hb[0];
-#pragma unroll
-        for (int e = 1; e < NE; ++e) hv = j >= 16 * e ? hb[e] : hv;
-        const uint8_t *vp = a.p.v + (hv + ((int64_t)vr << a.p.shift) + ((kb + j) & mask)) * ES;
+        const uint8_t *vp = a.p.v + (page * a.p.page_stride + hsize + ((int64_t)v_row(ln) << a.p.shift) + ((kb + vj) & mask)) * ES;
 #pragma unroll
         for (int i = 0; i < (P::VL + 3) / 4; ++i)  // 4 VR rows on: the same turn
             if (P::VL % 4 == 0 || wave + 4 * i < P::VL)
@@ -138,7 +142,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         uint32_t head;
     };
     auto place = [&](int r) {  // row r of this wavefront in q and o (past the last: the last)
-        const int z = r0 + min(wave * 32 + r, R - 1), t = z / G;
+        const int z = r0 + min(rg * 32 + r, R - 1), t = z / G;
         return Place{q.t0 + t, (uint32_t)((kvh * G + z - t * G) * HD)};
     };
     constexpr int QP = (HD + 31) / 32;
@@ -202,14 +206,15 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     float c = __FLT_MAX__, l = 0.0f;
 
     // where this lane's words are: the K row it gives, and the V^T row; word w of either at (place ^ 16 w)
-    const uint32_t k_at = (lane & 31) * P::KW * 16 + ((half * W) ^ turn<P::KW>(lane & 31)) * 16;
-    const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31)) * 16;
+    // (of the second block, where the wavefront takes that)
+    const uint32_t k_at = (pg * 32 + (lane & 31)) * P::KW * 16 + ((half * W) ^ turn<P::KW>(lane & 31)) * 16;
+    const uint32_t v_at = P::KBYTES + (lane & 31) * P::VW * 16 + ((half * W) ^ turn<P::VW>(lane & 31) ^ (pg * 4 * W)) * 16;
     const int first = max(sp.lo, k0), last = min(sp.hi, k1);  // the positions that count here
 
     // A tile in blocks of 32 positions, h: scores S(h), weights W(h), sums. The products of S(1) are issued among the
     // vector instructions of W(0), and those of the sums over block 0 among W(1)'s: a product takes the matrix pipe for 32 cycles, in which
     // the wavefront can issue 8 vector instructions.
-    constexpr int NH = KT / 32, AHEAD = P::NQ > 2 ? 2 : 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
+    constexpr int NH = KT / 32 / P::PW, AHEAD = P::NQ > 2 ? 2 : 3, SLOTS = AHEAD + 1;  // LDS words read ahead of the products that take them
     struct Weights {
         float v[2][8];  // scores, then weights, of this lane's positions 16 kk + 8 half + e of the block
         float mul;
@@ -337,7 +342,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         auto alone = [](int) {};
         scores(0, w0, alone);
         if constexpr (NH == 1) first_v();
-        const float top0 = forms(w0, kb, whole);
+        const float top0 = forms(w0, kb + pg * 32, whole);
         if (__builtin_amdgcn_ballot_w64(top0 + c > PTOP)) follow(top0);
         if constexpr (NH == 1) {
 #pragma unroll
@@ -407,6 +412,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         while (odd) {
             const int j = kb + __builtin_ctzll(odd);
             odd &= odd - 1;
+            if (P::PW > 1 && (j - kb) / 32 != pg) continue;
             int shift = a.p.shift;
             asm volatile("" : "+s"(shift));  // this rare path must not cost registers: no addresses formed ahead,
             const int64_t at = paged_head(a.p, table[j >> shift], kvh) + (j & mask) + ((int64_t)(4 * half) << shift);
@@ -425,18 +431,44 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         gone = gone_next;
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (P::PW > 1) {  // the pair's sums come together in the first of the two
+        pf4 *sum_l = (pf4 *)lds + rg * P::VB * 4 * 64 + lane;
+        pf2 *stat_l = (pf2 *)(lds + 2 * P::BYTES + 16) + rg * 64 + lane;
+        __syncthreads();
+        if (pg == 1) {
+            *stat_l = pf2{c, l};
+#pragma unroll
+            for (int b = 0; b < P::VB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum_l[(4 * b + i) * 64] = pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+        }
+        __syncthreads();
+        if (pg == 1) return;
+        const pf2 other = *stat_l;
+        const float cn = fminf(c, other.x), f = __builtin_amdgcn_exp2f(cn - c), g = __builtin_amdgcn_exp2f(cn - other.x);
+        c = cn;
+        l = l * f + other.y * g;
+#pragma unroll
+        for (int b = 0; b < P::VB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const pf4 z = sum_l[(4 * b + i) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[b][4 * i + e] = acc[b][4 * i + e] * f + z[e] * g;
+            }
+    }
     if (ch.used > 1) {  // sums as the lanes hold them
-        if (wave * 32 >= R) return;
-        pf4 *part = (pf4 *)a.psum.part + ((slot * a.ps + split) * 4 + wave) * (P::VB * 4 * 64) + lane;
+        if (rg * 32 >= R) return;
+        pf4 *part = (pf4 *)a.psum.part + ((slot * a.ps + split) * RW + rg) * (P::VB * 4 * 64) + lane;
 #pragma unroll
         for (int b = 0; b < P::VB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 part[(4 * b + i) * 64] = pf4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
-        if (half == 0) *(pf2 *)(a.psum.stat + ((slot * a.ps + split) * PRO_ROWS + wr) * 2) = pf2{c, l};
+        if (half == 0) *(pf2 *)(a.psum.stat + ((slot * a.ps + split) * P::ROWS + wr) * 2) = pf2{c, l};
         return;
     }
-    __syncthreads();  // the buffers have been read
+    if constexpr (P::PW == 1) __syncthreads();  // the buffers have been read
     const float inv = 1.0f / l;
     int ln = lane;
     asm volatile("" : "+v"(ln));  // the rows' places are formed again rather than kept
@@ -453,7 +485,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const pf4 z = *(const pf4 *)(own + (8 * u + rr) * 128 + (rw ^ rr) * 16);
-            if (wave * 32 + 8 * u + rr < R && (HD % 32 == 0 || 32 * b + 4 * rw < HD))
+            if (rg * 32 + 8 * u + rr < R && (HD % 32 == 0 || 32 * b + 4 * rw < HD))
                 *(pf4 *)(a.o + at[u].tok * a.ldo + at[u].head + 32 * b + 4 * rw) = z;
         }
     }

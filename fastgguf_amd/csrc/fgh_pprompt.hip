@@ -9,21 +9,28 @@ namespace fgh {
 
 namespace {
 
-template <int TYPE, int HD>
-__global__ __launch_bounds__(256, (Pro<TYPE, HD>::OCC)) void paged_prompt_kernel(PagedAttnArgs a, int nd) {
+template <int TYPE, int HD, int RW>
+__global__ __launch_bounds__(256, (Pro<TYPE, HD, RW>::OCC)) void paged_prompt_kernel(PagedAttnArgs a, int nd) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     // grid (tiles x K / V heads, prompt splits and what the decode workgroups need)
     const int block = blockIdx.x, y = blockIdx.y, d = (y - a.ps) * (int)gridDim.x + block;
-    if (y < a.ps) paged_prompt_block<TYPE, HD>(a, block, gridDim.x, y, lds);
+    if (y < a.ps) paged_prompt_block<TYPE, HD, RW>(a, block, gridDim.x, y, lds);
     else if (d < nd) paged_decode_block<TYPE, HD>(a, d, lds);
 }
 
+constexpr int ALONE = 82 * 1024;  // more than half a compute unit's LDS
+template <int TYPE, int HD, int RW>
+hipError_t launch_rows(const PagedAttnArgs &a, hipStream_t s) {
+    constexpr int pro = Pro<TYPE, HD, RW>::LDS, bytes = pro > dec_lds(HD) ? pro : dec_lds(HD);
+    const int x = (int)paged_tiles(a) * a.p.n_head_kv, nd = a.p.n_seq * a.ds * a.p.n_head_kv;
+    paged_prompt_kernel<TYPE, HD, RW><<<dim3((unsigned)x, (unsigned)(a.ps + (nd + x - 1) / x)), 256, a.alone ? std::max(bytes, ALONE) : bytes, s>>>(a, nd);
+    return hipGetLastError();
+}
 template <int TYPE, int HD>
 hipError_t launch_one(const PagedAttnArgs &a, hipStream_t s) {
-    constexpr int pro = 2 * Pro<TYPE, HD>::BYTES + 16, bytes = pro > dec_lds(HD) ? pro : dec_lds(HD);
-    const int x = (int)paged_tiles(a) * a.p.n_head_kv, nd = a.p.n_seq * a.ds * a.p.n_head_kv;
-    paged_prompt_kernel<TYPE, HD><<<dim3((unsigned)x, (unsigned)(a.ps + (nd + x - 1) / x)), 256, bytes, s>>>(a, nd);
-    return hipGetLastError();
+    if constexpr (pro_half(TYPE, HD))
+        if (a.prows == PRO_ROWS / 2) return launch_rows<TYPE, HD, 2>(a, s);
+    return launch_rows<TYPE, HD, 4>(a, s);
 }
 template <int TYPE>
 hipError_t launch_type(const PagedAttnArgs &a, hipStream_t s) {

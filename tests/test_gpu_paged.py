@@ -262,12 +262,11 @@ def test_damaged_sequences(backend, how, news):
 
 
 @pytest.mark.parametrize("page_no", [-1, 0x7FFFFFFF, -0x80000000, "n_pages"])
-@pytest.mark.parametrize("news", [[1, 1], [40, 5]])
+@pytest.mark.parametrize("news", [[1, 1], [40, 5], [40, 5] + [9] * 130])
 def test_bad_pages(backend, page_no, news):
     """A page that does not exist: the rows that see one of its positions are NaN, the others as they are; an append into it
     writes nothing."""
-    b = Batch(21, T_BF16, 64, 4, 2, 16, news, [news[0] + 70, 60])
-    b_good = Batch(21, T_BF16, 64, 4, 2, 16, news, [news[0] + 70, 60])
+    b, b_good = [Batch(21, T_BF16, 64, 4, 2, 16, news, [news[0] + 70, 60] + news[2:]) for _ in range(2)]
     bad_pos = (b.lens[0] - 10) // 16 * 16  # page of the last positions: early new tokens do not see it
     b.table[0, bad_pos // 16] = b.n_pages if page_no == "n_pages" else page_no
     want, tol, _ = attention(b_good, b.q, 0.125)
@@ -323,6 +322,11 @@ SHAPES = [  # type, hd, heads, K / V heads, page, news, lens
 ]
 
 
+def crowd(news, lens):
+    """The sequences and 130 short prompts: with two K / V heads too many workgroups for the prompt kernel's form of half the rows."""
+    return list(news) + [9] * 130, list(lens) + [9] * 130
+
+
 def shape(i, seed=0, **kw):
     t, hd, nh, nkv, page, news, lens = SHAPES[i]
     return Batch(300 + i + 1000 * seed, t, hd, nh, nkv, page, news, lens, **kw)
@@ -347,6 +351,19 @@ def test_attention_forms(backend, i, how):
         kw["window"] = [1, 7, 16, 40, 64, 129, 1000][i % 7]
     if how in ("prefix", "all"):
         kw["prefix"] = np.array([[0, m, m // 2, -3, 1, m + 100][(i + s) % 6] for s, m in enumerate(b.lens)], np.int32)
+    check_attention(backend, b, **kw)
+
+
+@pytest.mark.parametrize("t,hd", [(t, hd) for t in (T_F16, T_BF16, T_F32) for hd in (64, 80, 96, 128, 256)])
+@pytest.mark.parametrize("how", ["plain", "all"])
+def test_attention_crowded(backend, t, hd, how):
+    """Enough rows for whole workgroups of them, ranges in one part and in several, few-row sequences among them."""
+    b = Batch(51, t, hd, 4, 2, 32, *crowd([200, 1, 70, 0, 3, 130], [200, 90, 640, 0, 3, 333]), gap=8)
+    kw = {}
+    if how == "all":
+        kw = dict(softcap=5.0, slopes=np.exp2(-np.linspace(0.3, 8, 4)).astype(np.float32), window=129,
+                  prefix=np.resize([0, 50, 9, 300, 4, 20], len(b.news)).astype(np.int32))
+        b.q *= 4
     check_attention(backend, b, **kw)
 
 
@@ -445,11 +462,12 @@ def test_attention_stale_positions(backend, t, news):
 
 @pytest.mark.parametrize("what", ["k", "v", "q"])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("news", [4, 90])
-def test_attention_non_finite(backend, what, value, news):
+@pytest.mark.parametrize("news,crowded", [(4, False), (90, False), (90, True)])
+def test_attention_non_finite(backend, what, value, news, crowded):
     """A new token's value that is not finite: the tokens before it do not see it, whatever tile they share."""
     t, hd = T_F16, 128
-    b, clean = [Batch(44, t, hd, 4, 2, 16, [news], [news + 20]) for _ in range(2)]
+    batch = crowd([news], [news + 20]) if crowded else ([news], [news + 20])
+    b, clean = [Batch(44, t, hd, 4, 2, 16, *batch) for _ in range(2)]
     at = news // 2  # of the new tokens
     if what == "q":
         b.q[at, 1, 5] = value
