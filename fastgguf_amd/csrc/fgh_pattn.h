@@ -6,7 +6,7 @@
 //   BF16 cache  q and the weights as 3 bf16, cut so that they hold all 24 bits; 3 products
 //   F32 cache   K and V too as 3 bf16; the 6 products down to 2^-16 of the largest (the 3 left out are below 2^-24)
 // Halves have 5 bits of exponent, so a q row's largest value is brought to [2^14, 2^15) by a power of two (the scores take it
-// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the weights, 0 .. 1 beside the largest, are carried times 2^10 (PBIAS): down to 2^-24 of the
+// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the weights, 0 .. 1 beside the largest, are carried times 2^10: down to 2^-24 of the
 // largest both of a weight's halves are then normal numbers.
 #pragma once
 
@@ -28,6 +28,9 @@ struct PagedType {
     static constexpr int ES = TYPE == T_F32 ? 4 : 2;  // bytes a cached value
     static constexpr int NQ = TYPE == T_F16 ? 2 : 3;  // parts of q and of the weights
     static constexpr int NK = TYPE == T_F32 ? 3 : 1;  // parts of K and V
+    // Weights are 2^(PBIAS + s - m), s in powers of two, m a running reference of the row that follows a larger s where the exponent
+    // would pass PTOP. Halves: as large as their range allows (2^16). Elsewhere near 1, where the exponent of the largest is rounded least.
+    static constexpr float PBIAS = TYPE == T_F16 ? 10.0f : 0.0f, PTOP = PBIAS + 5.0f;
     static constexpr int NPROD = TYPE == T_F16 ? 2 : TYPE == T_F32 ? 6 : 3;  // products of parts
 };
 
@@ -127,10 +130,8 @@ __device__ __forceinline__ float cached(const uint8_t *base, int64_t i) {
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float PBIAS = 10.0f;  // weights are 2^(PBIAS + s - m): s in powers of two, m a running reference of the row
-constexpr float PTOP = 15.0f;   // m follows a larger s where the exponent would pass this: a half's largest is 2^16
 
-// tanh within 3 roundings: y + y^3 g(y^2) below 0.65 (g fitted at Chebyshev nodes), 1 - 2 / (e^(2 y) + 1) above
+// tanh within 3 roundings: y + y^3 g(y^2) below 0.65 (g fitted at Chebyshev nodes), 1 - 2 e / (1 + e), e = e^(-2 y), above
 __device__ __forceinline__ float tanh_below(float y) {
     const float z = y * y;
     float g = -0.005932980682700872f;
@@ -141,12 +142,13 @@ __device__ __forceinline__ float tanh_below(float y) {
     return __builtin_fmaf(y * z, g, y);
 }
 __device__ __forceinline__ float tanh_above(float y) {
-    const float e = __builtin_amdgcn_exp2f(fabsf(y) * (2.0f * LOG2E));
-    return copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), y);
+    const float e = __builtin_amdgcn_exp2f(fabsf(y) * (-2.0f * LOG2E)), d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
+    return copysignf(__builtin_fmaf(-2.0f * e, __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r), 1.0f), y);
 }
 constexpr float TANH_SPLIT = 0.65f;
 
-// What turns a row's products into scores in powers of two, s = v mul (v the products, unless a form has changed them)
+// What turns a row's products into scores in powers of two, s = v mul: v the products or, capped, their tanh, mul apply's result. The
+// product with mul is rounded once, in the sum that follows it.
 struct PagedScore {
     float mul;             // |scale| log2(e), times the power of two that q was divided by; above 0, so that -inf v
                            // are -inf scores (q takes the scale's sign, and a scale of 0 is 2^-126 here)
@@ -166,22 +168,19 @@ struct PagedScore {
             if (__builtin_amdgcn_ballot_w64(!(top < TANH_SPLIT))) {
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
-                    v[e] = cap_out * (fabsf(v[e]) < TANH_SPLIT ? tanh_below(v[e]) : tanh_above(v[e]));
+                    v[e] = fabsf(v[e]) < TANH_SPLIT ? tanh_below(v[e]) : tanh_above(v[e]);
                     if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: all at once would cost registers
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < NE; ++e) v[e] = cap_out * tanh_below(v[e]);
+                for (int e = 0; e < NE; ++e) v[e] = tanh_below(v[e]);
             }
-            if (!bias) return 1.0f;
-        } else if (bias) {
-#pragma unroll
-            for (int e = 0; e < NE; ++e) v[e] *= mul;
-        } else
-            return mul;
+        }
+        const float m = cap_out > 0.0f ? cap_out : mul;
+        if (!bias) return m;
         const float base = slope * (float)(p - j0);  // slope |p - j0 - e| = |slope (p - j0) - slope e|
 #pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = __builtin_fmaf(down, fabsf(__builtin_fmaf((float)-e, slope, base)), v[e]);
+        for (int e = 0; e < NE; ++e) v[e] = __builtin_fmaf(v[e], m, down * fabsf(__builtin_fmaf((float)-e, slope, base)));
         return 1.0f;
     }
 };

@@ -146,7 +146,10 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
     for (; st < end; st += 4) {
         const int kb = base + st * DEC_STEP, j0 = kb + quad * 8;
         const bool more = st + 4 < end;
-        pf4 sc[2] = {pf4{0.0f, 0.0f, 0.0f, 0.0f}, pf4{0.0f, 0.0f, 0.0f, 0.0f}};
+        // the first parts' products apart from the others', which are small: fewer roundings at the scores' size
+        pf4 sc[2], rest[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) sc[g] = rest[g] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -157,12 +160,12 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
                 for (int x = D::NQ - 1; x >= 0; --x)
 #pragma unroll
                     for (int y = D::NK - 1; y >= 0; --y)
-                        if (x + y < 3) mma16<TYPE>(sc[g], kp[y], qp[ks][x]);
+                        if (x + y < 3) mma16<TYPE>(x + y == 0 ? sc[g] : rest[g], kp[y], qp[ks][x]);
             }
         if (more) load_k(st + 4);
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sc[e / 4][e % 4];
+        for (int e = 0; e < 8; ++e) v[e] = sc[e / 4][e % 4] + rest[e / 4][e % 4];
         const float mul = score.apply(v, j0, pos);
         // positions that some row does not see: at the ends of the ranges
         const bool whole = kb >= sp.in_lo && kb + DEC_STEP - 1 <= sp.in_hi && !__builtin_amdgcn_ballot_w64(bad);
@@ -203,11 +206,11 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
 #pragma unroll
         for (int e = 1; e < 8; ++e) top = fmaxf(top, v[e]);
         top *= mul;
-        if (__builtin_amdgcn_ballot_w64(top + c > PTOP)) {
+        if (__builtin_amdgcn_ballot_w64(top + c > PagedType<TYPE>::PTOP)) {
             float mx = fmaxf(top, __shfl_xor(top, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (mx + c > PTOP) {  // of the whole row: its four lanes agree
-                const float cn = PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
+            if (mx + c > PagedType<TYPE>::PTOP) {  // of the whole row: its four lanes agree
+                const float cn = PagedType<TYPE>::PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
                 c = cn;
                 l *= f;
 #pragma unroll

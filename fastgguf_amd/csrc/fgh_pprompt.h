@@ -262,8 +262,8 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     auto follow = [&](float top) {
         const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
         float f = 1.0f;
-        if (mx + c > PTOP) {
-            const float cn = PBIAS - ceilf(mx);
+        if (mx + c > PagedType<TYPE>::PTOP) {
+            const float cn = PagedType<TYPE>::PBIAS - ceilf(mx);
             f = __builtin_amdgcn_exp2f(cn - c);
             c = cn;
             l *= f;
@@ -294,9 +294,11 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         };
         auto scores = [&](int h, Weights &out, auto side) {
             int m = 0;
-            pf16 sc;
+            // the first parts' products apart from the others', which are small: fewer roundings at the scores' size, where
+            // there are registers for it
+            pf16 sc, rest;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+            for (int r = 0; r < 16; ++r) sc[r] = rest[r] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < AHEAD; ++ks) read_k(h, ks);
 #pragma unroll
@@ -309,12 +311,12 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 #pragma unroll
                     for (int y = P::NK - 1; y >= 0; --y)
                         if (x + y < 3) {
-                            mma32<TYPE>(sc, kp[y], qp[ks][x]);
+                            mma32<TYPE>(x + y == 0 || P::PW == 1 ? sc : rest, kp[y], qp[ks][x]);
                             beside(m++, P::KS * NPROD, side);
                         }
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = sc[e];
+            for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = P::PW == 1 ? sc[e] : sc[e] + rest[e];
         };
         constexpr int NX = 2 * P::VB;  // V words of a block
         auto sums = [&](int h, const Weights &w, auto side) {
@@ -343,7 +345,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         scores(0, w0, alone);
         if constexpr (NH == 1) first_v();
         const float top0 = forms(w0, kb + pg * 32, whole);
-        if (__builtin_amdgcn_ballot_w64(top0 + c > PTOP)) follow(top0);
+        if (__builtin_amdgcn_ballot_w64(top0 + c > PagedType<TYPE>::PTOP)) follow(top0);
         if constexpr (NH == 1) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) weigh(w0, e);
@@ -353,7 +355,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
             scores(1, w1, [&](int e) { weigh(w0, e); });
             first_v();
             const float top1 = forms(w1, kb + 32, whole);
-            if (__builtin_amdgcn_ballot_w64(top1 + c > PTOP)) {  // block 0's weights wait for their sums
+            if (__builtin_amdgcn_ballot_w64(top1 + c > PagedType<TYPE>::PTOP)) {  // block 0's weights wait for their sums
                 const float f = follow(top1);
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
