@@ -139,10 +139,10 @@ struct PagedAttnArgs {
     int64_t ldq, ldo;
     int n_head, window;
     float scale, softcap;
-    // Sequences of few rows per K / V head (new tokens x query heads of the head) go to the decode kernel, the others
-    // to the prompt kernel; each kernel's ranges of positions are split over up to ds / ps workgroups (0: not
-    // launched) of at least dleast steps / pleast units each. Split ranges leave their sums in part and stat, by slot (a workgroup's
-    // rows) and split, and what the join has to know of a slot in info.
+    // Sequences of few rows per K / V head (new tokens x query heads of the head, at most drows) go to the decode kernel, the
+    // others to the prompt kernel, prows rows a workgroup; each kernel's ranges of positions are split over up to ds / ps
+    // workgroups (0: not launched). Split ranges leave their sums in part and stat, by slot (a workgroup's rows) and split, and
+    // what the join has to know of a slot in info. alone: one workgroup of the prompt launch to a compute unit.
     int ds, ps, drows, prows;
     bool alone;
     PagedSums dsum, psum;

@@ -6,8 +6,10 @@
 //   BF16 cache  q and the weights as 3 bf16, cut so that they hold all 24 bits; 3 products
 //   F32 cache   K and V too as 3 bf16; the 6 products down to 2^-16 of the largest (the 3 left out are below 2^-24)
 // Halves have 5 bits of exponent, so a q row's largest value is brought to [2^14, 2^15) by a power of two (the scores take it
-// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the weights, 0 .. 1 beside the largest, are carried times 2^10: down to 2^-24 of the
-// largest both of a weight's halves are then normal numbers.
+// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the
+// weights, 0 .. 1 beside the largest, are carried times 2^10: down to 2^-24 of the largest both of a weight's halves are
+// then normal numbers. The small products are summed apart where registers allow: an error of 1.0 instead of 1.5 to 2 times
+// a plain fp32 form's where few large scores decide.
 #pragma once
 
 #include "fgh_internal.h"

@@ -106,13 +106,23 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int np
 
 }  // namespace
 
-// Prompt: tiles of 128 rows for every compute unit twice over (what fits at once) and no further: a split saves nothing
-// where they are that many, and its join costs 5 to 20 us (2032 tokens behind 7168, 512 tiles: 600 us whole, 600 + 20 in two
-// splits; seven documents of up to 900 tokens, 252 tiles: 48.7 us whole, 33 + 5 in three). At least 4 units of 64 positions each (256 positions
-// of a tile take about 10 us, the join of a few splits 5), at most 8 splits: 64 tokens over 4096 positions take 28 + 5 us in 8, 27 + 7 in 16.
-// Decode: what fits at once too, of 4 steps and more, a step for every wavefront (4 sequences of 3000 positions at hd 256, of which one workgroup
-// fits a compute unit: 21.5 us in 256 workgroups, 28.8 in 512); up to eight for every compute unit where that leaves 16 steps each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take 137 us in 2 splits, 110 in 8, and 32 of 1024
-// 27 in 2, 35 in 8. At most 64, which is what the join holds. The bounds may be far above the lengths: the kernels split what is there.
+// Prompt: workgroups of 128 rows, since a tile of K and V is read out of LDS once for all of them. Where they would not give
+// every compute unit one in as many splits as there may be, of 64: 64 tokens behind 2000 positions, 8 heads over 4, take 32.7 us
+// in 128 rows and 24.7 in 64 (bf16, hd 256), 38.7 and 26.0 (f32, hd 128); with more workgroups than that 64 rows lose (32 tokens of each of
+// 4 sequences behind 1000, f16: 20.8 and 25.0).
+// Splits: as many as fit at once, two workgroups for every compute unit. More save nothing, and the join costs 5 to 20 us (2032 tokens behind
+// 7168, 512 tiles: 600 us whole, 600 + 20 in two splits; seven documents of up to 900 tokens, 252 tiles: 48.7 us whole,
+// 33 + 5 in three). At least 4 units of 64 positions each, at most 8 splits: 64 tokens over 4096 positions took 29 + 5 us in 8,
+// 27 + 7 in 16.
+// One workgroup to a compute unit where all fit so: the dispatcher would put two on one and leave others idle (128 tokens behind
+// 4000: 40.8 us, 34.0 so; 256 tokens, which do not fit, would take 59 instead of 46).
+// Decode: as many as fit at once too, of 4 steps and more, a step for every wavefront (4 sequences of 3000 positions at hd 256, of
+// which one workgroup fits a compute unit: 26.3 us with the join in 256 workgroups, 33.6 in 512); up to eight for every compute
+// unit where that leaves 16 steps each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take
+// 137 us in 2 splits, 110 in 8, and 32 of 1024 27 in 2, 35 in 8. At most 64: the join reads that many one after the other.
+// The bounds may be far above the lengths: the kernels split what is there.
+// The join is a launch of its own: a workgroup that arrives last and joins the others' sums within the same launch needs
+// stores that pass the L2 caches of the XCDs, and took longer (one sequence of 4096 positions 14 to 16 us against 12.3).
 PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
     const int G = a.n_head / a.p.n_head_kv;
     const int64_t most = (int64_t)a.p.max_tok * G;  // rows of a sequence and K / V head
@@ -128,13 +138,14 @@ PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
         int64_t wgs = paged_tiles(a) * a.p.n_head_kv;
         if (wgs * splits <= num_cu && pro_half(a.p.type, a.p.hd)) a.prows = PRO_ROWS / 2, wgs = paged_tiles(a) * a.p.n_head_kv;
         a.ps = (int)std::min<int64_t>(splits, std::max<int64_t>(1, (2 * (int64_t)num_cu + wgs / 2) / wgs));
-        // workgroups with rows, a sequence's last tile counted half: it may be there or not
+        // workgroups with rows, a sequence's last tile counted half: it may be there or not. A few too many still pay.
         a.alone = (paged_tiles(a) - a.p.n_seq / 2) * a.p.n_head_kv * a.ps * 4 <= (int64_t)num_cu * 5;
         if (a.ps > 1) n.pslot = (size_t)wgs, n.prow = n.pslot * a.ps * a.prows, n.ppart = n.prow * ((a.p.hd + 31) / 32 * 32);
     }
     if (a.ps == 0 || a.p.n_seq > 1) {
-        const int64_t steps = seen / DEC_STEP + 1;
-        const int64_t even = std::min<int64_t>(dec_resident(a.p.type, a.p.hd) * (int64_t)num_cu / heads, (steps + 3) / 4), more = std::min<int64_t>(8 * (int64_t)num_cu / heads, steps / 16);
+        const int64_t steps = seen / DEC_STEP + 1, at_once = dec_resident(a.p.type, a.p.hd) * (int64_t)num_cu;
+        const int64_t even = std::min<int64_t>(at_once / heads, (steps + 3) / 4);
+        const int64_t more = std::min<int64_t>(8 * (int64_t)num_cu / heads, steps / 16);
         a.ds = (int)std::min<int64_t>(64, std::max<int64_t>({1, even, more}));
         if (a.ds > 1) n.dslot = (size_t)heads, n.drow = n.dslot * a.ds * a.drows, n.dpart = n.drow * a.p.hd;
     }

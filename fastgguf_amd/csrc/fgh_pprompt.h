@@ -1,7 +1,8 @@
 // fgh_pprompt.h - paged attention of many rows per K / V head: prompts.
 //
 // A workgroup takes 128 rows of a sequence and K / V head (row = new token x the head's query heads + query head, so the
-// heads that share K and V share its tiles), 32 a wavefront, and goes over their positions in tiles of KT. K and V^T
+// heads that share K and V share its tiles), 32 a wavefront, and goes over their positions in tiles of KT; or 64 rows, with two
+// wavefronts to 32 of them that take half of every tile each and add their sums up at the end, where workgroups are few. K and V^T
 // tiles come into LDS by direct loads (16 bytes a lane), two tiles deep: the next one is on its way while this one is used.
 //   S^T = K q^T: 32 x 32 x 16 products, A = 32 K rows out of LDS, B = q in registers. LDS row m of a 16-position block holds position
 //         (m & 3) | (m & 8) >> 1 | (m & 4) << 1, so that a lane's 16 scores of 32 positions are two runs of 8 positions,
@@ -9,6 +10,12 @@
 //         one exchange with the lane 32 away, and only where the row's reference has to follow it.
 // 16-byte words of a row are kept in LDS at (word ^ row), so that lanes that read the same word of neighbouring rows
 // meet in no bank.
+//
+// Bound by the matrix pipe, for the 2 (F16) to 6 (F32) products that an fp32 result takes: 8192 tokens, f16, 32 heads over 8, hd 128 take
+// 924 to 1085 us by the card's clock: 1.19 to 1.01 PFLOP/s of products, 1.15 for a large f16 matrix product here, with the clock held
+// down by power. Small batches are bound by what a tile costs a wavefront that is alone on its SIMD (64 tokens behind
+// 4032: 23.6 us; asking for the next tile took 1500 of a tile's 5500 cycles there before its loads' places were formed from
+// one lane's by other bits). Three tiles deep gained nothing there: the tiles are in time.
 #pragma once
 
 #include "fgh_pattn.h"

@@ -23,7 +23,8 @@ template <int TYPE, int HD, int RW>
 hipError_t launch_rows(const PagedAttnArgs &a, hipStream_t s) {
     constexpr int pro = Pro<TYPE, HD, RW>::LDS, bytes = pro > dec_lds(HD) ? pro : dec_lds(HD);
     const int x = (int)paged_tiles(a) * a.p.n_head_kv, nd = a.p.n_seq * a.ds * a.p.n_head_kv;
-    paged_prompt_kernel<TYPE, HD, RW><<<dim3((unsigned)x, (unsigned)(a.ps + (nd + x - 1) / x)), 256, a.alone ? std::max(bytes, ALONE) : bytes, s>>>(a, nd);
+    const dim3 grid((unsigned)x, (unsigned)(a.ps + (nd + x - 1) / x));
+    paged_prompt_kernel<TYPE, HD, RW><<<grid, 256, a.alone ? std::max(bytes, ALONE) : bytes, s>>>(a, nd);
     return hipGetLastError();
 }
 template <int TYPE, int HD>

@@ -293,7 +293,7 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * Requires hd 64, 80, 96, 128 or 256; page a power of 2 from 16 to 256; k and v 16-byte aligned,
  * page_stride a multiple of 8. Offsets are 64-bit. At most 16383 heads, 4096 K / V heads, 65535 sequences,
  * and 2^24 - 1 workgroups a call (append: n_tok + (n_tok / 64 + 2 n_seq) n_head_kv + 65536, attention:
- * (n_tok n_head / n_head_kv / 128 + n_seq) n_head_kv); more is refused. */
+ * (n_tok n_head / n_head_kv + 127 n_seq) / 128 n_head_kv); more is refused. */
 typedef struct {
     void *k, *v;            /* device */
     const int32_t *table;   /* device, [n_seq][table_stride] */
