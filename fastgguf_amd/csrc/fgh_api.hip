@@ -1018,7 +1018,8 @@ static const char *paged_check(const fgh_paged_cache *c, const fgh_paged_batch *
         if (m->window < 0) return "window is negative";
         const int G = n_head / c->n_head_kv;
         if ((int64_t)b->n_tok * G > INT32_MAX / 2) return "too many rows";
-        if (fgh::paged_tiles(b->n_tok, b->n_seq, G, fgh::PRO_ROWS) * c->n_head_kv > fgh::PAGED_GRID) return "too many rows, sequences or K / V heads";
+        if (std::max<int64_t>(fgh::paged_tiles(b->n_tok, b->n_seq, G, fgh::PRO_ROWS), b->n_seq) * c->n_head_kv > fgh::PAGED_GRID)
+            return "too many rows, sequences or K / V heads";
     }
     return nullptr;
 }

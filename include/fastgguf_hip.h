@@ -284,7 +284,7 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * formulas to within 1e-5 relative per output vector, as long as fp32 scores do (a weight is off by its score's
  * rounding: scores of hundreds cost as many 2^-24). Both calls are asynchronous on the context's
  * stream and can be captured (the attention's scratch must have its size from an eager call with the same
- * descriptors, or larger ones, before).
+ * sizes in the descriptors before: fewer sequences or rows can take more).
  *
  * The cache: n_pages pages for `page` positions of n_head_kv heads of hd values of `type` (FGH_T_F32,
  * FGH_T_F16 or FGH_T_BF16). K page: [n_head_kv][page][hd]; V page, transposed: [n_head_kv][hd][page].
@@ -293,7 +293,7 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * Requires hd 64, 80, 96, 128 or 256; page a power of 2 from 16 to 256; k and v 16-byte aligned,
  * page_stride a multiple of 8. Offsets are 64-bit. At most 16383 heads, 4096 K / V heads, 65535 sequences,
  * and 2^24 - 1 workgroups a call (append: n_tok + (n_tok / 64 + 2 n_seq) n_head_kv + 65536, attention:
- * (n_tok n_head / n_head_kv + 127 n_seq) / 128 n_head_kv); more is refused. */
+ * (n_tok n_head / n_head_kv + 127 n_seq) / 128 n_head_kv and n_seq n_head_kv); more is refused. */
 typedef struct {
     void *k, *v;            /* device */
     const int32_t *table;   /* device, [n_seq][table_stride] */
@@ -338,7 +338,7 @@ FGH_API int fgh_paged_store_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, cons
  *   s_j = scale q . k_j; softcap > 0: s = softcap tanh(s / softcap); slopes (device, [n_head], or NULL):
  *   s -= slopes[h] |p - j|
  * over the positions j that position p sees: j <= p or j < prefix[s] (device, [n_seq], or NULL: a prefix
- * that all tokens see), j < len, and p - j < window (window > 0). Sequences do not see each other, so
+ * that all tokens see, taken as 0 .. len), j < len, and p - j < window (window > 0). Sequences do not see each other, so
  * packed documents are sequences. Pages without a visible position are not read (their table entries may
  * be anything); a row that sees a position whose page is not 0 .. n_pages - 1 is NaN. Values in
  * positions that no row of a sequence sees do not matter, NaN included; with a q or k that is not finite

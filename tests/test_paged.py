@@ -75,6 +75,8 @@ def test_refused_sizes():
     assert "too many" in B.paged_check(c, b, 4, rope=B.PagedRope())
     c, b = descriptors(n_head_kv=255, n_seq=65535, n_tok=1 << 15)
     assert B.paged_check(c, b, 255, mask=mask) == "" and B.paged_check(c, b, 255, rope=B.PagedRope()) == "too many rows, sequences or K / V heads"
+    c, b = descriptors(n_head_kv=257, n_seq=65535, n_tok=1)  # decode workgroups: one above 2^24 - 1 with fewer prompt tiles
+    assert "too many" in B.paged_check(c, b, 257, mask=mask)
     c, b = descriptors(n_pages=1 << 20, page_stride=1 << 30)
     assert "page_stride" in B.paged_check(c, b, 4, mask=mask)
     c, b = descriptors(n_pages=1 << 20, page_stride=1 << 28)
