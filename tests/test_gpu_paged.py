@@ -660,6 +660,44 @@ def test_graphs_share_scratch(backend):
                 backend.graph_destroy(x[4])
 
 
+def test_scratch_and_graphs():
+    """Scratch that would grow while a call is recorded is refused, and a recorded call keeps its own when a larger eager
+    call takes more."""
+    from fastgguf_amd.backend import Backend
+    be = Backend(0)
+    try:
+        with Dev(be) as d:
+            small = Batch(70, T_F16, 64, 4, 1, 16, [1], [900])
+            large = Batch(71, T_F16, 128, 8, 8, 16, [1, 60], [3000, 2000])
+            calls = []
+            for b in (small, large):
+                cache, batch = put_batch(d, b)
+                q, o, row = d.put(b.q), d.put(np.zeros_like(b.q)), b.n_head * b.hd
+                calls.append((lambda cache=cache, batch=batch, b=b, q=q, o=o, row=row: be.paged_attention_dev(
+                    cache, batch, PagedMask(0.125), b.n_head, q, row, o, row), b, o))
+
+            def check(b, o):
+                want, tol, _ = attention(b, b.q, 0.125)
+                assert (np.abs(d.get(o, b.q) - want) <= tol).all()
+                be.h2d(o, np.zeros_like(b.q))
+
+            calls[0][0]()
+            check(*calls[0][1:])
+            be.graph_begin()
+            calls[0][0]()
+            with pytest.raises(BackendError, match="grow"):
+                calls[1][0]()
+            g = be.graph_end()
+            for _ in range(2):
+                be.graph_launch(g)
+                check(*calls[0][1:])
+                calls[1][0]()  # takes more
+                check(*calls[1][1:])
+            be.graph_destroy(g)
+    finally:
+        be.close()
+
+
 def test_agrees_with_ring_attention(backend):
     """An fp32 paged cache against fgh_attention over the same positions in its ring."""
     b = Batch(62, T_F32, 128, 8, 2, 16, [5], [300])
