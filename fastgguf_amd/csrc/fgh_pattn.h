@@ -237,7 +237,11 @@ __device__ __forceinline__ int dec_steps(const PagedSpan &r) { return (r.hi - (r
 constexpr int PRO_UNIT = 64;                // positions are split in units of 64,
 constexpr int PRO_LEAST = 4;                // that many and more each
 __device__ __forceinline__ int pro_units(const PagedSpan &r) { return (r.hi - (r.lo & ~(PRO_UNIT - 1))) / PRO_UNIT + 1; }
-inline int64_t paged_tiles(const PagedAttnArgs &a) { return paged_tiles(a.p.n_tok, a.p.n_seq, a.n_head / a.p.n_head_kv, a.prows); }
+// at most as many sequences of a batch with several are the prompt kernel's, and the tiles they can have
+inline int64_t pro_seqs(const PagedAttnArgs &a) {
+    return std::min<int64_t>(a.p.n_seq, (int64_t)a.p.n_tok * (a.n_head / a.p.n_head_kv) / (DEC_ROWS + 1));
+}
+inline int64_t paged_tiles(const PagedAttnArgs &a) { return paged_tiles(a.p.n_tok, pro_seqs(a), a.n_head / a.p.n_head_kv, a.prows); }
 // whether there is a form of the prompt kernel with half the rows (not where its tiles are of 32 positions)
 constexpr bool pro_half(int type, int hd) { return !(type == T_F32 && hd > 128); }
 // Tile `index` of the batch: the sequences' tiles in order (of those that are the prompt kernel's). s = -1: there are fewer.

@@ -115,7 +115,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int np
 // 33 + 5 in three). At least 4 units of 64 positions each, at most 8 splits: 64 tokens over 4096 positions took 29 + 5 us in 8,
 // 27 + 7 in 16.
 // One workgroup to a compute unit where all fit so: the dispatcher would put two on one and leave others idle (128 tokens behind
-// 4000: 40.8 us, 34.0 so; 256 tokens, which do not fit, would take 59 instead of 46).
+// 4000: 40.8 us, 34.0 so; 256 tokens, which do not fit, would take 59 instead of 46). Not where the sequences beside the longest have few
+// rows, whose decode workgroups fit several (40 tokens of one sequence and one each of 63: 111 us, 91 without).
 // Decode: as many as fit at once too, of 4 steps and more, a step for every wavefront (4 sequences of 3000 positions at hd 256, of
 // which one workgroup fits a compute unit: 26.3 us with the join in 256 workgroups, 33.6 in 512); up to eight for every compute
 // unit where that leaves 16 steps each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take
@@ -139,7 +140,8 @@ PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
         if (wgs * splits <= num_cu && pro_half(a.p.type, a.p.hd)) a.prows = PRO_ROWS / 2, wgs = paged_tiles(a) * a.p.n_head_kv;
         a.ps = (int)std::min<int64_t>(splits, std::max<int64_t>(1, (2 * (int64_t)num_cu + wgs / 2) / wgs));
         // workgroups with rows, a sequence's last tile counted half: it may be there or not. A few too many still pay.
-        a.alone = (paged_tiles(a) - a.p.n_seq / 2) * a.p.n_head_kv * a.ps * 4 <= (int64_t)num_cu * 5;
+        const bool mixed = (int64_t)(a.p.n_tok - a.p.max_tok) * G <= (int64_t)(a.p.n_seq - 1) * DEC_ROWS && a.p.n_seq > 1;
+        a.alone = !mixed && (paged_tiles(a) - pro_seqs(a) / 2) * a.p.n_head_kv * a.ps * 4 <= (int64_t)num_cu * 5;
         if (a.ps > 1) n.pslot = (size_t)wgs, n.prow = n.pslot * a.ps * a.prows, n.ppart = n.prow * ((a.p.hd + 31) / 32 * 32);
     }
     if (a.ps == 0 || a.p.n_seq > 1) {
