@@ -2,14 +2,18 @@
 //
 // fp32 results from 16-bit matrix instructions: every operand is a sum of 16-bit parts, and the products of parts are
 // summed in the fp32 accumulators.
-//   F16 cache   q and the weights as 2 halves (22 bits); K and V as they are: 2 products
+//   F16 cache   q and the weights as 2 halves; K and V as they are: 2 products
 //   BF16 cache  q and the weights as 3 bf16, cut so that they hold all 24 bits; 3 products
-//   F32 cache   K and V too as 3 bf16; the 6 products down to 2^-16 of the largest (the 3 left out are below 2^-24)
-// Halves have 5 bits of exponent, so a q row's largest value is brought to [2^14, 2^15) by a power of two (the scores take it
-// back with the scale; values down to 2^-17 of the largest keep their 22 bits, smaller ones 2^-40 of it), and the
-// weights, 0 .. 1 beside the largest, are carried times 2^10: down to 2^-24 of the largest both of a weight's halves are
-// then normal numbers. The small products are summed apart where registers allow: an error of 1.0 instead of 1.5 to 2 times
-// a plain fp32 form's where few large scores decide.
+//   F32 cache   K and V too as 3 bf16; 6 products. The 3 left out are at most 2^-21 of the whole product, and 2^-24.6 on average:
+//               the parts are cut, not rounded, so that each is up to 2^-7 of the one before
+// Halves have 5 bits of exponent. So a q row's largest value is brought to [2^14, 2^15) by a power of two (the scores take it
+// back with the scale): values down to 2^-17 of the largest keep 22 bits, smaller ones count to 2^-40 of it. The weights' second halves,
+// which would leave the halves' range 12 bits before the first ones, are carried times 2^LOW and summed by themselves. With
+// the largest weight at 2^12 to 2^15.9 a weight keeps 22 bits down to 2^-26 of the largest, 17 (the 1e-5 of a result) down
+// to 2^-31, and is off by at most 2^-48 of it below: what decides where the largest weights stand at V near 0. (Both halves
+// on one scale, the largest at 2^10, held 17 bits down to 2^-18 only, for 6 % less time of a long prompt.)
+// q's small products are summed apart where registers allow: an error of 1.0 instead of 1.5 to 2 times a plain fp32 form's where few
+// large scores decide.
 #pragma once
 
 #include "fgh_internal.h"
@@ -31,8 +35,12 @@ struct PagedType {
     static constexpr int NQ = TYPE == T_F16 ? 2 : 3;  // parts of q and of the weights
     static constexpr int NK = TYPE == T_F32 ? 3 : 1;  // parts of K and V
     // Weights are 2^(PBIAS + s - m), s in powers of two, m a running reference of the row that follows a larger s where the exponent
-    // would pass PTOP. Halves: as large as their range allows (2^16). Elsewhere near 1, where the exponent of the largest is rounded least.
-    static constexpr float PBIAS = TYPE == T_F16 ? 10.0f : 0.0f, PTOP = PBIAS + 5.0f;
+    // would pass PTOP. Halves: up to what their range allows (2^16, and 2^15 for second ones times 2^LOW), and 2^3 below it after the
+    // reference has moved: in 2^2 it moves more often (8192 tokens 1013 us, 997 so), in 2^6 weights lose 3 bits for 6 us. Elsewhere near
+    // 1, where the exponent of the largest is rounded least.
+    static constexpr float PBIAS = TYPE == T_F16 ? 13.0f : 0.0f, PTOP = TYPE == T_F16 ? 15.9f : 5.0f;
+    static constexpr int LOW = TYPE == T_F16 ? 11 : 0;
+    static constexpr float LOW_UP = 1 << LOW, LOW_DOWN = 1.0f / LOW_UP;
     static constexpr int NPROD = TYPE == T_F16 ? 2 : TYPE == T_F32 ? 6 : 3;  // products of parts
 };
 
@@ -49,14 +57,15 @@ __device__ __forceinline__ void mma32(pf16 &d, pu4 x, pu4 y) {
     else d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pb8, x), __builtin_bit_cast(pb8, y), d, 0, 0, 0);
 }
 
-// values 2 i and 2 i + 1 of 8 as NP vectors of 16-bit parts
+// values 2 i and 2 i + 1 of 8 as NP vectors of 16-bit parts, a second half times `up`, a power of two
 template <int TYPE, int NP>
-__device__ __forceinline__ void parts2(float a, float b, int i, pu4 (&out)[NP]) {
+__device__ __forceinline__ void parts2(float a, float b, int i, pu4 (&out)[NP], float up = 1.0f) {
     if constexpr (TYPE == T_F16) {  // to nearest, then what is left to nearest
         const pf2 v = {a, b};
         const ph2 h = __builtin_convertvector(v, ph2);
         out[0][i] = __builtin_bit_cast(uint32_t, h);
-        out[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v - __builtin_convertvector(h, pf2), ph2));
+        const pf2 rest = {__builtin_fmaf((float)h.x, -up, a * up), __builtin_fmaf((float)h.y, -up, b * up)};  // exact
+        out[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, ph2));
     } else {  // the upper halves of the words, cut: what is left is exact, and 8 + 8 + 8 bits hold it all
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -69,21 +78,27 @@ __device__ __forceinline__ void parts2(float a, float b, int i, pu4 (&out)[NP]) 
 }
 // 8 fp32 values as NP vectors of 8 16-bit parts
 template <int TYPE, int NP>
-__device__ __forceinline__ void parts8(const float *x, pu4 (&out)[NP]) {
+__device__ __forceinline__ void parts8(const float *x, pu4 (&out)[NP], float up = 1.0f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) parts2<TYPE, NP>(x[2 * i], x[2 * i + 1], i, out);
+    for (int i = 0; i < 4; ++i) parts2<TYPE, NP>(x[2 * i], x[2 * i + 1], i, out, up);
 }
-// 8 16-bit parts times a power of two of at most 1
-template <int TYPE>
-__device__ __forceinline__ void scale8(pu4 &x, float f) {
-    if constexpr (TYPE == T_F16) {  // in two steps: a half goes down to 2^-24
-        const float r = f < 0x1p-20f ? 0x1p-20f : f;
-        const _Float16 a = (_Float16)r, b = (_Float16)(f / r);
-        x = __builtin_bit_cast(pu4, __builtin_bit_cast(ph8, x) * a * b);
+// 8 weights, as parts, times a power of two of at most 1. Halves are put together and taken apart again: each by itself would
+// lose what falls below 2^-24.
+template <int TYPE, int NP>
+__device__ __forceinline__ void scale8(pu4 (&x)[NP], float f) {
+    if constexpr (TYPE == T_F16) {
+        using T = PagedType<TYPE>;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const ph2 h = __builtin_bit_cast(ph2, (uint32_t)x[0][i]), r = __builtin_bit_cast(ph2, (uint32_t)x[1][i]);
+            parts2<TYPE, NP>(__builtin_fmaf((float)r.x, T::LOW_DOWN, (float)h.x) * f, __builtin_fmaf((float)r.y, T::LOW_DOWN, (float)h.y) * f, i, x, T::LOW_UP);
+        }
     } else
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x[i] = __builtin_amdgcn_perm(__float_as_uint(__uint_as_float(x[i] & 0xffff0000u) * f), __float_as_uint(__uint_as_float(x[i] << 16) * f), 0x07060302);
+        for (int k = 0; k < NP; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[k][i] = __builtin_amdgcn_perm(__float_as_uint(__uint_as_float(x[k][i] & 0xffff0000u) * f), __float_as_uint(__uint_as_float(x[k][i] << 16) * f), 0x07060302);
 }
 // 8 cached values (16 or 32 bytes) as parts
 template <int TYPE>

@@ -27,6 +27,7 @@ struct Dec {
     static constexpr int W = ES / 2;             // 16-byte words of 8 values
     static constexpr int KS = (HD + 31) / 32;    // steps of 32 along the head
     static constexpr int VB = HD / 16;           // blocks of 16 of V's values
+    static constexpr bool LOW = PagedType<TYPE>::LOW > 0;  // the weights' second parts are summed by themselves
     static constexpr int OCC = dec_resident(TYPE, HD);
 };
 
@@ -144,9 +145,9 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         score = paged_score(a, head, size);
     }
 
-    pf4 acc[D::VB];
+    pf4 acc[D::VB], low[D::VB];
 #pragma unroll
-    for (int b = 0; b < D::VB; ++b) acc[b] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b = 0; b < D::VB; ++b) acc[b] = low[b] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
     float c = __FLT_MAX__, l = 0.0f;  // c = PBIAS - m
 
     for (; st < end; st += 4) {
@@ -220,7 +221,10 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
                 c = cn;
                 l *= f;
 #pragma unroll
-                for (int b = 0; b < D::VB; ++b) acc[b] *= f;
+                for (int b = 0; b < D::VB; ++b) {
+                    acc[b] *= f;
+                    if (D::LOW) low[b] *= f;
+                }
             }
         }
         float p[8];
@@ -230,7 +234,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
             l += p[e];
         }
         pu4 pp[D::NQ];
-        parts8<TYPE, D::NQ>(p, pp);
+        parts8<TYPE, D::NQ>(p, pp, PagedType<TYPE>::LOW_UP);
 #pragma unroll
         for (int b = 0; b < D::VB; ++b) {
             pu4 vp[D::NK];
@@ -239,7 +243,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
             for (int x = D::NQ - 1; x >= 0; --x)
 #pragma unroll
                 for (int y = D::NK - 1; y >= 0; --y)
-                    if (x + y < 3) mma16<TYPE>(acc[b], vp[y], pp[x]);
+                    if (x + y < 3) mma16<TYPE>(D::LOW && x > 0 ? low[b] : acc[b], vp[y], pp[x]);
         }
         if (more) {
             load_v(st + 4);
@@ -267,6 +271,9 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         }
     }
 
+    if (D::LOW)
+#pragma unroll
+        for (int b = 0; b < D::VB; ++b) acc[b] += low[b] * PagedType<TYPE>::LOW_DOWN;
     // the row's sum over its four lanes, then the four wavefronts' sums
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);

@@ -11,10 +11,14 @@
 // 16-byte words of a row are kept in LDS at (word ^ row), so that lanes that read the same word of neighbouring rows
 // meet in no bank.
 //
+// F16's sums over the weights' second halves are formed apart (fgh_pattn.h), by blocks of 32 values, each over the whole tile and added to the
+// others while the next one's products run: registers for all of them at once there are none, and added per 32 positions they would take
+// twice the vector instructions.
+//
 // Bound by the matrix pipe, for the 2 (F16) to 6 (F32) products that an fp32 result takes: 8192 tokens, f16, 32 heads over 8, hd 128 take
-// 924 to 1085 us by the card's clock: 1.19 to 1.01 PFLOP/s of products, 1.15 for a large f16 matrix product here, with the clock held
+// 985 to 1000 us by the card, 1.12 PFLOP/s of products, 1.15 for a large f16 matrix product here, with the clock held
 // down by power. Small batches are bound by what a tile costs a wavefront that is alone on its SIMD (64 tokens behind
-// 4032: 23.6 us; asking for the next tile took 1500 of a tile's 5500 cycles there before its loads' places were formed from
+// 4032: 27.5 us with the join; asking for the next tile took 1500 of a tile's 5500 cycles there before its loads' places were formed from
 // one lane's by other bits). Three tiles deep gained nothing there: the tiles are in time.
 #pragma once
 
@@ -234,7 +238,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         l += v;
         asm volatile("" : "+v"(v), "+v"(l));  // here, not where they are used
         if (e % 2 == 1) {
-            parts2<TYPE, P::NQ>(w.v[e / 8][e % 8 - 1], v, e % 8 / 2, w.pp[e / 8]);
+            parts2<TYPE, P::NQ>(w.v[e / 8][e % 8 - 1], v, e % 8 / 2, w.pp[e / 8], PagedType<TYPE>::LOW_UP);
 #pragma unroll
             for (int i = 0; i < P::NQ; ++i) {
                 uint32_t z = w.pp[e / 8][i][e % 8 / 2];
@@ -287,10 +291,14 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 #pragma unroll
             for (int w = 0; w < W; ++w) raw[ks % SLOTS][w] = *(const pu4 *)(buf + (k_lane ^ (2 * ks * W + w) * 16) + h * 32 * P::KW * 16);
         };
-        auto read_v = [&](int x) {  // x: 16-position run, then block of values
-            const int k = x / P::VB, b = x % P::VB;
+        // V's words of the tile, in the order in which they are used: a block of positions' runs of 16, the blocks of values of each;
+        // where the weights' second parts are summed by themselves (LOW) the first block so, then both by blocks of values
+        constexpr bool LOW = PagedType<TYPE>::LOW > 0;
+        constexpr int NX = 2 * P::VB, NA = LOW && NH == 1 ? 0 : LOW ? NX : NH * NX, NV = NA + (LOW ? NH * NX : 0);
+        auto read_v = [&](int y) {
+            const int k = y < NA ? y / P::VB : (y - NA) % (2 * NH), b = y < NA ? y % P::VB : (y - NA) / (2 * NH);
 #pragma unroll
-            for (int w = 0; w < W; ++w) raw[x % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ (2 * k * W + w) * 16) + b * 32 * P::VW * 16);
+            for (int w = 0; w < W; ++w) raw[y % SLOTS][w] = *(const pu4 *)(buf + (v_lane ^ (2 * k * W + w) * 16) + b * 32 * P::VW * 16);
         };
         constexpr int NPROD = PagedType<TYPE>::NPROD;
         auto beside = [&](int m, int of, auto side) {  // product m of `of`: its share of the 16 weights beside it
@@ -325,23 +333,52 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 #pragma unroll
             for (int e = 0; e < 16; ++e) out.v[e / 8][e % 8] = P::PW == 1 ? sc[e] : sc[e] + rest[e];
         };
-        constexpr int NX = 2 * P::VB;  // V words of a block
         auto sums = [&](int h, const Weights &w, auto side) {
+            constexpr int NS = LOW ? 1 : NPROD;  // products of a word
             int m = 0;
 #pragma unroll
             for (int x = 0; x < NX; ++x) {
-                if (h * NX + x + AHEAD < NH * NX) read_v(h * NX + x + AHEAD);
+                const int at = h * NX + x;
+                if (at + AHEAD < NV) read_v(at + AHEAD);
                 pu4 vp[P::NK];
-                cache8<TYPE>(raw[(h * NX + x) % SLOTS], vp);
+                cache8<TYPE>(raw[at % SLOTS], vp);
 #pragma unroll
                 for (int i = P::NQ - 1; i >= 0; --i)
 #pragma unroll
                     for (int y = P::NK - 1; y >= 0; --y)
-                        if (i + y < 3) {
+                        if (i + y < 3 && !(LOW && i > 0)) {
                             mma32<TYPE>(acc[x % P::VB], vp[y], w.pp[x / P::VB][i]);
-                            beside(m++, NX * NPROD, side);
+                            beside(m++, NX * NS, side);
                         }
             }
+        };
+        // what is left of the tile's sums, by blocks of values: those of the second parts, added while the next block's are formed, and
+        // those of the first parts that `sums` has not taken
+        auto sums_low = [&](const Weights &w0, const Weights &w1) {
+            pf16 low[2];
+            auto add = [&](int b, int r) { acc[b][r] = __builtin_fmaf(low[b % 2][r], PagedType<TYPE>::LOW_DOWN, acc[b][r]); };
+#pragma unroll
+            for (int b = 0; b < P::VB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) low[b % 2][r] = 0.0f;
+                int m = 0;
+#pragma unroll
+                for (int k = 0; k < 2 * NH; ++k) {
+                    const int at = NA + b * 2 * NH + k;
+                    if (at + AHEAD < NV) read_v(at + AHEAD);
+                    const Weights &w = k < 2 ? w0 : w1;
+#pragma unroll
+                    for (int i = 1; i >= 0; --i)
+                        if (i == 1 || k >= 2 * NH - 2) {
+                            mma32<TYPE>(i == 1 ? low[b % 2] : acc[b], raw[at % SLOTS][0], w.pp[k % 2][i]);
+                            beside(m++, 2 * NH + 2, [&](int e) {
+                                if (b > 0) add(b - 1, e);
+                            });
+                        }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add(P::VB - 1, r);
         };
         auto first_v = [&]() {
 #pragma unroll
@@ -356,7 +393,8 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         if constexpr (NH == 1) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) weigh(w0, e);
-            sums(0, w0, alone);
+            if constexpr (LOW) sums_low(w0, w0);
+            else sums(0, w0, alone);
         } else {
             Weights w1;
             scores(1, w1, [&](int e) { weigh(w0, e); });
@@ -365,12 +403,11 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
             if (__builtin_amdgcn_ballot_w64(top1 + c > PagedType<TYPE>::PTOP)) {  // block 0's weights wait for their sums
                 const float f = follow(top1);
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-                    for (int i = 0; i < P::NQ; ++i) scale8<TYPE>(w0.pp[kk][i], f);
+                for (int kk = 0; kk < 2; ++kk) scale8<TYPE, P::NQ>(w0.pp[kk], f);
             }
             sums(0, w0, [&](int e) { weigh(w1, e); });
-            sums(1, w1, alone);
+            if constexpr (LOW) sums_low(w0, w1);
+            else sums(1, w1, alone);
         }
     };
 

@@ -281,10 +281,13 @@ FGH_API int fgh_kvq_attention_dev(fgh_ctx *ctx, int n_tok, int n_head, int n_hea
  * stand between the QKV and the O projection of a layer: the append of a batch's keys and values
  * with the head norms and the position rotation (the reference's rope, for GGUF's rope types), and
  * the attention over the pages. Activations are fp32, as everywhere here; results agree with the
- * formulas to within 1e-5 relative per output vector, as long as fp32 scores do (a weight is off by its score's
- * rounding: scores of hundreds cost as many 2^-24). Both calls are asynchronous on the context's
- * stream and can be captured (the attention's scratch must have its size from an eager call with the same
- * sizes in the descriptors before: fewer sequences or rows can take more).
+ * formulas to within 1e-5 relative per output vector, as long as fp32 scores do (a weight is off by its
+ * score's rounding: scores of hundreds cost as many 2^-24). With an F16 cache q counts to 2^-40 of a row's
+ * largest value, and a weight to 2^-48 of the row's largest: an output at 2^-31 and less of the values that
+ * its row sees, left by a largest weight whose v is 0, keeps fewer bits.
+ * Both calls are asynchronous on the context's stream and can be captured (the attention's scratch must
+ * have its size from an eager call with the same sizes in the descriptors before: fewer sequences or
+ * rows can take more).
  *
  * The cache: n_pages pages for `page` positions of n_head_kv heads of hd values of `type` (FGH_T_F32,
  * FGH_T_F16 or FGH_T_BF16). K page: [n_head_kv][page][hd]; V page, transposed: [n_head_kv][hd][page].

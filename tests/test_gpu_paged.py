@@ -749,3 +749,58 @@ def test_refusals(backend):
             refused(st, word)
             setattr(cache, field, old)
         at()
+
+
+# ---- weights far below the row's largest ----
+
+def with_null_key(t, news, lens, gap, at, hd=128, n_kv=2, group=2):
+    """A batch whose rows all see one key (position `at` of every sequence long enough) that scores `gap` above the others and whose V is 0,
+    so that the others, exp(-gap) of it, make the output. q and that key are few-bit numbers: their product is exact."""
+    b = Batch(80 + news[0], t, hd, group * n_kv, n_kv, 16, news, lens, sigma=0.1)
+    sign = np.where(b.rng.random(hd) < 0.5, -1.0, 1.0)
+    b.q[:] = sign
+    scale = 0.125 if hd < 256 else 0.0625
+    size = round(gap / (hd * scale) * 256) / 256
+    for s, (n, m) in enumerate(zip(news, lens)):
+        if m - n < at:
+            continue
+        for h in range(n_kv):
+            b.k[b.at(s, at, h, False)] = encode(sign * size, t)
+            b.v[b.at(s, at, h, True)] = 0
+    return b, scale
+
+
+NULL_KEYS = [  # new tokens, lengths, position of the key
+    ([1], [120], 0), ([1], [120], 100), ([1], [600], 37), ([4], [300], 2),  # few rows
+    ([1] * 140, [130] * 140, 5), ([1] * 140, [130] * 140, 64),  # so many that no range is split
+    ([40], [100], 0), ([40], [600], 33), ([20], [64], 40),  # prompts
+    ([20] * 260, [64] * 260, 40), ([20] * 260, [64] * 260, 3), ([20] * 260, [60] * 260, 36),  # that fill the device: 128 rows, ranges whole
+]
+
+
+def of_vectors(o, want):
+    """The largest error of a row and head, relative to that vector's length."""
+    return float((np.linalg.norm(o - want, axis=-1) / np.linalg.norm(want, axis=-1)).max())
+
+
+@pytest.mark.parametrize("gap", [12, 14, 16, 18, 20, 22])
+@pytest.mark.parametrize("i", range(len(NULL_KEYS)))
+def test_attention_null_key(backend, i, gap):
+    """Weights of a row's output at 2^-17 to 2^-32 of its largest: 1e-5 per output vector, as everywhere. (Of the 1e-5: a weight at
+    2^-31.7 of the largest is off by at most 2^-48 of it, evenly spread, which is 2^-16.3 / sqrt(3) = 7.3e-6 of a sum over
+    many; the factor of a score of 31.7 powers of two rounded to fp32 is 31.7 ln 2 2^-24 = 1.3e-6.)"""
+    b, scale = with_null_key(T_F16, *NULL_KEYS[i][:2], gap, NULL_KEYS[i][2])
+    o = run_attention(backend, b, scale=scale)
+    want, _, _ = attention(b, b.q, scale)
+    assert of_vectors(o, want) <= 1e-5
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("hd", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("news,lens,at", [([1], [200], 7), ([40], [200], 7), ([20] * 260, [64] * 260, 40)])
+def test_attention_null_key_types(backend, t, hd, news, lens, at):
+    """The same for every type and head size, at a gap of 20."""
+    b, scale = with_null_key(t, news, lens, 20, at, hd=hd)
+    o = run_attention(backend, b, scale=scale)
+    want, _, _ = attention(b, b.q, scale)
+    assert of_vectors(o, want) <= 1e-5
