@@ -48,6 +48,30 @@ __device__ __forceinline__ PagedSeq paged_useq(const Paged &a, int s) {
     q.ok = __builtin_amdgcn_readfirstlane(q.ok);
     return q;
 }
+// The rows that lane i's sequence, of 64 in order, has for itself: not those below the start of an earlier one (`top`: of the
+// sequences before the 64, 0 at first). Only where starts decrease there are such: rows that are in two sequences, or in none. What is left of
+// the sequences is then disjoint, so that launches sized by n_tok hold all of it; positions do not change, since the first rows go.
+__device__ __forceinline__ void paged_own_rows(const Paged &a, int s, PagedSeq &q, int &top) {
+    const bool falls = s < a.n_seq && a.tok[s + 1] < a.tok[s];
+    int m = q.t0;  // 0 behind the last sequence
+    if (__builtin_amdgcn_ballot_w64(falls) || __builtin_amdgcn_readfirstlane(m) < top) {
+        const int lane = threadIdx.x & 63;
+        for (int o = 1; o < 64; o <<= 1) m = max(m, __shfl_up(m, o, 64));  // lanes below o get their own
+        const int before = __shfl_up(m, 1, 64), from = max(q.t0, max(lane > 0 ? before : 0, top));
+        q.n = max(q.t0 + q.n - from, 0);
+        q.t0 = from;
+    }
+    top = max(top, __builtin_amdgcn_readlane(m, 63));
+}
+// the same for one sequence s, uniform
+__device__ __forceinline__ void paged_own_rows(const Paged &a, int s, PagedSeq &q) {
+    int m = q.t0;
+    for (int i = threadIdx.x & 63; i < s; i += 64) m = max(m, min(a.tok[i], a.n_tok));
+    for (int o = 1; o < 64; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
+    const int from = __builtin_amdgcn_readfirstlane(m);
+    q.n = max(q.t0 + q.n - from, 0);
+    q.t0 = from;
+}
 // the sequence of row t, or -1: the last s with tok[s] <= t, if t < tok[s + 1]. Every wavefront finds
 // it for itself, 64 starts a load.
 __device__ __forceinline__ int paged_find(const Paged &a, int t) {
@@ -74,15 +98,16 @@ struct PagedVTile {
 };
 __device__ __forceinline__ PagedVTile paged_vtile(const Paged &a, int index) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    int before = 0, top = 0;
     PagedVTile t;
     t.s = -1, t.base = 0, t.q = PagedSeq{};
     for (int b = 0; b < a.n_seq; b += 64) {
         const int s = b + lane;
         int own = 0, first = 0;
         PagedSeq q{};
+        if (s < a.n_seq) q = paged_seq(a, s);
+        paged_own_rows(a, s, q, top);
         if (s < a.n_seq) {
-            q = paged_seq(a, s);
             first = (q.len - q.n) / 64;
             own = q.n > 0 && q.ok ? (q.len - 1) / 64 - first + 1 : 0;
         }

@@ -266,15 +266,16 @@ struct PagedTile {
 };
 __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs &a, int tile_rows, int index) {
     const int lane = threadIdx.x & 63, G = a.n_head / a.p.n_head_kv;
-    int before = 0;  // tiles of the sequences before the 64 looked at
+    int before = 0, top = 0;  // tiles of the sequences before the 64 looked at
     PagedTile t;
     t.s = -1, t.r0 = 0, t.index = index, t.q = PagedSeq{};
     for (int b = 0; b < a.p.n_seq; b += 64) {
         const int s = b + lane;
         int own = 0;
         PagedSeq q{};
+        if (s < a.p.n_seq) q = paged_seq(a.p, s);
+        paged_own_rows(a.p, s, q, top);
         if (s < a.p.n_seq) {
-            q = paged_seq(a.p, s);
             const int64_t rows = (int64_t)q.n * G;
             own = a.ds > 0 && rows <= DEC_ROWS ? 0 : (int)((rows + tile_rows - 1) / tile_rows);
         }

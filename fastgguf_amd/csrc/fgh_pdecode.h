@@ -42,9 +42,11 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
     const int nkv = a.p.n_head_kv, G = a.n_head / nkv;
     const int kvh = block % nkv, split = block / nkv % a.ds, s = block / nkv / a.ds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const PagedSeq q = paged_useq(a.p, s);
+    PagedSeq q = paged_useq(a.p, s);
+    // the prompt kernel's, unless starts decrease and only few of the rows are the sequence's own
+    if (a.ps > 0 && (int64_t)q.n * G > DEC_ROWS) paged_own_rows(a.p, s, q);
     const int64_t rows = (int64_t)q.n * G;
-    const bool none = q.n == 0 || (a.ps > 0 && rows > DEC_ROWS);  // the prompt kernel's
+    const bool none = q.n == 0 || (a.ps > 0 && rows > DEC_ROWS);
     if (a.ds > 1 && split == 0 && tid == 0 && (none || !q.ok)) a.dsum.info[s * nkv + kvh].used = 0;
     if (none) return;
     if (!q.ok) {

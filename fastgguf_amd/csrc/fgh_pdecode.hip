@@ -10,6 +10,7 @@ namespace {
 template <int TYPE, int HD>
 __global__ __launch_bounds__(256, (Dec<TYPE, HD>::OCC)) void paged_decode_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    a.ps = 0;  // as the plan says: without what only batches with prompts need
     paged_decode_block<TYPE, HD>(a, blockIdx.x, lds);
 }
 

@@ -311,7 +311,8 @@ typedef struct {
  * sequence's new tokens and length. As these stay on the device, a sequence that breaks a bound
  * (more than max_tok tokens, len above max_len or the table's positions or below its
  * number of tokens, rows outside 0 .. n_tok) is no error: its rows are NaN and nothing is appended.
- * tok is read as non-decreasing: rows in two sequences of one that is not hold anything. */
+ * tok is read as non-decreasing. Where it decreases, rows that are in two sequences, before tok[0] or from
+ * tok[n_seq] on hold anything, and so do their places in the pages; the other rows are as ever. */
 typedef struct {
     const int32_t *tok;     /* device, [n_seq + 1] */
     const int32_t *len;     /* device, [n_seq] */

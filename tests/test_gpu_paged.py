@@ -804,3 +804,58 @@ def test_attention_null_key_types(backend, t, hd, news, lens, at):
     o = run_attention(backend, b, scale=scale)
     want, _, _ = attention(b, b.q, scale)
     assert of_vectors(o, want) <= 1e-5
+
+
+# ---- starts that decrease ----
+
+def falling(t, tok, pasts, hd=64, n_head=2, n_kv=1):
+    """A batch of these starts, and of every row whether it is in one sequence only."""
+    n_tok = max(tok)
+    news = [max(0, e - s) for s, e in zip(tok, tok[1:])]
+    b = Batch(90, t, hd, n_head, n_kv, 32, news, [n + p for n, p in zip(news, pasts)])
+    b.tok, b.n_tok, b.q = np.array(tok, np.int32), n_tok, b.q[:n_tok]
+    times = np.zeros(n_tok, int)
+    for s, e in zip(tok, tok[1:]):
+        times[s:e] += 1
+    once = times == 1
+    once[tok[-1]:] = False
+    return b, once
+
+
+FALLS = [  # starts, cached positions, query heads
+    ([0, 900, 100, 1000], [0, 0, 0], 2),  # more tiles of rows and of positions than 1000 tokens have otherwise
+    ([0, 40, 30, 50, 46, 70], [0, 0, 100, 0, 5], 1),  # the third sequence's 20 rows, 10 of them its own
+    ([0, 40, 30, 50, 46, 70], [2000, 0, 1500, 0, 5], 1),  # in several splits
+    ([v + 70 * i for i in range(30) for v in (0, 40, 30, 50, 46)] + [2100], [3, 0, 40, 0, 5] * 30, 1),  # more than 64 sequences
+]
+
+
+@pytest.mark.parametrize("i", range(len(FALLS)))
+@pytest.mark.parametrize("broken", [False, True])
+def test_falling_starts(backend, i, broken):
+    """Rows that are in one sequence are appended, keys and values, and attended, however many tiles the others make; a broken
+    sequence's are NaN and not appended."""
+    tok, pasts, nh = FALLS[i]
+    b, once = falling(T_F16, tok, pasts, n_head=nh)
+    max_len = max(b.lens)
+    want, tol, _ = attention(b, b.q, 0.125)
+    bad = np.zeros(b.n_tok, bool)
+    if broken:
+        bad[b.tok[2]:b.tok[3]] = True
+        b.len[2] = max_len + 1
+    o = run_attention(backend, b, scale=0.125, max_len=max_len)
+    assert np.isnan(o[once & bad]).all()
+    fine = once & ~bad
+    assert (np.abs(o - want)[fine] <= tol[fine]).all()
+    qkv = b.rng.standard_normal((b.n_tok, nh + 2, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b, max_len=max_len)
+        x, od, row = d.put(qkv), d.put(np.full((b.n_tok, nh, 64), 777.0, np.float32)), (nh + 2) * 64
+        backend.paged_store_dev(cache, batch, PagedRope(), nh, x, row, x + 256 * nh, x + 256 * (nh + 1), row, od, 64 * nh)
+        got, kc, vc = d.get(od, np.zeros((b.n_tok, nh, 64), np.float32)), d.get(cache.k, b.k), d.get(cache.v, b.v)
+    assert np.array_equal(got[fine], qkv[fine][:, :nh]) and np.isnan(got[once & bad]).all()
+    for t, s, pos in b.tokens():
+        if once[t]:
+            for h, is_v, code, old in ((nh, False, kc, b.k), (nh + 1, True, vc, b.v)):
+                at = b.at(s, pos, 0, is_v)
+                assert np.array_equal(code[at], old[at] if bad[t] else encode(qkv[t, h], T_F16)), (t, s, pos, is_v)
