@@ -151,6 +151,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
 #pragma unroll
     for (int b = 0; b < D::VB; ++b) acc[b] = low[b] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
     float c = __FLT_MAX__, l = 0.0f;  // c = PBIAS - m
+    bool big = false;                 // a reference beyond SCORE_BIG
 
     for (; st < end; st += 4) {
         const int kb = base + st * DEC_STEP, j0 = kb + quad * 8;
@@ -175,7 +176,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sc[e / 4][e % 4] + rest[e / 4][e % 4];
-        const float mul = score.apply(v, j0, pos);
+        float mul = score.apply(v, j0, pos);
         // positions that some row does not see: at the ends of the ranges
         const bool whole = kb >= sp.in_lo && kb + DEC_STEP - 1 <= sp.in_hi && !__builtin_amdgcn_ballot_w64(bad);
         bool odd = false;  // a V value that only some rows see is not finite
@@ -218,8 +219,9 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         if (__builtin_amdgcn_ballot_w64(top + c > PagedType<TYPE>::PTOP)) {
             float mx = fmaxf(top, __shfl_xor(top, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && fabsf(mx) > SCORE_BIG) != 0;
             if (mx + c > PagedType<TYPE>::PTOP) {  // of the whole row: its four lanes agree
-                const float cn = PagedType<TYPE>::PBIAS - mx, f = __builtin_amdgcn_exp2f(cn - c);
+                const float cn = score_bias<TYPE>(mx) - mx, f = __builtin_amdgcn_exp2f(cn - c);
                 c = cn;
                 l *= f;
 #pragma unroll
@@ -228,6 +230,11 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
                     if (D::LOW) low[b] *= f;
                 }
             }
+        }
+        if (big) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= mul;
+            mul = 1.0f;
         }
         float p[8];
 #pragma unroll

@@ -269,12 +269,14 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         for (int e = 1; e < 16; ++e) top = fmaxf(top, w.v[e / 8][e % 8]);
         return top * w.mul;
     };
+    bool big = false;  // a reference beyond SCORE_BIG
     // the row's reference follows a larger score, in whole powers of two; the factor of what was formed before
     auto follow = [&](float top) {
         const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
         float f = 1.0f;
+        big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && fabsf(mx) > SCORE_BIG) != 0;
         if (mx + c > PagedType<TYPE>::PTOP) {
-            const float cn = PagedType<TYPE>::PBIAS - ceilf(mx);
+            const float cn = score_bias<TYPE>(mx) - ceilf(mx);
             f = __builtin_amdgcn_exp2f(cn - c);
             c = cn;
             l *= f;
@@ -282,6 +284,13 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
             for (int b = 0; b < P::VB; ++b) acc[b] *= f;
         }
         return f;
+    };
+    auto round_big = [&](Weights &w) {
+        if (big) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w.v[e / 8][e % 8] *= w.mul;
+            w.mul = 1.0f;
+        }
     };
     auto tile = [&](const uint8_t *buf, bool whole) {
         uint32_t k_lane = k_at, v_lane = v_at;
@@ -390,6 +399,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
         if constexpr (NH == 1) first_v();
         const float top0 = forms(w0, kb + pg * 32, whole);
         if (__builtin_amdgcn_ballot_w64(top0 + c > PagedType<TYPE>::PTOP)) follow(top0);
+        round_big(w0);
         if constexpr (NH == 1) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) weigh(w0, e);
@@ -405,6 +415,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) scale8<TYPE, P::NQ>(w0.pp[kk], f);
             }
+            round_big(w1);
             sums(0, w0, [&](int e) { weigh(w1, e); });
             if constexpr (LOW) sums_low(w0, w1);
             else sums(1, w1, alone);

@@ -859,3 +859,41 @@ def test_falling_starts(backend, i, broken):
             for h, is_v, code, old in ((nh, False, kc, b.k), (nh + 1, True, vc, b.v)):
                 at = b.at(s, pos, 0, is_v)
                 assert np.array_equal(code[at], old[at] if bad[t] else encode(qkv[t, h], T_F16)), (t, s, pos, is_v)
+
+
+# ---- scores of millions and more ----
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("news,lens", [([1, 3], [70, 3000]), ([40], [90]), ([20] * 260, [64] * 260)])
+def test_attention_huge_scores(backend, t, size, news, lens):
+    """Scores whose fp32 steps are powers of two apart: a row is the value at its largest score, as it is in fp32, where the next one is
+    out of the scores' rounding (72 roundings of the largest sum of products, for 64 and the forms) and 30 more away.
+    Its weight times that value, over the weight: 2^-21 for the products that an F32 cache leaves out (parts of w and v of 2^-7 and 2^-15
+    of them: 2 x 2^-22), 8 roundings of the 6 products' sum, the weights' sum, its reciprocal and the last product: 2^-20 in all."""
+    b = Batch(95, t, 64, 4, 2, 16, news, lens)
+    b.q = (b.q * (size / 8)).astype(np.float32)
+    rows = [r for r in b.tokens() if r[0] % 7 == 0 or len(news) < 3]
+    keys = {(s, h): (b.rows(s, h, False), b.rows(s, h, True)) for s in {r[1] for r in rows} for h in range(2)}
+    for kw in ({}, {"slopes": np.float32([0.0, size / 100, size, size * 10])}, {"softcap": 1e15}):
+        o = run_attention(backend, b, scale=1.0, **kw)
+        assert np.isfinite(o).all()
+        if "softcap" in kw and size > 1e12:
+            continue  # all at the cap: any of them
+        clear = 0
+        for row, s, p in rows:
+            for h in range(4):
+                k, v = (x[:p + 1] for x in keys[s, h // 2])
+                z = k @ b.q[row, h].astype(np.float64)
+                off = 72 * 2.0**-24 * (np.abs(k) @ np.abs(b.q[row, h])).max()
+                if "softcap" in kw:
+                    z = 1e15 * np.tanh(z / 1e15)
+                if "slopes" in kw:
+                    z = z - np.float64(kw["slopes"][h]) * (p - np.arange(p + 1))
+                    off += 72 * 2.0**-24 * np.abs(z).max()
+                order = np.argsort(z)
+                if p == 0 or z[order[-1]] - z[order[-2]] > 2 * off + 30:
+                    clear += 1
+                    want = v[order[-1]]
+                    assert (np.abs(o[row, h] - want) <= 2.0**-20 * np.abs(want) + 1e-9).all(), (row, h)
+        assert clear > len(rows)
