@@ -174,8 +174,8 @@ __device__ __forceinline__ float score_bias(float mx) { return fabsf(mx) > SCORE
 // What turns a row's products into scores in powers of two, s = v mul: v the products or, capped, their tanh, mul apply's result. The
 // product with mul is rounded once, in the sum that follows it.
 struct PagedScore {
-    float mul;             // |scale| log2(e), times the power of two that q was divided by; above 0, so that -inf v
-                           // are -inf scores (q takes the scale's sign, and a scale of 0 is 2^-126 here)
+    float mul;             // |scale| log2(e), times the power of two that q was divided by; above 0 and finite, so that -inf v
+                           // are -inf scores and 0 is 0 (q takes the scale's sign, and is 0 for a scale of 0)
     float cap_in, cap_out; // |scale| / softcap (with that power), softcap log2(e); cap_out 0: none
     float slope, down;     // |slopes[h]| log2(e), and -1 or 1 with the slope's sign turned around
     bool bias;
@@ -210,8 +210,9 @@ struct PagedScore {
 };
 __device__ __forceinline__ PagedScore paged_score(const PagedAttnArgs &a, int head, float q_size) {
     PagedScore c;
-    c.mul = fmaxf(fabsf(a.scale) * LOG2E * q_size, __FLT_MIN__);
-    c.cap_in = a.softcap > 0.0f ? fabsf(a.scale) / a.softcap * q_size : 0.0f;
+    const float scale = fabsf(a.scale) * q_size;
+    c.mul = fminf(fmaxf(scale * LOG2E, __FLT_MIN__), __FLT_MAX__);
+    c.cap_in = a.softcap > 0.0f ? fminf(scale / a.softcap, __FLT_MAX__) : 0.0f;
     c.cap_out = a.softcap * LOG2E;
     c.bias = a.slopes != nullptr;
     const float slope = c.bias ? a.slopes[head] : 0.0f;
@@ -226,6 +227,12 @@ __device__ __forceinline__ float row_size(float amax) {
     const uint32_t e = __float_as_uint(amax) >> 23;
     return e == 255 ? 1.0f : __uint_as_float((e > 15 ? e - 14 : 1u) << 23);
 }
+
+// that power of two where q keeps its size (not F16): with scales below 2^-64 q and the scale meet halfway, since products
+// of up to 2^128 would otherwise meet a factor below an fp32's normal ones
+__device__ __forceinline__ float scale_size(float scale) { return fabsf(scale) < 0x1p-64f ? 0x1p64f : 1.0f; }
+// and what q is multiplied by
+__device__ __forceinline__ float q_factor(float scale, float size) { return (scale < 0.0f ? -1.0f : scale > 0.0f ? 1.0f : 0.0f) / size; }
 
 // positions lo .. hi that the new tokens i0 .. i1 of a sequence see, and those that all of them see
 struct PagedSpan {

@@ -131,13 +131,13 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         for (int ks = 0; ks < D::KS; ++ks)
 #pragma unroll
             for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[ks][e]));
-        float size = 1.0f;
+        float size = scale_size(a.scale);
         if constexpr (TYPE == T_F16) {
             amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
             amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
             size = row_size(amax);
         }
-        const float inv = (a.scale < 0.0f ? -1.0f : 1.0f) / size;
+        const float inv = q_factor(a.scale, size);
 #pragma unroll
         for (int ks = 0; ks < D::KS; ++ks) {
 #pragma unroll

@@ -173,7 +173,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     pu4 qp[P::KS][P::NQ];
     PagedScore score;
     {
-        float size = 1.0f;
+        float size = scale_size(a.scale);
         if constexpr (TYPE == T_F16) {  // the rows' largest magnitudes
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -188,7 +188,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
             }
             size = row_size(((const float *)own)[lane & 31]);
         }
-        const float inv = (a.scale < 0.0f ? -1.0f : 1.0f) / size;
+        const float inv = q_factor(a.scale, size);
 #pragma unroll
         for (int g = 0; g < QP; ++g) {
 #pragma unroll

@@ -897,3 +897,37 @@ def test_attention_huge_scores(backend, t, size, news, lens):
                     want = v[order[-1]]
                     assert (np.abs(o[row, h] - want) <= 2.0**-20 * np.abs(want) + 1e-9).all(), (row, h)
         assert clear > len(rows)
+
+
+# ---- scales at the ends of their range ----
+
+@pytest.mark.parametrize("t,k_size", [(T_F16, 1e4), (T_BF16, 1e18), (T_F32, 1e18)])
+@pytest.mark.parametrize("scale", [0.0, 1e-36, -1e-37, 1e-39, -2e-42])
+@pytest.mark.parametrize("news,lens", [([1, 3], [70, 3000]), ([40], [90]), ([20] * 260, [64] * 260)])
+def test_attention_tiny_scales(backend, t, k_size, scale, news, lens):
+    """Products near an fp32's largest, by scales near or below its smallest normal number, and by 0."""
+    b = Batch(96, t, 64, 4, 2, 16, news, lens)
+    b.k = encode(decode(b.k, t) * k_size, t)
+    b.q = (b.q * (1e36 / k_size)).astype(np.float32)
+    check_attention(backend, b, scale=scale)
+    check_attention(backend, b, scale=scale, softcap=0.5)
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("news,lens", [([1, 3], [70, 3000]), ([40], [90])])
+@pytest.mark.parametrize("softcap", [0.0, 1e-15])
+def test_attention_zero_products(backend, t, softcap, news, lens):
+    """Products that are 0 are scores of 0 at the largest scale and queries too: beside others that the cap makes +-1e-15, or alone."""
+    b = Batch(97, t, 64, 4, 2, 16, news, lens)
+    for s, m in enumerate(lens):
+        for pos in range(m):
+            for h in range(2):
+                if pos % 3 == 0 or not softcap:
+                    b.k[b.at(s, pos, h, False)] = 0
+    b.q = (b.q * 1e30).astype(np.float32) if t == T_F16 else b.q
+    o = run_attention(backend, b, scale=1e15, softcap=softcap)
+    for row, s, p in b.tokens():
+        for h in range(4):
+            v = b.rows(s, h // 2, True)[:p + 1]
+            # all weights the same: off by 16 roundings as in the others' bound
+            assert (np.abs(o[row, h] - v.mean(0)) <= 32 * 2.0**-24 * np.abs(v).mean(0)).all()
