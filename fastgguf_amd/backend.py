@@ -33,7 +33,7 @@ EXPORTS = (
     "fgh_dev_alloc", "fgh_dev_free", "fgh_copy_h2d", "fgh_copy_d2h", "fgh_copy_d2d", "fgh_checksum_dev", "fgh_memcpy_dev", "fgh_mfma_peak_dev", "fgh_sync",
     "fgh_event_create", "fgh_event_record", "fgh_event_elapsed_ms", "fgh_event_destroy",
     "fgh_quantize", "fgh_block_ints", "fgh_gemm_block_ints", "fgh_moe_block_ints", "fgh_expf", "fgh_fp16_to_f32", "fgh_matvec_shape", "fgh_matmul_path",
-    "fgh_paged_slot", "fgh_paged_check",
+    "fgh_paged_slot", "fgh_paged_check", "fgh_paged_plan",
     "fgh_gguf_open", "fgh_gguf_close", "fgh_gguf_summary", "fgh_gguf_tensor", "fgh_gguf_find",
     "fgh_gguf_kv_num", "fgh_gguf_kv_str", "fgh_gguf_data", "fgh_upload_gguf",
 )
@@ -110,6 +110,17 @@ def paged_check(cache: PagedCache, batch: PagedBatch, n_head: int, *, rope: Page
     return "" if rc == OK else err.value.decode()
 
 
+def paged_plan(cache: PagedCache, batch: PagedBatch, n_head: int, mask: PagedMask, num_cu: int = 256) -> tuple[int, int, int, bool]:
+    """What the paged attention launches (no device needed): the splits of the kernel for sequences with few rows
+    (0: not launched), those of the prompt kernel, its rows a workgroup, and whether one of them has a compute unit
+    for itself."""
+    plan = np.zeros(4, np.int32)
+    rc = load_library().fgh_paged_plan(C.byref(cache), C.byref(batch), C.byref(mask), n_head, num_cu, _p(plan))
+    if rc != OK:
+        raise BackendError(rc, "paged_plan: bad arguments")
+    return int(plan[0]), int(plan[1]), int(plan[2]), bool(plan[3])
+
+
 def paged_slot(cache: PagedCache, table: np.ndarray, seq: int, pos: int, head: int, d: int, v: bool = False) -> int:
     """The offset in values at which the paged kernels find value d of a head of a position in the K (or
     V) pages, or -1 where they read and write nothing; table: host int32 [n_seq][table_stride] (no device needed)."""
@@ -162,6 +173,7 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "fgh_paged_slot": (i64, [C.POINTER(PagedCache), vp, i32, i32, i32, i32, i32]),
         "fgh_paged_check": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedRope), C.POINTER(PagedMask), i32,
                                   i64, i64, i64, C.c_char_p, C.c_size_t]),
+        "fgh_paged_plan": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedMask), i32, i32, vp]),
         "fgh_graph_begin": (i32, [vp]),
         "fgh_graph_end": (i32, [vp, C.POINTER(vp)]),
         "fgh_graph_launch": (i32, [vp, vp]),

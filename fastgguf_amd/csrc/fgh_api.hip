@@ -1032,11 +1032,25 @@ static fgh::Paged paged_args(const fgh_paged_cache *c, const fgh_paged_batch *b)
     p.max_len = (int)std::min<int64_t>(b->max_len, std::min<int64_t>((int64_t)c->table_stride * c->page, INT32_MAX / 2));
     return p;
 }
+static fgh::PagedAttnArgs paged_attn_args(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_mask *m, int n_head) {
+    fgh::PagedAttnArgs a{};
+    a.p = paged_args(c, b);
+    a.n_head = n_head, a.window = m->window, a.scale = m->scale;
+    a.softcap = m->softcap, a.slopes = m->slopes, a.prefix = m->prefix;
+    return a;
+}
 int fgh_paged_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_rope *r, const fgh_paged_mask *m,
                     int n_head, int64_t ldq, int64_t ldkv, int64_t ldo, char *err, size_t err_len) {
     const char *why = paged_check(c, b, r, m, n_head, ldq, ldkv, ldo);
     if (why && err && err_len) snprintf(err, err_len, "%s", why);
     return why ? FGH_ERR_ARG : FGH_OK;
+}
+int fgh_paged_plan(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_mask *m, int n_head, int num_cu, int32_t *plan) {
+    if (!m || !plan || num_cu < 1 || !c || paged_check(c, b, nullptr, m, n_head, (int64_t)n_head * c->hd, 0, (int64_t)n_head * c->hd)) return FGH_ERR_ARG;
+    fgh::PagedAttnArgs a = paged_attn_args(c, b, m, n_head);
+    (void)fgh::paged_attention_plan(a, num_cu);
+    plan[0] = a.ds, plan[1] = a.ps, plan[2] = a.ps ? a.prows : 0, plan[3] = a.alone;
+    return FGH_OK;
 }
 int64_t fgh_paged_slot(const fgh_paged_cache *c, const int32_t *table, int s, int pos, int kvh, int d, int is_v) {
     if (!c || !table || c->page < 16 || (c->page & (c->page - 1)) || s < 0 || pos < 0 || pos >= (int64_t)c->table_stride * c->page || kvh < 0 || kvh >= c->n_head_kv || d < 0 || d >= c->hd) return -1;
@@ -1085,10 +1099,8 @@ int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_
         return fail(c, FGH_ERR_ARG, "paged_attention: the cache, q and o must be 16-byte aligned");
     INJECT(c);
     HIP_TRY(c, hipSetDevice(c->device));
-    fgh::PagedAttnArgs a{};
-    a.p = paged_args(cache, batch);
-    a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo, a.n_head = n_head, a.window = mask->window, a.scale = mask->scale;
-    a.softcap = mask->softcap, a.slopes = mask->slopes, a.prefix = mask->prefix;
+    fgh::PagedAttnArgs a = paged_attn_args(cache, batch, mask, n_head);
+    a.q = q, a.o = o, a.ldq = ldq, a.ldo = ldo;
     const fgh::PagedScratch need = fgh::paged_attention_plan(a, c->num_cu);
     if (const size_t bytes = need.bytes()) {
         if (int rc = grow(c, c->pa, bytes)) return rc;

@@ -435,7 +435,11 @@ FGH_API int fgh_event_destroy(fgh_ctx *ctx, void *ev);
  * (cache->table is not used). Needs no device.
  * fgh_paged_check: the argument checks of fgh_paged_store_dev (rope not NULL) and fgh_paged_attention_dev
  * (mask not NULL) on descriptors and strides, without pointers being read: FGH_OK, or FGH_ERR_ARG with a message in
- * err. Needs no device. */
+ * err. Needs no device.
+ * fgh_paged_plan: what fgh_paged_attention_dev launches on a device of num_cu compute units: plan[0] over how many
+ * workgroups the ranges of positions of sequences with few rows are split at most (0: no such kernel), plan[1] the same
+ * of the others, plan[2] the rows of a workgroup of these, plan[3] whether only one of them runs on a compute
+ * unit. Needs no device; FGH_ERR_ARG for what fgh_paged_check refuses. */
 #define FGH_MATMUL_DECODE 0
 #define FGH_MATMUL_GEMM 1
 #define FGH_MATMUL_TOKENS 2
@@ -460,6 +464,8 @@ FGH_API int64_t fgh_paged_slot(const fgh_paged_cache *cache, const int32_t *tabl
 FGH_API int fgh_paged_check(const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_rope *rope,
                     const fgh_paged_mask *mask, int n_head, int64_t ldq, int64_t ldkv, int64_t ldo, char *err,
                     size_t err_len);
+FGH_API int fgh_paged_plan(const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_mask *mask, int n_head,
+                   int num_cu, int32_t *plan);
 
 #ifdef __cplusplus
 }

@@ -795,9 +795,12 @@ def test_attention_null_key(backend, i, gap):
     assert of_vectors(o, want) <= 1e-5
 
 
+NULL_TYPES = [([1], [200], 7), ([40], [150], 7), ([40], [200], 7), ([40], [600], 7), ([20] * 260, [64] * 260, 40)]
+
+
 @pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
 @pytest.mark.parametrize("hd", [64, 80, 96, 128, 256])
-@pytest.mark.parametrize("news,lens,at", [([1], [200], 7), ([40], [200], 7), ([20] * 260, [64] * 260, 40)])
+@pytest.mark.parametrize("news,lens,at", NULL_TYPES)
 def test_attention_null_key_types(backend, t, hd, news, lens, at):
     """The same for every type and head size, at a gap of 20."""
     b, scale = with_null_key(t, news, lens, 20, at, hd=hd)

@@ -126,3 +126,63 @@ def test_slots_are_64_bit():
     table = np.array([[(1 << 20) - 1] * 4], np.int32)
     assert B.paged_slot(c, table, 0, 17, 1, 3) == ((1 << 20) - 1 << 20) + 64 * 16 + 64 + 3
     assert B.paged_slot(c, table, 0, 17, 1, 3, True) == ((1 << 20) - 1 << 20) + 64 * 16 + 3 * 16 + 1
+
+
+def plan(b, **kw):
+    """What the attention of a batch of paged_ref launches on 256 compute units."""
+    c = B.PagedCache(b.type, 16, 16, 16, n_pages=b.n_pages, page=b.page, table_stride=b.stride, n_head_kv=b.n_kv, hd=b.hd, page_stride=b.page_stride)
+    batch = B.PagedBatch(16, 16, n_seq=len(b.news), n_tok=b.n_tok, max_tok=max(b.news + [1]), max_len=max(b.lens + [1]))
+    return B.paged_plan(c, batch, b.n_head, B.PagedMask(0.125, **kw))
+
+
+def test_plan():
+    """Few rows, prompts, and both: which kernels, over how many splits, in which rows."""
+    def of(news, lens, hd=128, heads=8, kv=2, t=T_F16, **kw):
+        return plan(Batch(1, t, hd, heads, kv, 16, news, lens, sigma=0.0), **kw)
+
+    assert of([1], [4096]) == (33, 0, 0, False)              # a step for every wavefront
+    assert of([1] * 300, [40] * 300) == (1, 0, 0, False)     # more workgroups than fit: whole ranges
+    assert of([4], [300], kv=2) == (3, 0, 0, False)          # 16 rows a K / V head
+    assert of([5], [300], kv=2) == (0, 2, 64, True)          # 20
+    assert of([64], [4096]) == (0, 8, 64, True)
+    assert of([64], [4096], t=T_F32, hd=256) == (0, 8, 128, True)  # no form of half the rows
+    assert of([64], [4096], window=100) == (0, 1, 64, True)  # 163 positions
+    assert of([64], [4096], window=100, prefix=16) == (0, 8, 64, True)
+    ds, ps, rows, alone = of([900] * 8, [900] * 8)
+    assert (ds, ps, rows) == (8, 1, 128) and not alone
+    assert of([40, 1, 0, 3], [2100, 1500, 9, 3])[:3] == (17, 8, 64)
+    with pytest.raises(B.BackendError):
+        of([1], [16], hd=100)
+
+
+def test_gpu_tests_take_every_form():
+    """The batches of the GPU tests reach every kernel form that there is, for every head size and type."""
+    import test_gpu_paged as G
+    seen = set()
+
+    def add(b, **kw):
+        ds, ps, rows, alone = plan(b, **kw)
+        for form in (("few rows", "split" if ds > 1 else "whole") if ds else None, (rows, "split" if ps > 1 else "whole") if ps else None):
+            if form:
+                seen.add((b.type, b.hd) + form)
+        if ds and ps:
+            seen.add((b.type, b.hd, "both"))
+        if alone:
+            seen.add("alone")
+
+    types, hds = (T_F16, T_BF16, T_F32), (64, 80, 96, 128, 256)
+    for t in types:
+        for hd in hds:
+            for news, lens, at in G.NULL_TYPES:
+                add(G.with_null_key(t, news, lens, 20, at, hd=hd)[0])
+            add(Batch(51, t, hd, 4, 2, 32, *G.crowd([200, 1, 70, 0, 3, 130], [200, 90, 640, 0, 3, 333]), sigma=0.0))
+    for i in range(len(G.SHAPES)):
+        add(G.shape(i))
+    for t, hd, nh in G.SPLITS:
+        for news, lens in (([1], [2500]), ([3, 1], [2500, 700]), ([40], [2500]), ([40, 1, 0, 3], [2100, 1500, 9, 3])):
+            add(Batch(50, t, hd, nh, 1, 32, news, lens, sigma=0.0))
+    want = {(t, hd) + f for t in types for hd in hds for f in (("few rows", "whole"), ("few rows", "split"), (128, "whole"), (128, "split"),
+                                                              (64, "whole"), (64, "split"), ("both",))}
+    want -= {(T_F32, 256, 64, w) for w in ("whole", "split")}
+    assert "alone" in seen
+    assert not want - seen, sorted(want - seen, key=str)
