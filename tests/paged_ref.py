@@ -139,3 +139,34 @@ def attention(b, q, scale, softcap=0.0, window=0, slopes=None, prefix=None):
             out[t, h] = w @ v
             tol[t, h] = (2 * d + 16 * U32) * 2 * (w @ np.abs(v))
     return out, tol, mine
+
+
+def of_vectors(o, want):
+    """The largest error of a row and head, relative to that vector's length."""
+    return float((np.linalg.norm(o - want, axis=-1) / np.linalg.norm(want, axis=-1)).max())
+
+
+def cut(x, bits):
+    """fp32 values without the bits behind the first `bits` of their 24: what is left of a value taken apart, a part short."""
+    return (np.ascontiguousarray(x, np.float32).view(np.uint32) & np.uint32(-(1 << 24 - bits) & 0xFFFFFFFF)).view(np.float32)
+
+
+def plain32(b, q, scale, bits_q=24, bits_w=24):
+    """The causal attention of a batch in fp32 throughout (rows of no sequence: 0), q and the weights to so many bits."""
+    out = np.zeros((b.n_tok, b.n_head, b.hd), np.float32)
+    q, scale = cut(q, bits_q), np.float32(scale)
+    for s in range(len(b.news)):
+        rows = [(t, p) for t, x, p in b.tokens() if x == s]
+        for h in range(b.n_head if rows else 0):
+            k, v = (b.rows(s, h * b.n_kv // b.n_head, is_v).astype(np.float32) for is_v in (False, True))
+            for t, p in rows:
+                z = (k[:p + 1] @ q[t, h]) * scale
+                w = cut(np.exp(z - z.max()), bits_w)
+                out[t, h] = (w @ v[:p + 1]) / w.sum(dtype=np.float32)
+    return out
+
+
+def vector_bound(b, q, scale, want, mine):
+    """What a result may be off by, of a vector's length: 4 times the worst of plain32, which rounds as often in another order, and
+    2^-22 for the rounding of q, of the weights and of the result, that do not depend on the sums' order."""
+    return 4 * of_vectors(plain32(b, q, scale)[mine], want[mine]) + 2.0**-22

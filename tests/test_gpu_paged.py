@@ -5,7 +5,7 @@ Tolerances are per value, from the inputs: half a step of the cache's type for w
 bounds that paged_ref derives for the fp32 arithmetic."""
 import numpy as np
 import pytest
-from paged_ref import HALF_STEP, T_BF16, T_F16, T_F32, Batch, attention, decode, encode, store
+from paged_ref import HALF_STEP, T_BF16, T_F16, T_F32, Batch, attention, decode, encode, of_vectors, store, vector_bound
 
 from fastgguf_amd.backend import ERR_ARG, BackendError, PagedBatch, PagedCache, PagedMask, PagedRope
 
@@ -778,11 +778,6 @@ NULL_KEYS = [  # new tokens, lengths, position of the key
 ]
 
 
-def of_vectors(o, want):
-    """The largest error of a row and head, relative to that vector's length."""
-    return float((np.linalg.norm(o - want, axis=-1) / np.linalg.norm(want, axis=-1)).max())
-
-
 @pytest.mark.parametrize("gap", [12, 14, 16, 18, 20, 22])
 @pytest.mark.parametrize("i", range(len(NULL_KEYS)))
 def test_attention_null_key(backend, i, gap):
@@ -934,3 +929,71 @@ def test_attention_zero_products(backend, t, softcap, news, lens):
             v = b.rows(s, h // 2, True)[:p + 1]
             # all weights the same: off by 16 roundings as in the others' bound
             assert (np.abs(o[row, h] - v.mean(0)) <= 32 * 2.0**-24 * np.abs(v).mean(0)).all()
+
+
+# ---- results as vectors, values in bad pages, values that are not finite in every type ----
+
+VECTORS = [([1], [4096]), ([1, 3], [700, 600]), ([40], [600]), ([9] * 130 + [40], [60] * 130 + [300])]
+
+
+def ordinary(t, i, hd=128):
+    return Batch(110 + i, t, hd, 4, 2, 32, *VECTORS[i])
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("i", range(len(VECTORS)))
+def test_attention_vectors(backend, t, hd, i):
+    """Ordinary scores: an error per output vector as small as a plain fp32 form's (test_paged.py: a part of q or of the weights
+    less would be more)."""
+    b = ordinary(t, i, hd)
+    scale = float(np.float32(hd**-0.5))
+    want, _, mine = attention(b, b.q, scale)
+    off = of_vectors(run_attention(backend, b, scale=scale)[mine], want[mine])
+    assert off <= vector_bound(b, b.q, scale, want, mine) and off <= 1e-5
+
+
+@pytest.mark.parametrize("page_no", [-1, 0x7FFFFFFF, "n_pages"])
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("news", [[1, 1], [40, 5], [150, 70, 1]])
+def test_bad_pages_values(backend, t, news, page_no):
+    """An append into a page that does not exist: values as well as keys go nowhere, the others to their places."""
+    b = Batch(22, t, 64, 4, 2, 16, news, [n + 33 for n in news])
+    there = b.table.copy()
+    bad = {(0, (b.lens[0] - 1) // 16), (1, (b.lens[1] - news[1]) // 16)}
+    for s, at in bad:
+        b.table[s, at] = b.n_pages if page_no == "n_pages" else page_no
+    kv = b.rng.standard_normal((2, b.n_tok, 2, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        backend.paged_store_dev(cache, batch, PagedRope(), 0, 0, 0, d.put(kv[0]), d.put(kv[1]), 128, 0, 0)
+        got = d.get(cache.k, b.k), d.get(cache.v, b.v)
+    b.table = there
+    for is_v, old in ((False, b.k), (True, b.v)):
+        want = old.copy()
+        for row, s, p in b.tokens():
+            for h in range(2):
+                if (s, p // 16) not in bad:
+                    want[b.at(s, p, h, is_v)] = encode(kv[int(is_v), row, h], t)
+        assert np.array_equal(got[is_v], want)
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("hd", [80, 128, 256])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("news,lens", [([4], [24]), ([4], [2000]), ([90], [110]), ([90] + [9] * 130, [110] + [9] * 130)])
+def test_attention_non_finite_values(backend, t, hd, value, news, lens):
+    """Values that are not finite at a few new positions, in every type: the rows that see one get it in that value of theirs, the
+    others and their other values are as they were."""
+    b, clean = [Batch(112, t, hd, 4, 2, 16, news, lens) for _ in range(2)]
+    marks = [(news[0] // 2, 1, 7), (news[0] - 1, 0, hd - 1), (news[0] // 3, 0, 0)]  # new token, K / V head, value
+    for at, h, x in marks:
+        b.v[b.at(0, lens[0] - news[0] + at, h, True)[x]] = encode(np.float32([value]), t)[0]
+    scale = float(np.float32(hd**-0.5))
+    o = run_attention(backend, b, scale=scale)
+    want, tol, _ = attention(clean, clean.q, scale)
+    hit = np.zeros(o.shape, bool)
+    for at, h, x in marks:
+        hit[at:news[0], 2 * h:2 * h + 2, x] = True
+    assert not np.isfinite(o[hit]).any()
+    assert (np.abs(o - want)[~hit] <= tol[~hit]).all()

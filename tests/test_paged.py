@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from fastgguf_amd import backend as B
-from paged_ref import Batch, T_BF16, T_F16, T_F32
+from paged_ref import Batch, T_BF16, T_F16, T_F32, attention, of_vectors, plain32, vector_bound
 
 
 def descriptors(**kw):
@@ -186,3 +186,16 @@ def test_gpu_tests_take_every_form():
     want -= {(T_F32, 256, 64, w) for w in ("whole", "split")}
     assert "alone" in seen
     assert not want - seen, sorted(want - seen, key=str)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_vector_bound_holds_every_part(i):
+    """The bound of the GPU tests' output vectors is passed by q or weights that lack their last 8 of 24 bits."""
+    import test_gpu_paged as G
+    b = G.ordinary(T_BF16, i)
+    scale = float(np.float32(128**-0.5))
+    want, _, mine = attention(b, b.q, scale)
+    bound = vector_bound(b, b.q, scale, want, mine)
+    assert of_vectors(plain32(b, b.q, scale)[mine], want[mine]) < bound < 5e-6
+    for bits in ({"bits_q": 16}, {"bits_w": 16}):
+        assert of_vectors(plain32(b, b.q, scale, **bits)[mine], want[mine]) > bound
