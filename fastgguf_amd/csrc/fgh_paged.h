@@ -34,7 +34,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const Paged &a, int s) {
     const int b = a.tok[s], e = a.tok[s + 1], len = a.len[s];
     PagedSeq q;
     q.t0 = min(max(b, 0), a.n_tok);
-    q.n = max(min(e, a.n_tok) - q.t0, 0);
+    q.n = max(min(max(e, 0), a.n_tok) - q.t0, 0);  // e may be anything: a difference with it as it is could wrap to many rows
     q.len = len;
     q.ok = b >= 0 && e <= a.n_tok && q.n <= a.max_tok && len >= q.n && len <= a.max_len;
     return q;

@@ -997,3 +997,42 @@ def test_attention_non_finite_values(backend, t, hd, value, news, lens):
         hit[at:news[0], 2 * h:2 * h + 2, x] = True
     assert not np.isfinite(o[hit]).any()
     assert (np.abs(o - want)[~hit] <= tol[~hit]).all()
+
+
+# ---- starts that are no starts ----
+
+LOW, HIGH = -2**31, 2**31 - 1
+
+
+@pytest.mark.parametrize("tok,nan,fine", [
+    ([0, LOW, 7, 9], range(7), range(7, 9)),
+    ([5, LOW, 7, 9], range(5, 7), range(7, 9)),
+    ([0, 3, LOW, HIGH], range(3, 9), ()),
+    ([0, HIGH, HIGH, HIGH], range(9), ()),
+    ([0, 4, 4, HIGH], range(4, 9), range(4)),
+    ([HIGH, LOW, HIGH, LOW], (), ()),
+    ([LOW, 2, 5, 9], range(2), range(2, 9)),
+    ([-1, -1, LOW, LOW], (), ()),
+    ([HIGH, HIGH, HIGH, HIGH], (), ()),
+])
+@pytest.mark.parametrize("heads", [1, 32])
+def test_wild_starts(backend, tok, nan, fine, heads):
+    """Starts at the ends of an int: the rows in 0 .. n_tok of a sequence that reaches out of it are NaN, those of others as ever, and
+    nothing around them is written. (Rows in two sequences or before tok[0] hold anything.)"""
+    b = Batch(120, T_F16, 64, heads, 1, 16, [3, 3, 3], [30, 31, 32])
+    b.tok = np.array(tok, np.int32)
+    n, pad, row = 9, 64, heads * 64
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b, max_len=40, max_tok=9)
+        q = np.full((n + 2 * pad, row), 777.0, np.float32)
+        q[pad:pad + n] = b.q.reshape(n, row)
+        qd, od, kv = d.put(q), d.put(np.full_like(q, 777.0)), d.put(np.zeros((n, 64), np.float32))
+        at = pad * row * 4
+        for call in (lambda: backend.paged_attention_dev(cache, batch, PagedMask(0.125), heads, qd + at, row, od + at, row),
+                     lambda: backend.paged_store_dev(cache, batch, PagedRope(), heads, qd + at, row, kv, kv, 64, od + at, row)):
+            backend.h2d(od, np.full_like(q, 777.0))
+            call()
+            o = d.get(od, q)
+            assert (o[:pad] == 777.0).all() and (o[pad + n:] == 777.0).all()
+            o = o[pad:pad + n]
+            assert np.isnan(o[list(nan)]).all() and np.isfinite(o[list(fine)]).all() and (o[list(fine)] != 777.0).all()
