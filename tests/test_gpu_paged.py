@@ -1036,3 +1036,60 @@ def test_wild_starts(backend, tok, nan, fine, heads):
             assert (o[:pad] == 777.0).all() and (o[pad + n:] == 777.0).all()
             o = o[pad:pad + n]
             assert np.isnan(o[list(nan)]).all() and np.isfinite(o[list(fine)]).all() and (o[list(fine)] != 777.0).all()
+
+
+# ---- the largest batches and head counts ----
+
+@pytest.mark.parametrize("most", [1, 9])
+def test_most_sequences(backend, most):
+    """65535 sequences, few of them with tokens; single tokens, and a prompt of the last one."""
+    n_seq, page = 65535, 16
+    b = Batch(130, T_F16, 64, 2, 1, page, [1, 1, 20 if most > 1 else 1], [5, 40, 50])
+    at = [0, 30000, n_seq - 1]
+    rows = np.zeros(n_seq, np.int32)
+    rows[at] = b.news
+    lens, table = np.zeros(n_seq, np.int32), np.full((n_seq, b.stride), -1, np.int32)
+    lens[at], table[at] = b.lens, b.table
+    qkv = b.rng.standard_normal((b.n_tok, 4, 64)).astype(np.float32)
+    want, tol, _ = attention(b, b.q, 0.125)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        cache.table = d.put(table)
+        batch = PagedBatch(d.put(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)), d.put(lens), n_seq=n_seq, n_tok=b.n_tok,
+                           max_tok=max(b.news), max_len=50)
+        q, o = d.put(b.q), d.put(np.full_like(b.q, 777.0))
+        backend.paged_attention_dev(cache, batch, PagedMask(0.125), 2, q, 128, o, 128)
+        got = d.get(o, b.q)
+        assert (np.abs(got - want) <= tol).all()
+        x = d.put(qkv)
+        backend.paged_store_dev(cache, batch, PagedRope(), 2, x, 256, x + 512, x + 768, 256, o, 128)
+        got, kc, vc = d.get(o, b.q), d.get(cache.k, b.k), d.get(cache.v, b.v)
+    assert np.array_equal(got, qkv[:, :2])
+    for t, s, pos in b.tokens():
+        assert np.array_equal(kc[b.at(s, pos, 0, False)], encode(qkv[t, 2], T_F16))
+        assert np.array_equal(vc[b.at(s, pos, 0, True)], encode(qkv[t, 3], T_F16))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4000, 1), (16383, 1), (4096, 4096), (8192, 4096)])
+def test_most_heads(backend, heads, kv_heads):
+    """One token of very many heads over one K / V head, and of very many K / V heads."""
+    b = Batch(131, T_F16, 64, heads, kv_heads, 16, [1], [20])
+    check_attention(backend, b)
+    qkv = b.rng.standard_normal((1, heads + 2 * kv_heads, 64)).astype(np.float32)
+    with Dev(backend) as d:
+        cache, batch = put_batch(d, b)
+        x, o, row = d.put(qkv), d.put(np.zeros((1, heads, 64), np.float32)), (heads + 2 * kv_heads) * 64
+        backend.paged_store_dev(cache, batch, PagedRope(), heads, x, row, x + 256 * heads, x + 256 * (heads + kv_heads), row, o, heads * 64)
+        got, kc, vc = d.get(o, qkv[:, :heads]), d.get(cache.k, b.k), d.get(cache.v, b.v)
+    assert np.array_equal(got, qkv[:, :heads])
+    for h in range(kv_heads):
+        assert np.array_equal(kc[b.at(0, 19, h, False)], encode(qkv[0, heads + h], T_F16))
+        assert np.array_equal(vc[b.at(0, 19, h, True)], encode(qkv[0, heads + kv_heads + h], T_F16))
+
+
+@pytest.mark.parametrize("news", [1, 40])
+def test_attention_rising_bias(backend, news):
+    """Slopes below 0 raise what is far away; 0 leaves a head without a bias."""
+    b = Batch(132, T_BF16, 64, 4, 2, 16, [news], [news + 300])
+    check_attention(backend, b, slopes=np.float32([-0.25, 0.0, 0.125, -1.0]), prefix=np.array([200], np.int32))
+    check_attention(backend, b, slopes=np.float32([-0.25, 0.0, 0.125, -1.0]), softcap=3.0)
