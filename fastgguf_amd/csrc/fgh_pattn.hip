@@ -106,21 +106,27 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int np
 
 }  // namespace
 
+// Times here are of calls one after the other, the join with them.
 // Prompt: workgroups of 128 rows, since a tile of K and V is read out of LDS once for all of them. Where they would not give
-// every compute unit one in as many splits as there may be, of 64: 64 tokens behind 2000 positions, 8 heads over 4, take 32.7 us
-// in 128 rows and 24.7 in 64 (bf16, hd 256), 38.7 and 26.0 (f32, hd 128); with more workgroups than that 64 rows lose (32 tokens of each of
-// 4 sequences behind 1000, f16: 20.8 and 25.0).
-// Splits: as many as fit at once, two workgroups for every compute unit. More save nothing, and the join costs 5 to 20 us (2032 tokens behind
-// 7168, 512 tiles: 600 us whole, 600 + 20 in two splits; seven documents of up to 900 tokens, 252 tiles: 48.7 us whole,
-// 33 + 5 in three). At least 4 units of 64 positions each, at most 8 splits: 64 tokens over 4096 positions took 29 + 5 us in 8,
-// 27 + 7 in 16.
-// One workgroup to a compute unit where all fit so: the dispatcher would put two on one and leave others idle (128 tokens behind
-// 4000: 40.8 us, 34.0 so; 256 tokens, which do not fit, would take 59 instead of 46). Not where the sequences beside the longest have few
-// rows, whose decode workgroups fit several (40 tokens of one sequence and one each of 63: 111 us, 91 without).
+// every compute unit one in as many splits as there may be, of 64: 64 tokens behind 2000 positions, 8 heads over 4, take 34.9 us
+// in 128 rows and 28.3 in 64 (bf16, hd 256), 42.0 and 29.8 (f32, hd 128); with more workgroups than that 64 rows gain nothing (32 tokens
+// of each of 4 sequences behind 1000, f16: 25.4 and 25.7).
+// Splits: as many as fit at once, two workgroups for every compute unit. More save nothing, and the join has its price (2032 tokens
+// behind 7168, 512 tiles: 510 us whole, 513 in two splits; seven documents of up to 900 tokens, 252 tiles: 46.2 us whole, 36.8 in
+// three). At least 4 units of 64 positions each, at most 8 splits: 64 tokens over 4096 positions take 27.7 us in 8, 31.3 in 16. These
+// 8 are measured where they fill the device. Where a K / V head has only one or two tiles over a long range they leave compute units
+// idle, and no rule for more is there yet: 3 tokens of 32 heads over 4 at 16384 positions take 54 us, 2 tokens, which are the
+// decode kernel's, 18; one token of 48 heads over one 53, of 16 heads 16. Nor do the splits know how many of the tiles that a
+// batch could have it has: the 64 tokens over 4096 with one token each of 63 short sequences take 105 us.
+// One workgroup to a compute unit where all fit so: the dispatcher may put two on one and leave others idle (2 sequences of 64 tokens
+// behind 4000, f16, 256 workgroups: 41.0 us, 34.7 so; most batches that fit take the same either way). A few too many lose a whole turn (150
+// tokens behind 2000, 320 workgroups: 35 us, 43 so; 40 tokens of each of 4 behind 1000, bf16, hd 64: 16.1 and 21.4). Not where the
+// sequences beside the longest have few rows, whose decode workgroups fit several (40 tokens of one sequence and one each of 63: 125
+// us so, 105).
 // Decode: as many as fit at once too, of 4 steps and more, a step for every wavefront (4 sequences of 3000 positions at hd 256, of
-// which one workgroup fits a compute unit: 26.3 us with the join in 256 workgroups, 33.6 in 512); up to eight for every compute
+// which one workgroup fits a compute unit: 26.1 us in 256 workgroups, 33.9 in 512); up to eight for every compute
 // unit where that leaves 16 steps each, since sequences' lengths differ: 32 sequences of 65 to 8192 positions take
-// 137 us in 2 splits, 110 in 8, and 32 of 1024 27 in 2, 35 in 8. At most 64: the join reads that many one after the other.
+// 141 us in 2 splits, 115 in 8, and 32 of 1024 31.5 in 2, 40.6 in 8. All sequences get as many splits, short ones leave theirs unused. At most 64: the join reads that many one after the other.
 // The bounds may be far above the lengths: the kernels split what is there.
 // The join is a launch of its own: a workgroup that arrives last and joins the others' sums within the same launch needs
 // stores that pass the L2 caches of the XCDs, and took longer (one sequence of 4096 positions 14 to 16 us against 12.3).
@@ -139,9 +145,10 @@ PagedScratch paged_attention_plan(PagedAttnArgs &a, int num_cu) {
         int64_t wgs = paged_tiles(a) * a.p.n_head_kv;
         if (wgs * splits <= num_cu && pro_half(a.p.type, a.p.hd)) a.prows = PRO_ROWS / 2, wgs = paged_tiles(a) * a.p.n_head_kv;
         a.ps = (int)std::min<int64_t>(splits, std::max<int64_t>(1, (2 * (int64_t)num_cu + wgs / 2) / wgs));
-        // workgroups with rows, a sequence's last tile counted half: it may be there or not. A few too many still pay.
         const bool mixed = (int64_t)(a.p.n_tok - a.p.max_tok) * G <= (int64_t)(a.p.n_seq - 1) * DEC_ROWS && a.p.n_seq > 1;
-        a.alone = !mixed && (paged_tiles(a) - pro_seqs(a) / 2) * a.p.n_head_kv * a.ps * 4 <= (int64_t)num_cu * 5;
+        // workgroups with rows, for tokens spread evenly over the sequences
+        const int64_t seqs = pro_seqs(a), each = ((a.p.n_tok + seqs - 1) / seqs * G + a.prows - 1) / a.prows;
+        a.alone = !mixed && std::min(paged_tiles(a), seqs * each) * a.p.n_head_kv * a.ps <= num_cu;
         if (a.ps > 1) n.pslot = (size_t)wgs, n.prow = n.pslot * a.ps * a.prows, n.ppart = n.prow * ((a.p.hd + 31) / 32 * 32);
     }
     if (a.ps == 0 || a.p.n_seq > 1) {

@@ -151,6 +151,10 @@ def test_plan():
     ds, ps, rows, alone = of([900] * 8, [900] * 8)
     assert (ds, ps, rows) == (8, 1, 128) and not alone
     assert of([40, 1, 0, 3], [2100, 1500, 9, 3])[:3] == (17, 8, 64)
+    # a compute unit each only for as many workgroups as there are: 256, and 320, which would take two turns
+    assert of([64, 64], [4064, 4064], heads=32, kv=8) == (32, 8, 128, True)
+    assert of([150], [2150], heads=32, kv=8) == (0, 8, 128, False)
+    assert of([40] * 4, [1040] * 4, heads=16, kv=8, hd=64, t=T_BF16) == (9, 5, 64, False)
     with pytest.raises(B.BackendError):
         of([1], [16], hd=100)
 
