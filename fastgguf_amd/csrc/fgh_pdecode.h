@@ -10,11 +10,12 @@
 // the rows' sums stay in their lanes to the end. Each wavefront takes every fourth step of the workgroup's positions; the next step's K
 // is asked for when the scores are done, its V when the sums are; the four wavefronts are joined in LDS.
 //
-// Bound by the cache's bytes, as long as there are many: a step's 16 to 64 KB of K and V are in flight for each wavefront while
-// the one before is used. 16 rows, since that is the narrowest matrix product: fewer rows cost nothing less, more are the prompt
-// kernel's. Measured with the join: 32 sequences of 65 to 8192 positions, f16, 32 heads over 8, hd 128: 535 MB in 115 us, 4.6 TB/s (a large
-// copy here: 4.76); 8 of up to 4096 in a window, capped, bf16, hd 256: 239 MB in 56 us; 4 tokens of 6 sequences over an f32 cache: 79 MB in
-// 28 us; one sequence of 4096 positions: 17 MB in 11.4 us, of which two launches that wait for each other are 8.
+// Bound by the rate of the cache's reads, as long as there are many: a step's 16 to 64 KB of K and V are in flight for each wavefront while
+// the one before is used, and no byte is asked of memory twice. 16 rows, since that is the narrowest matrix product: fewer rows cost
+// nothing less, more are the prompt kernel's. Measured with the join: 32 sequences of 65 to 8192 positions, f16, 32 heads over 8, hd 128: 535 MB
+// in 115.5 us, 4.6 TB/s (a large copy here: 4.8, a plain read of 1 GB: 6.7); 8 of up to 4096 in a window, capped, bf16, hd 256: 239 MB in 56
+// us; 4 tokens of 6 sequences over an f32 cache: 79 MB in 28 us; one sequence of 4096 positions: 17 MB in 11.9 us, of which two launches that
+// wait for each other are 8.
 #pragma once
 
 #include "fgh_pattn.h"

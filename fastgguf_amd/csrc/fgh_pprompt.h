@@ -16,7 +16,7 @@
 // twice the vector instructions.
 //
 // Bound by the matrix pipe, for the 2 (F16) to 6 (F32) products that an fp32 result takes: 8192 tokens, f16, 32 heads over 8, hd 128 take
-// 985 to 1000 us by the card, 1.12 PFLOP/s of products, 1.15 for a large f16 matrix product here, with the clock held
+// 975 to 1000 us by the card, 1.10 to 1.13 PFLOP/s of products, 1.15 for a large f16 matrix product here, with the clock held
 // down by power. Small batches are bound by what a tile costs a wavefront that is alone on its SIMD (64 tokens behind
 // 4032: 27.5 us with the join; asking for the next tile took 1500 of a tile's 5500 cycles there before its loads' places were formed from
 // one lane's by other bits). Three tiles deep gained nothing there: the tiles are in time.
@@ -45,8 +45,8 @@ struct Pro {
     static constexpr int LDS = 2 * BYTES + 16 + (PW > 1 ? RW * 512 : 0);
     static_assert(PW == 1 || (KT == 64 && RW * VB * 4096 <= 2 * BYTES - 16384), "a block for every wavefront, its sums beside the rows' staging");
     static constexpr int OCC = HD > 128 || (TYPE == T_F32 && HD > 64) ? 1 : 2;
-    // The loads' places kept in registers, where there are any left: 8192 tokens, f16, hd 128 take 1035 us so and 1075 otherwise;
-    // 1008 tokens behind 7168, bf16, 342 with spills and 320.
+    // The loads' places kept in registers, where there are any left: 64 tokens behind 4032, f16, hd 128 take 27.7 us so and 28.7
+    // otherwise, 8192 975 and 985; 1008 tokens behind 7168, bf16, 327 with spills and 309.
     static constexpr bool KEEP = !(NQ > 2 && HD == 128 && RW == 4);
     static constexpr int KL = KT / 4 * KW / 64;           // direct loads of a wavefront for its KT / 4 K rows
     static constexpr int VL = HD * VW / 64;               // and of all four for V

@@ -319,7 +319,7 @@ typedef struct {
     int32_t n_seq, n_tok, max_tok, max_len;
 } fgh_paged_batch;
 /* What happens to the heads of q and k on the way. RMS norm, where q_norm / k_norm (device, [hd]) is
- * not NULL: x * w / sqrt(mean(x^2) + eps). Rotation of the first n_rot values (even, 0: none) of each
+ * not NULL: x * w / sqrt(mean(x^2) + eps), squares and their sum in fp32. Rotation of the first n_rot values (even, 0: none) of each
  * head by the angles p * freq_scale * freq_base^(-2i / n_rot) / freq_factors[i] (device, [n_rot / 2],
  * or NULL for 1) of position p, formed in 64 bits; pairs (2i, 2i + 1) with FGH_ROPE_PAIRS, (i, i + n_rot / 2)
  * with FGH_ROPE_HALVES. */
