@@ -167,7 +167,9 @@ constexpr float TANH_SPLIT = 0.65f;
 // Scores above 2^20 leave fewer than 4 bits behind the point: a score rounded for the maximum and the same score unrounded in its
 // weight's sum would differ by powers of two, enough to pass a half's range, or from 2^30 on an fp32's. Once a reference of a wavefront's
 // rows is that far from 0, scores are rounded before they are used, and such a reference is the maximum itself.
+// (Not for an infinite one, which leaves its own row undefined and the others as they are.)
 constexpr float SCORE_BIG = 0x1p20f;
+__device__ __forceinline__ bool score_big(float mx) { return fabsf(mx) > SCORE_BIG && fabsf(mx) <= __FLT_MAX__; }
 template <int TYPE>
 __device__ __forceinline__ float score_bias(float mx) { return fabsf(mx) > SCORE_BIG ? 0.0f : PagedType<TYPE>::PBIAS; }
 

@@ -220,7 +220,7 @@ __device__ __forceinline__ void paged_decode_block(const PagedAttnArgs &a, int b
         if (__builtin_amdgcn_ballot_w64(top + c > PagedType<TYPE>::PTOP)) {
             float mx = fmaxf(top, __shfl_xor(top, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && fabsf(mx) > SCORE_BIG) != 0;
+            big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && score_big(mx)) != 0;
             if (mx + c > PagedType<TYPE>::PTOP) {  // of the whole row: its four lanes agree
                 const float cn = score_bias<TYPE>(mx) - mx, f = __builtin_amdgcn_exp2f(cn - c);
                 c = cn;

@@ -274,7 +274,7 @@ __device__ __forceinline__ void paged_prompt_block(const PagedAttnArgs &a, int b
     auto follow = [&](float top) {
         const float mx = fmaxf(top, __shfl_xor(top, 32, 64));
         float f = 1.0f;
-        big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && fabsf(mx) > SCORE_BIG) != 0;
+        big = big || __builtin_amdgcn_ballot_w64(mx + c > PagedType<TYPE>::PTOP && score_big(mx)) != 0;
         if (mx + c > PagedType<TYPE>::PTOP) {
             const float cn = score_bias<TYPE>(mx) - ceilf(mx);
             f = __builtin_amdgcn_exp2f(cn - c);

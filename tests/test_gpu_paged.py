@@ -1093,3 +1093,18 @@ def test_attention_rising_bias(backend, news):
     b = Batch(132, T_BF16, 64, 4, 2, 16, [news], [news + 300])
     check_attention(backend, b, slopes=np.float32([-0.25, 0.0, 0.125, -1.0]), prefix=np.array([200], np.int32))
     check_attention(backend, b, slopes=np.float32([-0.25, 0.0, 0.125, -1.0]), softcap=3.0)
+
+
+@pytest.mark.parametrize("t", [T_F16, T_BF16, T_F32])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("news", [[4], [90], [20] * 260])
+def test_infinite_key_of_a_later_row(backend, t, value, news):
+    """A key that is not finite leaves the rows that do not see it as they are, bit for bit, also where it makes infinite scores."""
+    b = Batch(133, t, 64, 4, 2, 16, news, [n + 40 for n in news])
+    before = run_attention(backend, b)
+    at = news[0] // 2
+    b.k[b.at(0, 40 + at, 1, False)[3]] = encode(np.float32([value]), t)[0]
+    after = run_attention(backend, b)
+    same = np.ones(after.shape[:2], bool)
+    same[at:news[0], 2:] = False
+    assert np.array_equal(after[same].view(np.uint32), before[same].view(np.uint32))
