@@ -1108,3 +1108,23 @@ def test_infinite_key_of_a_later_row(backend, t, value, news):
     same = np.ones(after.shape[:2], bool)
     same[at:news[0], 2:] = False
     assert np.array_equal(after[same].view(np.uint32), before[same].view(np.uint32))
+
+
+@pytest.mark.parametrize("past", [0, 2000])
+def test_most_sequences_and_one_prompt(backend, past):
+    """One tile of a prompt beside 65535 sequences: the most rows of workgroups that a launch can have."""
+    n_seq = 65535
+    b = Batch(134, T_F16, 64, 1, 1, 256, [1, 20, 1], [5, 20 + past, 9])
+    at = [1, 40000, n_seq - 1]
+    rows, lens, table = np.zeros(n_seq, np.int32), np.zeros(n_seq, np.int32), np.full((n_seq, b.stride), -1, np.int32)
+    rows[at], lens[at], table[at] = b.news, b.lens, b.table
+    with Dev(backend) as d:
+        cache, _ = put_batch(d, b)
+        cache.table = d.put(table)
+        batch = PagedBatch(d.put(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)), d.put(lens), n_seq=n_seq, n_tok=b.n_tok,
+                           max_tok=20, max_len=20 + past)
+        q, o = d.put(b.q), d.put(np.full_like(b.q, 777.0))
+        backend.paged_attention_dev(cache, batch, PagedMask(0.125), 1, q, 64, o, 64)
+        got = d.get(o, b.q)
+    want, tol, _ = attention(b, b.q, 0.125)
+    assert (np.abs(got - want) <= tol).all()
