@@ -269,7 +269,7 @@ def _bind(state):
     p = {k: v.data_ptr() for k, v in state.i.items()}
     o = {k: v.data_ptr() for k, v in state.out.items()}
     if case["op"] == "reserve":
-        stride, pages, _ = _reserve_sizes(case)
+        stride, pages = state.i["table"].shape[1], state.i["queue"].shape[0]
         cache = PagedCache(GGML["f16"], 0, 0, p["table"], n_pages=pages, page=case["page"], table_stride=stride, n_head_kv=1, hd=64)
         batch = PagedBatch(o["tok"], o["len"], n_seq=case["seqs"], n_tok=case["rows"], max_tok=case["rows"], max_len=stride * case["page"])
         pool = PagedPool(p["keep"], p["add"], p["held"], o["held"], p["queue"], p["free"], o["free"], seq=o["seq"], pos=o["pos"], slot=o["slot"])
