@@ -29,11 +29,12 @@ EXPORTS = (
     "fgh_matvec", "fgh_matvec_multi", "fgh_matmul", "fgh_moe_ffn", "fgh_attention",
     "fgh_matvec_dev", "fgh_matvec_multi_dev", "fgh_matvec_silu_dev", "fgh_matvec_gate_up_silu_dev", "fgh_ffn_dev", "fgh_matmul_dev", "fgh_matmul_dev_noalloc", "fgh_moe_ffn_dev",
     "fgh_attention_dev", "fgh_kvq_store_dev", "fgh_kvq_attention_dev", "fgh_paged_store_dev", "fgh_paged_attention_dev",
+    "fgh_paged_reserve_dev", "fgh_draft_verify_dev", "fgh_lora_dev",
     "fgh_graph_begin", "fgh_graph_end", "fgh_graph_launch", "fgh_graph_destroy",
     "fgh_dev_alloc", "fgh_dev_free", "fgh_copy_h2d", "fgh_copy_d2h", "fgh_copy_d2d", "fgh_checksum_dev", "fgh_memcpy_dev", "fgh_mfma_peak_dev", "fgh_sync",
     "fgh_event_create", "fgh_event_record", "fgh_event_elapsed_ms", "fgh_event_destroy",
     "fgh_quantize", "fgh_block_ints", "fgh_gemm_block_ints", "fgh_moe_block_ints", "fgh_expf", "fgh_fp16_to_f32", "fgh_matvec_shape", "fgh_matmul_path",
-    "fgh_paged_slot", "fgh_paged_check", "fgh_paged_plan",
+    "fgh_paged_slot", "fgh_paged_check", "fgh_paged_plan", "fgh_paged_reserve_check", "fgh_draft_check", "fgh_lora_check",
     "fgh_gguf_open", "fgh_gguf_close", "fgh_gguf_summary", "fgh_gguf_tensor", "fgh_gguf_find",
     "fgh_gguf_kv_num", "fgh_gguf_kv_str", "fgh_gguf_data", "fgh_upload_gguf",
 )
@@ -96,6 +97,64 @@ class PagedMask(C.Structure):
 
     def __init__(self, scale: float, *, softcap: float = 0.0, window: int = 0, slopes: int = 0, prefix: int = 0):
         super().__init__(scale, softcap, window, slopes, prefix)
+
+
+class PagedPool(C.Structure):
+    """fgh_paged_pool: device pointers to keep, add, held and held_out int32 [n_seq], the ring of free pages int32 [n_pages], its
+    first entry and their number int32 [2] before and after, and the rows' maps [n_tok] (seq and pos int32, slot int64; 0: none)."""
+    _fields_ = [("keep", C.c_void_p), ("add", C.c_void_p), ("held", C.c_void_p), ("held_out", C.c_void_p), ("queue", C.c_void_p),
+                ("free", C.c_void_p), ("free_out", C.c_void_p), ("seq", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p)]
+
+    def __init__(self, keep_dev: int, add_dev: int, held_dev: int, held_out_dev: int, queue_dev: int, free_dev: int, free_out_dev: int,
+                 *, seq: int = 0, pos: int = 0, slot: int = 0):
+        super().__init__(keep_dev, add_dev, held_dev, held_out_dev, queue_dev, free_dev, free_out_dev, seq, pos, slot)
+
+
+class Drafts(C.Structure):
+    """fgh_drafts: device pointers to the target's logits [n_tok][ld], tok int32 [n_seq + 1], the rows' tokens int32 [n_tok], the numbers u
+    [n_tok] and v [n_seq], temperatures and lengths [n_seq], and the drafter's logits [n_tok][ldq] with their log sum exp
+    [n_tok] (0: none)."""
+    _fields_ = [("logits", C.c_void_p), ("q", C.c_void_p), ("q_lse", C.c_void_p), ("tok", C.c_void_p), ("tokens", C.c_void_p),
+                ("len", C.c_void_p), ("temp", C.c_void_p), ("u", C.c_void_p), ("v", C.c_void_p), ("ld", C.c_int64), ("ldq", C.c_int64),
+                ("n_seq", C.c_int32), ("n_tok", C.c_int32), ("max_tok", C.c_int32), ("vocab", C.c_int32)]
+
+    def __init__(self, logits_dev: int, tok_dev: int, tokens_dev: int, u_dev: int, v_dev: int, *, n_seq: int, n_tok: int, max_tok: int,
+                 vocab: int, temp: int = 0, len: int = 0, q: int = 0, q_lse: int = 0, ld: int = 0, ldq: int = 0):
+        super().__init__(logits_dev, q, q_lse, tok_dev, tokens_dev, len, temp, u_dev, v_dev, ld or vocab, ldq or vocab, n_seq, n_tok, max_tok,
+                         vocab)
+
+
+class Lora(C.Structure):
+    """fgh_lora: device pointers to the adapters A [n_adapter][max_rank][cols] and B [n_adapter][rows][max_rank] and to their ranks
+    and scales [n_adapter] (0: max_rank, 1)."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p), ("type", C.c_uint32),
+                ("n_adapter", C.c_int32), ("max_rank", C.c_int32), ("cols", C.c_int32), ("rows", C.c_int32)]
+
+    def __init__(self, type_: int, a_dev: int, b_dev: int, *, n_adapter: int, max_rank: int, cols: int, rows: int, rank: int = 0,
+                 scale: int = 0):
+        super().__init__(a_dev, b_dev, rank, scale, type_, n_adapter, max_rank, cols, rows)
+
+
+def paged_reserve_check(cache: PagedCache, batch: PagedBatch, pool: PagedPool) -> str:
+    """What paged_reserve_dev would refuse about these descriptors, or "" (no device needed)."""
+    err = C.create_string_buffer(256)
+    rc = load_library().fgh_paged_reserve_check(C.byref(cache), C.byref(batch), C.byref(pool), err, len(err))
+    return "" if rc == OK else err.value.decode()
+
+
+def draft_check(drafts: Drafts) -> str:
+    """What draft_verify_dev would refuse about its descriptor, or "" (no device needed)."""
+    err = C.create_string_buffer(256)
+    rc = load_library().fgh_draft_check(C.byref(drafts), err, len(err))
+    return "" if rc == OK else err.value.decode()
+
+
+def lora_check(lora: Lora, tok_dev: int, id_dev: int, n_seq: int, n_tok: int, x_dev: int, ldx: int, y_dev: int, ldy: int, *,
+               y_in_dev: int = 0, ldyi: int = 0) -> str:
+    """What lora_dev would refuse about its arguments, or "" (no device needed)."""
+    err = C.create_string_buffer(256)
+    rc = load_library().fgh_lora_check(C.byref(lora), tok_dev, id_dev, n_seq, n_tok, x_dev, ldx, y_in_dev, ldyi, y_dev, ldy, err, len(err))
+    return "" if rc == OK else err.value.decode()
 
 
 def paged_check(cache: PagedCache, batch: PagedBatch, n_head: int, *, rope: PagedRope | None = None,
@@ -174,6 +233,12 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "fgh_paged_check": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedRope), C.POINTER(PagedMask), i32,
                                   i64, i64, i64, C.c_char_p, C.c_size_t]),
         "fgh_paged_plan": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedMask), i32, i32, vp]),
+        "fgh_paged_reserve_dev": (i32, [vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedPool)]),
+        "fgh_draft_verify_dev": (i32, [vp, C.POINTER(Drafts), vp, vp, vp, vp]),
+        "fgh_lora_dev": (i32, [vp, C.POINTER(Lora), vp, vp, i32, i32, vp, i64, vp, i64, vp, i64]),
+        "fgh_paged_reserve_check": (i32, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedPool), C.c_char_p, C.c_size_t]),
+        "fgh_draft_check": (i32, [C.POINTER(Drafts), C.c_char_p, C.c_size_t]),
+        "fgh_lora_check": (i32, [C.POINTER(Lora), vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, C.c_char_p, C.c_size_t]),
         "fgh_graph_begin": (i32, [vp]),
         "fgh_graph_end": (i32, [vp, C.POINTER(vp)]),
         "fgh_graph_launch": (i32, [vp, vp]),
@@ -653,6 +718,19 @@ class Backend:
                             o_dev: int, ldo: int):
         self._check(self.lib.fgh_paged_attention_dev(self.ctx, cache, batch, mask, n_head, q_dev, ldq, o_dev, ldo))
 
+    def paged_reserve_dev(self, cache: PagedCache, batch: PagedBatch, pool: PagedPool):
+        """The pages of a batch's new tokens, and its tok, len and maps of rows."""
+        self._check(self.lib.fgh_paged_reserve_dev(self.ctx, cache, batch, pool))
+
+    def draft_verify_dev(self, drafts: Drafts, n_ok_dev: int, next_dev: int, *, keep_dev: int = 0, lse_dev: int = 0):
+        """How many drafts of each sequence stay, and the token that follows them."""
+        self._check(self.lib.fgh_draft_verify_dev(self.ctx, drafts, n_ok_dev, next_dev, keep_dev, lse_dev))
+
+    def lora_dev(self, lora: Lora, tok_dev: int, id_dev: int, n_seq: int, n_tok: int, x_dev: int, ldx: int, y_dev: int, ldy: int, *,
+                 y_in_dev: int = 0, ldyi: int = 0):
+        """y = y_in + scale B (A x), every row with the adapter of its sequence (y_in_dev may be y_dev, or 0)."""
+        self._check(self.lib.fgh_lora_dev(self.ctx, lora, tok_dev, id_dev, n_seq, n_tok, x_dev, ldx, y_in_dev, ldyi, y_dev, ldy))
+
     def kvq_store(self, k, v, pos, kq, vq, kbits: int, vbits: int):
         """Writes rows k / v ([n_tok][n_head_kv][hd]) at positions pos into host copies of the
         quantized caches kq / vq ([cap][slot bytes]), on the device; returns the new caches."""
@@ -699,5 +777,5 @@ class Backend:
                 self.dev_free(b)
 
 
-__all__ = ["Backend", "BackendError", "Gguf", "PagedBatch", "PagedCache", "PagedMask", "PagedRope", "Tensor", "load_library", "EXPORTS", "T_Q4_K", "T_Q5_0", "T_Q5_K", "T_Q6_K", "T_Q8_0",
+__all__ = ["Backend", "BackendError", "Drafts", "Gguf", "Lora", "PagedBatch", "PagedCache", "PagedMask", "PagedPool", "PagedRope", "Tensor", "load_library", "EXPORTS", "T_Q4_K", "T_Q5_0", "T_Q5_K", "T_Q6_K", "T_Q8_0",
            "ORDER_AUTO", "ORDER_ROW", "ORDER_REPACKED"]

@@ -19,6 +19,7 @@
 #include "../../include/fastgguf_hip.h"
 #include "fgh_internal.h"
 #include "fgh_paged.h"
+#include "fgh_serve.h"
 
 static const int FG_BATCH = 64;  // prompt batch limit (fastgguf.c:2139)
 
@@ -39,6 +40,7 @@ struct fgh_ctx {
     DevBuf gq;          // prompt-GEMM activation records (launch_gemm_quant layout)
     DevBuf as;          // attention scores / weights
     DevBuf pa;          // paged attention: sums of split ranges
+    DevBuf pr, dv, lo;  // pages of a batch: its sums; drafts: parts of rows; adapters: A x
     DevBuf kqr, kor;    // TurboQuant attention: rotated queries, rotated outputs
     DevBuf msel, mw, mg, mu, md, mlog;  // MoE: selection, weights, gate / up / down outputs
     DevBuf mseg, mslot, mimx, mimh;         // MoE: per-expert slot counts and buckets, Q8_K images of x and h
@@ -520,7 +522,7 @@ void fgh_close(fgh_ctx *c) {
     (void)hipSetDevice(c->device);
     (void)hipStreamSynchronize(c->stream);
     for (DevBuf *b : {&c->x, &c->y, &c->aqs, &c->ad, &c->abs, &c->gq, &c->msel, &c->mw, &c->mg,
-                      &c->mu, &c->md, &c->mlog, &c->mseg, &c->mslot, &c->mimx, &c->mimh, &c->ck, &c->as, &c->pa, &c->kqr,
+                      &c->mu, &c->md, &c->mlog, &c->mseg, &c->mslot, &c->mimx, &c->mimh, &c->ck, &c->as, &c->pa, &c->pr, &c->dv, &c->lo, &c->kqr,
                       &c->kor, &c->h})
         if (b->p) (void)hipFree(b->p);
     free_retired(c);
@@ -1112,6 +1114,118 @@ int fgh_paged_attention_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_
         a.psum.stat = a.dsum.stat + need.drow * 2;
     }
     HIP_TRY(c, fgh::launch_paged_attention(a, c->stream));
+    return FGH_OK;
+}
+// what is wrong with the arguments of the calls around the paged cache, or null
+static bool off4(std::initializer_list<const void *> p) {
+    uintptr_t all = 0;
+    for (const void *q : p) all |= (uintptr_t)q;
+    return all % 4 != 0;
+}
+static const char *reserve_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_pool *p) {
+    if (!c || !b || !p) return "null descriptor";
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return "page is not a power of 2 from 16 to 256";
+    if (c->n_pages < 1 || c->table_stride < 1) return "bad n_pages or table_stride";
+    if (b->n_seq < 1 || b->n_seq > 65535 || b->n_tok < 1 || b->max_tok < 1 || b->max_len < 1) return "bad n_seq, n_tok, max_tok or max_len";
+    if (!c->table || !b->tok || !b->len || !p->keep || !p->add || !p->held || !p->held_out || !p->queue || !p->free || !p->free_out) return "null pointer";
+    if (off4({c->table, b->tok, b->len, p->keep, p->add, p->held, p->held_out, p->queue, p->free, p->free_out, p->seq, p->pos}) || (uintptr_t)p->slot % 8 != 0)
+        return "pointers must be 4-byte aligned, slot 8";
+    return nullptr;
+}
+static const char *draft_check(const fgh_drafts *d) {
+    if (!d) return "null descriptor";
+    if (d->n_seq < 1 || d->n_seq > 65535 || d->n_tok < 1 || d->n_tok > (1 << 18) - 1 || d->max_tok < 1) return "bad n_seq, n_tok or max_tok";
+    if (d->vocab < 1 || d->vocab > 1 << 24) return "vocab is not 1 .. 2^24";
+    if (d->ld < d->vocab || d->ld > (int64_t)1 << 31 || (d->q && (d->ldq < d->vocab || d->ldq > (int64_t)1 << 31))) return "ld or ldq is smaller than a row or too large";
+    if (!d->logits || !d->tok || !d->tokens || !d->u || !d->v || (d->q && !d->q_lse)) return "null pointer";
+    if (off4({d->logits, d->tok, d->tokens, d->u, d->v, d->temp, d->len, d->q, d->q_lse})) return "pointers must be 4-byte aligned";
+    return nullptr;
+}
+static const char *lora_check(const fgh_lora *l, const int32_t *tok, const int32_t *id, int n_seq, int n_tok, const float *x, int64_t ldx,
+                              const float *yin, int64_t ldyi, const float *y, int64_t ldy) {
+    if (!l) return "null descriptor";
+    if (l->type != FGH_T_F32 && l->type != FGH_T_F16 && l->type != FGH_T_BF16) return "the adapters' type is not F32, F16 or BF16";
+    if (l->cols < 8 || l->cols % 8 != 0 || l->cols > 1 << 24 || l->rows < 1 || l->rows > 1 << 24) return "cols is no multiple of 8, or cols or rows is out of range";
+    if (l->max_rank < 8 || l->max_rank % 8 != 0 || l->max_rank > 512) return "max_rank is no multiple of 8 up to 512";
+    if (l->n_adapter < 1) return "bad n_adapter";
+    if (n_seq < 1 || n_seq > 65535 || n_tok < 1 || n_tok > 1 << 30) return "bad n_seq or n_tok";
+    const int64_t most = (int64_t)1 << 31;
+    if (ldx < l->cols || ldy < l->rows || (yin && ldyi < l->rows) || ldx > most || ldy > most || (yin && ldyi > most)) return "ldx, ldyi or ldy is smaller than a row or too large";
+    if (!l->a || !l->b || !tok || !id || !x || !y) return "null pointer";
+    if (off4({l->rank, l->scale, tok, id, x, yin, y})) return "pointers must be 4-byte aligned";
+    if (((uintptr_t)l->a | (uintptr_t)l->b) % 16 != 0) return "the adapters must be 16-byte aligned";
+    if (yin == y && ldyi != ldy) return "y_in is y, with another stride";
+    return nullptr;
+}
+static fgh::LoraArgs lora_args(const fgh_lora *l, int n_seq, int n_tok) {
+    fgh::LoraArgs a{};
+    a.a = (const uint8_t *)l->a, a.b = (const uint8_t *)l->b, a.rank = l->rank, a.scale = l->scale;
+    a.type = (int)l->type, a.n_adapter = l->n_adapter, a.max_rank = l->max_rank, a.cols = l->cols, a.rows = l->rows, a.n_seq = n_seq, a.n_tok = n_tok;
+    return a;
+}
+static int told(const char *why, char *err, size_t err_len) {
+    if (why && err && err_len) snprintf(err, err_len, "%s", why);
+    return why ? FGH_ERR_ARG : FGH_OK;
+}
+int fgh_paged_reserve_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_pool *p, char *err, size_t err_len) {
+    return told(reserve_check(c, b, p), err, err_len);
+}
+int fgh_draft_check(const fgh_drafts *d, char *err, size_t err_len) { return told(draft_check(d), err, err_len); }
+int fgh_lora_check(const fgh_lora *l, const int32_t *tok, const int32_t *id, int n_seq, int n_tok, const float *x, int64_t ldx, const float *yin,
+                   int64_t ldyi, const float *y, int64_t ldy, char *err, size_t err_len) {
+    const char *why = lora_check(l, tok, id, n_seq, n_tok, x, ldx, yin, ldyi, y, ldy);
+    if (!why) {
+        fgh::LoraArgs a = lora_args(l, n_seq, n_tok);
+        (void)fgh::lora_plan(a, 1024);  // more compute units than there are: the largest grids
+        if (fgh::lora_grid(a) > fgh::PAGED_GRID) why = "too many rows or outputs";
+    }
+    return told(why, err, err_len);
+}
+int fgh_paged_reserve_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_pool *pool) {
+    if (!c) return FGH_ERR_ARG;
+    if (const char *why = reserve_check(cache, batch, pool)) return fail(c, FGH_ERR_ARG, "paged_reserve: %s", why);
+    INJECT(c);
+    HIP_TRY(c, hipSetDevice(c->device));
+    fgh::ReserveArgs a{};
+    a.keep = pool->keep, a.add = pool->add, a.held = pool->held, a.free = pool->free;
+    a.held_out = pool->held_out, a.free_out = pool->free_out, a.queue = pool->queue;
+    a.table = const_cast<int32_t *>(cache->table), a.tok = const_cast<int32_t *>(batch->tok), a.len = const_cast<int32_t *>(batch->len);
+    a.seq = pool->seq, a.pos = pool->pos, a.slot = pool->slot;
+    const fgh::Paged p = paged_args(cache, batch);  // its bounds
+    a.n_seq = p.n_seq, a.n_tok = p.n_tok, a.max_tok = p.max_tok, a.max_len = p.max_len, a.n_pages = p.n_pages, a.shift = p.shift, a.table_stride = p.table_stride;
+    if (int rc = grow(c, c->pr, fgh::reserve_scratch(a))) return rc;
+    a.pre = (int32_t *)c->pr.p;
+    HIP_TRY(c, fgh::launch_reserve(a, c->num_cu, c->stream));
+    return FGH_OK;
+}
+int fgh_draft_verify_dev(fgh_ctx *c, const fgh_drafts *d, int32_t *n_ok, int32_t *next, int32_t *keep, float *lse) {
+    if (!c) return FGH_ERR_ARG;
+    if (const char *why = draft_check(d)) return fail(c, FGH_ERR_ARG, "draft_verify: %s", why);
+    if (!n_ok || !next || (keep && !d->len)) return fail(c, FGH_ERR_ARG, "draft_verify: null pointer");
+    if (off4({n_ok, next, keep, lse})) return fail(c, FGH_ERR_ARG, "draft_verify: pointers must be 4-byte aligned");
+    INJECT(c);
+    HIP_TRY(c, hipSetDevice(c->device));
+    fgh::VerifyArgs a{};
+    a.logits = d->logits, a.q = d->q, a.q_lse = d->q_lse, a.temp = d->temp, a.u = d->u, a.v = d->v, a.tok = d->tok, a.tokens = d->tokens, a.len = d->len;
+    a.n_ok = n_ok, a.next = next, a.keep = keep, a.lse = lse, a.ld = d->ld, a.ldq = d->ldq;
+    a.n_seq = d->n_seq, a.n_tok = d->n_tok, a.max_tok = std::min(d->max_tok, d->n_tok), a.vocab = d->vocab;
+    if (int rc = grow(c, c->dv, fgh::verify_plan(a, c->num_cu))) return rc;
+    fgh::verify_scratch(a, c->dv.p);
+    HIP_TRY(c, fgh::launch_verify(a, c->stream));
+    return FGH_OK;
+}
+int fgh_lora_dev(fgh_ctx *c, const fgh_lora *l, const int32_t *tok, const int32_t *id, int n_seq, int n_tok, const float *x, int64_t ldx,
+                 const float *yin, int64_t ldyi, float *y, int64_t ldy) {
+    if (!c) return FGH_ERR_ARG;
+    char err[128];
+    if (fgh_lora_check(l, tok, id, n_seq, n_tok, x, ldx, yin, ldyi, y, ldy, err, sizeof(err))) return fail(c, FGH_ERR_ARG, "lora: %s", err);
+    INJECT(c);
+    HIP_TRY(c, hipSetDevice(c->device));
+    fgh::LoraArgs a = lora_args(l, n_seq, n_tok);
+    a.tok = tok, a.id = id, a.x = x, a.ldx = ldx, a.yin = yin, a.ldyi = ldyi, a.y = y, a.ldy = ldy;
+    if (int rc = grow(c, c->lo, fgh::lora_plan(a, c->num_cu))) return rc;
+    a.part = (float *)c->lo.p;
+    HIP_TRY(c, fgh::launch_lora(a, c->stream));
     return FGH_OK;
 }
 int fgh_kvq_store_dev(fgh_ctx *c, int n_tok, int n_head_kv, int hd, int kbits, int vbits, const float *k,

@@ -1,0 +1,69 @@
+// fgh_serve.h - what a server of many sequences does around the paged cache: pages and rows of a batch (fgh_reserve.hip), drafted
+// tokens checked and tokens drawn (fgh_verify.hip), adapters of many requests (fgh_lora.hip). Internal.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace fgh {
+
+// The sequence of row t, or -1: the last s with tok[s] <= t, if t < tok[s + 1]; tok[0 .. n_seq] does not decrease. A wavefront's 64
+// lanes look at 64 starts at a time, evenly apart: 65535 sequences take three loads that wait for each other.
+__device__ __forceinline__ int seq_of_row(const int32_t *tok, int n_seq, int t) {
+    const int lane = threadIdx.x & 63;
+    int base = 0, len = n_seq + 1;
+    while (len > 64) {
+        const int step = (len + 63) / 64, i = lane * step;
+        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < len && tok[base + (i < len ? i : 0)] <= t));
+        if (c == 0) return -1;
+        base += (c - 1) * step;
+        len = min(step, len - (c - 1) * step);
+    }
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < len && tok[base + (lane < len ? lane : 0)] <= t));
+    const int s = base + c - 1;
+    return s >= n_seq ? -1 : s;
+}
+
+struct ReserveArgs {
+    const int32_t *keep, *add, *held, *free;
+    int32_t *held_out, *free_out, *queue, *table, *tok, *len, *seq, *pos;
+    int64_t *slot;
+    int n_seq, n_tok, max_tok, max_len, n_pages, shift, table_stride;  // max_len: at most the table's positions
+    int32_t *pre;  // reserve_scratch bytes
+};
+size_t reserve_scratch(const ReserveArgs &a);
+hipError_t launch_reserve(const ReserveArgs &a, int num_cu, hipStream_t s);
+
+struct VerifyArgs {
+    const float *logits, *q, *q_lse, *temp, *u, *v;
+    const int32_t *tok, *tokens, *len;
+    int32_t *n_ok, *next, *keep;
+    float *lse;
+    int64_t ld, ldq;
+    int n_seq, n_tok, max_tok, vocab;
+    // set by verify_plan: a row's words over `splits` workgroups, `per` words each, in blocks of 1024 nv
+    int splits, per, nv;
+    double *sum, *rest;  // [n_tok][splits], [n_seq][splits]
+    float *top;          // [n_tok][splits]
+    int32_t *at;         // [n_tok][splits]
+};
+size_t verify_plan(VerifyArgs &a, int num_cu);  // the scratch it takes
+void verify_scratch(VerifyArgs &a, void *p);
+hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
+
+struct LoraArgs {
+    const uint8_t *a, *b;
+    const int32_t *rank, *tok, *id;
+    const float *scale, *x, *yin;
+    float *y, *part;
+    int64_t ldx, ldyi, ldy;
+    int type, n_adapter, max_rank, cols, rows, n_seq, n_tok;
+    // set by lora_plan: tiles of `tile` rows, `slots` workgroups for the runs of one adapter in a tile, A x over ks workgroups of kper
+    // columns, ranks in blocks of 16 nr
+    int tile, slots, ks, kper, nr;
+};
+size_t lora_plan(LoraArgs &a, int num_cu);  // the scratch it takes
+int64_t lora_grid(const LoraArgs &a);       // workgroups of the larger launch
+hipError_t launch_lora(const LoraArgs &a, hipStream_t s);
+
+}  // namespace fgh

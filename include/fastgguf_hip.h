@@ -360,6 +360,79 @@ FGH_API int fgh_paged_attention_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, 
                             const fgh_paged_mask *mask, int n_head, const float *q_dev, int64_t ldq, float *o_dev,
                             int64_t ldo);
 
+/* ---- around the paged cache: a batch's pages and rows, drafted tokens, adapters. No counterpart in the
+ * reference, which serves one sequence at a time. With the two calls above and the matmuls they keep the step of a server of many
+ * sequences on the device: reserve, the projections with their adapters, append, attention, the LM head, verify, whose
+ * `keep` the next reserve takes. All are asynchronous on the context's stream and can be captured (after an eager call with the same
+ * sizes, which sizes the scratch). tok is read as non-decreasing everywhere; where it decreases, the rows and the outputs
+ * of the sequences concerned hold anything. */
+/* The pages of a batch. Sequence s holds held[s] pages, the first entries of its table row; keep[s] of its positions stay
+ * (fewer than before where drafts were rejected, 0 where it has ended), add[s] new tokens want to follow. The free pages are
+ * a ring of n_pages entries: `free` holds the place of the first and their number. The call
+ *   gives back the pages behind the positions that a sequence then has, to the ring's end, in the sequences' order;
+ *   takes the pages that are missing from its front, in the sequences' order (pages that the same call gives back are its last);
+ *   writes the cache's table, the batch's tok and len (the descriptors' memory: the inputs of the two calls above), held_out and
+ *   free_out, and of every row its sequence, its position and its slot, page * cache->page + place in the page
+ *   (seq, pos, slot: [n_tok], each may be NULL; -1 in rows of no sequence, slot -1 where the page is not 0 .. n_pages - 1).
+ * A sequence gets no new tokens (an empty range, len = keep) where add is not 0 .. max_tok, keep + add passes max_len or the table,
+ * or, with the sequences before it, the ring's pages or n_tok rows do not suffice: sequences are served in order, and one
+ * that needs no page does not wait for pages. It gives back pages behind keep all the same. One with a keep below 0 or above its
+ * pages, or a held that is not 0 .. table_stride, gets no tokens and len 0, and its pages stay. A `free` that is no such pair is an
+ * empty ring; a ring whose pages would be more than n_pages takes no more. Of the cache only table, n_pages, page and
+ * table_stride are used. keep may be len, held held_out and free free_out: nothing else may overlap. */
+typedef struct {
+    const int32_t *keep, *add, *held;   /* device, [n_seq] */
+    int32_t *held_out;                  /* device, [n_seq] */
+    int32_t *queue;                     /* device, [n_pages] */
+    const int32_t *free;                /* device, [2]: first, number */
+    int32_t *free_out;                  /* device, [2] */
+    int32_t *seq, *pos;                 /* device, [n_tok], or NULL */
+    int64_t *slot;                      /* device, [n_tok], or NULL */
+} fgh_paged_pool;
+FGH_API int fgh_paged_reserve_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, const fgh_paged_batch *batch,
+                          const fgh_paged_pool *pool);
+/* Drafted tokens against the target's probabilities. Sequence s has rows tok[s] .. tok[s + 1] - 1 (n of them, at most max_tok);
+ * tokens[t] is what row t was computed from, so row i's logits judge token i + 1: the first row's token is known, the
+ * n - 1 others are drafts. With p = softmax(logits / temp[s]) of a row, draft d stays while u[row] q(d) < p(d); n_ok[s] is how many do.
+ * next[s] follows them: at the first rejected draft, the first word whose running sum of max(p - q, 0) passes v[s] times the
+ * whole (p itself where nothing is left, or the draft is no word); behind the last row, the same of p. So next is distributed as
+ * the target's own sampling, given uniform u and v of 0 <= u, v < 1. With one row a sequence this draws a token.
+ * q: the drafter's logits, row t its distribution for token t + 1, and q_lse their log sum exp at the same temperature:
+ * q(j) = exp(q[t][j] / temp[s] - q_lse[t]) (log probabilities with q_lse 0 are such a pair at temperature 1). NULL: drafts without probabilities, q(d) = 1.
+ * temp (NULL: 1) 0: a draft stays if it is the largest logit's word (the lowest of equal ones), which next is, too; u, v, q are not
+ * used. lse[t], if not NULL: log sum exp(logits / temp) of the row (temp 0: of the logits), the q_lse of a drafter that samples with
+ * this call. keep[s], if not NULL (it may be len): len[s] without the rejected drafts, not below 0.
+ * Logits of -infinity are words that cannot be; a row with NaN, +infinity or nothing else, or a temp below 0 or NaN, has no
+ * distribution: its draft is rejected and next is -1. A q that is NaN counts as 0 in the sums, and its draft is rejected. A sequence without
+ * rows, or with more than max_tok or outside 0 .. n_tok: n_ok 0, next -1, keep as len. Exponentials, sums and
+ * comparisons are in 64 bits. vocab up to 2^24, n_tok below 2^18, pointers 4-byte aligned, any strides. Inputs and outputs do not overlap but for keep. */
+typedef struct {
+    const float *logits;                /* device, [n_tok][ld] */
+    const float *q, *q_lse;             /* device, [n_tok][ldq] and [n_tok], or NULL */
+    const int32_t *tok, *tokens, *len;  /* device, [n_seq + 1], [n_tok], [n_seq] (len NULL without keep) */
+    const float *temp, *u, *v;          /* device, [n_seq] or NULL, [n_tok], [n_seq] */
+    int64_t ld, ldq;
+    int32_t n_seq, n_tok, max_tok, vocab;
+} fgh_drafts;
+FGH_API int fgh_draft_verify_dev(fgh_ctx *ctx, const fgh_drafts *drafts, int32_t *n_ok_dev, int32_t *next_dev, int32_t *keep_dev,
+                         float *lse_dev);
+/* Low-rank adapters of many requests beside a projection: y[t] = y_in[t] + scale B (A x[t]) for the rows t of each sequence, with the
+ * adapter id[s] of n_adapter: A [max_rank][cols] and B [rows][max_rank], of which the first rank[id] (0 .. max_rank; NULL: max_rank) count;
+ * scale [n_adapter] (NULL: 1). id -1: y = y_in; any other id or rank: NaN rows. y_in NULL: 0. y_in may be y (ldyi == ldy); else
+ * y overlaps no input. Rows before tok[0] and from tok[n_seq] on are left as they were. Results are those of fp32 sums,
+ * whatever the type. Rows of one adapter that stand together share its reads: order sequences by adapter. x that is not
+ * finite, or above 2^127, makes its row anything. n_seq up to 65535.
+ * cols and max_rank multiples of 8 (max_rank up to 512), a and b 16-byte aligned, the others 4-byte; any strides. */
+typedef struct {
+    const void *a, *b;                  /* device, [n_adapter][max_rank][cols] and [n_adapter][rows][max_rank] */
+    const int32_t *rank;                /* device, [n_adapter], or NULL */
+    const float *scale;                 /* device, [n_adapter], or NULL */
+    uint32_t type;                      /* FGH_T_F32, FGH_T_F16 or FGH_T_BF16 */
+    int32_t n_adapter, max_rank, cols, rows;
+} fgh_lora;
+FGH_API int fgh_lora_dev(fgh_ctx *ctx, const fgh_lora *lora, const int32_t *tok_dev, const int32_t *id_dev, int n_seq, int n_tok,
+                 const float *x_dev, int64_t ldx, const float *y_in_dev, int64_t ldyi, float *y_dev, int64_t ldy);
+
 /* ---- HIP graphs of device-resident calls (launch-bound decode loops) ----
  * fgh_graph_begin starts capturing the context stream; the *_dev calls that follow are recorded,
  * not run; fgh_graph_end instantiates them as one executable graph that fgh_graph_launch replays
@@ -439,7 +512,9 @@ FGH_API int fgh_event_destroy(fgh_ctx *ctx, void *ev);
  * fgh_paged_plan: what fgh_paged_attention_dev launches on a device of num_cu compute units: plan[0] over how many
  * workgroups the ranges of positions of sequences with few rows are split at most (0: no such kernel), plan[1] the same
  * of the others, plan[2] the rows of a workgroup of these, plan[3] whether only one of them runs on a compute
- * unit. Needs no device; FGH_ERR_ARG for what fgh_paged_check refuses. */
+ * unit. Needs no device; FGH_ERR_ARG for what fgh_paged_check refuses.
+ * fgh_paged_reserve_check, fgh_draft_check, fgh_lora_check: the argument checks of fgh_paged_reserve_dev, fgh_draft_verify_dev
+ * (its descriptor's) and fgh_lora_dev, without pointers being read: FGH_OK, or FGH_ERR_ARG with a message in err. Need no device. */
 #define FGH_MATMUL_DECODE 0
 #define FGH_MATMUL_GEMM 1
 #define FGH_MATMUL_TOKENS 2
@@ -466,6 +541,11 @@ FGH_API int fgh_paged_check(const fgh_paged_cache *cache, const fgh_paged_batch 
                     size_t err_len);
 FGH_API int fgh_paged_plan(const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_mask *mask, int n_head,
                    int num_cu, int32_t *plan);
+FGH_API int fgh_paged_reserve_check(const fgh_paged_cache *cache, const fgh_paged_batch *batch, const fgh_paged_pool *pool, char *err,
+                            size_t err_len);
+FGH_API int fgh_draft_check(const fgh_drafts *drafts, char *err, size_t err_len);
+FGH_API int fgh_lora_check(const fgh_lora *lora, const int32_t *tok, const int32_t *id, int n_seq, int n_tok, const float *x, int64_t ldx,
+                   const float *y_in, int64_t ldyi, const float *y, int64_t ldy, char *err, size_t err_len);
 
 #ifdef __cplusplus
 }
