@@ -34,6 +34,13 @@ struct ReserveArgs {
 size_t reserve_scratch(const ReserveArgs &a);
 hipError_t launch_reserve(const ReserveArgs &a, int num_cu, hipStream_t s);
 
+// what a sequence's rows come to: the row t that the next token is drawn from, its sum, largest value and the place of that; the draft d that
+// it rejects, or -1; the rows n (0: no token) and the accepted drafts
+struct VerifyChoice {
+    double sum;
+    float top;
+    int at, t, d, n, good;
+};
 struct VerifyArgs {
     const float *logits, *q, *q_lse, *temp, *u, *v;
     const int32_t *tok, *tokens, *len;
@@ -46,6 +53,7 @@ struct VerifyArgs {
     double *sum, *rest;  // [n_tok][splits], [n_seq][splits]
     float *top;          // [n_tok][splits]
     int32_t *at;         // [n_tok][splits]
+    VerifyChoice *choice;  // [n_seq]
 };
 size_t verify_plan(VerifyArgs &a, int num_cu);  // the scratch it takes
 void verify_scratch(VerifyArgs &a, void *p);

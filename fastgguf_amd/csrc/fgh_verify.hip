@@ -8,6 +8,8 @@
 // from those.
 #include "fgh_serve.h"
 
+#include <limits.h>
+
 #include <algorithm>
 
 namespace fgh {
@@ -19,23 +21,27 @@ typedef float vf4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
-// 2^t, off by at most 1e-14 of it: t - rint(t) in the exponential's series to the 11th power. -infinity and NaN give 0.
+// 2^t for -1000 <= t <= 1000, off by 9e-13 of it: t's nearest whole number by an addition that leaves it in the low bits, which go into the
+// exponent, and a polynomial of what is left, at most 1/2 (its coefficients: the least largest error, 1 exact at 0).
+// 16 instructions of 64 bits a value with the sum; rint, a conversion and an exponent function instead cost twice the time.
+__device__ __forceinline__ double exp2_near(double t) {
+    const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);
+    double r = 1.3178933573679677e-06;
+    r = __builtin_fma(r, f, 1.5309156297959352e-05);
+    r = __builtin_fma(r, f, 1.5403825462941963e-04);
+    r = __builtin_fma(r, f, 1.3333454860108985e-03);
+    r = __builtin_fma(r, f, 9.6181286161221811e-03);
+    r = __builtin_fma(r, f, 5.5504109352666739e-02);
+    r = __builtin_fma(r, f, 2.4022650698110606e-01);
+    r = __builtin_fma(r, f, 6.9314718054821234e-01);
+    r = __builtin_fma(r, f, 1.0);
+    const uint64_t u = __builtin_bit_cast(uint64_t, r), n = __builtin_bit_cast(uint64_t, whole);
+    return __builtin_bit_cast(double, u + (n << 52));
+}
+// 2^t: 0 below 2^-1000 and where t is NaN, 2^1000 at most
 __device__ __forceinline__ double exp2_of(double t) {
-    t = fmin(fmax(t, -1100.0), 1100.0);
-    const double n = rint(t), f = (t - n) * LN2;
-    double r = 1.0 / 39916800;
-    r = __builtin_fma(r, f, 1.0 / 3628800);
-    r = __builtin_fma(r, f, 1.0 / 362880);
-    r = __builtin_fma(r, f, 1.0 / 40320);
-    r = __builtin_fma(r, f, 1.0 / 5040);
-    r = __builtin_fma(r, f, 1.0 / 720);
-    r = __builtin_fma(r, f, 1.0 / 120);
-    r = __builtin_fma(r, f, 1.0 / 24);
-    r = __builtin_fma(r, f, 1.0 / 6);
-    r = __builtin_fma(r, f, 0.5);
-    r = __builtin_fma(r, f, 1.0);
-    r = __builtin_fma(r, f, 1.0);
-    return __builtin_amdgcn_ldexp(r, (int)n);
+    const double r = exp2_near(fmin(fmax(t, -1000.0), 1000.0));
+    return t >= -1000.0 ? r : 0.0;
 }
 
 // log2(e) / T of a sequence; T = 0, the largest value, has 1's. A T below 0 or NaN makes NaN.
@@ -45,7 +51,8 @@ __device__ __forceinline__ double heat_of(const VerifyArgs &a, int s, bool &gree
     return greedy ? LOG2E : t > 0.0f ? LOG2E / (double)t : (double)__builtin_nanf("");
 }
 
-// a row, or a part of one: its largest value (NaN where it has a NaN), the first place of it, sum of 2^((x - top) c)
+// a row, or a part of one: its largest value (NaN where it has a NaN), the first place of it where the largest is asked for, sum of
+// 2^((x - top) c)
 struct Part {
     double sum;
     float top;
@@ -53,25 +60,18 @@ struct Part {
 };
 // the largest value to take others relative to: 0 where there is none
 __device__ __forceinline__ double level(float top) { return fabsf(top) <= 3.4028235e38f ? (double)top : 0.0; }
-__device__ __forceinline__ Part join(const Part &x, const Part &y, double c) {  // x's words stand before y's
-    Part r;
-    const bool nan = x.top != x.top || y.top != y.top, second = y.top > x.top;
-    r.top = nan ? __builtin_nanf("") : second ? y.top : x.top;
-    r.at = second ? y.at : x.at;
-    const double m = level(r.top);
-    r.sum = x.sum * exp2_of(((double)x.top - m) * c) + y.sum * exp2_of(((double)y.top - m) * c);  // 0 for a part without words
-    return r;
-}
-__device__ __forceinline__ Part shfl_part(const Part &p, int mask) {
-    return Part{__shfl_xor(p.sum, mask, 64), __shfl_xor(p.top, mask, 64), __shfl_xor(p.at, mask, 64)};
-}
-// over a wavefront's lanes, in the lanes' order; every lane gets it
-__device__ __forceinline__ Part join_wave(Part p, double c) {
-    const int lane = threadIdx.x & 63;
-    for (int o = 1; o < 64; o <<= 1) {
-        const Part z = shfl_part(p, o);
-        p = lane & o ? join(z, p, c) : join(p, z, c);
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }  // NaN if either is
+// over `lanes` lanes that have a part each (a power of two); every one gets the whole
+__device__ __forceinline__ Part join_lanes(Part p, double c, int lanes) {
+    const float own = p.top;
+    for (int o = 1; o < lanes; o <<= 1) {
+        const float y = __shfl_xor(p.top, o, 64);
+        const int at = __shfl_xor(p.at, o, 64);
+        p.at = y > p.top ? at : y == p.top ? min(p.at, at) : p.at;
+        p.top = larger(p.top, y);
     }
+    p.sum *= exp2_of(((double)own - level(p.top)) * c);  // 0 for a part without words
+    for (int o = 1; o < lanes; o <<= 1) p.sum += __shfl_xor(p.sum, o, 64);
     return p;
 }
 
@@ -97,113 +97,94 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     if (s < 0) return;
     bool greedy;
     const double c = heat_of(a, s, greedy);
-    Part p{0.0, -__builtin_inff(), from};
+    Part p{0.0, -__builtin_inff(), INT_MAX};
     for (int base = from; base < to; base += 1024 * NV) {
         if (base != from) load(base);
-        Part b{0.0, -__builtin_inff(), base};
-        bool nan = false;
+        const float was = p.top;
+        float top = was;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) top = larger(larger(top, larger(v[i].x, v[i].y)), larger(v[i].z, v[i].w));
+        if (greedy && top > was)  // a lane's words rise: its first one that is as large
+#pragma unroll
+            for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+                for (int e = 3; e >= 0; --e)
+                    if (v[i][e] == top) p.at = base + i * 1024 + 4 * tid + e;
+        const double m = level(top);
+        if (base != from) p.sum *= exp2_of(((double)was - m) * c);
+        p.top = top;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float y = v[i][e];
-                nan |= y != y;
-                if (y > b.top) b.top = y, b.at = base + i * 1024 + 4 * tid + e;
-            }
-        const double m = level(b.top);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b.sum += exp2_of(((double)v[i][e] - m) * c);
-        if (nan) b.top = __builtin_nanf("");
-        // lanes' words are not in order: the smaller place of two equal ones
-        Part r = join(p, b, c);
-        p = r;
+            for (int e = 0; e < 4; ++e) p.sum += exp2_near(fmax(((double)v[i][e] - m) * c, -1000.0));
     }
-    // a lane's words lie between other lanes': equal largest values go to the lower place
-    for (int o = 1; o < 64; o <<= 1) {
-        const Part z = shfl_part(p, o);
-        const int at = p.top == z.top ? min(p.at, z.at) : z.top > p.top ? z.at : p.at;
-        p = (tid & o) ? join(z, p, c) : join(p, z, c);
-        p.at = at;
-    }
+    p = join_lanes(p, c, 64);
     if ((tid & 63) == 0) lds[tid >> 6] = p;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < 4; ++w) {
-            const Part z = lds[w];
-            const int at = p.top == z.top ? min(p.at, z.at) : z.top > p.top ? z.at : p.at;
-            p = join(p, z, c);
-            p.at = at;
+    if (tid < 4) {
+        p = join_lanes(lds[tid], c, 4);
+        if (tid == 0) {
+            const int64_t i = (int64_t)row * a.splits + split;
+            a.sum[i] = p.sum, a.top[i] = p.top, a.at[i] = p.at;
         }
-        const int64_t i = (int64_t)row * a.splits + split;
-        a.sum[i] = p.sum, a.top[i] = p.top, a.at[i] = p.at;
     }
 }
 
-// what a sequence's rows come to
-struct Choice {
-    Part row;       // of the row that the next token is drawn from
-    int t, d;       // that row; the draft that it rejects, or -1
-    int n, good;    // rows, accepted drafts; n = 0: no token
-};
-// the sequence's rows, their ends in the buffers: none for what a batch cannot mean
+constexpr int WG = 512;  // threads that decide: 8 rows at a time
+
+// the sequence's rows: none for what a batch cannot mean
 __device__ __forceinline__ int2 rows_of(const VerifyArgs &a, int s) {
     const int b = a.tok[s], e = a.tok[s + 1];
     if (b < 0 || e > a.n_tok || e <= b || e - b > a.max_tok) return int2{0, 0};
     return int2{b, e - b};
 }
-__device__ __forceinline__ Part row_part(const VerifyArgs &a, int t, double c) {
-    const int lane = threadIdx.x & 63;
-    Part p{0.0, -__builtin_inff(), 0};
-    if (lane < a.splits) {
-        const int64_t i = (int64_t)t * a.splits + lane;
-        p = Part{a.sum[i], a.top[i], a.at[i]};
-    }
-    return join_wave(p, c);
-}
-// the draft's probability under q; NaN, which passes no test, where q has one
-__device__ __forceinline__ double q_at(const VerifyArgs &a, int t, int d, double c) {
-    const double x = (double)a.q[t * a.ldq + d] * c - (double)a.q_lse[t] * LOG2E;
-    return x == x ? exp2_of(x) : x;
-}
-// by a workgroup of 256, a wavefront to a row, four rows at a time until one is rejected (all of them where `lse` is written)
-__device__ Choice decide(const VerifyArgs &a, int s, double c, bool greedy, bool lse) {
-    __shared__ Part rows[4];
-    __shared__ int ok[4];
-    const int wave = threadIdx.x >> 6;
+// by a workgroup, a wavefront to a row, 8 rows at a time until one is rejected (all of them where `lse` is written)
+__device__ VerifyChoice decide(const VerifyArgs &a, int s, double c, bool greedy, bool lse) {
+    __shared__ Part rows[WG / 64];
+    __shared__ int ok[WG / 64], word[WG / 64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int2 r = rows_of(a, s);
-    Choice ch;
-    ch.n = r.y, ch.good = 0, ch.t = -1, ch.d = -1, ch.row = Part{0.0, 0.0f, 0};
+    VerifyChoice ch{0.0, 0.0f, 0, -1, -1, r.y, 0};
     bool open = true;
-    for (int i0 = 0; i0 < r.y && (open || lse); i0 += 4) {
+    for (int i0 = 0; i0 < r.y && (open || lse); i0 += WG / 64) {
         const int i = i0 + wave, t = r.x + i;
         if (i < r.y) {
-            const Part p = row_part(a, t, c);
+            Part p{0.0, -__builtin_inff(), INT_MAX};
+            if (lane < a.splits) {
+                const int64_t k = (int64_t)t * a.splits + lane;
+                p = Part{a.sum[k], a.top[k], a.at[k]};
+            }
+            const int d = i < r.y - 1 ? a.tokens[t + 1] : -1;
+            const bool is_word = (uint32_t)d < (uint32_t)a.vocab;
+            float x = 0.0f, u = 0.0f, q = 0.0f, q_lse = 0.0f;
+            if (is_word) {
+                x = a.logits[t * a.ld + d], u = a.u[t];
+                if (a.q) q = a.q[t * a.ldq + d], q_lse = a.q_lse[t];
+            }
+            p = join_lanes(p, c, 64);
             bool good = false;
-            if (i < r.y - 1) {
-                const int d = a.tokens[t + 1];
-                if ((uint32_t)d < (uint32_t)a.vocab && fabsf(p.top) <= 3.4028235e38f) {
-                    if (greedy) good = d == p.at;
-                    else {
-                        const double w = exp2_of(((double)a.logits[t * a.ld + d] - p.top) * c) / p.sum;
-                        good = (double)a.u[t] * (a.q ? q_at(a, t, d, c) : 1.0) < w && c == c;
-                    }
+            if (is_word && fabsf(p.top) <= 3.4028235e38f) {
+                if (greedy) good = d == p.at;
+                else {
+                    const double under = (double)q * c - (double)q_lse * LOG2E;  // NaN passes no test
+                    const double chance = !a.q ? 1.0 : under == under ? exp2_of(under) : under;
+                    good = (double)u * chance < exp2_of(((double)x - p.top) * c) / p.sum && c == c;
                 }
             }
-            if ((threadIdx.x & 63) == 0) {
-                rows[wave] = p, ok[wave] = good;
-                if (lse) a.lse[t] = p.top != p.top || c != c ? __builtin_nanf("") : fabsf(p.top) <= 3.4028235e38f ? (float)(level(p.top) * c * LN2 + log(p.sum)) : p.top;
+            if (lane == 0) {
+                rows[wave] = p, ok[wave] = good, word[wave] = is_word ? d : -1;  // no word: the token is drawn from p
+                if (lse) a.lse[t] = p.top != p.top || c != c ? __builtin_nanf("") : fabsf(p.top) <= 3.4028235e38f ? (float)((double)p.top * c * LN2 + log(p.sum)) : p.top;
             }
         }
         __syncthreads();
-        for (int w = 0; w < 4 && open && i0 + w < r.y; ++w) {
-            ch.row = rows[w], ch.t = r.x + i0 + w;
-            if (i0 + w == r.y - 1 || !ok[w]) {
-                open = false;
-                ch.d = i0 + w == r.y - 1 ? -1 : a.tokens[ch.t + 1];
-                if ((uint32_t)ch.d >= (uint32_t)a.vocab) ch.d = -1;  // no word: the token is drawn from p
-            } else ++ch.good;
+        for (int w = 0; w < WG / 64 && open && i0 + w < r.y; ++w) {
+            const bool last = i0 + w == r.y - 1;
+            if (!last && ok[w]) {
+                ++ch.good;
+                continue;
+            }
+            open = false;
+            ch.sum = rows[w].sum, ch.top = rows[w].top, ch.at = rows[w].at, ch.t = r.x + i0 + w, ch.d = last ? -1 : word[w];
         }
         __syncthreads();
     }
@@ -218,42 +199,69 @@ struct Weigh {
     int d;
 };
 template <int MODE>
-__device__ __forceinline__ double weight(const Weigh &w, int j) {
+__device__ __forceinline__ double weight(const Weigh &w, int j, float x, float q) {
+    const double p = exp2_of(((double)x - w.m) * w.c);
     if (MODE == WITHOUT_DRAFT && j == w.d) return 0.0;
-    const double p = exp2_of(((double)w.x[j] - w.m) * w.c);
-    if (MODE != FROM_REST) return p;
-    const double q = exp2_of((double)w.q[j] * w.c - w.lse);
-    return fmax(p * w.z - q, 0.0);
+    return MODE == FROM_REST ? fmax(p * w.z - exp2_of((double)q * w.c - w.lse), 0.0) : p;
 }
-__device__ __forceinline__ Weigh weigh_of(const VerifyArgs &a, const Choice &ch, double c) {
+__device__ __forceinline__ Weigh weigh_of(const VerifyArgs &a, const VerifyChoice &ch, double c) {
     Weigh w;
     w.x = a.logits + ch.t * a.ld, w.q = a.q ? a.q + ch.t * a.ldq : nullptr;
-    w.m = level(ch.row.top), w.c = c, w.z = 1.0 / ch.row.sum, w.lse = a.q ? (double)a.q_lse[ch.t] * LOG2E : 0.0, w.d = ch.d;
+    w.m = level(ch.top), w.c = c, w.z = 1.0 / ch.sum, w.lse = a.q ? (double)a.q_lse[ch.t] * LOG2E : 0.0, w.d = ch.d;
     return w;
 }
-__device__ __forceinline__ double sum_block(double v) {
-    __shared__ double lds[4];
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+// f(first word, weights of 4) of a thread's words b .. e - 1
+template <int MODE, class F>
+__device__ __forceinline__ void each4(const Weigh &w, int b, int e, F &&f) {
+    for (int j = b; j < e; j += 4) {
+        double x[4];
+        if (j + 4 <= e) {
+            const vf4 p = *(const vf4 *)(w.x + j);
+            vf4 q = p;
+            if (MODE == FROM_REST) q = *(const vf4 *)(w.q + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = weight<MODE>(w, j + i, p[i], q[i]);
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = j + i < e ? weight<MODE>(w, j + i, w.x[j + i], MODE == FROM_REST ? w.q[j + i] : 0.0f) : 0.0;
+        f(j, x);
+    }
+}
+// over the workgroup: the sum of the threads before, and the whole
+__device__ __forceinline__ double2 scan_block(double v) {
+    __shared__ double lds[WG / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double upto = v;
+    for (int o = 1; o < 64; o <<= 1) {
+        const double z = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += z;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    if (lane == 63) lds[wave] = upto;
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    double before = 0.0, all = 0.0;
+    for (int i = 0; i < WG / 64; ++i) {
+        if (i < wave) before += lds[i];
+        all += lds[i];
+    }
+    return double2{before + (upto - v), all};
 }
 template <int MODE>
 __device__ __forceinline__ double sum_words(const Weigh &w, int from, int to) {
     double v = 0.0;
-    for (int j = from + threadIdx.x; j < to; j += 256) v += weight<MODE>(w, j);
-    return sum_block(v);
+    for (int b = from + 4 * (int)threadIdx.x; b < to; b += 4 * WG) each4<MODE>(w, b, min(to, b + 4), [&](int, const double (&x)[4]) { v += (x[0] + x[1]) + (x[2] + x[3]); });
+    return scan_block(v).y;
 }
 
-// sums of max(p - q, 0) of a rejected row, by parts
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs a) {
+// the decision where the drafts have probabilities, and the sums of max(p - q, 0) of a rejected row, by parts
+__global__ __launch_bounds__(WG) void verify_rest_kernel(VerifyArgs a) {
     const int s = blockIdx.x / a.splits, split = blockIdx.x - s * a.splits;
     bool greedy;
     const double c = heat_of(a, s, greedy);
-    if (greedy || !(c == c)) return;
-    const Choice ch = decide(a, s, c, greedy, false);
-    if (ch.d < 0) return;
+    if (split > 0 && (greedy || !(c == c))) return;
+    const VerifyChoice ch = decide(a, s, c, greedy, a.lse && split == 0);
+    if (split == 0 && threadIdx.x == 0) a.choice[s] = ch;
+    if (greedy || !(c == c) || ch.d < 0) return;
     const double v = sum_words<FROM_REST>(weigh_of(a, ch, c), split * a.per, min(a.vocab, (split + 1) * a.per));
     if (threadIdx.x == 0) a.rest[(int64_t)s * a.splits + split] = v;
 }
@@ -261,97 +269,79 @@ __global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs a) {
 // the first of words from .. to - 1 whose running sum passes `aim`, or the last of any weight (-1: none has)
 template <int MODE>
 __device__ int pick(const Weigh &w, int from, int to, double aim) {
-    __shared__ double sums[4];
-    __shared__ int word, last;
-    const int per = (to - from + 255) / 256, b = min(to, from + (int)threadIdx.x * per), e = min(to, b + per), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ int first, last;
+    const int per = ((to - from + WG - 1) / WG + 3) & ~3, b = min(to, from + (int)threadIdx.x * per), e = min(to, b + per);
     double own = 0.0;
-    for (int j = b; j < e; ++j) own += weight<MODE>(w, j);
-    double upto = own;
+    each4<MODE>(w, b, e, [&](int, const double (&x)[4]) { own += (x[0] + x[1]) + (x[2] + x[3]); });
+    if (threadIdx.x == 0) first = WG, last = -1;
+    double run = scan_block(own).x;  // its barriers stand before what follows
+    if (own > 0.0) {
+        atomicMax(&last, (int)threadIdx.x);
+        if (run + own > aim) atomicMin(&first, (int)threadIdx.x);
+    }
+    __syncthreads();
+    const int mine = first < WG ? first : last;
+    __syncthreads();
+    if (mine < 0) return -1;
+    if (threadIdx.x == mine) {
+        int at = -1;
+        bool found = false;
+        each4<MODE>(w, b, e, [&](int j, const double (&x)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[i] > 0.0 && !found) {
+                    at = j + i;
+                    run += x[i];
+                    found = run > aim;
+                }
+        });
+        first = at;
+    }
+    __syncthreads();
+    return first;
+}
+
+// the part, then the word; a lane has a part's sum, the same in every wavefront
+template <int MODE>
+__device__ int draw(const VerifyArgs &a, const Weigh &w, double sum, double v) {
+    const int lane = threadIdx.x & 63;
+    double upto = sum;
     for (int o = 1; o < 64; o <<= 1) {
         const double z = __shfl_up(upto, o, 64);
         if (lane >= o) upto += z;
     }
-    if (lane == 63) sums[wave] = upto;
-    if (threadIdx.x == 0) word = to, last = -1;
-    __syncthreads();
-    for (int i = 0; i < wave; ++i) upto += sums[i];
-    double run = upto - own;
-    if (own > 0.0) {
-        int at = to, end = -1;
-        for (int j = b; j < e; ++j) {
-            const double x = weight<MODE>(w, j);
-            run += x;
-            if (x > 0.0) {
-                end = j;
-                if (run > aim && at == to) at = j;
-            }
-        }
-        if (at < to) atomicMin(&word, at);
-        if (end >= 0) atomicMax(&last, end);
-    }
-    __syncthreads();
-    return word < to ? word : last;
+    const double aim = v * __shfl(upto, 63, 64);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(sum > 0.0), past = __builtin_amdgcn_ballot_w64(sum > 0.0 && upto > aim);
+    if (!some) return -1;
+    const int part = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // none passes by a rounding, or v is 1 or more: the last
+    return pick<MODE>(w, part * a.per, min(a.vocab, (part + 1) * a.per), aim - __shfl(upto - sum, part, 64));
 }
 
-// chooses the part, then the word; sums[] holds the parts' sums
-template <int MODE>
-__device__ int draw(const VerifyArgs &a, const Weigh &w, const double *sums, double aim) {
-    double run = 0.0;
-    int part = -1;
-    double before = 0.0;
-    for (int i = 0; i < a.splits; ++i) {  // the first part that passes the aim, or the last of any weight
-        const double x = sums[i];
-        if (x > 0.0) {
-            part = i, before = run;
-            run += x;
-            if (run > aim) break;
-        }
-    }
-    if (part < 0) return -1;
-    return pick<MODE>(w, part * a.per, min(a.vocab, (part + 1) * a.per), aim - before);
-}
-
-__global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
-    __shared__ double sums[64];
-    const int s = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     bool greedy;
     const double c = heat_of(a, s, greedy);
-    const Choice ch = decide(a, s, c, greedy, a.lse != nullptr);
+    const VerifyChoice ch = a.q ? a.choice[s] : decide(a, s, c, greedy, a.lse != nullptr);
     int word = -1;
-    if (ch.n > 0 && fabsf(ch.row.top) <= 3.4028235e38f && c == c) {
-        if (greedy) word = ch.row.at;
+    if (ch.n > 0 && fabsf(ch.top) <= 3.4028235e38f && c == c) {
+        if (greedy) word = ch.at;
         else {
             const Weigh w = weigh_of(a, ch, c);
             const double v = a.v[s];
-            auto parts = [&] {  // of p: what the rows' pass left, on the row's level
-                if (tid < a.splits) {
-                    const int64_t i = (int64_t)ch.t * a.splits + tid;
-                    sums[tid] = a.sum[i] * exp2_of(((double)a.top[i] - w.m) * c);
-                }
-                __syncthreads();
-            };
-            auto whole = [&] {
-                double r = 0.0;
-                for (int i = 0; i < a.splits; ++i) r += sums[i];
-                return r;
-            };
-            if (ch.d >= 0 && a.q) {
-                if (tid < a.splits) sums[tid] = a.rest[(int64_t)s * a.splits + tid];
-                __syncthreads();
-                word = draw<FROM_REST>(a, w, sums, v * whole());
-            } else if (ch.d >= 0) {
-                parts();
-                const int mine = ch.d / a.per;  // the draft's part without it
-                const double left = sum_words<WITHOUT_DRAFT>(w, mine * a.per, min(a.vocab, (mine + 1) * a.per));
-                if (tid == 0) sums[mine] = left;
-                __syncthreads();
-                word = draw<WITHOUT_DRAFT>(a, w, sums, v * whole());
+            double part = 0.0;  // of p: what the rows' pass left, on the row's level
+            if (lane < a.splits) {
+                const int64_t i = (int64_t)ch.t * a.splits + lane;
+                part = a.sum[i] * exp2_of(((double)a.top[i] - w.m) * c);
             }
-            if (word < 0) {  // behind the last row, or nothing is left of p
-                __syncthreads();
-                parts();
-                word = draw<FROM_P>(a, w, sums, v * whole());
+            if (ch.d >= 0 && a.q) word = draw<FROM_REST>(a, w, lane < a.splits ? a.rest[(int64_t)s * a.splits + lane] : 0.0, v);
+            else if (ch.d >= 0) {
+                // the draft's part without it: by a difference where that loses a bit at most, else anew
+                const int mine = ch.d / a.per;
+                const double with = __shfl(part, mine, 64), x = weight<FROM_P>(w, ch.d, w.x[ch.d], 0.0f);
+                const double left = x <= 0.5 * with ? with - x : sum_words<WITHOUT_DRAFT>(w, mine * a.per, min(a.vocab, (mine + 1) * a.per));
+                word = draw<WITHOUT_DRAFT>(a, w, lane == mine ? left : part, v);
             }
+            if (word < 0) word = draw<FROM_P>(a, w, part, v);  // behind the last row, or nothing is left of p
         }
     }
     if (tid == 0) {
@@ -366,19 +356,20 @@ __global__ __launch_bounds__(256) void verify_next_kernel(VerifyArgs a) {
 size_t verify_plan(VerifyArgs &a, int num_cu) {
     auto parts = [&](int nv) { return (a.vocab + 1024 * nv - 1) / (1024 * nv); };
     a.nv = 8;
-    while (a.nv > 1 && (int64_t)a.n_tok * parts(a.nv) < 2 * num_cu) a.nv /= 2;
+    while (a.nv > 1 && (int64_t)a.n_tok * parts(a.nv) < 4 * num_cu) a.nv /= 2;
     const int blocks = parts(a.nv);
     a.splits = std::min(64, blocks);  // a wavefront joins them
     a.per = (blocks + a.splits - 1) / a.splits * 1024 * a.nv;
     a.splits = (a.vocab + a.per - 1) / a.per;
     const size_t n = (size_t)a.n_tok * a.splits;
-    return n * 16 + (a.q ? (size_t)a.n_seq * a.splits * 8 : 0);
+    return n * 16 + (a.q ? (size_t)a.n_seq * (a.splits * 8 + sizeof(VerifyChoice)) : 0);
 }
 void verify_scratch(VerifyArgs &a, void *p) {
-    const size_t n = (size_t)a.n_tok * a.splits;
+    const size_t n = (size_t)a.n_tok * a.splits, m = a.q ? a.n_seq : 0;
     a.sum = (double *)p;
     a.rest = a.sum + n;
-    a.top = (float *)(a.rest + (a.q ? (size_t)a.n_seq * a.splits : 0));
+    a.choice = (VerifyChoice *)(a.rest + m * a.splits);
+    a.top = (float *)(a.choice + m);
     a.at = (int32_t *)(a.top + n);
 }
 
@@ -390,8 +381,8 @@ hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) {
     case 4: verify_rows_kernel<4><<<grid, 256, 0, s>>>(a); break;
     default: verify_rows_kernel<8><<<grid, 256, 0, s>>>(a); break;
     }
-    if (a.q) verify_rest_kernel<<<(unsigned)((int64_t)a.n_seq * a.splits), 256, 0, s>>>(a);
-    verify_next_kernel<<<(unsigned)a.n_seq, 256, 0, s>>>(a);
+    if (a.q) verify_rest_kernel<<<(unsigned)((int64_t)a.n_seq * a.splits), WG, 0, s>>>(a);
+    verify_next_kernel<<<(unsigned)a.n_seq, WG, 0, s>>>(a);
     return hipGetLastError();
 }
 
