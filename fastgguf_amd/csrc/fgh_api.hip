@@ -1224,7 +1224,7 @@ int fgh_lora_dev(fgh_ctx *c, const fgh_lora *l, const int32_t *tok, const int32_
     fgh::LoraArgs a = lora_args(l, n_seq, n_tok);
     a.tok = tok, a.id = id, a.x = x, a.ldx = ldx, a.yin = yin, a.ldyi = ldyi, a.y = y, a.ldy = ldy;
     if (int rc = grow(c, c->lo, fgh::lora_plan(a, c->num_cu))) return rc;
-    a.part = (float *)c->lo.p;
+    fgh::lora_scratch(a, c->lo.p);
     HIP_TRY(c, fgh::launch_lora(a, c->stream));
     return FGH_OK;
 }

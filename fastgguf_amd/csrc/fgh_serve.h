@@ -59,6 +59,11 @@ size_t verify_plan(VerifyArgs &a, int num_cu);  // the scratch it takes
 void verify_scratch(VerifyArgs &a, void *p);
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 
+// rows of one adapter that stand together in a tile of a batch. adapter -1: none, -2: what is no adapter; n = 0: no rows
+struct LoraRun {
+    int row, n, adapter, rank;
+    float scale;
+};
 struct LoraArgs {
     const uint8_t *a, *b;
     const int32_t *rank, *tok, *id;
@@ -66,12 +71,14 @@ struct LoraArgs {
     float *y, *part;
     int64_t ldx, ldyi, ldy;
     int type, n_adapter, max_rank, cols, rows, n_seq, n_tok;
-    // set by lora_plan: tiles of `tile` rows, `slots` workgroups for the runs of one adapter in a tile, A x over ks workgroups of kper
-    // columns, ranks in blocks of 16 nr
-    int tile, slots, ks, kper, nr;
+    LoraRun *runs;  // [tiles][most]: the second launch takes them from the first
+    // set by lora_plan: tiles of `tile` rows, with up to `most` runs each over `slots` workgroups, A x over ks workgroups of kper
+    // columns, ranks in blocks of 16 nr; ucols outputs to a workgroup of the second launch
+    int tile, most, slots, ks, kper, nr, ucols;
 };
 size_t lora_plan(LoraArgs &a, int num_cu);  // the scratch it takes
-int64_t lora_grid(const LoraArgs &a);       // workgroups of the larger launch
+void lora_scratch(LoraArgs &a, void *p);
+int64_t lora_grid(const LoraArgs &a);  // workgroups of the larger launch, of 256 threads
 hipError_t launch_lora(const LoraArgs &a, hipStream_t s);
 
 }  // namespace fgh
