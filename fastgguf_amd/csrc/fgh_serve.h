@@ -59,9 +59,10 @@ size_t verify_plan(VerifyArgs &a, int num_cu);  // the scratch it takes
 void verify_scratch(VerifyArgs &a, void *p);
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s);
 
-// rows of one adapter that stand together in a tile of a batch. adapter -1: none, -2: what is no adapter; n = 0: no rows
+// rows of a tile of a batch that have one adapter, a bit each. adapter -1: none, -2: what is no adapter
 struct LoraRun {
-    int row, n, adapter, rank;
+    uint64_t rows;
+    int adapter, rank;
     float scale;
 };
 struct LoraArgs {
@@ -74,7 +75,9 @@ struct LoraArgs {
     LoraRun *runs;  // [tiles][most]: the second launch takes them from the first
     // set by lora_plan: tiles of `tile` rows, with up to `most` runs each over `slots` workgroups, A x over ks workgroups of kper
     // columns, ranks in blocks of 16 nr; ucols outputs to a workgroup of the second launch
+    // `whole`: tiles mostly of one sequence's rows
     int tile, most, slots, ks, kper, nr, ucols;
+    bool whole;
 };
 size_t lora_plan(LoraArgs &a, int num_cu);  // the scratch it takes
 void lora_scratch(LoraArgs &a, void *p);
