@@ -115,24 +115,24 @@ __device__ __forceinline__ void multiply(pf4 *d, const pu4 (&w)[J][Weights<TYPE>
                 for (int j = 0; j < J; ++j) mma16<T_BF16>(d[j], w[j][i], x[sum - i]);
 }
 
-// Adapter values of 64 rows (of A: ranks, of B: outputs) and 64 values along them, shared by a workgroup: a thread takes 8 values of a row,
-// 8 threads a row's 64, so that an access finds whole lines, and leaves their parts in LDS as the products take them: [4 tiles][2 steps]
-// [parts][64 lanes]. (Loaded as the products take them, neighbouring lanes in 16 different rows, every lane was an access of its own to
-// the first cache: 1.0 a cycle, the bound of such a kernel.) Lanes are exchanged so that 8 threads write to different banks.
-template <int TYPE>
+// Adapter values of 64 rows (of A: ranks, of B: outputs) and 32 or 64 (SB 1, 2) values along them, shared by a workgroup: a thread takes 8 values of a
+// row, its neighbours the row's next ones, so that an access finds whole lines, and leaves their parts in LDS as the products take them:
+// [4 tiles][SB steps][parts][64 lanes]. (Loaded as the products take them, neighbouring lanes in 16 different rows, every lane was an access of its own to
+// the first cache: 1.0 a cycle, the bound of such a kernel.) Lanes are exchanged so that neighbours write to different banks.
+template <int TYPE, int SB>
 struct Stage {
-    static constexpr int NW = Weights<TYPE>::NW, ES = Weights<TYPE>::ES, VALUES = 8 * NW * 64;  // 16-byte values in LDS
+    static constexpr int NW = Weights<TYPE>::NW, ES = Weights<TYPE>::ES, VALUES = 4 * SB * NW * 64;  // 16-byte values in LDS
     static __device__ __forceinline__ int slot(int c, int g, int k) { return 16 * g + (c ^ (4 * g + k)); }
     static __device__ __forceinline__ void put(pu4 *lds, int row, int chunk, const Raw<TYPE> &raw) {
         const int j = row >> 4, k = chunk >> 2;
         pu4 w[NW];
         weights8<TYPE>(raw, w);
 #pragma unroll
-        for (int e = 0; e < NW; ++e) lds[((2 * j + k) * NW + e) * 64 + slot(row & 15, chunk & 3, k)] = w[e];
+        for (int e = 0; e < NW; ++e) lds[((SB * j + k) * NW + e) * 64 + slot(row & 15, chunk & 3, k)] = w[e];
     }
     static __device__ __forceinline__ void get(const pu4 *lds, int j, int k, int lane, pu4 (&w)[NW]) {
 #pragma unroll
-        for (int e = 0; e < NW; ++e) w[e] = lds[((2 * j + k) * NW + e) * 64 + slot(lane & 15, lane >> 4, k)];
+        for (int e = 0; e < NW; ++e) w[e] = lds[((SB * j + k) * NW + e) * 64 + slot(lane & 15, lane >> 4, k)];
     }
 };
 constexpr int LD = 68;  // floats between rows of 64 in LDS: 16 rows start in 16 different groups of banks
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 4) void lora_down_split_kernel(Lor
 // values on their way during the products of some. x too goes through LDS, each wavefront's by itself: 16 lanes read 256 bytes of a row.
 template <int TYPE, int NR>
 __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
-    using S = Stage<TYPE>;
+    using S = Stage<TYPE, 2>;
     constexpr int ES = S::ES, UNITS = (128 * NR + 255) / 256;
     __shared__ __attribute__((aligned(16))) pu4 wl[2][S::VALUES * NR / 4];
     __shared__ __attribute__((aligned(16))) float xl[4][16 * LD];
@@ -254,19 +254,23 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     int b = blockIdx.x;
     const int part = b % a.ks;
     b /= a.ks;
-    const int block = b % blocks, tile = b / blocks, base = tile * a.tile;
+    const int block = b % blocks;
+    b /= blocks;
+    const int slot = b % a.slots, tile = b / a.slots, base = tile * a.tile;
     const int from = part * a.kper, to = min(a.cols, from + a.kper), r0 = block * 16 * NR;
     const int padded = (a.max_rank + 15) & ~15;
     int *list = lists + 64 * wave;
     const int mark = adapters_of(a, base, list);
     uint64_t left = __builtin_amdgcn_ballot_w64(mark != 0);
-    for (int which = 0;; ++which) {
+    for (int which = 0, mine = slot;; ++which) {  // the tile's runs; every `slots`-th one is this workgroup's
         const int m = left ? __builtin_amdgcn_readlane(mark, __builtin_ctzll(left)) : 0;
         const uint64_t rows_of = __builtin_amdgcn_ballot_w64(mark == m) & left;
         left &= ~rows_of;
+        if (m && which != mine) continue;
         const LoraRun run = m ? run_of(a, rows_of, m) : LoraRun{};
-        if (part == 0 && block == 0 && tid == 0 && which < a.most) a.runs[(int64_t)tile * a.most + which] = run;  // behind the last: no rows
+        if (part == 0 && block == 0 && tid == 0 && mine < a.most) a.runs[(int64_t)tile * a.most + mine] = run;  // behind the last: no rows
         if (!m) break;
+        mine += a.slots;
         if (run.adapter < 0 || r0 >= run.rank) continue;
         const int n = list_rows(rows_of, list);
         const uint8_t *A = a.a + (int64_t)run.adapter * a.max_rank * a.cols * ES;
@@ -277,37 +281,51 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
         for (int i = 0; i < 4; ++i) xo[i] = 4 * ((uint32_t)list[min(16 * wave + 4 * i + g, n - 1)] * (uint32_t)a.ldx);
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) wo[u] = ES * ((uint32_t)min(r0 + (tid >> 3) + 32 * u, run.rank - 1) * (uint32_t)a.cols);
-        lf4 xn[4];
-        Raw<TYPE> wn[UNITS];
-        auto load = [&](int k0) {  // behind the last column the last ones again
-            const uint32_t kx = min(k0 + 4 * c, a.cols - 4), kw = min(k0 + 8 * (tid & 7), a.cols - 8);
+        lf4 xn[2][4];  // of the next two steps
+        Raw<TYPE> wn[2][UNITS];
+        // behind the last column the last ones again
+        auto load_w = [&](Raw<TYPE> (&v)[UNITS], int k0) {
+            const uint32_t k = min(k0 + 8 * (tid & 7), a.cols - 8);
 #pragma unroll
-            for (int u = 0; u < UNITS; ++u) wn[u] = raw8<TYPE>(A + wo[u] + ES * kw);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) xn[i] = *(const lf4 *)(X + xo[i] + 4 * kx);
+            for (int u = 0; u < UNITS; ++u) v[u] = raw8<TYPE>(A + (uint32_t)(wo[u] + ES * k));
         };
-        auto put_w = [&](pu4 *lds, int k0) {  // times 0 behind the last column
+        auto load_x = [&](lf4 (&v)[4], int k0) {
+            const uint32_t k = min(k0 + 4 * c, a.cols - 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *(const lf4 *)(X + (uint32_t)(xo[i] + 4 * k));
+        };
+        auto put_w = [&](pu4 *lds, Raw<TYPE> (&v)[UNITS], int k0) {  // times 0 behind the last column
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
-                if (k0 + 8 * (tid & 7) >= to) wn[u] = Raw<TYPE>{};
-                if (NR > 1 || tid < 128) S::put(lds, (tid >> 3) + 32 * u, tid & 7, wn[u]);
+                if (k0 + 8 * (tid & 7) >= to) v[u] = Raw<TYPE>{};
+                if (NR > 1 || tid < 128) S::put(lds, (tid >> 3) + 32 * u, tid & 7, v[u]);
             }
         };
         pf4 acc[NR];
 #pragma unroll
         for (int j = 0; j < NR; ++j) acc[j] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
         float *own = xl[wave];
-        load(from);
-        put_w(wl[0], from);
-        int at = 0;
-#pragma clang loop unroll(disable)
-        for (int k0 = from; k0 < to; k0 += 64, at ^= 1) {
+        // The steps start at another column in each tile and go round: rows lie a power of two apart, and workgroups that read the same columns
+        // of their rows at a time would ask few of the memory's channels.
+        const int steps = (to - from + 63) / 64, turn = (int)((unsigned)(tile * 5) % (unsigned)steps);
+        // Every step asks for the next ones' values, the last two for the last ones' again: loads in branches would be waited for at once.
+        auto column = [&](int i) {
+            const int j = min(i, steps - 1) + turn;
+            return from + 64 * (j < steps ? j : j - steps);
+        };
+        load_w(wn[0], column(0));
+        load_x(xn[0], column(0));
+        load_w(wn[1], column(1));
+        load_x(xn[1], column(1));
+        put_w(wl[0], wn[0], column(0));
+        auto step = [&](int i, int at) {
             // LDS serves a wavefront in order: only the compiler must keep it
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(pf4 *)(own + (4 * i + g) * LD + 4 * c) = xn[i];
+            for (int j = 0; j < 4; ++j) *(pf4 *)(own + (4 * j + g) * LD + 4 * c) = xn[at][j];
             __builtin_amdgcn_wave_barrier();
-            if (k0 + 64 < to) load(k0 + 64);
+            load_w(wn[at], column(i + 2));
+            load_x(xn[at], column(i + 2));
             lds_barrier();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -315,15 +333,23 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
                 float v[8];
                 *(pf4 *)v = *(const pf4 *)(own + c * LD + 32 * k + 8 * g), *(pf4 *)(v + 4) = *(const pf4 *)(own + c * LD + 32 * k + 8 * g + 4);
                 parts8<T_BF16, 3>(v, p);
+                constexpr int J = NR > 1 ? 2 : 1;
 #pragma unroll
-                for (int j = 0; j < NR; ++j) {
-                    pu4 w[1][S::NW];
-                    S::get(wl[at], j, k, lane, w[0]);
-                    multiply<TYPE, 1>(acc + j, w, p);
+                for (int j0 = 0; j0 < NR; j0 += J) {
+                    pu4 w[J][S::NW];
+#pragma unroll
+                    for (int j = 0; j < J; ++j) S::get(wl[at], j0 + j, k, lane, w[j]);
+                    multiply<TYPE, J>(acc + j0, w, p);
                 }
             }
-            if (k0 + 64 < to) put_w(wl[at ^ 1], k0 + 64);
+            put_w(wl[at ^ 1], wn[at ^ 1], column(i + 1));
+        };
+#pragma clang loop unroll(disable)
+        for (int i = 0; i + 1 < steps; i += 2) {
+            step(i, 0);
+            step(i + 1, 1);
         }
+        if (steps & 1) step(steps - 1, 0);
         lds_barrier();
         const int row = 16 * wave + c;
 #pragma unroll
@@ -334,16 +360,16 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     }
 }
 
-// y of rows that have an adapter in common, ucols of the outputs, 64 at a time and 64 ranks of them, the next ones' values on their way
+// y of rows that have an adapter in common, ucols of the outputs, 64 at a time and 32 SB ranks of them, the next ones' values on their way
 // during the products of some. ROWS (prompts): each wavefront has 16 rows and all 64 outputs; else (few rows) 16 of the outputs and the
 // same rows. Products: lane l has output l % 16 of a tile and row l % 16, ranks 8 (l / 16) .. + 7, and gets outputs 4 (l / 16) .. + 3 of its row;
-// through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: blocks of 64 ranks, whose h stays in registers; 0: any number,
+// through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: such blocks of ranks, whose h stays in registers; 0: any number,
 // which does not.
-template <int TYPE, int KB, bool ROWS>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
-    using S = Stage<TYPE>;
-    constexpr int ES = S::ES, NW = S::NW, J = ROWS ? 4 : 1, KH = KB ? 2 * KB : 1;
-    __shared__ __attribute__((aligned(16))) pu4 wl[2][S::VALUES];
+template <int TYPE, int SB, int KB, bool ROWS>
+__global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lora_up_kernel(LoraArgs a) {
+    using S = Stage<TYPE, SB>;
+    constexpr int ES = S::ES, NW = S::NW, J = ROWS ? 4 : 1, P = ROWS ? 2 : 1, KH = KB ? SB * KB : 1, CH = 4 * SB;  // CH: threads to a row's values
+    __shared__ __attribute__((aligned(16))) pu4 wl[S::VALUES];
     __shared__ __attribute__((aligned(16))) float tiles[ROWS ? 4 : 1][16 * LD];
     __shared__ int lists[4 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
@@ -353,13 +379,14 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
     b /= blocks;
     const int slot = b % a.slots, tile = b / a.slots, base = tile * a.tile;
     const int padded = (a.max_rank + 15) & ~15;
-    float *out = tiles[ROWS ? wave : 0];
+    float *out = tiles[ROWS ? wave : 0], *y = a.y + base * a.ldy;
+    const float *yin = a.yin + base * a.ldyi;
     int *list = lists + 64 * wave;
     for (int which = slot; which < a.most; which += a.slots) {
         const LoraRun run = a.runs[(int64_t)tile * a.most + which];
         if (run.rows == 0) break;
         if (run.adapter == -1 && a.y == a.yin) continue;
-        const int n = list_rows(run.rows, list), steps = (run.rank + 31) / 32, kbs = max(1, (run.rank + 63) / 64);
+        const int n = list_rows(run.rows, list), steps = (run.rank + 31) / 32, kbs = max(1, (run.rank + 32 * SB - 1) / (32 * SB));
         const uint8_t *B = a.b + (int64_t)max(run.adapter, 0) * a.rows * a.max_rank * ES;
         for (int t0 = 0; t0 < n; t0 += ROWS ? 64 : 16) {
             const int mine = t0 + (ROWS ? 16 * wave : 0);  // the wavefront's first row
@@ -371,32 +398,27 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
                 const uint32_t row = list[min(ROWS ? mine + 4 * i + g : t0 + (tid >> 4), n - 1)];
                 yo[i] = 4 * (row * (uint32_t)a.ldy), yio[i] = 4 * (row * (uint32_t)a.ldyi);
             }
-            lf4 yn[I] = {};
-            Raw<TYPE> wn[2];
+            lf4 yn[2][I] = {};  // of the next two turns
+            Raw<TYPE> wn[SB];
             auto load_w = [&](int n0, int kb) {  // outputs and ranks behind the last: others, which are not used, or cut
-                const int r = min(64 * kb + 8 * (tid & 7), a.max_rank - 8);
+                const int r = min(32 * SB * kb + 8 * (tid % CH), a.max_rank - 8);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) wn[u] = raw8<TYPE>(B + ES * ((int64_t)min(n0 + (tid >> 3) + 32 * u, a.rows - 1) * a.max_rank + r));
+                for (int u = 0; u < SB; ++u) wn[u] = raw8<TYPE>(B + ES * ((int64_t)min(n0 + tid / CH + 256 / CH * u, a.rows - 1) * a.max_rank + r));
             };
-            auto put_w = [&](pu4 *lds, int kb) {
-                const int have = run.rank - 64 * kb - 8 * (tid & 7);
+            auto put_w = [&](int kb) {
+                const int have = run.rank - 32 * SB * kb - 8 * (tid % CH);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < SB; ++u) {
                     if (have < 8) mask8<TYPE>(wn[u], first8<TYPE>(have));
-                    S::put(lds, (tid >> 3) + 32 * u, tid & 7, wn[u]);
+                    S::put(wl, tid / CH + 256 / CH * u, tid % CH, wn[u]);
                 }
             };
-            auto load_y = [&](int n0) {  // a row's last values one by one
-                const uint8_t *p = (const uint8_t *)(a.yin + base * a.ldyi + n0 + 4 * c);
-                if (n0 + 64 <= a.rows)
+            // a row's last 4 values for lanes behind them: what is not four whole values is read again where it is written
+            const bool ahead = a.yin && a.rows >= 4;
+            auto load_y = [&](lf4 (&v)[I], int n0) {
+                const uint32_t o = 4 * (uint32_t)min(n0 + 4 * c, a.rows - 4);
 #pragma unroll
-                    for (int i = 0; i < I; ++i) yn[i] = *(const lf4 *)(p + yio[i]);
-                else
-#pragma unroll
-                    for (int i = 0; i < I; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (n0 + 4 * c + e < a.rows) yn[i][e] = *(const float *)(p + yio[i] + 4 * e);
+                for (int i = 0; i < I; ++i) v[i] = *(const lf4 *)((const uint8_t *)yin + (uint32_t)(yio[i] + o));
             };
             const float *part = a.part + (int64_t)(base + list[min(mine + c, n - 1)]) * padded + 8 * g;
             auto sums = [&](int k, pu4 (&x)[3]) {  // h of a row, 8 ranks, as parts
@@ -412,45 +434,46 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
                 parts8<T_BF16, 3>(h, x);
             };
             load_w(first, 0);
-            if (a.yin) load_y(first);
+            if (ahead) {
+                load_y(yn[0], first);
+                load_y(yn[1], first + 64);
+            }
             pu4 x[KH][3];
             if (KB)
 #pragma unroll
                 for (int k = 0; k < KH; ++k)
                     if (k < steps) sums(k, x[k]);
-            put_w(wl[0], 0);
-            int at = 0;
-#pragma clang loop unroll(disable)
-            for (int n0 = first; n0 < end; n0 += 64) {
+            auto turn = [&](lf4 (&v)[I], int n0) {
                 pf4 acc[J];
 #pragma unroll
                 for (int j = 0; j < J; ++j) acc[j] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-                auto block = [&](int kb, const pu4 (&h0)[3], const pu4 (&h1)[3]) {
-                    const bool last = kb + 1 == kbs, more = !last || n0 + 64 < end;
-                    if (more) load_w(last ? n0 + 64 : n0, last ? 0 : kb + 1);
+                auto block = [&](int kb, const pu4 (*h)[3]) {
+                    const bool last = kb + 1 == kbs;
+                    lds_barrier();  // the products before are done
+                    put_w(kb);
+                    load_w(last ? n0 + 64 : n0, last ? 0 : kb + 1);  // behind the last the last again: in a branch it would be waited for at once
                     lds_barrier();
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (2 * kb + k < steps)
+                    for (int k = 0; k < SB; ++k)
+                        if (SB * kb + k < steps)
 #pragma unroll
-                            for (int j = 0; j < J; ++j) {
-                                pu4 w[1][NW];
-                                S::get(wl[at], ROWS ? j : wave, k, lane, w[0]);
-                                multiply<TYPE, 1>(acc + j, w, k ? h1 : h0);
+                            for (int j0 = 0; j0 < J; j0 += P) {
+                                pu4 w[P][NW];
+#pragma unroll
+                                for (int j = 0; j < P; ++j) S::get(wl, ROWS ? j0 + j : wave, k, lane, w[j]);
+                                multiply<TYPE, P>(acc + j0, w, h[k]);
                             }
-                    at ^= 1;
-                    if (more) put_w(wl[at], last ? 0 : kb + 1);
                 };
                 if constexpr (KB > 0) {
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb)
-                        if (kb < kbs) block(kb, x[2 * kb], x[2 * kb + 1]);
+                        if (kb < kbs) block(kb, x + SB * kb);
                 } else
                     for (int kb = 0; kb < kbs; ++kb) {
-                        pu4 h[2][3];
-                        sums(2 * kb, h[0]);
-                        sums(2 * kb + 1, h[1]);
-                        block(kb, h[0], h[1]);
+                        pu4 h[SB][3];
+#pragma unroll
+                        for (int k = 0; k < SB; ++k) sums(SB * kb + k, h[k]);
+                        block(kb, h);
                     }
                 // LDS serves a wavefront in order: only the compiler must keep it, and the workgroup where the rows are shared
                 if (ROWS) __builtin_amdgcn_wave_barrier();
@@ -458,22 +481,39 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraArgs a) {
                 for (int j = 0; j < J; ++j) *(pf4 *)(out + c * LD + 16 * (ROWS ? j : wave) + 4 * g) = acc[j];
                 if (ROWS) __builtin_amdgcn_wave_barrier();
                 else lds_barrier();
-                uint8_t *y = (uint8_t *)(a.y + base * a.ldy + n0 + 4 * c);
+                const uint32_t o = 4 * (n0 + 4 * c);
+                if (n0 + 64 <= a.rows) {
+                    pf4 d[I];
 #pragma unroll
-                for (int i = 0; i < I; ++i) {
-                    const pf4 d = *(const pf4 *)(out + (ROWS ? 4 * i + g : tid >> 4) * LD + 4 * c);
-                    lf4 v = yn[i];
+                    for (int i = 0; i < I; ++i) d[i] = *(const pf4 *)(out + (ROWS ? 4 * i + g : tid >> 4) * LD + 4 * c);
                     if (run.adapter != -1)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] += run.scale * d[e];
-                    if ((ROWS ? mine + 4 * i + g : t0 + (tid >> 4)) >= n) continue;
-                    if (n0 + 64 <= a.rows) *(lf4 *)(y + yo[i]) = v;
-                    else
+                        for (int i = 0; i < I; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (n0 + 4 * c + e < a.rows) *(float *)(y + yo[i] + 4 * e) = v[e];
+                            for (int e = 0; e < 4; ++e) v[i][e] += run.scale * d[i][e];
+#pragma unroll
+                    for (int i = 0; i < I; ++i)
+                        if ((ROWS ? mine + 4 * i + g : t0 + (tid >> 4)) < n) *(lf4 *)((uint8_t *)y + (uint32_t)(yo[i] + o)) = v[i];
+                } else {  // a row's last outputs, fewer than 64: one by one
+#pragma clang loop unroll(disable)
+                    for (int i = ROWS ? lane : tid; i < 1024; i += ROWS ? 64 : 256) {
+                        const int row = i >> 6, col = i & 63;
+                        if (mine + row >= n || n0 + col >= a.rows) continue;
+                        const int64_t at = list[mine + row];
+                        const float u = a.yin ? yin[at * a.ldyi + n0 + col] : 0.0f;
+                        y[at * a.ldy + n0 + col] = run.adapter != -1 ? u + run.scale * out[row * LD + col] : u;
+                    }
                 }
-                if (a.yin && n0 + 64 < end) load_y(n0 + 64);
+                if (ahead) load_y(v, n0 + 128);
+                else
+#pragma unroll
+                    for (int i = 0; i < I; ++i) v[i] = lf4{0.0f, 0.0f, 0.0f, 0.0f};
+            };
+#pragma clang loop unroll(disable)
+            for (int n0 = first; n0 < end; n0 += 128) {
+                turn(yn[0], n0);
+                if (n0 + 64 >= end) break;
+                turn(yn[1], n0 + 64);
             }
             lds_barrier();  // the next rows' values go where these were
         }
@@ -485,9 +525,10 @@ int64_t tiles_of(const LoraArgs &a) { return ((int64_t)a.n_tok + a.tile - 1) / a
 
 template <int TYPE, bool ROWS>
 void launch_up(const LoraArgs &a, unsigned grid, hipStream_t s) {
-    if (a.max_rank <= 64) lora_up_kernel<TYPE, 1, ROWS><<<grid, 256, 0, s>>>(a);
-    else if (a.max_rank <= 128) lora_up_kernel<TYPE, 2, ROWS><<<grid, 256, 0, s>>>(a);
-    else lora_up_kernel<TYPE, 0, ROWS><<<grid, 256, 0, s>>>(a);
+    if (a.max_rank <= 32) lora_up_kernel<TYPE, 1, 1, ROWS><<<grid, 256, 0, s>>>(a);
+    else if (a.max_rank <= 64) lora_up_kernel<TYPE, 2, 1, ROWS><<<grid, 256, 0, s>>>(a);
+    else if (a.max_rank <= 128) lora_up_kernel<TYPE, 2, 2, ROWS><<<grid, 256, 0, s>>>(a);
+    else lora_up_kernel<TYPE, 2, 0, ROWS><<<grid, 256, 0, s>>>(a);
 }
 template <int TYPE>
 hipError_t launch_type(const LoraArgs &a, hipStream_t s) {
@@ -517,15 +558,15 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     const int64_t tiles = tiles_of(a);
     a.most = (int)std::min<int64_t>(std::min(a.n_seq, a.tile), (int64_t)a.n_adapter + 2);
     a.nr = a.max_rank <= 16 ? 1 : a.max_rank <= 32 ? 2 : 4;
-    // a workgroup for every run that a tile of short sequences could have, while that fills the device twice at most
-    a.slots = prompts ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(a.most, 2 * num_cu / tiles));
+    // a workgroup for every run that a tile could have, while that fills the device twice at most; one run after the other is as long again
+    a.slots = (int)std::max<int64_t>(1, std::min<int64_t>(prompts ? std::min(a.most, 3) : a.most, 2 * num_cu / tiles));
     // columns over as many workgroups as that leaves room for, a step of each wavefront, or of the workgroup, at the least
     const int64_t unit = a.whole ? 64 : 32 * DOWN_WAVES, units = (a.cols + unit - 1) / unit;
-    const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * a.slots * rank_blocks(a))}));
+    const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
     // outputs over so many workgroups that the device is filled, 256 at the least
-    const int64_t steps = (a.rows + 255) / 256, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * num_cu / (tiles * a.slots)));
+    const int64_t steps = (a.rows + 255) / 256, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * num_cu / (tiles * (prompts ? 1 : a.slots))));
     a.ucols = (int)((steps + chunks - 1) / chunks * 256);
     return (size_t)tiles * a.most * sizeof(LoraRun) + (size_t)a.ks * a.n_tok * ((a.max_rank + 15) & ~15) * 4;
 }
