@@ -1193,9 +1193,10 @@ int fgh_paged_reserve_dev(fgh_ctx *c, const fgh_paged_cache *cache, const fgh_pa
     a.seq = pool->seq, a.pos = pool->pos, a.slot = pool->slot;
     const fgh::Paged p = paged_args(cache, batch);  // its bounds
     a.n_seq = p.n_seq, a.n_tok = p.n_tok, a.max_tok = p.max_tok, a.max_len = p.max_len, a.n_pages = p.n_pages, a.shift = p.shift, a.table_stride = p.table_stride;
-    if (int rc = grow(c, c->pr, fgh::reserve_scratch(a))) return rc;
+    if (const size_t bytes = fgh::reserve_scratch(a))
+        if (int rc = grow(c, c->pr, bytes)) return rc;
     a.pre = (int32_t *)c->pr.p;
-    HIP_TRY(c, fgh::launch_reserve(a, c->num_cu, c->stream));
+    HIP_TRY(c, fgh::launch_reserve(a, c->stream));
     return FGH_OK;
 }
 int fgh_draft_verify_dev(fgh_ctx *c, const fgh_drafts *d, int32_t *n_ok, int32_t *next, int32_t *keep, float *lse) {

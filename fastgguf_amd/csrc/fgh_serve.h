@@ -32,7 +32,7 @@ struct ReserveArgs {
     int32_t *pre;  // reserve_scratch bytes
 };
 size_t reserve_scratch(const ReserveArgs &a);
-hipError_t launch_reserve(const ReserveArgs &a, int num_cu, hipStream_t s);
+hipError_t launch_reserve(const ReserveArgs &a, hipStream_t s);
 
 // what a sequence's rows come to: the row t that the next token is drawn from, its sum, largest value and the place of that; the draft d that
 // it rejects, or -1; the rows n (0: no token) and the accepted drafts
