@@ -8,20 +8,23 @@
 namespace fgh {
 
 // The sequence of row t, or -1: the last s with tok[s] <= t, if t < tok[s + 1]; tok[0 .. n_seq] does not decrease. A wavefront's 64
-// lanes look at 64 starts at a time, evenly apart: 65535 sequences take three loads that wait for each other.
+// lanes look at 256 starts at a time, evenly apart: 65535 sequences take two loads that wait for each other.
 __device__ __forceinline__ int seq_of_row(const int32_t *tok, int n_seq, int t) {
     const int lane = threadIdx.x & 63;
     int base = 0, len = n_seq + 1;
-    while (len > 64) {
-        const int step = (len + 63) / 64, i = lane * step;
-        const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < len && tok[base + (i < len ? i : 0)] <= t));
-        if (c == 0) return -1;
+    while (true) {
+        const int step = (len + 255) / 256;
+        int c = 0;
+        int32_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = tok[base + min((lane + 64 * i) * step, len - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64((lane + 64 * i) * step < len && at[i] <= t));
+        if (c == 0) return base - 1;
         base += (c - 1) * step;
         len = min(step, len - (c - 1) * step);
+        if (len == 1) return base >= n_seq ? -1 : base;
     }
-    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < len && tok[base + (lane < len ? lane : 0)] <= t));
-    const int s = base + c - 1;
-    return s >= n_seq ? -1 : s;
 }
 
 struct ReserveArgs {
@@ -50,7 +53,7 @@ struct VerifyArgs {
     int n_seq, n_tok, max_tok, vocab;
     // set by verify_plan: a row's words over `splits` workgroups, `per` words each, in blocks of 1024 nv
     int splits, per, nv;
-    double *sum, *rest;  // [n_tok][splits], [n_seq][splits]
+    double *sum, *rest;  // [n_tok][splits], [n_seq][splits][per / 2048 + 1]
     float *top;          // [n_tok][splits]
     int32_t *at;         // [n_tok][splits]
     VerifyChoice *choice;  // [n_seq]

@@ -61,17 +61,55 @@ struct Part {
 // the largest value to take others relative to: 0 where there is none
 __device__ __forceinline__ double level(float top) { return fabsf(top) <= 3.4028235e38f ? (double)top : 0.0; }
 __device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }  // NaN if either is
-// over `lanes` lanes that have a part each (a power of two); every one gets the whole
-__device__ __forceinline__ Part join_lanes(Part p, double c, int lanes) {
-    const float own = p.top;
-    for (int o = 1; o < lanes; o <<= 1) {
-        const float y = __shfl_xor(p.top, o, 64);
-        const int at = __shfl_xor(p.at, o, 64);
-        p.at = y > p.top ? at : y == p.top ? min(p.at, at) : p.at;
-        p.top = larger(p.top, y);
+// over a wavefront, every lane gets it: 8 steps without LDS
+template <class F>
+__device__ __forceinline__ int over_lanes(int v, F &&f) {
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
+    return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+__device__ __forceinline__ float largest(float x) {
+    return __int_as_float(over_lanes(__float_as_int(x), [](int a, int b) { return __float_as_int(larger(__int_as_float(a), __int_as_float(b))); }));
+}
+__device__ __forceinline__ int least(int x) {
+    return over_lanes(x, [](int a, int b) { return min(a, b); });
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)u, (int)u, CTRL, 0xF, 0xF, false),
+                   hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(u >> 32), (int)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double total(double x) {
+    x += dpp<0xB1>(x);
+    x += dpp<0x4E>(x);
+    x += dpp<0x141>(x);
+    x += dpp<0x140>(x);
+    return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+// the sum with the lanes before
+__device__ __forceinline__ double upto_lane(double x) {
+    const int lane = threadIdx.x & 63;
+    for (int o = 1; o < 64; o <<= 1) {
+        const double z = __shfl_up(x, o, 64);
+        if (lane >= o) x += z;
     }
-    p.sum *= exp2_of(((double)own - level(p.top)) * c);  // 0 for a part without words
-    for (int o = 1; o < lanes; o <<= 1) p.sum += __shfl_xor(p.sum, o, 64);
+    return x;
+}
+// the parts of a wavefront's lanes, as one; places only where the largest is asked for
+__device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
+    const float own = p.top;
+    p.top = largest(own);
+    if (greedy) p.at = least(own == p.top ? p.at : INT_MAX);
+    p.sum = total(p.sum * exp2_of(((double)own - level(p.top)) * c));  // 0 for a part without words
     return p;
 }
 
@@ -83,14 +121,14 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     const float *x = a.logits + row * a.ld;
     vf4 v[NV];
     auto load = [&](int base) {
+        if (base + 1024 * NV <= to)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = base + i * 1024 + 4 * tid;
-            if (j + 4 <= to) v[i] = *(const vf4 *)(x + j);
-            else
+            for (int i = 0; i < NV; ++i) v[i] = *(const vf4 *)(x + base + i * 1024 + 4 * tid);
+        else  // behind the last word that one again, which becomes none
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] = j + e < to ? x[j + e] : -__builtin_inff();
-        }
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] = x[min(base + i * 1024 + 4 * tid + e, to - 1)];
     };
     load(from);  // on its way while the row's sequence is found
     const int s = seq_of_row(a.tok, a.n_seq, row);
@@ -100,6 +138,12 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     Part p{0.0, -__builtin_inff(), INT_MAX};
     for (int base = from; base < to; base += 1024 * NV) {
         if (base != from) load(base);
+        if (base + 1024 * NV > to)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (base + i * 1024 + 4 * tid + e >= to) v[i][e] = -__builtin_inff();
         const float was = p.top;
         float top = was;
 #pragma unroll
@@ -118,11 +162,11 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) p.sum += exp2_near(fmax(((double)v[i][e] - m) * c, -1000.0));
     }
-    p = join_lanes(p, c, 64);
+    p = join_lanes(p, c, greedy);
     if ((tid & 63) == 0) lds[tid >> 6] = p;
     __syncthreads();
-    if (tid < 4) {
-        p = join_lanes(lds[tid], c, 4);
+    if (tid < 64) {
+        p = join_lanes(tid < 4 ? lds[tid] : Part{0.0, -__builtin_inff(), INT_MAX}, c, greedy);
         if (tid == 0) {
             const int64_t i = (int64_t)row * a.splits + split;
             a.sum[i] = p.sum, a.top[i] = p.top, a.at[i] = p.at;
@@ -161,7 +205,7 @@ __device__ VerifyChoice decide(const VerifyArgs &a, int s, double c, bool greedy
                 x = a.logits[t * a.ld + d], u = a.u[t];
                 if (a.q) q = a.q[t * a.ldq + d], q_lse = a.q_lse[t];
             }
-            p = join_lanes(p, c, 64);
+            p = join_lanes(p, c, greedy);
             bool good = false;
             if (is_word && fabsf(p.top) <= 3.4028235e38f) {
                 if (greedy) good = d == p.at;
@@ -227,94 +271,105 @@ __device__ __forceinline__ void each4(const Weigh &w, int b, int e, F &&f) {
         f(j, x);
     }
 }
-// over the workgroup: the sum of the threads before, and the whole
-__device__ __forceinline__ double2 scan_block(double v) {
+// over the workgroup: the sum of the wavefronts before, and the whole (v: a wavefront's, the same in its lanes)
+__device__ __forceinline__ double2 scan_waves(double v) {
     __shared__ double lds[WG / 64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double upto = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double z = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += z;
-    }
+    const int wave = threadIdx.x >> 6;
     __syncthreads();
-    if (lane == 63) lds[wave] = upto;
+    if ((threadIdx.x & 63) == 0) lds[wave] = v;
     __syncthreads();
     double before = 0.0, all = 0.0;
     for (int i = 0; i < WG / 64; ++i) {
         if (i < wave) before += lds[i];
         all += lds[i];
     }
-    return double2{before + (upto - v), all};
+    return double2{before, all};
 }
+constexpr int SUB = 4 * WG;  // words that the workgroup takes at a time
 template <int MODE>
 __device__ __forceinline__ double sum_words(const Weigh &w, int from, int to) {
     double v = 0.0;
-    for (int b = from + 4 * (int)threadIdx.x; b < to; b += 4 * WG) each4<MODE>(w, b, min(to, b + 4), [&](int, const double (&x)[4]) { v += (x[0] + x[1]) + (x[2] + x[3]); });
-    return scan_block(v).y;
+    for (int b = from + 4 * (int)threadIdx.x; b < to; b += SUB) each4<MODE>(w, b, min(to, b + 4), [&](int, const double (&x)[4]) { v += (x[0] + x[1]) + (x[2] + x[3]); });
+    return scan_waves(total(v)).y;
 }
 
-// the decision where the drafts have probabilities, and the sums of max(p - q, 0) of a rejected row, by parts
+// the decision where the drafts have probabilities, and the sums of max(p - q, 0) of a rejected row, by parts of SUB words
 __global__ __launch_bounds__(WG) void verify_rest_kernel(VerifyArgs a) {
-    const int s = blockIdx.x / a.splits, split = blockIdx.x - s * a.splits;
+    const int s = blockIdx.x / a.splits, split = blockIdx.x - s * a.splits, subs = (a.per + SUB - 1) / SUB;
     bool greedy;
     const double c = heat_of(a, s, greedy);
     if (split > 0 && (greedy || !(c == c))) return;
     const VerifyChoice ch = decide(a, s, c, greedy, a.lse && split == 0);
     if (split == 0 && threadIdx.x == 0) a.choice[s] = ch;
     if (greedy || !(c == c) || ch.d < 0) return;
-    const double v = sum_words<FROM_REST>(weigh_of(a, ch, c), split * a.per, min(a.vocab, (split + 1) * a.per));
-    if (threadIdx.x == 0) a.rest[(int64_t)s * a.splits + split] = v;
+    const Weigh w = weigh_of(a, ch, c);
+    const int to = min(a.vocab, (split + 1) * a.per);
+    for (int i = 0; i < subs; ++i) {
+        const int from = split * a.per + i * SUB;
+        const double v = sum_words<FROM_REST>(w, from, min(from + SUB, to));
+        if (threadIdx.x == 0) a.rest[((int64_t)s * a.splits + split) * subs + i] = v;
+    }
 }
 
 // the first of words from .. to - 1 whose running sum passes `aim`, or the last of any weight (-1: none has)
 template <int MODE>
 __device__ int pick(const Weigh &w, int from, int to, double aim) {
     __shared__ int first, last;
-    const int per = ((to - from + WG - 1) / WG + 3) & ~3, b = min(to, from + (int)threadIdx.x * per), e = min(to, b + per);
+    __shared__ double sum;
+    const int per = ((to - from + WG - 1) / WG + 3) & ~3, b = min(to, from + (int)threadIdx.x * per), e = min(to, b + per), lane = threadIdx.x & 63;
     double own = 0.0;
     each4<MODE>(w, b, e, [&](int, const double (&x)[4]) { own += (x[0] + x[1]) + (x[2] + x[3]); });
     if (threadIdx.x == 0) first = WG, last = -1;
-    double run = scan_block(own).x;  // its barriers stand before what follows
+    double run = upto_lane(own);
+    run += scan_waves(lane_of(run, 63)).x;  // its barriers stand before what follows
     if (own > 0.0) {
         atomicMax(&last, (int)threadIdx.x);
-        if (run + own > aim) atomicMin(&first, (int)threadIdx.x);
+        if (run > aim) atomicMin(&first, (int)threadIdx.x);
     }
     __syncthreads();
     const int mine = first < WG ? first : last;
-    __syncthreads();
     if (mine < 0) return -1;
-    if (threadIdx.x == mine) {
-        int at = -1;
-        bool found = false;
-        each4<MODE>(w, b, e, [&](int j, const double (&x)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (x[i] > 0.0 && !found) {
-                    at = j + i;
-                    run += x[i];
-                    found = run > aim;
-                }
-        });
-        first = at;
-    }
+    if ((int)threadIdx.x == mine) sum = run - own;
     __syncthreads();
-    return first;
+    // that thread's words, one to a lane
+    const int b1 = min(to, from + mine * per), e1 = min(to, b1 + per);
+    run = sum;
+    int at = -1;
+    for (int j0 = b1; j0 < e1; j0 += 64) {
+        const int j = j0 + lane;
+        const double x = j < e1 ? weight<MODE>(w, j, w.x[j], MODE == FROM_REST ? w.q[j] : 0.0f) : 0.0, upto = run + upto_lane(x);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0), past = __builtin_amdgcn_ballot_w64(x > 0.0 && upto > aim);
+        if (past) return j0 + __builtin_ctzll(past);
+        if (some) at = j0 + 63 - __builtin_clzll(some);
+        run = lane_of(upto, 63);
+    }
+    return at;
 }
 
-// the part, then the word; a lane has a part's sum, the same in every wavefront
-template <int MODE>
-__device__ int draw(const VerifyArgs &a, const Weigh &w, double sum, double v) {
+// The part, then the word. part(i): the sum of part i; there are `subs` of up to `words` words to each split. Each wavefront goes through them for
+// itself.
+template <int MODE, class F>
+__device__ int draw(const VerifyArgs &a, const Weigh &w, int subs, int words, double v, F &&part) {
+    const int n = a.splits * subs;
     const int lane = threadIdx.x & 63;
-    double upto = sum;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double z = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += z;
+    double whole = 0.0;
+    for (int i = 0; i < n; i += 64) whole += total(i + lane < n ? part(i + lane) : 0.0);
+    const double aim = v * whole;
+    int at = -1;
+    double run = 0.0, before = 0.0;
+    for (int i = 0; i < n; i += 64) {
+        const double x = i + lane < n ? part(i + lane) : 0.0, upto = run + upto_lane(x);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0), past = __builtin_amdgcn_ballot_w64(x > 0.0 && upto > aim);
+        if (some) {  // none passes by a rounding, or v is 1 or more: the last
+            const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+            at = i + l, before = l ? lane_of(upto, l - 1) : run;
+        }
+        if (past) break;
+        run = lane_of(upto, 63);
     }
-    const double aim = v * __shfl(upto, 63, 64);
-    const uint64_t some = __builtin_amdgcn_ballot_w64(sum > 0.0), past = __builtin_amdgcn_ballot_w64(sum > 0.0 && upto > aim);
-    if (!some) return -1;
-    const int part = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);  // none passes by a rounding, or v is 1 or more: the last
-    return pick<MODE>(w, part * a.per, min(a.vocab, (part + 1) * a.per), aim - __shfl(upto - sum, part, 64));
+    if (at < 0) return -1;
+    const int split = at / subs, from = split * a.per + (at - split * subs) * words;
+    return pick<MODE>(w, from, min(from + words, min((split + 1) * a.per, a.vocab)), aim - before);
 }
 
 __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
@@ -333,15 +388,18 @@ __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
                 const int64_t i = (int64_t)ch.t * a.splits + lane;
                 part = a.sum[i] * exp2_of(((double)a.top[i] - w.m) * c);
             }
-            if (ch.d >= 0 && a.q) word = draw<FROM_REST>(a, w, lane < a.splits ? a.rest[(int64_t)s * a.splits + lane] : 0.0, v);
-            else if (ch.d >= 0) {
+            if (ch.d >= 0 && a.q) {
+                const int subs = (a.per + SUB - 1) / SUB;
+                const double *rest = a.rest + (int64_t)s * a.splits * subs;
+                word = draw<FROM_REST>(a, w, subs, SUB, v, [&](int i) { return rest[i]; });
+            } else if (ch.d >= 0) {
                 // the draft's part without it: by a difference where that loses a bit at most, else anew
                 const int mine = ch.d / a.per;
-                const double with = __shfl(part, mine, 64), x = weight<FROM_P>(w, ch.d, w.x[ch.d], 0.0f);
+                const double with = lane_of(part, mine), x = weight<FROM_P>(w, ch.d, w.x[ch.d], 0.0f);
                 const double left = x <= 0.5 * with ? with - x : sum_words<WITHOUT_DRAFT>(w, mine * a.per, min(a.vocab, (mine + 1) * a.per));
-                word = draw<WITHOUT_DRAFT>(a, w, lane == mine ? left : part, v);
+                word = draw<WITHOUT_DRAFT>(a, w, 1, a.per, v, [&](int) { return lane == mine ? left : part; });
             }
-            if (word < 0) word = draw<FROM_P>(a, w, part, v);  // behind the last row, or nothing is left of p
+            if (word < 0) word = draw<FROM_P>(a, w, 1, a.per, v, [&](int) { return part; });  // behind the last row, or nothing is left of p
         }
     }
     if (tid == 0) {
@@ -351,6 +409,7 @@ __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     }
 }
 
+size_t subs_of(const VerifyArgs &a) { return (a.per + SUB - 1) / SUB; }
 }  // namespace
 
 size_t verify_plan(VerifyArgs &a, int num_cu) {
@@ -362,13 +421,13 @@ size_t verify_plan(VerifyArgs &a, int num_cu) {
     a.per = (blocks + a.splits - 1) / a.splits * 1024 * a.nv;
     a.splits = (a.vocab + a.per - 1) / a.per;
     const size_t n = (size_t)a.n_tok * a.splits;
-    return n * 16 + (a.q ? (size_t)a.n_seq * (a.splits * 8 + sizeof(VerifyChoice)) : 0);
+    return n * 16 + (a.q ? (size_t)a.n_seq * ((size_t)a.splits * subs_of(a) * 8 + sizeof(VerifyChoice)) : 0);
 }
 void verify_scratch(VerifyArgs &a, void *p) {
     const size_t n = (size_t)a.n_tok * a.splits, m = a.q ? a.n_seq : 0;
     a.sum = (double *)p;
     a.rest = a.sum + n;
-    a.choice = (VerifyChoice *)(a.rest + m * a.splits);
+    a.choice = (VerifyChoice *)(a.rest + m * a.splits * subs_of(a));
     a.top = (float *)(a.choice + m);
     a.at = (int32_t *)(a.top + n);
 }
