@@ -565,9 +565,9 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
-    // outputs over so many workgroups that the device is filled, 256 at the least
-    const int64_t steps = (a.rows + 255) / 256, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * num_cu / (tiles * (prompts ? 1 : a.slots))));
-    a.ucols = (int)((steps + chunks - 1) / chunks * 256);
+    // outputs over so many workgroups that the device is filled, a turn of 64 at the least
+    const int64_t steps = (a.rows + 63) / 64, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * num_cu / (tiles * (prompts ? 1 : a.slots))));
+    a.ucols = (int)((steps + chunks - 1) / chunks * 64);
     return (size_t)tiles * a.most * sizeof(LoraRun) + (size_t)a.ks * a.n_tok * ((a.max_rank + 15) & ~15) * 4;
 }
 void lora_scratch(LoraArgs &a, void *p) {

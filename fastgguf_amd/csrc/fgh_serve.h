@@ -51,8 +51,8 @@ struct VerifyArgs {
     float *lse;
     int64_t ld, ldq;
     int n_seq, n_tok, max_tok, vocab;
-    // set by verify_plan: a row's words over `splits` workgroups, `per` words each, in blocks of 1024 nv
-    int splits, per, nv;
+    // set by verify_plan: a row's words over `splits` workgroups, `per` words each, in blocks of 1024 nv; `group` such parts to a workgroup
+    int splits, per, nv, group;
     double *sum, *rest;  // [n_tok][splits], [n_seq][splits][per / 2048 + 1]
     float *top;          // [n_tok][splits]
     int32_t *at;         // [n_tok][splits]

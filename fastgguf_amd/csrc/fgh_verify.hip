@@ -21,11 +21,11 @@ typedef float vf4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.69314718055994530942;
 
-// 2^t for -1000 <= t <= 1000, off by 9e-13 of it: t's nearest whole number by an addition that leaves it in the low bits, which go into the
-// exponent, and a polynomial of what is left, at most 1/2 (its coefficients: the least largest error, 1 exact at 0).
-// 16 instructions of 64 bits a value with the sum; rint, a conversion and an exponent function instead cost twice the time.
-__device__ __forceinline__ double exp2_near(double t) {
-    const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);
+// 2^(d c) for -1000 <= d c <= 1000, off by 9e-13 of it: the product's nearest whole number by a sum that leaves it in the low bits, which go
+// into the exponent, and a polynomial of what is left, at most 1/2 (its coefficients: the least largest error, 1 exactly at 0).
+// 12 instructions of 64 bits; with rint, a conversion and an exponent function instead it took twice the time.
+__device__ __forceinline__ double exp2_near(double d, double c) {
+    const double whole = __builtin_fma(d, c, 0x1.8p52), f = __builtin_fma(d, c, 0x1.8p52 - whole);
     double r = 1.3178933573679677e-06;
     r = __builtin_fma(r, f, 1.5309156297959352e-05);
     r = __builtin_fma(r, f, 1.5403825462941963e-04);
@@ -40,15 +40,16 @@ __device__ __forceinline__ double exp2_near(double t) {
 }
 // 2^t: 0 below 2^-1000 and where t is NaN, 2^1000 at most
 __device__ __forceinline__ double exp2_of(double t) {
-    const double r = exp2_near(fmin(fmax(t, -1000.0), 1000.0));
+    const double r = exp2_near(fmin(fmax(t, -1000.0), 1000.0), 1.0);
     return t >= -1000.0 ? r : 0.0;
 }
 
-// log2(e) / T of a sequence; T = 0, the largest value, has 1's. A T below 0 or NaN makes NaN.
+// log2(e) / T of a sequence; T = 0, the largest value, has 1's; an infinite one a number that makes every word as likely. A T below 0 or NaN
+// makes NaN.
 __device__ __forceinline__ double heat_of(const VerifyArgs &a, int s, bool &greedy) {
     const float t = a.temp ? a.temp[s] : 1.0f;
     greedy = t == 0.0f;
-    return greedy ? LOG2E : t > 0.0f ? LOG2E / (double)t : (double)__builtin_nanf("");
+    return greedy ? LOG2E : t > 0.0f ? fmax(LOG2E / (double)t, 1e-290) : (double)__builtin_nanf("");
 }
 
 // a row, or a part of one: its largest value (NaN where it has a NaN), the first place of it where the largest is asked for, sum of
@@ -95,14 +96,21 @@ __device__ __forceinline__ double total(double x) {
     x += dpp<0x140>(x);
     return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
 }
-// the sum with the lanes before
+template <int CTRL>
+__device__ __forceinline__ double dpp0(double x) {  // 0 where no lane is
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, true), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// the sum with the lanes before: in rows of 16 lanes (row_shr 1, 2, 4, 8), then over the rows
 __device__ __forceinline__ double upto_lane(double x) {
     const int lane = threadIdx.x & 63;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double z = __shfl_up(x, o, 64);
-        if (lane >= o) x += z;
-    }
-    return x;
+    x += dpp0<0x111>(x);
+    x += dpp0<0x112>(x);
+    x += dpp0<0x114>(x);
+    x += dpp0<0x118>(x);
+    const double a = lane_of(x, 15), b = a + lane_of(x, 31), c = b + lane_of(x, 47);
+    return x + (lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 // the parts of a wavefront's lanes, as one; places only where the largest is asked for
 __device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
@@ -116,60 +124,70 @@ __device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
 template <int NV>
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ Part lds[4];
-    const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits, tid = threadIdx.x;
-    const int from = split * a.per, to = min(a.vocab, from + a.per);
+    const int groups = (a.splits + a.group - 1) / a.group, row = blockIdx.x / groups, split0 = (blockIdx.x - row * groups) * a.group, tid = threadIdx.x;
     const float *x = a.logits + row * a.ld;
-    vf4 v[NV];
-    auto load = [&](int base) {
-        if (base + 1024 * NV <= to)
+    vf4 v[NV] = {};
+    auto load = [&](int base) {  // behind the last four words those again
+        if (a.vocab >= 4)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = *(const vf4 *)(x + base + i * 1024 + 4 * tid);
-        else  // behind the last word that one again, which becomes none
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] = x[min(base + i * 1024 + 4 * tid + e, to - 1)];
+            for (int i = 0; i < NV; ++i) v[i] = *(const vf4 *)((const uint8_t *)x + 4 * (uint32_t)min(base + i * 1024 + 4 * tid, a.vocab - 4));
+        else
+            for (int e = 0; e < a.vocab; ++e) v[0][e] = x[e];
     };
-    load(from);  // on its way while the row's sequence is found
+    auto cut = [&](int base) {  // a row's last block: a lane's words from its first one on, then none
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = base + i * 1024 + 4 * tid, over = a.vocab >= 4 ? max(0, j - (a.vocab - 4)) : 0;
+            if (over & 1) v[i] = vf4{v[i].y, v[i].z, v[i].w, v[i].w};
+            if (over & 2) v[i] = vf4{v[i].z, v[i].w, v[i].w, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e >= a.vocab) v[i][e] = -__builtin_inff();
+        }
+    };
+    load(split0 * a.per);  // on its way while the row's sequence is found
     const int s = seq_of_row(a.tok, a.n_seq, row);
     if (s < 0) return;
     bool greedy;
-    const double c = heat_of(a, s, greedy);
-    Part p{0.0, -__builtin_inff(), INT_MAX};
-    for (int base = from; base < to; base += 1024 * NV) {
-        if (base != from) load(base);
-        if (base + 1024 * NV > to)
+    const double c = heat_of(a, s, greedy), least_d = -1000.0 / c;
+    for (int split = split0; split < min(a.splits, split0 + a.group); ++split) {
+        const int from = split * a.per, to = min(a.vocab, from + a.per);
+        Part p{0.0, -__builtin_inff(), INT_MAX};  // a wavefront's: the sum still a lane's
+        for (int base = from; base < to; base += 1024 * NV) {
+            if (base != split0 * a.per) load(base);
+            if (base + 1024 * NV > a.vocab) cut(base);
+            const float was = p.top;
+            float own = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) own = larger(larger(own, larger(v[i].x, v[i].y)), larger(v[i].z, v[i].w));
+            p.top = larger(was, largest(own));
+            if (greedy && p.top > was) {  // a lane's words rise: its first one that is as large
+                p.at = INT_MAX;
+#pragma unroll
+                for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+                    for (int e = 3; e >= 0; --e)
+                        if (v[i][e] == p.top) p.at = base + i * 1024 + 4 * tid + e;
+            }
+            const double m = level(p.top);
+            if (base != from) p.sum *= exp2_of(((double)was - m) * c);
+            // a word that is none, and a NaN, add 2^-1000
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (base + i * 1024 + 4 * tid + e >= to) v[i][e] = -__builtin_inff();
-        const float was = p.top;
-        float top = was;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) top = larger(larger(top, larger(v[i].x, v[i].y)), larger(v[i].z, v[i].w));
-        if (greedy && top > was)  // a lane's words rise: its first one that is as large
-#pragma unroll
-            for (int i = NV - 1; i >= 0; --i)
-#pragma unroll
-                for (int e = 3; e >= 0; --e)
-                    if (v[i][e] == top) p.at = base + i * 1024 + 4 * tid + e;
-        const double m = level(top);
-        if (base != from) p.sum *= exp2_of(((double)was - m) * c);
-        p.top = top;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p.sum += exp2_near(fmax(((double)v[i][e] - m) * c, -1000.0));
-    }
-    p = join_lanes(p, c, greedy);
-    if ((tid & 63) == 0) lds[tid >> 6] = p;
-    __syncthreads();
-    if (tid < 64) {
-        p = join_lanes(tid < 4 ? lds[tid] : Part{0.0, -__builtin_inff(), INT_MAX}, c, greedy);
-        if (tid == 0) {
-            const int64_t i = (int64_t)row * a.splits + split;
-            a.sum[i] = p.sum, a.top[i] = p.top, a.at[i] = p.at;
+                for (int e = 0; e < 4; ++e) p.sum += exp2_near(fmax((double)v[i][e] - m, least_d), c);
+        }
+        p.sum = total(p.sum);
+        if (greedy) p.at = least(p.at);
+        if (split != split0) __syncthreads();
+        if ((tid & 63) == 0) lds[tid >> 6] = p;
+        __syncthreads();
+        if (tid < 64) {
+            p = join_lanes(tid < 4 ? lds[tid] : Part{0.0, -__builtin_inff(), INT_MAX}, c, greedy);
+            if (tid == 0) {
+                const int64_t i = (int64_t)row * a.splits + split;
+                a.sum[i] = p.sum, a.top[i] = p.top, a.at[i] = p.at;
+            }
         }
     }
 }
@@ -239,19 +257,20 @@ __device__ VerifyChoice decide(const VerifyArgs &a, int s, double c, bool greedy
 enum { FROM_P, WITHOUT_DRAFT, FROM_REST };
 struct Weigh {
     const float *x, *q;
-    double m, c, z, lse;  // the row's largest, log2(e) / T, 1 / the sum, the draft row's lse in powers of two
+    double m, c, z, lse, least_d;  // the row's largest, log2(e) / T, 1 / the sum, the draft row's lse in powers of two, -1000 / c
     int d;
 };
 template <int MODE>
 __device__ __forceinline__ double weight(const Weigh &w, int j, float x, float q) {
+    if (MODE == FROM_REST)  // a word that cannot be has 2^-1000 in p, and 2^-990 or more in q
+        return fmax(__builtin_fma(exp2_near(fmax((double)x - w.m, w.least_d), w.c), w.z, -exp2_near(fmin(fmax(__builtin_fma((double)q, w.c, -w.lse), -990.0), 1000.0), 1.0)), 0.0);
     const double p = exp2_of(((double)x - w.m) * w.c);
-    if (MODE == WITHOUT_DRAFT && j == w.d) return 0.0;
-    return MODE == FROM_REST ? fmax(p * w.z - exp2_of((double)q * w.c - w.lse), 0.0) : p;
+    return MODE == WITHOUT_DRAFT && j == w.d ? 0.0 : p;
 }
 __device__ __forceinline__ Weigh weigh_of(const VerifyArgs &a, const VerifyChoice &ch, double c) {
     Weigh w;
     w.x = a.logits + ch.t * a.ld, w.q = a.q ? a.q + ch.t * a.ldq : nullptr;
-    w.m = level(ch.top), w.c = c, w.z = 1.0 / ch.sum, w.lse = a.q ? (double)a.q_lse[ch.t] * LOG2E : 0.0, w.d = ch.d;
+    w.m = level(ch.top), w.c = c, w.z = 1.0 / ch.sum, w.lse = a.q ? (double)a.q_lse[ch.t] * LOG2E : 0.0, w.d = ch.d, w.least_d = -1000.0 / c;
     return w;
 }
 // f(first word, weights of 4) of a thread's words b .. e - 1
@@ -293,7 +312,8 @@ __device__ __forceinline__ double sum_words(const Weigh &w, int from, int to) {
     return scan_waves(total(v)).y;
 }
 
-// the decision where the drafts have probabilities, and the sums of max(p - q, 0) of a rejected row, by parts of SUB words
+// the decision where the drafts have probabilities, and the sums of max(p - q, 0) of a rejected row, by parts of SUB words. Each of a sequence's
+// workgroups decides for itself; the first one keeps it for the draw. (A launch for the decisions alone took as long.)
 __global__ __launch_bounds__(WG) void verify_rest_kernel(VerifyArgs a) {
     const int s = blockIdx.x / a.splits, split = blockIdx.x - s * a.splits, subs = (a.per + SUB - 1) / SUB;
     bool greedy;
@@ -376,13 +396,14 @@ __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     bool greedy;
     const double c = heat_of(a, s, greedy);
+    const double v = a.v[s];
+    const int len = a.keep ? a.len[s] : 0;
     const VerifyChoice ch = a.q ? a.choice[s] : decide(a, s, c, greedy, a.lse != nullptr);
     int word = -1;
     if (ch.n > 0 && fabsf(ch.top) <= 3.4028235e38f && c == c) {
         if (greedy) word = ch.at;
         else {
             const Weigh w = weigh_of(a, ch, c);
-            const double v = a.v[s];
             double part = 0.0;  // of p: what the rows' pass left, on the row's level
             if (lane < a.splits) {
                 const int64_t i = (int64_t)ch.t * a.splits + lane;
@@ -405,7 +426,7 @@ __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     if (tid == 0) {
         a.n_ok[s] = ch.good;
         a.next[s] = word;
-        if (a.keep) a.keep[s] = ch.n > 0 ? max(0, a.len[s] - (ch.n - 1 - ch.good)) : a.len[s];
+        if (a.keep) a.keep[s] = ch.n > 0 ? max(0, len - (ch.n - 1 - ch.good)) : len;
     }
 }
 
@@ -414,12 +435,13 @@ size_t subs_of(const VerifyArgs &a) { return (a.per + SUB - 1) / SUB; }
 
 size_t verify_plan(VerifyArgs &a, int num_cu) {
     auto parts = [&](int nv) { return (a.vocab + 1024 * nv - 1) / (1024 * nv); };
-    a.nv = 8;
+    a.nv = 4;
     while (a.nv > 1 && (int64_t)a.n_tok * parts(a.nv) < 4 * num_cu) a.nv /= 2;
-    const int blocks = parts(a.nv);
-    a.splits = std::min(64, blocks);  // a wavefront joins them
+    const int blocks = parts(a.nv), two = (int64_t)a.n_tok * blocks >= 8 * num_cu ? 2 : 1;
+    a.splits = std::min(64, (blocks + two - 1) / two);  // a wavefront joins them
     a.per = (blocks + a.splits - 1) / a.splits * 1024 * a.nv;
     a.splits = (a.vocab + a.per - 1) / a.per;
+    a.group = (int64_t)a.n_tok * a.splits >= 8 * num_cu ? 2 : 1;
     const size_t n = (size_t)a.n_tok * a.splits;
     return n * 16 + (a.q ? (size_t)a.n_seq * ((size_t)a.splits * subs_of(a) * 8 + sizeof(VerifyChoice)) : 0);
 }
@@ -433,12 +455,11 @@ void verify_scratch(VerifyArgs &a, void *p) {
 }
 
 hipError_t launch_verify(const VerifyArgs &a, hipStream_t s) {
-    const unsigned grid = (unsigned)((int64_t)a.n_tok * a.splits);
+    const unsigned grid = (unsigned)((int64_t)a.n_tok * ((a.splits + a.group - 1) / a.group));
     switch (a.nv) {
     case 1: verify_rows_kernel<1><<<grid, 256, 0, s>>>(a); break;
     case 2: verify_rows_kernel<2><<<grid, 256, 0, s>>>(a); break;
-    case 4: verify_rows_kernel<4><<<grid, 256, 0, s>>>(a); break;
-    default: verify_rows_kernel<8><<<grid, 256, 0, s>>>(a); break;
+    default: verify_rows_kernel<4><<<grid, 256, 0, s>>>(a); break;
     }
     if (a.q) verify_rest_kernel<<<(unsigned)((int64_t)a.n_seq * a.splits), WG, 0, s>>>(a);
     verify_next_kernel<<<(unsigned)a.n_seq, WG, 0, s>>>(a);
