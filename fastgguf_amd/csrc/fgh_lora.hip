@@ -137,15 +137,16 @@ struct Stage {
 };
 constexpr int LD = 68;  // floats between rows of 64 in LDS: 16 rows start in 16 different groups of banks
 
-constexpr int DOWN_WAVES = 8;
-
-// h of few rows that have an adapter in common, 16 NR ranks, over a part of the columns: the wavefronts take steps of 32 columns in turn, the next one's values on their
-// way during the products of one. Lane l: rank l % 16 of a tile and row l % 16, columns 8 (l / 16) .. + 7.
+// h of few rows that have an adapter in common, 16 NR ranks, over a part of the columns: the wavefronts take steps of 64 columns in turn, the
+// next one's values on their way during the products of one. A's values and x's go through a wavefront's own LDS, so that neighbouring lanes
+// read neighbouring values: as the products take them, 16 rows an access, the first cache gave one lane a cycle.
 template <int TYPE, int NR>
-__global__ __launch_bounds__(64 * DOWN_WAVES, 4) void lora_down_split_kernel(LoraArgs a) {
-    constexpr int ES = Weights<TYPE>::ES, NW = Weights<TYPE>::NW, HALF = DOWN_WAVES / 2;
-    __shared__ __attribute__((aligned(16))) pf4 lds[HALF * NR * 64];
-    __shared__ int marks[DOWN_WAVES * 64];
+__global__ __launch_bounds__(256) void lora_down_split_kernel(LoraArgs a) {
+    constexpr int ES = Weights<TYPE>::ES, NW = Weights<TYPE>::NW;
+    constexpr int CH = 4 * ES, PER = 64 / CH, LOADS = 16 * NR / PER, ROW = 64 * ES + 16;  // 16-byte values of a row, rows of an access; bytes of a row in LDS
+    __shared__ __attribute__((aligned(16))) uint8_t wl[4][16 * NR * ROW];
+    __shared__ __attribute__((aligned(16))) float xl[4][16 * LD];
+    __shared__ int marks[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int blocks = (a.max_rank + 16 * NR - 1) / (16 * NR);
     int b = blockIdx.x;
@@ -157,6 +158,8 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 4) void lora_down_split_kernel(Lor
     const int from = part * a.kper, to = min(a.cols, from + a.kper), r0 = block * 16 * NR;
     const int padded = (a.max_rank + 15) & ~15;
     int *list = marks + 64 * wave;
+    uint8_t *wo = wl[wave];
+    float *xo = xl[wave];
     const int mark = adapters_of(a, base, list);
     uint64_t left = __builtin_amdgcn_ballot_w64(mark != 0);
     for (int which = 0, mine = slot;; ++which) {  // the tile's runs; every `slots`-th one is this workgroup's
@@ -169,70 +172,64 @@ __global__ __launch_bounds__(64 * DOWN_WAVES, 4) void lora_down_split_kernel(Lor
         if (!m) break;
         mine += a.slots;
         if (run.adapter < 0 || r0 >= run.rank) continue;
-        const int n = list_rows(rows_of, list);
-        const uint8_t *A = a.a + (int64_t)run.adapter * a.max_rank * a.cols * ES;
+        const int n = list_rows(rows_of, list), tiles = min(NR, (run.rank - r0 + 15) / 16);
+        const uint8_t *A = a.a + ((int64_t)run.adapter * a.max_rank + r0) * a.cols * ES;
+        const uint8_t *X = (const uint8_t *)(a.x + base * a.ldx);
         for (int t0 = 0; t0 < n; t0 += 16) {
             pf4 acc[NR];
 #pragma unroll
             for (int j = 0; j < NR; ++j) acc[j] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-            // a lane's place in its rows of x and of A, from addresses that move along the columns: offsets of 32 bits
-            const uint32_t xo = 4 * ((uint32_t)list[min(t0 + c, n - 1)] * (uint32_t)a.ldx + 8 * g);
-            uint32_t wo[NR];
-            // behind the last rank that one again: what it gives is not used
+            uint32_t xr[4];
 #pragma unroll
-            for (int j = 0; j < NR; ++j) wo[j] = ES * ((uint32_t)min(r0 + 16 * j + c, run.rank - 1) * (uint32_t)a.cols + 8 * g);
-            const uint8_t *X = (const uint8_t *)(a.x + base * a.ldx);
-            const int tiles = min(NR, (run.rank - r0 + 15) / 16);
-            lf4 xn[2];
-            Raw<TYPE> wn[NR];
-            // columns end at a multiple of 8: lanes behind them look back to the last ones
-            auto back = [&](int k0) { return (uint32_t)max(0, k0 + 8 * g + 8 - a.cols); };
-            auto load_x = [&](int k0) {
-                const uint8_t *p = X + 4 * (int64_t)k0;
-                const uint32_t z = k0 + 32 <= a.cols ? 0 : 4 * back(k0);
-                xn[0] = *(const lf4 *)(p + xo - z), xn[1] = *(const lf4 *)(p + xo - z + 16);
+            for (int i = 0; i < 4; ++i) xr[i] = 4 * ((uint32_t)list[min(t0 + 4 * i + g, n - 1)] * (uint32_t)a.ldx);
+            pu4 wn[LOADS];
+            lf4 xn[4];
+            auto load = [&](int k0) {  // behind the last column and the last rank those again
+                const uint32_t k = ES * (uint32_t)min(k0 + 16 / ES * (lane % CH), a.cols - 16 / ES), kx = 4 * (uint32_t)min(k0 + 4 * c, a.cols - 4);
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i)
+                    if (i * PER < 16 * tiles) wn[i] = *(const pu4 *)(A + (uint32_t)(ES * ((uint32_t)min(i * PER + lane / CH, run.rank - r0 - 1) * (uint32_t)a.cols) + k));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t0 + 4 * i < n) xn[i] = *(const lf4 *)(X + (uint32_t)(xr[i] + kx));
             };
-            auto load_w = [&](int j, int k0) {
-                const uint32_t z = k0 + 32 <= a.cols ? 0 : ES * back(k0);
-                if (j < tiles) wn[j] = raw8<TYPE>(A + (int64_t)ES * k0 + wo[j] - z);
-            };
-            int k0 = from + 32 * wave;
-            if (k0 < to) {
+            int k0 = from + 64 * wave;
+            if (k0 < to) load(k0);
+            for (; k0 < to; k0 += 256) {
+                // LDS serves a wavefront in order: only the compiler must keep it
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int j = 0; j < NR; ++j) load_w(j, k0);
-                load_x(k0);
-            }
-            for (; k0 < to; k0 += 32 * DOWN_WAVES) {
-                const bool more = k0 + 32 * DOWN_WAVES < to, whole = k0 + 32 <= to;
-                const float v[8] = {xn[0].x, xn[0].y, xn[0].z, xn[0].w, xn[1].x, xn[1].y, xn[1].z, xn[1].w};
-                pu4 p[3];
-                parts8<T_BF16, 3>(v, p);
-                if (more) load_x(k0 + 32 * DOWN_WAVES);
+                for (int i = 0; i < LOADS; ++i) *(pu4 *)(wo + (i * PER + lane / CH) * ROW + 16 * (lane % CH)) = wn[i];
 #pragma unroll
-                for (int j = 0; j < NR; ++j) {
-                    if (j >= tiles) break;
-                    pu4 q[1][NW];
-                    if (!whole && k0 + 8 * g >= to) wn[j] = Raw<TYPE>{};
-                    weights8<TYPE>(wn[j], q[0]);
-                    if (more) load_w(j, k0 + 32 * DOWN_WAVES);
-                    multiply<TYPE, 1>(acc + j, q, p);
+                for (int i = 0; i < 4; ++i) *(pf4 *)(xo + (4 * i + g) * LD + 4 * c) = xn[i];
+                __builtin_amdgcn_wave_barrier();
+                if (k0 + 256 < to) load(k0 + 256);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float v[8];
+                    *(pf4 *)v = *(const pf4 *)(xo + c * LD + 32 * k + 8 * g), *(pf4 *)(v + 4) = *(const pf4 *)(xo + c * LD + 32 * k + 8 * g + 4);
+                    pu4 p[3];
+                    parts8<T_BF16, 3>(v, p);
+#pragma unroll
+                    for (int j = 0; j < NR; ++j) {
+                        if (j >= tiles) break;
+                        Raw<TYPE> raw = raw8<TYPE>(wo + (16 * j + c) * ROW + ES * (32 * k + 8 * g));
+                        if (k0 + 32 * k + 8 * g >= to) raw = Raw<TYPE>{};  // times 0 behind the last column
+                        pu4 w[1][NW];
+                        weights8<TYPE>(raw, w[0]);
+                        multiply<TYPE, 1>(acc + j, w, p);
+                    }
                 }
             }
-            // the wavefronts' sums: the second half to the first, then all to the first ones
-            auto at = [&](int w, int i) -> pf4 & { return lds[(w * NR + i) * 64 + lane]; };
-            if (wave >= HALF)
-#pragma unroll
-                for (int i = 0; i < NR; ++i) at(wave - HALF, i) = acc[i];
+            // the wavefronts' sums, in the order of the wavefronts
             __syncthreads();
-            if (wave < HALF)
+            pf4 *sums = (pf4 *)wl;  // [4][NR][64]
 #pragma unroll
-                for (int i = 0; i < NR; ++i) at(wave, i) += acc[i];
+            for (int j = 0; j < NR; ++j) sums[(wave * NR + j) * 64 + lane] = acc[j];
             __syncthreads();
-            for (int i = wave; i < NR; i += DOWN_WAVES) {
-                const int row = t0 + c, r = r0 + 16 * i + 4 * g;
-                pf4 v = at(0, i);
-#pragma unroll
-                for (int w = 1; w < HALF; ++w) v += at(w, i);
+            for (int j = wave; j < NR; j += 4) {
+                const int row = t0 + c, r = r0 + 16 * j + 4 * g;
+                const pf4 v = (sums[j * 64 + lane] + sums[(NR + j) * 64 + lane]) + (sums[(2 * NR + j) * 64 + lane] + sums[(3 * NR + j) * 64 + lane]);
                 if (row < n && r < padded) *(pf4 *)(a.part + ((int64_t)part * a.n_tok + base + list[row]) * padded + r) = v;
             }
             __syncthreads();
@@ -438,11 +435,34 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                 load_y(yn[0], first);
                 load_y(yn[1], first + 64);
             }
+            // h, summed over the parts by neighbouring threads for the workgroup, through the LDS of the results
             pu4 x[KH][3];
-            if (KB)
+            if constexpr (KB > 0) {
+                constexpr int Q = 8 * SB;  // threads to a row
 #pragma unroll
-                for (int k = 0; k < KH; ++k)
-                    if (k < steps) sums(k, x[k]);
+                for (int kb = 0; kb < KB; ++kb) {
+                    if (kb) lds_barrier();
+                    for (int i = tid; i < (ROWS ? 64 : 16) * Q; i += 256) {
+                        const int row = i / Q, r = 32 * SB * kb + 4 * (i % Q);
+                        if (t0 + row >= n || r >= run.rank) continue;
+                        const float *p = a.part + (int64_t)(base + list[t0 + row]) * padded + r;
+                        pf4 h = *(const pf4 *)p;
+#pragma unroll 4
+                        for (int s = 1; s < a.ks; ++s) h += *(const pf4 *)(p + (int64_t)s * a.n_tok * padded);
+                        *(pf4 *)(&tiles[0][0] + row * LD + 4 * (i % Q)) = h;
+                    }
+                    lds_barrier();
+#pragma unroll
+                    for (int k = 0; k < SB; ++k) {
+                        const float *p = out + c * LD + 32 * k + 8 * g;
+                        float h[8];
+                        *(pf4 *)h = *(const pf4 *)p, *(pf4 *)(h + 4) = *(const pf4 *)(p + 4);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = 32 * (SB * kb + k) + 8 * g < run.rank ? h[e] : 0.0f;
+                        parts8<T_BF16, 3>(h, x[SB * kb + k]);
+                    }
+                }
+            }
             auto turn = [&](lf4 (&v)[I], int n0) {
                 pf4 acc[J];
 #pragma unroll
@@ -540,9 +560,9 @@ hipError_t launch_type(const LoraArgs &a, hipStream_t s) {
         else lora_down_kernel<TYPE, 4><<<down, 256, 0, s>>>(a);
         launch_up<TYPE, true>(a, up, s);
     } else {
-        if (a.nr == 1) lora_down_split_kernel<TYPE, 1><<<down, 64 * DOWN_WAVES, 0, s>>>(a);
-        else if (a.nr == 2) lora_down_split_kernel<TYPE, 2><<<down, 64 * DOWN_WAVES, 0, s>>>(a);
-        else lora_down_split_kernel<TYPE, 4><<<down, 64 * DOWN_WAVES, 0, s>>>(a);
+        if (a.nr == 1) lora_down_split_kernel<TYPE, 1><<<down, 256, 0, s>>>(a);
+        else if (a.nr == 2) lora_down_split_kernel<TYPE, 2><<<down, 256, 0, s>>>(a);
+        else lora_down_split_kernel<TYPE, 4><<<down, 256, 0, s>>>(a);
         launch_up<TYPE, false>(a, up, s);
     }
     return hipGetLastError();
@@ -561,7 +581,7 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     // a workgroup for every run that a tile could have, while that fills the device twice at most; one run after the other is as long again
     a.slots = (int)std::max<int64_t>(1, std::min<int64_t>(prompts ? std::min(a.most, 3) : a.most, 2 * num_cu / tiles));
     // columns over as many workgroups as that leaves room for, a step of each wavefront, or of the workgroup, at the least
-    const int64_t unit = a.whole ? 64 : 32 * DOWN_WAVES, units = (a.cols + unit - 1) / unit;
+    const int64_t unit = a.whole ? 64 : 256, units = (a.cols + unit - 1) / unit;
     const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
