@@ -444,7 +444,7 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                     if (kb) lds_barrier();
                     for (int i = tid; i < (ROWS ? 64 : 16) * Q; i += 256) {
                         const int row = i / Q, r = 32 * SB * kb + 4 * (i % Q);
-                        if (t0 + row >= n || r >= run.rank) continue;
+                        if (t0 + row >= n || (r & ~7) >= run.rank) continue;  // eights of ranks: what is behind the last one is finite if that is
                         const float *p = a.part + (int64_t)(base + list[t0 + row]) * padded + r;
                         pf4 h = *(const pf4 *)p;
 #pragma unroll 4
@@ -596,7 +596,7 @@ void lora_scratch(LoraArgs &a, void *p) {
 }
 int64_t lora_grid(const LoraArgs &a) {
     const int64_t tiles = tiles_of(a) * a.slots;
-    return std::max(2 * tiles * a.ks * rank_blocks(a), tiles * ((a.rows + a.ucols - 1) / a.ucols));
+    return std::max(2 * tiles * a.ks * rank_blocks(a), tiles * ((a.rows + 63) / 64));  // at the most
 }
 
 hipError_t launch_lora(const LoraArgs &a, hipStream_t s) {

@@ -314,6 +314,14 @@ def test_verify(backend, i, drafter):
         assert 0 < n_ok.sum() < sum(max(0, n - 1) for n in rows)
 
 
+@pytest.mark.parametrize("drafter", [False, True])
+def test_verify_many_rows(backend, drafter):
+    """More rows than fill the device: each part of one takes two blocks, each workgroup two parts."""
+    c = Case(113, [6] * 190 + [1, 0, 11], 9001, drafter, (1, 2), 3)
+    n_ok, _ = c.run(backend)
+    assert 0 < n_ok.sum() < c.n_tok - c.n
+
+
 def test_verify_long_rows(backend):
     """A vocabulary whose parts take several blocks of a workgroup."""
     c = Case(20, [2], 1000003, True)
@@ -552,6 +560,42 @@ def test_lora(backend, i, t):
     check_lora(backend, *lora_case(40 + i, t, n, max_rank, cols, rows, news, ids, ranks, pad), pad=i % 4, form=form)
 
 
+PROMPTS = [  # the same, of prompts long enough to have workgroups of 64 rows
+    (3, 8, 200, 130, [700, 1, 1, 1, 1, 400], [0, 1, 2, 0, 1, 2], [8, 3, 5], (3, 9)),
+    (2, 32, 1000, 515, [600, 499], [1, 0], [32, 9], (0, 0)),
+    (3, 64, 136, 70, [301] * 4, [0, 1, 2, -1], [64, 33, 1], (0, 2)),
+    (2, 128, 320, 384, [513, 0, 600], [1, 7, 0], [128, 100], (1, 0)),
+    (2, 200, 264, 65, [1025, 40], [1, 0], [200, 140], (0, 0)),
+    (1, 512, 72, 64, [1100], [0], None, (0, 0)),
+    (2, 16, 2048, 3, [1500, 20], [0, 1], [16, 10], (0, 0)),
+    (1, 24, 8, 1, [2000], [0], [17], (5, 0)),
+    (4, 16, 64, 200, [16] * 70, [s % 6 - 1 for s in range(70)], [16, 0, 2, 11], (0, 0)),
+    (2, 40, 448, 1030, [64, 63, 65, 1000], [0, 1, 1, 0], [40, 24], (0, 0)),
+]
+
+
+@pytest.mark.parametrize("t", R.TYPES)
+@pytest.mark.parametrize("i", range(len(PROMPTS)))
+def test_lora_prompts(backend, i, t):
+    n, max_rank, cols, rows, news, ids, ranks, pad = PROMPTS[i]
+    form = ["in place", "apart", "alone"][i % 3]
+    check_lora(backend, *lora_case(140 + i, t, n, max_rank, cols, rows, news, ids, ranks, pad), pad=i % 4, form=form)
+
+
+@pytest.mark.parametrize("news", [[4, 1, 1, 1, 1, 1100], [4, 1, 1, 1, 1, 300], [4, 1, 1, 1, 1, 1] * 300])
+@pytest.mark.parametrize("rank", [1, 2, 4, 9])
+def test_lora_beside_nan(backend, news, rank):
+    """A tile's rows whose results are NaN leave nothing to others of the same tile, whose ranks end inside the next eight."""
+    ids = [s % 6 for s in range(len(news))]
+    ad, tok, ids, x, y_in = lora_case(160 + rank, T_F16, 6, 64, 128, 128, news, ids, [64, 0, 64, rank, rank, rank])
+    spoilt = np.isin(np.repeat(ids, news), (0, 2))
+    x[spoilt, 3] = np.nan
+    got, _ = run_lora(backend, ad, tok, ids, x, y_in)
+    want, tol, _ = R.lora(ad, tok, ids, np.where(np.isfinite(x), x, 0).astype(np.float32), y_in)
+    assert np.isnan(got[spoilt]).all()
+    assert (np.abs(got - want) <= tol)[~spoilt].all()
+
+
 @pytest.mark.parametrize("form", ["apart", "in place", "alone"])
 @pytest.mark.parametrize("pad", [0, 1, 4])
 def test_lora_forms(backend, form, pad):
@@ -675,6 +719,30 @@ def test_lora_captured(backend):
         finally:
             for g in graphs:
                 backend.graph_destroy(g)
+
+
+def test_lora_prompt_captured(backend):
+    """A recorded call of a prompt, beside eager ones of few rows."""
+    ad, tok, ids, x, y_in = lora_case(74, T_BF16, 2, 32, 264, 190, [1000, 90], [1, 0])
+    with Dev(backend) as d:
+        set_ = Lora(ad.type, d.put(ad.a), d.put(ad.b), n_adapter=ad.n, max_rank=ad.max_rank, cols=ad.cols, rows=ad.rows, rank=d.put(ad.rank),
+                    scale=d.put(ad.scale))
+        xd, yd, yi = d.put(x), d.put(np.zeros_like(y_in)), d.put(y_in)
+        args = (set_, d.put(tok.astype(np.int32)), d.put(np.array(ids, np.int32)), len(ids), len(x), xd, ad.cols, yd, ad.rows)
+        backend.lora_dev(*args, y_in_dev=yi, ldyi=ad.rows)
+        backend.graph_begin()
+        backend.lora_dev(*args, y_in_dev=yi, ldyi=ad.rows)
+        graph = backend.graph_end()
+        try:
+            for step in range(3):
+                x += 1.0
+                backend.h2d(xd, x)
+                check_lora(backend, *lora_case(75 + step, T_F16, 3, 16, 512, 200, [1, 2, 1], [0, 1, 2]))
+                backend.graph_launch(graph)
+                want, tol, _ = R.lora(ad, tok, ids, x, y_in)
+                assert (np.abs(d.get(yd, y_in) - want) <= tol).all()
+        finally:
+            backend.graph_destroy(graph)
 
 
 def test_same_results_twice(backend):

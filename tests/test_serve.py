@@ -76,6 +76,14 @@ def test_lora_refused(kw):
     assert lora_check(**kw) != ""
 
 
+def test_lora_largest():
+    """A tile's offsets in 32 bits."""
+    most = dict(cols=1 << 20, ldx=1 << 24, ldy=1 << 24, ldyi=1 << 24)
+    assert lora_check(**most) == ""
+    for kw in (dict(cols=(1 << 20) + 8), dict(ldx=(1 << 24) + 1), dict(ldy=(1 << 24) + 1), dict(ldyi=(1 << 24) + 1)):
+        assert lora_check(**{**most, **kw}) != ""
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_pages_are_never_lost(seed):
     """After any steps of the host's form, every page is held once or free once, and sequences hold what their lengths take."""
