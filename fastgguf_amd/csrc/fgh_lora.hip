@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void lora_down_split_kernel(LoraArgs a) {
     b /= a.ks;
     const int block = b % blocks;
     b /= blocks;
-    const int slot = b % a.slots, tile = b / a.slots, base = tile * a.tile;
+    const int all = (a.n_tok + a.tile - 1) / a.tile, tile = b % all, slot = b / all, base = tile * a.tile;  // first the first runs, which every tile has
     const int from = part * a.kper, to = min(a.cols, from + a.kper), r0 = block * 16 * NR;
     const int padded = (a.max_rank + 15) & ~15;
     int *list = marks + 64 * wave;
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     b /= a.ks;
     const int block = b % blocks;
     b /= blocks;
-    const int slot = b % a.slots, tile = b / a.slots, base = tile * a.tile;
+    const int all = (a.n_tok + a.tile - 1) / a.tile, tile = b % all, slot = b / all, base = tile * a.tile;  // first the first runs, which every tile has
     const int from = part * a.kper, to = min(a.cols, from + a.kper), r0 = block * 16 * NR;
     const int padded = (a.max_rank + 15) & ~15;
     int *list = lists + 64 * wave;
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
 // through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: such blocks of ranks, whose h stays in registers; 0: any number,
 // which does not.
 template <int TYPE, int SB, int KB, bool ROWS>
-__global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lora_up_kernel(LoraArgs a) {
+__global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS ? 3 : 4) void lora_up_kernel(LoraArgs a) {
     using S = Stage<TYPE, SB>;
     constexpr int ES = S::ES, NW = S::NW, J = ROWS ? 4 : 1, P = ROWS ? 2 : 1, KH = KB ? SB * KB : 1, CH = 4 * SB;  // CH: threads to a row's values
     __shared__ __attribute__((aligned(16))) pu4 wl[S::VALUES];
@@ -372,13 +372,20 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int blocks = (a.rows + a.ucols - 1) / a.ucols;
     int b = blockIdx.x;
-    const int first = b % blocks * a.ucols, end = min(a.rows, first + a.ucols);
+    const int b_chunk = b % blocks, first = b_chunk * a.ucols, end = min(a.rows, first + a.ucols);
     b /= blocks;
-    const int slot = b % a.slots, tile = b / a.slots, base = tile * a.tile;
+    const int all = (a.n_tok + a.tile - 1) / a.tile, tile = b % all, slot = b / all, base = tile * a.tile;  // first the first runs, which every tile has
     const int padded = (a.max_rank + 15) & ~15;
     float *out = tiles[ROWS ? wave : 0], *y = a.y + base * a.ldy;
     const float *yin = a.yin + base * a.ldyi;
     int *list = lists + 64 * wave;
+    // The turns start at another one in each tile and go round: rows lie a power of two or a few apart, and workgroups that read and write the same
+    // columns of their rows at a time would ask few of the memory's channels.
+    const int turns = (end - first + 63) / 64, rot = (int)((unsigned)(tile + b_chunk) % (unsigned)turns);
+    auto column = [&](int i) {  // behind the last turn the last one again
+        const int j = min(i, turns - 1) + rot;
+        return first + 64 * (j < turns ? j : j - turns);
+    };
     for (int which = slot; which < a.most; which += a.slots) {
         const LoraRun run = a.runs[(int64_t)tile * a.most + which];
         if (run.rows == 0) break;
@@ -430,10 +437,10 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                     }
                 parts8<T_BF16, 3>(h, x);
             };
-            load_w(first, 0);
+            load_w(column(0), 0);
             if (ahead) {
-                load_y(yn[0], first);
-                load_y(yn[1], first + 64);
+                load_y(yn[0], column(0));
+                load_y(yn[1], column(1));
             }
             // h, summed over the parts by neighbouring threads for the workgroup, through the LDS of the results
             pu4 x[KH][3];
@@ -463,7 +470,8 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                     }
                 }
             }
-            auto turn = [&](lf4 (&v)[I], int n0) {
+            auto turn = [&](lf4 (&v)[I], int i) {
+                const int n0 = column(i), next = column(i + 1);
                 pf4 acc[J];
 #pragma unroll
                 for (int j = 0; j < J; ++j) acc[j] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -471,7 +479,7 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                     const bool last = kb + 1 == kbs;
                     lds_barrier();  // the products before are done
                     put_w(kb);
-                    load_w(last ? n0 + 64 : n0, last ? 0 : kb + 1);  // behind the last the last again: in a branch it would be waited for at once
+                    load_w(last ? next : n0, last ? 0 : kb + 1);  // behind the last the last again: in a branch it would be waited for at once
                     lds_barrier();
 #pragma unroll
                     for (int k = 0; k < SB; ++k)
@@ -524,16 +532,16 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS && SB == 2 ? 3 : 4) void lo
                         y[at * a.ldy + n0 + col] = run.adapter != -1 ? u + run.scale * out[row * LD + col] : u;
                     }
                 }
-                if (ahead) load_y(v, n0 + 128);
+                if (ahead) load_y(v, column(i + 2));
                 else
 #pragma unroll
                     for (int i = 0; i < I; ++i) v[i] = lf4{0.0f, 0.0f, 0.0f, 0.0f};
             };
 #pragma clang loop unroll(disable)
-            for (int n0 = first; n0 < end; n0 += 128) {
-                turn(yn[0], n0);
-                if (n0 + 64 >= end) break;
-                turn(yn[1], n0 + 64);
+            for (int i = 0; i < turns; i += 2) {
+                turn(yn[0], i);
+                if (i + 1 >= turns) break;
+                turn(yn[1], i + 1);
             }
             lds_barrier();  // the next rows' values go where these were
         }
@@ -586,7 +594,7 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
     // outputs over so many workgroups that the device is filled, a turn of 64 at the least
-    const int64_t steps = (a.rows + 63) / 64, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, 4 * num_cu / (tiles * (prompts ? 1 : a.slots))));
+    const int64_t steps = (a.rows + 63) / 64, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, (a.whole ? 2 : 4) * num_cu / (tiles * (prompts ? 1 : a.slots))));
     a.ucols = (int)((steps + chunks - 1) / chunks * 64);
     return (size_t)tiles * a.most * sizeof(LoraRun) + (size_t)a.ks * a.n_tok * ((a.max_rank + 15) & ~15) * 4;
 }
