@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS ? 3 : 4) void lora_up_kerne
             lf4 yn[2][I] = {};  // of the next two turns
             Raw<TYPE> wn[SB];
             auto load_w = [&](int n0, int kb) {  // outputs and ranks behind the last: others, which are not used, or cut
-                const int r = min(32 * SB * kb + 8 * (tid % CH), a.max_rank - 8);
+                const int r = min(32 * SB * kb + 8 * (tid % CH), max(run.rank - 1, 0) & ~7);
 #pragma unroll
                 for (int u = 0; u < SB; ++u) wn[u] = raw8<TYPE>(B + ES * ((int64_t)min(n0 + tid / CH + 256 / CH * u, a.rows - 1) * a.max_rank + r));
             };
@@ -579,21 +579,27 @@ hipError_t launch_type(const LoraArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t lora_plan(LoraArgs &a, int num_cu) {
-    // tiles of 64 rows, whose rows of one adapter share its reads; prompts with few rows take tiles of 16
+    // Tiles of 64 rows, whose rows of one adapter share its reads. In prompts most of a tile is one sequence's, and each wavefront has rows of its own,
+    // if there are tiles for the device; few rows, and many short prompts, are better in tiles of 16 (4096 -> 14336, F16, rank 64; one prompt of 512: 27 us,
+    // 34 with 64; of 1024: 48 and 49; of 2048: 82 and 76; 64 of 63: 220 and 200. 4096 -> 6144, F32, rank 32; 128 of 16: 46 and 74; 256 of 4, which are
+    // tiles of 64 again: 40, of 16: 69).
     const bool prompts = a.n_tok >= 16 * (int64_t)a.n_seq;
-    a.whole = prompts && a.n_tok >= 4 * num_cu;
+    a.whole = a.n_tok >= 32 * (int64_t)a.n_seq && a.n_tok >= 4 * num_cu;
     a.tile = a.whole || !prompts ? 64 : 16;
     const int64_t tiles = tiles_of(a);
     a.most = (int)std::min<int64_t>(std::min(a.n_seq, a.tile), (int64_t)a.n_adapter + 2);
     a.nr = a.max_rank <= 16 ? 1 : a.max_rank <= 32 ? 2 : 4;
-    // a workgroup for every run that a tile could have, while that fills the device twice at most; one run after the other is as long again
+    // A workgroup for every run that a tile could have, while that fills the device twice at most: one after the other they add up (64 tokens of 24
+    // adapters: 139 us by one workgroup a tile, 31 by 8, 21 by 26). In prompts 3, more are mostly idle.
     a.slots = (int)std::max<int64_t>(1, std::min<int64_t>(prompts ? std::min(a.most, 3) : a.most, 2 * num_cu / tiles));
-    // columns over as many workgroups as that leaves room for, a step of each wavefront, or of the workgroup, at the least
+    // Columns over as many workgroups as that leaves room for, a step of each wavefront, or of the workgroup, at the least; 8 parts at most, since the
+    // second launch sums them (64 tokens: 4 parts 22.5 us, 8 21.1, 16 21.1).
     const int64_t unit = a.whole ? 64 : 256, units = (a.cols + unit - 1) / unit;
     const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
-    // outputs over so many workgroups that the device is filled, a turn of 64 at the least
+    // Outputs over so many workgroups that the device is filled, a turn of 64 at the least; long ones where a prompt's rows fill it (8192 tokens: 2 a
+    // compute unit 189 us, 3 196, 4 215, 1 290).
     const int64_t steps = (a.rows + 63) / 64, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, (a.whole ? 2 : 4) * num_cu / (tiles * (prompts ? 1 : a.slots))));
     a.ucols = (int)((steps + chunks - 1) / chunks * 64);
     return (size_t)tiles * a.most * sizeof(LoraRun) + (size_t)a.ks * a.n_tok * ((a.max_rank + 15) & ~15) * 4;
