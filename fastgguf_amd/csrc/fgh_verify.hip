@@ -6,6 +6,10 @@
 // comparisons are in 64 bits. A row is read once: each workgroup leaves the largest value of its words, its
 // place and the sum of exp((x - largest) / T); whole rows, and the sums that a number has to be compared with, are joined
 // from those.
+//
+// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 51 us: the rows 27 (20 for reading alone, 25 for the
+// exponentials alone, in one kernel they overlap), the rejected rows' sums 16, the choice 10.5. Few rows are a matter of launches that wait for each
+// other and, in the choice, of five loads that do: 12 us for one token of one row.
 #include "fgh_serve.h"
 
 #include <limits.h>
@@ -121,6 +125,8 @@ __device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
     return p;
 }
 
+// Each row's largest value and sum, a workgroup to a part of its words, 4 NV words a thread at a time, all of whose loads are under way at
+// once. Bound by 64-bit instructions: 13 a word, 75 to 85 % of the cycles.
 template <int NV>
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ Part lds[4];
@@ -392,6 +398,9 @@ __device__ int draw(const VerifyArgs &a, const Weigh &w, int subs, int words, do
     return pick<MODE>(w, from, min(from + words, min((split + 1) * a.per, a.vocab)), aim - before);
 }
 
+// The decision where drafts have no probabilities, and the draw: the part of the words that v falls on by the parts' sums, a thread's words
+// in it by a scan over the workgroup, the word by one over a wavefront. One workgroup a sequence: 8 to 13 us whatever the vocabulary, waits for loads
+// that depend on each other. (Keeping the parts' sums and the thread's words from step to step saved nothing that could be measured.)
 __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     bool greedy;
@@ -433,6 +442,10 @@ __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
 size_t subs_of(const VerifyArgs &a) { return (a.per + SUB - 1) / SUB; }
 }  // namespace
 
+// Blocks of 4096 words, smaller while the device would not be filled (64 rows of 32768 words: 4096 5.5 us, 2048 4.8, 1024 7.0); parts of two
+// blocks where rows are many, which leaves fewer sums to write and join (189 rows of 128256: 31.1 us with one, 27.8 with two, and the rejected rows'
+// sums 17.8 and 16.3; 106 of 50021, below the limit: 11.0 and 9.5, but 13.0 and 15.2 for the choice, which goes through a part word by word); two
+// parts a workgroup where those are still many (27.8 and 27.1; with 800 workgroups left: 11.4 and 12.2).
 size_t verify_plan(VerifyArgs &a, int num_cu) {
     auto parts = [&](int nv) { return (a.vocab + 1024 * nv - 1) / (1024 * nv); };
     a.nv = 4;

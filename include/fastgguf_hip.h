@@ -420,9 +420,9 @@ FGH_API int fgh_draft_verify_dev(fgh_ctx *ctx, const fgh_drafts *drafts, int32_t
  * adapter id[s] of n_adapter: A [max_rank][cols] and B [rows][max_rank], of which the first rank[id] (0 .. max_rank; NULL: max_rank) count;
  * scale [n_adapter] (NULL: 1). id -1: y = y_in; any other id or rank: NaN rows. y_in NULL: 0. y_in may be y (ldyi == ldy); else
  * y overlaps no input. Rows before tok[0] and from tok[n_seq] on are left as they were. Results are those of fp32 sums,
- * whatever the type. Rows of one adapter that stand together share its reads: order sequences by adapter. x that is not
- * finite, or above 2^127, makes its row anything. n_seq up to 65535.
- * cols and max_rank multiples of 8 (max_rank up to 512), a and b 16-byte aligned, the others 4-byte; any strides. */
+ * whatever the type. Rows of one adapter among 64 neighbouring ones share its reads: order sequences by adapter. x that is not
+ * finite makes its own row anything, and no other. n_seq up to 65535.
+ * cols and max_rank multiples of 8 (cols up to 2^20, max_rank up to 512), a and b 16-byte aligned, the others 4-byte; any strides up to 2^24. */
 typedef struct {
     const void *a, *b;                  /* device, [n_adapter][max_rank][cols] and [n_adapter][rows][max_rank] */
     const int32_t *rank;                /* device, [n_adapter], or NULL */
