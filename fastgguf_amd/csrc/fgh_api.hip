@@ -1147,7 +1147,7 @@ static const char *lora_check(const fgh_lora *l, const int32_t *tok, const int32
     if (l->type != FGH_T_F32 && l->type != FGH_T_F16 && l->type != FGH_T_BF16) return "the adapters' type is not F32, F16 or BF16";
     if (l->cols < 8 || l->cols % 8 != 0 || l->cols > 1 << 20 || l->rows < 1 || l->rows > 1 << 24) return "cols is no multiple of 8, or cols or rows is out of range";
     if (l->max_rank < 8 || l->max_rank % 8 != 0 || l->max_rank > 512) return "max_rank is no multiple of 8 up to 512";
-    if (l->n_adapter < 1) return "bad n_adapter";
+    if (l->n_adapter < 1 || l->n_adapter > 1 << 30) return "bad n_adapter";
     if (n_seq < 1 || n_seq > 65535 || n_tok < 1 || n_tok > 1 << 30) return "bad n_seq or n_tok";
     const int64_t most = 1 << 24;  // offsets of a tile's rows in 32 bits
     if (ldx < l->cols || ldy < l->rows || (yin && ldyi < l->rows) || ldx > most || ldy > most || (yin && ldyi > most)) return "ldx, ldyi or ldy is smaller than a row or too large";

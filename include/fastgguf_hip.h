@@ -369,14 +369,14 @@ FGH_API int fgh_paged_attention_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, 
 /* The pages of a batch. Sequence s holds held[s] pages, the first entries of its table row; keep[s] of its positions stay
  * (fewer than before where drafts were rejected, 0 where it has ended), add[s] new tokens want to follow. The free pages are
  * a ring of n_pages entries: `free` holds the place of the first and their number. The call
- *   gives back the pages behind the positions that a sequence then has, to the ring's end, in the sequences' order;
+ *   gives back the pages behind a sequence's keep + add positions, to the ring's end, in the sequences' order;
  *   takes the pages that are missing from its front, in the sequences' order (pages that the same call gives back are its last);
  *   writes the cache's table, the batch's tok and len (the descriptors' memory: the inputs of the two calls above), held_out and
  *   free_out, and of every row its sequence, its position and its slot, page * cache->page + place in the page
  *   (seq, pos, slot: [n_tok], each may be NULL; -1 in rows of no sequence, slot -1 where the page is not 0 .. n_pages - 1).
- * A sequence gets no new tokens (an empty range, len = keep) where add is not 0 .. max_tok, keep + add passes max_len or the table,
- * or, with the sequences before it, the ring's pages or n_tok rows do not suffice: sequences are served in order, and one
- * that needs no page does not wait for pages. It gives back pages behind keep all the same. One with a keep below 0 or above its
+ * A sequence gets no new tokens (an empty range, len = keep) where add is not 0 .. max_tok or keep + add passes max_len or the table
+ * (add then counts as 0), or where, with the sequences before it, the ring's pages or n_tok rows do not suffice: sequences are
+ * served in order, and one that needs no page does not wait for pages. What it gives back it does all the same. One with a keep below 0 or above its
  * pages, or a held that is not 0 .. table_stride, gets no tokens and len 0, and its pages stay. A `free` that is no such pair is an
  * empty ring; a ring whose pages would be more than n_pages takes no more. Of the cache only table, n_pages, page and
  * table_stride are used. keep may be len, held held_out and free free_out: nothing else may overlap. */
@@ -392,7 +392,7 @@ typedef struct {
 FGH_API int fgh_paged_reserve_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, const fgh_paged_batch *batch,
                           const fgh_paged_pool *pool);
 /* Drafted tokens against the target's probabilities. Sequence s has rows tok[s] .. tok[s + 1] - 1 (n of them, at most max_tok);
- * tokens[t] is what row t was computed from, so row i's logits judge token i + 1: the first row's token is known, the
+ * tokens[t] is what row t was computed from, so row i's logits are those of token i + 1: the first row's token is known, the
  * n - 1 others are drafts. With p = softmax(logits / temp[s]) of a row, draft d stays while u[row] q(d) < p(d); n_ok[s] is how many do.
  * next[s] follows them: at the first rejected draft, the first word whose running sum of max(p - q, 0) passes v[s] times the
  * whole (p itself where nothing is left, or the draft is no word); behind the last row, the same of p. So next is distributed as

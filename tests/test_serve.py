@@ -80,7 +80,7 @@ def test_lora_largest():
     """A tile's offsets in 32 bits."""
     most = dict(cols=1 << 20, ldx=1 << 24, ldy=1 << 24, ldyi=1 << 24)
     assert lora_check(**most) == ""
-    for kw in (dict(cols=(1 << 20) + 8), dict(ldx=(1 << 24) + 1), dict(ldy=(1 << 24) + 1), dict(ldyi=(1 << 24) + 1)):
+    for kw in (dict(n_adapter=(1 << 30) + 1), dict(cols=(1 << 20) + 8), dict(ldx=(1 << 24) + 1), dict(ldy=(1 << 24) + 1), dict(ldyi=(1 << 24) + 1)):
         assert lora_check(**{**most, **kw}) != ""
 
 
