@@ -340,19 +340,24 @@ __global__ __launch_bounds__(WG) void verify_rest_kernel(VerifyArgs a) {
 // the first of words from .. to - 1 whose running sum passes `aim`, or the last of any weight (-1: none has)
 template <int MODE>
 __device__ int pick(const Weigh &w, int from, int to, double aim) {
-    __shared__ int first, last;
+    __shared__ int firsts[WG / 64], lasts[WG / 64];
     __shared__ double sum;
     const int per = ((to - from + WG - 1) / WG + 3) & ~3, b = min(to, from + (int)threadIdx.x * per), e = min(to, b + per), lane = threadIdx.x & 63;
     double own = 0.0;
     each4<MODE>(w, b, e, [&](int, const double (&x)[4]) { own += (x[0] + x[1]) + (x[2] + x[3]); });
-    if (threadIdx.x == 0) first = WG, last = -1;
     double run = upto_lane(own);
-    run += scan_waves(lane_of(run, 63)).x;  // its barriers stand before what follows
-    if (own > 0.0) {
-        atomicMax(&last, (int)threadIdx.x);
-        if (run > aim) atomicMin(&first, (int)threadIdx.x);
+    run += scan_waves(lane_of(run, 63)).x;
+    // the first thread that passes, or the last of any weight (by atomics in LDS, one lane after the other, this took 5 us)
+    const uint64_t any = __builtin_amdgcn_ballot_w64(own > 0.0), over = __builtin_amdgcn_ballot_w64(own > 0.0 && run > aim);
+    if (lane == 0) {
+        const int t = (int)threadIdx.x;
+        firsts[t >> 6] = over ? t + __builtin_ctzll(over) : WG;
+        lasts[t >> 6] = any ? t + 63 - __builtin_clzll(any) : -1;
     }
     __syncthreads();
+    int first = WG, last = -1;
+#pragma unroll
+    for (int i = 0; i < WG / 64; ++i) first = min(first, firsts[i]), last = max(last, lasts[i]);
     const int mine = first < WG ? first : last;
     if (mine < 0) return -1;
     if ((int)threadIdx.x == mine) sum = run - own;
