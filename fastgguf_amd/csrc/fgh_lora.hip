@@ -9,6 +9,7 @@
 // Bound by memory where rows are many: 8192 tokens, 4096 -> 14336, rank 64, F16: 238 us for 1.08 GB, 4.5 TB/s; y alone at 5.0. By loads that wait for
 // each other where they are few: 64 tokens with 24 adapters 21 us (38 MB), one token 9.
 #include <algorithm>
+#include <type_traits>
 
 #include "fgh_pattn.h"
 #include "fgh_serve.h"
@@ -138,6 +139,7 @@ struct Stage {
         for (int e = 0; e < NW; ++e) w[e] = lds[((SB * j + k) * NW + e) * 64 + slot(lane & 15, lane >> 4, k)];
     }
 };
+constexpr int MOST_PARTS = 8;  // of h
 constexpr int LD = 68;  // floats between rows of 64 in LDS: 16 rows start in 16 different groups of banks
 
 // h of few rows that have an adapter in common (64 tokens of 24 adapters, BF16, rank 64: 8.7 us, of which 5 are the way to the first load; one token:
@@ -449,19 +451,28 @@ __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS ? 3 : 4) void lora_up_kerne
             // h, summed over the parts by neighbouring threads for the workgroup, through the LDS of the results
             pu4 x[KH][3];
             if constexpr (KB > 0) {
-                constexpr int Q = 8 * SB;  // threads to a row
+                constexpr int Q = 8 * SB, ALL = (ROWS ? 64 : 16) * Q;  // threads to a row, and to all
+                auto sum = [&](int kb, auto parts) {  // every load is under way before the first is waited for
+                    constexpr int N = decltype(parts)::value;
+#pragma unroll
+                    for (int i0 = 0; i0 < ALL; i0 += 256) {
+                        const int i = i0 + tid, row = min(i / Q, (ROWS ? 64 : 16) - 1), r = 32 * SB * kb + 4 * (i % Q);
+                        // eights of ranks: what is behind the last one is finite if that is; behind them, and behind the rows, others, which are not used
+                        const float *p = a.part + (int64_t)(base + list[min(t0 + row, n - 1)]) * padded + ((r & ~7) < run.rank ? r : 0);
+                        pf4 v[N];
+#pragma unroll
+                        for (int s = 0; s < N; ++s) v[s] = *(const pf4 *)(p + (int64_t)min(s, a.ks - 1) * a.n_tok * padded);
+#pragma unroll
+                        for (int s = 1; s < N; ++s)
+                            if (s < a.ks) v[0] += v[s];
+                        if (ALL >= 256 || i < ALL) *(pf4 *)(&tiles[0][0] + row * LD + 4 * (i % Q)) = v[0];
+                    }
+                };
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     if (kb) lds_barrier();
-                    for (int i = tid; i < (ROWS ? 64 : 16) * Q; i += 256) {
-                        const int row = i / Q, r = 32 * SB * kb + 4 * (i % Q);
-                        if (t0 + row >= n || (r & ~7) >= run.rank) continue;  // eights of ranks: what is behind the last one is finite if that is
-                        const float *p = a.part + (int64_t)(base + list[t0 + row]) * padded + r;
-                        pf4 h = *(const pf4 *)p;
-#pragma unroll 4
-                        for (int s = 1; s < a.ks; ++s) h += *(const pf4 *)(p + (int64_t)s * a.n_tok * padded);
-                        *(pf4 *)(&tiles[0][0] + row * LD + 4 * (i % Q)) = h;
-                    }
+                    if (a.ks > 4) sum(kb, std::integral_constant<int, MOST_PARTS>{});
+                    else sum(kb, std::integral_constant<int, 4>{});
                     lds_barrier();
 #pragma unroll
                     for (int k = 0; k < SB; ++k) {
@@ -599,7 +610,7 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     // Columns over as many workgroups as that leaves room for, a step of each wavefront, or of the workgroup, at the least; 8 parts at most, since the
     // second launch sums them (64 tokens: 4 parts 22.5 us, 8 21.1, 16 21.1).
     const int64_t unit = a.whole ? 64 : 256, units = (a.cols + unit - 1) / unit;
-    const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, 8, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
+    const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, MOST_PARTS, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
     // Outputs over so many workgroups that the device is filled, a turn of 64 at the least; long ones where a prompt's rows fill it (8192 tokens: 2 a

@@ -54,35 +54,36 @@ __device__ __forceinline__ Ask ask_of(const ReserveArgs &a, int s) {
 // Sums of numbers that are not negative, kept at 2^32 - 1 where they would pass it: one instruction, in any order the same. What is
 // compared with them is below that.
 __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
-// over a wavefront: the sum with the lanes before
+// over each row of 16 lanes: the sum with the lanes before
+__device__ __forceinline__ uint32_t scan_row(uint32_t v) {
+    v = add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true));  // row_shr 1, 2, 4, 8; 0 from before the row
+    v = add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true));
+    v = add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true));
+    return add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true));
+}
+// the same over a wavefront
 __device__ __forceinline__ uint32_t scan_wave(uint32_t v) {
     const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {  // in rows of 16 lanes, by DPP: row_shr o, 0 from before the row
-        const uint32_t z = o == 1 ? __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true)
-                         : o == 2 ? __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true)
-                         : o == 4 ? __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true)
-                                  : __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
-        v = add(v, z);
-    }
+    v = scan_row(v);
     const uint32_t a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31), c = __builtin_amdgcn_readlane(v, 47);
     const uint32_t ab = add(a, b), abc = add(ab, c);
     return add(v, lane < 16 ? 0u : lane < 32 ? a : lane < 48 ? ab : abc);
 }
-// N sums over the workgroup's wavefronts before this one (v: a wavefront's, the same in its lanes), and of all in `all`
+// N sums over the workgroup's wavefronts before this one (v: a wavefront's, the same in its lanes), and of all in `all`: a row of lanes to each
 template <int THREADS, int N>
 __device__ __forceinline__ void scan_waves(uint32_t (&v)[N], uint32_t (&all)[N], uint32_t (*lds)[16]) {
     constexpr int W = THREADS / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < N; ++i)
         if (lane == 0) lds[i][wave] = v[i];
     __syncthreads();
+    static_assert(N <= 4 && W <= 16);
+    const uint32_t w = scan_row(lane >> 4 < N && (lane & 15) < W ? lds[lane >> 4][lane & 15] : 0u);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const uint32_t w = scan_wave(lane < W ? lds[i][lane] : 0u);
-        all[i] = __builtin_amdgcn_readlane(w, W - 1);
-        v[i] = wave ? (uint32_t)__shfl((int)w, wave - 1, 64) : 0u;
+        all[i] = __builtin_amdgcn_readlane(w, 16 * i + W - 1);
+        v[i] = wave ? (uint32_t)__builtin_amdgcn_readlane(w, 16 * i + wave - 1) : 0u;
     }
     __syncthreads();
 }
@@ -204,17 +205,18 @@ __device__ __forceinline__ void map_row(const ReserveArgs &a, const Sums &z, con
     if (a.pos) a.pos[r] = pos;
     if (a.slot) a.slot[r] = slot;
 }
-// The pages that change hands, and the rows' maps, by one workgroup with the sums in LDS: each finds its sequence by halves.
+// The pages that change hands, and the rows' maps, with the sums in LDS: each finds its sequence by halves. Where they are few each of the three has
+// wavefronts of its own.
 __device__ __forceinline__ void reserve_fill(const ReserveArgs &a, const Sums &z, int thread, int threads) {
     const int n = a.n_seq, gives = min(z.give[n], a.n_pages), takes = z.take[n], total = z.row[n];
     const Pages p(a, z);
     for (int k = thread; k < gives; k += threads) p.give(k, p.given(k));
-    for (int k = thread; k < takes; k += threads) {
+    for (int k = (thread + 64) % threads; k < takes; k += threads) {
         const int s = find(z.take, n, k);
         a.table[(int64_t)s * a.table_stride + z.held[s] + (k - z.take[s])] = p.taken(k);
     }
     if (a.seq || a.pos || a.slot)
-        for (int r = thread; r < a.n_tok; r += threads) map_row(a, z, p, r, r < total ? find(z.row, n, r) : -1);
+        for (int r = (thread + 128) % threads; r < a.n_tok; r += threads) map_row(a, z, p, r, r < total ? find(z.row, n, r) : -1);
 }
 
 // All of it in one launch, the sums in LDS: each workgroup makes them for itself, the first one writes what is not pages or rows (kernel alone: 4.9 us
