@@ -198,6 +198,7 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     }
 }
 
+constexpr int MOST_SPLITS = 64;  // parts of a row: a wavefront joins them
 constexpr int WG = 512;  // threads that decide: 8 rows at a time
 
 // the sequence's rows: none for what a batch cannot mean
@@ -310,7 +311,8 @@ __device__ __forceinline__ double2 scan_waves(double v) {
     }
     return double2{before, all};
 }
-constexpr int SUB = 4 * WG;  // words that the workgroup takes at a time
+constexpr int SUB = 4 * WG;                                // words that the workgroup takes at a time
+constexpr int MOST_SUBS = (1 << 24) / (MOST_SPLITS * SUB);  // of a part
 template <int MODE>
 __device__ __forceinline__ double sum_words(const Weigh &w, int from, int to) {
     double v = 0.0;
@@ -329,11 +331,39 @@ __global__ __launch_bounds__(WG) void verify_rest_kernel(VerifyArgs a) {
     if (split == 0 && threadIdx.x == 0) a.choice[s] = ch;
     if (greedy || !(c == c) || ch.d < 0) return;
     const Weigh w = weigh_of(a, ch, c);
-    const int to = min(a.vocab, (split + 1) * a.per);
-    for (int i = 0; i < subs; ++i) {
-        const int from = split * a.per + i * SUB;
-        const double v = sum_words<FROM_REST>(w, from, min(from + SUB, to));
-        if (threadIdx.x == 0) a.rest[((int64_t)s * a.splits + split) * subs + i] = v;
+    __shared__ double sums[MOST_SUBS][WG / 64];
+    const int first = split * a.per, to = min(a.vocab, first + a.per), wave = threadIdx.x >> 6;
+    auto load = [&](int i, vf4 &x, vf4 &q) {  // words behind the last: the last again, no weight
+        const int j = first + i * SUB + 4 * (int)threadIdx.x;
+        if (a.vocab >= 4) {
+            const uint32_t o = 4 * (uint32_t)min(j, a.vocab - 4);
+            x = *(const vf4 *)((const uint8_t *)w.x + o), q = *(const vf4 *)((const uint8_t *)w.q + o);
+        } else
+            for (int e = 0; e < a.vocab; ++e) x[e] = w.x[e], q[e] = w.q[e];
+    };
+    vf4 x{}, q{}, xn{}, qn{};
+    load(0, x, q);
+    for (int i = 0; i < subs; ++i) {  // the next words on their way, no wavefront waits for another
+        if (i + 1 < subs) load(i + 1, xn, qn);
+        const int j = first + i * SUB + 4 * (int)threadIdx.x, over = a.vocab >= 4 ? max(0, j - (a.vocab - 4)) : 0;
+        double v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = weight<FROM_REST>(w, j, x[e], q[e]);
+        if (first + (i + 1) * SUB > to) {  // a row's last words: of four, those from j on
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < over || j - over + e >= to) v[e] = 0.0;
+        }
+        const double sum = total((v[0] + v[1]) + (v[2] + v[3]));
+        if ((threadIdx.x & 63) == 0) sums[i][wave] = sum;
+        x = xn, q = qn;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < subs; i += WG) {
+        double v = 0.0;
+#pragma unroll
+        for (int k = 0; k < WG / 64; ++k) v += sums[i][k];
+        a.rest[((int64_t)s * a.splits + split) * subs + i] = v;
     }
 }
 
@@ -456,7 +486,7 @@ size_t verify_plan(VerifyArgs &a, int num_cu) {
     a.nv = 4;
     while (a.nv > 1 && (int64_t)a.n_tok * parts(a.nv) < 4 * num_cu) a.nv /= 2;
     const int blocks = parts(a.nv), two = (int64_t)a.n_tok * blocks >= 8 * num_cu ? 2 : 1;
-    a.splits = std::min(64, (blocks + two - 1) / two);  // a wavefront joins them
+    a.splits = std::min(MOST_SPLITS, (blocks + two - 1) / two);
     a.per = (blocks + a.splits - 1) / a.splits * 1024 * a.nv;
     a.splits = (a.vocab + a.per - 1) / a.per;
     a.group = (int64_t)a.n_tok * a.splits >= 8 * num_cu ? 2 : 1;
