@@ -143,9 +143,9 @@ constexpr int MOST_PARTS = 8;  // of h
 constexpr int LD = 68;  // floats between rows of 64 in LDS: 16 rows start in 16 different groups of banks
 
 // h of few rows that have an adapter in common (64 tokens of 24 adapters, BF16, rank 64: 8.7 us, of which 5 are the way to the first load; one token:
-// 5.0), 16 NR ranks, over a part of the columns: the wavefronts take steps of 64 columns in turn, the
-// next one's values on their way during the products of one. A's values and x's go through a wavefront's own LDS, so that neighbouring lanes
-// read neighbouring values: as the products take them, 16 rows an access, the first cache gave one lane a cycle.
+// 5.0), 16 NR ranks, over a part of the columns: the wavefronts take steps of 64 columns in turn, the next one's values on their way during the
+// products of one. A's values and x's go through a wavefront's own LDS, so that neighbouring lanes read neighbouring values: as the products take
+// them, 16 rows an access, the first cache gave one lane a cycle.
 template <int TYPE, int NR>
 __global__ __launch_bounds__(256) void lora_down_split_kernel(LoraArgs a) {
     constexpr int ES = Weights<TYPE>::ES, NW = Weights<TYPE>::NW;
@@ -243,8 +243,9 @@ __global__ __launch_bounds__(256) void lora_down_split_kernel(LoraArgs a) {
     }
 }
 
-// h of a prompt's rows (8192 tokens of 4096 columns, F16, rank 64: 53 us, 2.5 TB/s of x), 16 NR ranks, over a part of the columns: 64 rows to a workgroup, 16 to a wavefront, 64 columns at a time, the next ones'
-// values on their way during the products of some. x too goes through LDS, each wavefront's by itself: 16 lanes read 256 bytes of a row.
+// h of a prompt's rows (8192 tokens of 4096 columns, F16, rank 64: 52 us, 2.6 TB/s of x), 16 NR ranks, over a part of the columns: 64 rows to a
+// workgroup, 16 to a wavefront, 64 columns at a time, the next ones' values on their way during the products of some. x too goes through LDS, each
+// wavefront's by itself: 16 lanes read 256 bytes of a row.
 template <int TYPE, int NR>
 __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     using S = Stage<TYPE, 2>;
@@ -363,11 +364,12 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
     }
 }
 
-// y of rows that have an adapter in common (8192 tokens of 14336 outputs: 187 us, 5.0 TB/s; 64 tokens of 24 adapters: 12.5), ucols of the outputs, 64 at a time and 32 SB ranks of them, the next ones' values on their way
-// during the products of some. ROWS (prompts): each wavefront has 16 rows and all 64 outputs; else (few rows) 16 of the outputs and the
-// same rows. Products: lane l has output l % 16 of a tile and row l % 16, ranks 8 (l / 16) .. + 7, and gets outputs 4 (l / 16) .. + 3 of its row;
-// through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: such blocks of ranks, whose h stays in registers; 0: any number,
-// which does not. ROWS: three workgroups a compute unit, since at four registers spill (2500 tokens, F32: 46.8 us, without 35.7).
+// y of rows that have an adapter in common (8192 tokens of 14336 outputs: 187 us, 5.0 TB/s; 64 tokens of 24 adapters: 12.5), ucols of the outputs, 64
+// at a time and 32 SB ranks of them, the next ones' values on their way during the products of some. ROWS (prompts): each wavefront has 16 rows and
+// all 64 outputs; else (few rows) 16 of the outputs and the same rows. Products: lane l has output l % 16 of a tile and row l % 16, ranks 8 (l / 16)
+// .. + 7, and gets outputs 4 (l / 16) .. + 3 of its row; through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: such blocks of
+// ranks, whose h stays in registers; 0: any number, which does not. ROWS: three workgroups a compute unit, since at four registers spill (2500
+// tokens, F32: 46.8 us, without 35.7).
 template <int TYPE, int SB, int KB, bool ROWS>
 __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS ? 3 : 4) void lora_up_kernel(LoraArgs a) {
     using S = Stage<TYPE, SB>;

@@ -6,7 +6,7 @@
 // pages given and rows asked for, a second one of the rows granted.
 //
 // A step's bytes are few (32 sequences: 1 KB; 4100 of them with 96000 pages and 60000 rows: 2 MB): what it takes is launches and loads that wait for
-// each other, 5 to 7 us in one launch, 14 in two.
+// each other, 4 to 6 us in one launch, 14 in two.
 #include "fgh_serve.h"
 
 #include <algorithm>
@@ -219,8 +219,8 @@ __device__ __forceinline__ void reserve_fill(const ReserveArgs &a, const Sums &z
         for (int r = (thread + 128) % threads; r < a.n_tok; r += threads) map_row(a, z, p, r, r < total ? find(z.row, n, r) : -1);
 }
 
-// All of it in one launch, the sums in LDS: each workgroup makes them for itself, the first one writes what is not pages or rows (kernel alone: 4.9 us
-// for 32 sequences, 6.3 for 250 with 11000 rows in 11 workgroups, 5.6 for prompts of 20000 rows in 20)
+// All of it in one launch, the sums in LDS: each workgroup makes them for itself, the first one writes what is not pages or rows (kernel alone: 3.8 us
+// for 32 sequences, 6.0 for 250 with 11000 rows in 11 workgroups, 5.1 for prompts of 20000 rows in 20)
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveArgs a) {
     extern __shared__ int32_t sums[];

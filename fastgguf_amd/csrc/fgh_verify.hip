@@ -7,9 +7,9 @@
 // place and the sum of exp((x - largest) / T); whole rows, and the sums that a number has to be compared with, are joined
 // from those.
 //
-// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 51 us: the rows 27 (20 for reading alone, 25 for the
-// exponentials alone, in one kernel they overlap), the rejected rows' sums 16, the choice 10.5. Few rows are a matter of launches that wait for each
-// other and, in the choice, of five loads that do: 12 us for one token of one row.
+// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 46 us: the rows 27 (20 for reading alone, 25 for the
+// exponentials alone, in one kernel they overlap), the rejected rows' sums 15, the choice 7. Few rows are a matter of launches that wait for each
+// other and, in the choice, of five loads that do: 8.2 us for one token of one row.
 #include "fgh_serve.h"
 
 #include <limits.h>
@@ -126,7 +126,8 @@ __device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
 }
 
 // Each row's largest value and sum, a workgroup to a part of its words, 4 NV words a thread at a time, all of whose loads are under way at
-// once. Bound by 64-bit instructions: 13 a word, 75 to 85 % of the cycles.
+// once. Bound by vector instructions, 76 % of the cycles: 17 a word, of which 13 are of 64 bits, and a third as many again around them. (The next
+// block's loads a block ahead, at 86 registers instead of 63, gained nothing.)
 template <int NV>
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
     __shared__ Part lds[4];
@@ -434,8 +435,8 @@ __device__ int draw(const VerifyArgs &a, const Weigh &w, int subs, int words, do
 }
 
 // The decision where drafts have no probabilities, and the draw: the part of the words that v falls on by the parts' sums, a thread's words
-// in it by a scan over the workgroup, the word by one over a wavefront. One workgroup a sequence: 8 to 13 us whatever the vocabulary, waits for loads
-// that depend on each other. (Keeping the parts' sums and the thread's words from step to step saved nothing that could be measured.)
+// in it by a scan over the workgroup, the word by one over a wavefront. One workgroup a sequence: 5 to 9 us whatever the vocabulary, waits for loads
+// that depend on each other. (Keeping the parts' sums from step to step saved nothing that could be measured.)
 __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     bool greedy;

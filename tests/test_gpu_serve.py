@@ -322,6 +322,13 @@ def test_verify_many_rows(backend, drafter):
     assert 0 < n_ok.sum() < c.n_tok - c.n
 
 
+@pytest.mark.parametrize("drafter", [False, True])
+def test_verify_widest(backend, drafter):
+    """2^24 words, the most that a row may have: parts of 262144."""
+    c = Case(114, [2], 1 << 24, drafter, temps=(30.0,))
+    c.run(backend)
+
+
 def test_verify_long_rows(backend):
     """A vocabulary whose parts take several blocks of a workgroup."""
     c = Case(20, [2], 1000003, True)
