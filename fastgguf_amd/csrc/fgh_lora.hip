@@ -32,7 +32,7 @@ __device__ __forceinline__ int adapters_of(const LoraArgs &a, int base, int *mar
         const int s = min(b + lane, a.n_seq - 1), id = a.id[s];
         const int from = max(a.tok[s], base), to = min(a.tok[s + 1], top);
         if (b + lane < a.n_seq && from < to) mark[from - base] = id == -1 ? NONE : (uint32_t)id < (uint32_t)a.n_adapter ? FIRST + id : BAD;
-        if (__builtin_amdgcn_ballot_w64(b + lane >= a.n_seq || to >= end)) break;
+        if (__builtin_amdgcn_ballot_w64(b + lane >= a.n_seq || to >= end || base >= end)) break;
     }
     __builtin_amdgcn_wave_barrier();
     const int m = mark[lane];

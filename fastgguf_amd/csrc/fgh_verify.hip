@@ -152,9 +152,9 @@ __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
                 if (j + e >= a.vocab) v[i][e] = -__builtin_inff();
         }
     };
-    load(split0 * a.per);  // on its way while the row's sequence is found
     const int s = seq_of_row(a.tok, a.n_seq, row);
     if (s < 0) return;
+    load(split0 * a.per);  // rows of no sequence, of which a recorded call may have many, are not read (asked for before the search: 0.3 to 1.4 us more)
     bool greedy;
     const double c = heat_of(a, s, greedy), least_d = -1000.0 / c;
     for (int split = split0; split < min(a.splits, split0 + a.group); ++split) {
