@@ -615,8 +615,8 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     const int64_t ks = std::max<int64_t>(1, std::min<int64_t>({units, MOST_PARTS, 2 * num_cu / (tiles * (prompts ? 1 : a.slots) * rank_blocks(a))}));
     a.kper = (int)((units + ks - 1) / ks * unit);
     a.ks = (a.cols + a.kper - 1) / a.kper;
-    // Outputs over so many workgroups that the device is filled, a turn of 64 at the least; long ones where a prompt's rows fill it (8192 tokens: 2 a
-    // compute unit 189 us, 3 196, 4 215, 1 290).
+    // Outputs over so many workgroups that the device is filled, a turn of 64 at the least: 4 a compute unit (64 tokens: 12.7 us; 2 14.0, 3 13.8, 6 15.1,
+    // 8 15.8), 2 where a prompt's rows fill it (8192 tokens: 189 us; 1 290, 3 196, 4 215).
     const int64_t steps = (a.rows + 63) / 64, chunks = std::max<int64_t>(1, std::min<int64_t>(steps, (a.whole ? 2 : 4) * num_cu / (tiles * (prompts ? 1 : a.slots))));
     a.ucols = (int)((steps + chunks - 1) / chunks * 64);
     return (size_t)tiles * a.most * sizeof(LoraRun) + (size_t)a.ks * a.n_tok * ((a.max_rank + 15) & ~15) * 4;
