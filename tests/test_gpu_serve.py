@@ -323,6 +323,12 @@ def test_verify_many_rows(backend, drafter):
 
 
 @pytest.mark.parametrize("drafter", [False, True])
+def test_verify_padded(backend, drafter):
+    """Many rows of no sequence before the first and behind the last."""
+    Case(115, [3, 1, 4], 5000, drafter, (130, 600)).run(backend)
+
+
+@pytest.mark.parametrize("drafter", [False, True])
 def test_verify_widest(backend, drafter):
     """2^24 words, the most that a row may have: parts of 262144."""
     c = Case(114, [2], 1 << 24, drafter, temps=(30.0,))
@@ -669,6 +675,12 @@ def test_lora_many_sequences(backend):
     news[[0, 70, 71, 4000, 65534]] = 1, 2, 1, 3, 1
     ids = [s % 3 for s in range(65535)]
     check_lora(backend, *lora_case(66, T_BF16, 3, 8, 64, 30, news, ids, None, (1, 1)))
+
+
+@pytest.mark.parametrize("news, pad", [([1] * 300, (0, 800)), ([1] * 20, (70, 300)), ([400, 3], (0, 1500)), ([5], (1100, 40))])
+def test_lora_padded(backend, news, pad):
+    """Whole tiles before the first row and behind the last are left as they were."""
+    check_lora(backend, *lora_case(78, T_BF16, 3, 24, 72, 70, news, [s % 4 - 1 for s in range(len(news))], None, pad), form="apart")
 
 
 def test_lora_far_adapters(backend):
