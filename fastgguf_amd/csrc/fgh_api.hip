@@ -1125,8 +1125,9 @@ static bool off4(std::initializer_list<const void *> p) {
 static const char *reserve_check(const fgh_paged_cache *c, const fgh_paged_batch *b, const fgh_paged_pool *p) {
     if (!c || !b || !p) return "null descriptor";
     if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return "page is not a power of 2 from 16 to 256";
-    if (c->n_pages < 1 || c->table_stride < 1) return "bad n_pages or table_stride";
-    if (b->n_seq < 1 || b->n_seq > 65535 || b->n_tok < 1 || b->max_tok < 1 || b->max_len < 1) return "bad n_seq, n_tok, max_tok or max_len";
+    // rows and pages are gone through in 32 bits, by steps of up to 131072 past the last one
+    if (c->n_pages < 1 || c->n_pages > 1 << 30 || c->table_stride < 1) return "bad n_pages or table_stride";
+    if (b->n_seq < 1 || b->n_seq > 65535 || b->n_tok < 1 || b->n_tok > 1 << 30 || b->max_tok < 1 || b->max_len < 1) return "bad n_seq, n_tok, max_tok or max_len";
     if (!c->table || !b->tok || !b->len || !p->keep || !p->add || !p->held || !p->held_out || !p->queue || !p->free || !p->free_out) return "null pointer";
     if (off4({c->table, b->tok, b->len, p->keep, p->add, p->held, p->held_out, p->queue, p->free, p->free_out, p->seq, p->pos}) || (uintptr_t)p->slot % 8 != 0)
         return "pointers must be 4-byte aligned, slot 8";

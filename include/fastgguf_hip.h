@@ -379,7 +379,7 @@ FGH_API int fgh_paged_attention_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, 
  * served in order, and one that needs no page does not wait for pages. What it gives back it does all the same. One with a keep below 0 or above its
  * pages, or a held that is not 0 .. table_stride, gets no tokens and len 0, and its pages stay. A `free` that is no such pair is an
  * empty ring; a ring whose pages would be more than n_pages takes no more. Of the cache only table, n_pages, page and
- * table_stride are used. keep may be len, held held_out and free free_out: nothing else may overlap. */
+ * table_stride are used; n_pages and n_tok up to 2^30. keep may be len, held held_out and free free_out: nothing else may overlap. */
 typedef struct {
     const int32_t *keep, *add, *held;   /* device, [n_seq] */
     int32_t *held_out;                  /* device, [n_seq] */

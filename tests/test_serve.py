@@ -33,6 +33,14 @@ def test_reserve_refused(kw):
     assert B.paged_reserve_check(*pool(**kw)) != ""
 
 
+@pytest.mark.parametrize("most", ["n_tok", "n_pages"])
+def test_reserve_largest(most):
+    """Rows and pages are counted in 32 bits, by steps of up to 131072 past the last one."""
+    assert B.paged_reserve_check(*pool(**{most: 1 << 30})) == ""
+    for n in ((1 << 30) + 1, 2**31 - 131072, 2**31 - 1):
+        assert most in B.paged_reserve_check(*pool(**{most: n}))
+
+
 def drafts(**kw):
     d = dict(logits_dev=P, tok_dev=P, tokens_dev=P, u_dev=P, v_dev=P, n_seq=2, n_tok=5, max_tok=3, vocab=100)
     d.update(kw)
