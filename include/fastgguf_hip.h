@@ -375,8 +375,11 @@ FGH_API int fgh_paged_attention_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, 
  *   free_out, and of every row its sequence, its position and its slot, page * cache->page + place in the page
  *   (seq, pos, slot: [n_tok], each may be NULL; -1 in rows of no sequence, slot -1 where the page is not 0 .. n_pages - 1).
  * A sequence gets no new tokens (an empty range, len = keep) where add is not 0 .. max_tok or keep + add passes max_len or the table
- * (add then counts as 0), or where, with the sequences before it, the ring's pages or n_tok rows do not suffice: sequences are
- * served in order, and one that needs no page does not wait for pages. What it gives back it does all the same. One with a keep below 0 or above its
+ * (add then counts as 0), or where, with all that the sequences before it ask for, the ring's pages or n_tok rows do not suffice.
+ * That holds for pages and for rows by themselves, and what was asked for counts whether it was granted or not: sequences are served in
+ * order, one that needs no page may go ahead of one that waits for pages, but not with the rows that this one asks for. So a prompt
+ * that waits for pages and asks for most of n_tok leaves no rows to those behind it, call after call: give it add 0 until pages are
+ * free, or less to add. What a sequence gives back it does all the same. One with a keep below 0 or above its
  * pages, or a held that is not 0 .. table_stride, gets no tokens and len 0, and its pages stay. A `free` that is no such pair is an
  * empty ring; a ring whose pages would be more than n_pages takes no more. Of the cache only table, n_pages, page and
  * table_stride are used; n_pages and n_tok up to 2^30. keep may be len, held held_out and free free_out: nothing else may overlap. */

@@ -161,6 +161,19 @@ def test_reserve_bad_ring(backend, free):
         dev.check(p, R.reserve(p, keep, add, 60, 30, 160))
 
 
+@pytest.mark.parametrize("first, tok", [(512, [0, 0, 0, 0, 0]), (0, [0, 0, 1, 2, 3]), (160, [0, 160, 161, 162, 163]), (161, [0, 0, 1, 2, 3])])
+def test_reserve_rows_of_one_that_waits(backend, first, tok):
+    """A prompt without pages keeps the rows it asked for from those behind it, which need no page."""
+    p = R.Pool(1, 4, 16, [0, 5, 20, 35], 10, 64)
+    with Dev(backend) as d:
+        dev = DevPool(d, p, 4, 512, 512, 1024, True)
+        dev.ask(p.len, [first, 1, 1, 1])
+        backend.paged_reserve_dev(dev.cache, dev.batch, dev.pool)
+        want = R.reserve(p, p.len, [first, 1, 1, 1], 512, 512, 1024)
+        assert want[0].tolist() == tok
+        dev.check(p, want)
+
+
 def test_reserve_full_ring(backend):
     """Pages given back to a ring that has them already: nothing is written past it, and its number stays that of the pages."""
     p = R.Pool(8, 3, 16, [40, 16, 90], 6, 10)

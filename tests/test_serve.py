@@ -41,6 +41,22 @@ def test_reserve_largest(most):
         assert most in B.paged_reserve_check(*pool(**{most: n}))
 
 
+def test_rows_of_one_that_waits():
+    """A prompt without pages keeps the rows it asked for from those behind it, call after call; with add 0, or for a piece of the prompt that
+    there are pages for, they are served."""
+    def step(first, times=1):
+        p = R.Pool(1, 4, 16, [0, 5, 20, 35], 10, 64)
+        keep = p.len
+        for _ in range(times):
+            tok, keep, *_ = R.reserve(p, keep, [first, 1, 1, 1], 512, 512, 1024)
+        return tok.tolist()
+
+    assert step(512) == step(512, 3) == [0, 0, 0, 0, 0]
+    assert step(0) == [0, 0, 1, 2, 3]
+    assert step(160) == [0, 160, 161, 162, 163]
+    assert step(161) == [0, 0, 1, 2, 3]  # no pages, but few rows
+
+
 def drafts(**kw):
     d = dict(logits_dev=P, tok_dev=P, tokens_dev=P, u_dev=P, v_dev=P, n_seq=2, n_tok=5, max_tok=3, vocab=100)
     d.update(kw)
