@@ -98,6 +98,44 @@ def test_reserve(backend, i, form):
             p.len = want[1]
 
 
+MANY = [  # sequences, page, positions before, new tokens up to, free pages, rows, share of sequences that end
+    (250, 16, (10, 9000), 60, 90, 11000, 0.0),     # more than 4096 rows: several workgroups; a ring that runs out
+    (250, 16, (10, 9000), 60, 0, 11000, 0.004),    # no free pages: those of the same call
+    (9, 64, (0, 1), 4000, 400, 20000, 0.1),
+    (1024, 16, (0, 300), 12, 800, 5000, 0.1),      # rows run out
+    (1000, 32, (0, 300), 60, 40, 25001, 0.3),
+    (600, 16, (1000, 9000), 2, 20, 900, 0.0),      # few rows, more than 2^17 pages
+    (600, 16, (1000, 9000), 40, 3, 24001, 0.002),
+]
+
+
+@pytest.mark.parametrize("form", ["apart", "in place", "without maps"])
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_reserve_by_many(backend, i, form):
+    """Up to 1024 sequences whose rows or pages take several workgroups: one launch where outputs are apart from inputs, two where they are not."""
+    n, page, lens, most, free, rows, ends = MANY[i]
+    r = np.random.default_rng(300 + i)
+    stride = -(-(lens[1] + 3 * most) // page)
+    p = R.Pool(300 + i, n, page, r.integers(*lens, n), free, stride)
+    assert rows > 4096 or min(p.n_pages, n * stride) > 1 << 17
+    short = False
+    with Dev(backend) as d:
+        dev = DevPool(d, p, n, rows, most, stride * page, form == "in place", form != "without maps")
+        for _ in range(3):
+            keep = np.where(r.random(n) < ends, 0, np.maximum(0, p.len - r.integers(0, 4, n)))
+            add = r.integers(0, most + 1, n)
+            dev.ask(keep, add)
+            backend.paged_reserve_dev(dev.cache, dev.batch, dev.pool)
+            want = R.reserve(p, keep, add, rows, most, stride * page)
+            short |= bool((np.diff(want[0]) < add).any())
+            dev.check(p, want, form != "without maps")
+            if form != "in place":
+                backend.h2d(dev.held, p.held)
+                backend.h2d(dev.free, p.free)
+            p.len = want[1]
+    assert short or rows < 4096  # where rows or pages are many, some find none
+
+
 def test_reserve_again(backend):
     """The same inputs give the same outputs again, also where pages moved."""
     r = np.random.default_rng(5)
