@@ -660,6 +660,29 @@ def test_lora_beside_nan(backend, news, rank):
     assert (np.abs(got - want) <= tol)[~spoilt].all()
 
 
+MIXED = [  # adapters, max_rank, cols, rows, new tokens: more runs in a tile than workgroups for them
+    (40, 16, 72, 70, [1] * 2000),
+    (40, 24, 64, 130, [1, 2, 1, 0, 1] * 500),
+    (9, 8, 64, 66, [1] * 33000),                   # a workgroup for all of a tile's runs
+    (24, 64, 264, 200, [4100] + [1] * 63),         # a prompt beside single tokens
+    (24, 16, 136, 130, [1] * 40 + [1500] + [1] * 23 + [600]),
+    (30, 32, 200, 70, [512] + [1] * 255),
+    (5, 136, 72, 70, [300] + [1] * 90),
+]
+
+
+@pytest.mark.parametrize("t", R.TYPES)
+@pytest.mark.parametrize("i", range(len(MIXED)))
+def test_lora_mixed(backend, i, t):
+    """Tiles of many adapters, without one, with ids and ranks that mean nothing among them."""
+    n, max_rank, cols, rows, news = MIXED[i]
+    r = np.random.default_rng(180 + i)
+    ids = r.integers(-2, n, len(news)).tolist()
+    ranks = r.integers(0, max_rank + 1, n)
+    ranks[:2] = max_rank, max_rank + 1
+    check_lora(backend, *lora_case(180 + i, t, n, max_rank, cols, rows, news, ids, ranks.tolist(), (i % 3, 5)), pad=i % 4, form=["apart", "in place", "alone"][i % 3])
+
+
 @pytest.mark.parametrize("form", ["apart", "in place", "alone"])
 @pytest.mark.parametrize("pad", [0, 1, 4])
 def test_lora_forms(backend, form, pad):
