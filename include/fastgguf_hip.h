@@ -408,7 +408,10 @@ FGH_API int fgh_paged_reserve_dev(fgh_ctx *ctx, const fgh_paged_cache *cache, co
  * Logits of -infinity are words that cannot be; a row with NaN, +infinity or nothing else, or a temp below 0 or NaN, has no
  * distribution: its draft is rejected and next is -1. A q that is NaN counts as 0 in the sums, and its draft is rejected. A sequence without
  * rows, or with more than max_tok or outside 0 .. n_tok: n_ok 0, next -1, keep as len. Exponentials, sums and
- * comparisons are in 64 bits. vocab up to 2^24, n_tok below 2^18, pointers 4-byte aligned, any strides. Inputs and outputs do not overlap but for keep. */
+ * comparisons are in 64 bits. An exponential is off by up to 9e-13 of itself (besides its argument's rounding), and one below 2^-990
+ * counts as 0: where u q(d) is that near p(d), or v that near the place in the running sum where a word ends, the outcome may be the other
+ * one. Where p and q are nearly equal, that place is unsure by p / (p - q) times as much. vocab up to 2^24, n_tok below 2^18,
+ * pointers 4-byte aligned, any strides. Inputs and outputs do not overlap but for keep. */
 typedef struct {
     const float *logits;                /* device, [n_tok][ld] */
     const float *q, *q_lse;             /* device, [n_tok][ldq] and [n_tok], or NULL */
