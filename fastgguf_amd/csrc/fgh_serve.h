@@ -53,7 +53,7 @@ struct VerifyArgs {
     int n_seq, n_tok, max_tok, vocab;
     // set by verify_plan: a row's words over `splits` workgroups, `per` words each, in blocks of 1024 nv; `group` such parts to a workgroup
     int splits, per, nv, group;
-    double *sum, *rest;  // [n_tok][splits], [n_seq][splits][per / 2048 + 1]
+    double *sum, *rest;  // [n_tok][splits], [n_seq][splits][(per + 2047) / 2048]
     float *top;          // [n_tok][splits]
     int32_t *at;         // [n_tok][splits]
     VerifyChoice *choice;  // [n_seq]

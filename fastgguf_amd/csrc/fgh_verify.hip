@@ -435,8 +435,9 @@ __device__ int draw(const VerifyArgs &a, const Weigh &w, int subs, int words, do
 }
 
 // The decision where drafts have no probabilities, and the draw: the part of the words that v falls on by the parts' sums, a thread's words
-// in it by a scan over the workgroup, the word by one over a wavefront. One workgroup a sequence: 5 to 9 us whatever the vocabulary, waits for loads
-// that depend on each other. (Keeping the parts' sums from step to step saved nothing that could be measured.)
+// in it by a scan over the workgroup, the word by one over a wavefront. One workgroup a sequence: 5 to 9 us up to 262144 words, waits for loads
+// that depend on each other; 8 for a row of 2^20 and 70 for one of 2^24, whose parts are 16384 and 262144 words, all gone through by that
+// workgroup. (Keeping the parts' sums from step to step saved nothing that could be measured.)
 __global__ __launch_bounds__(WG) void verify_next_kernel(VerifyArgs a) {
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     bool greedy;
