@@ -4,7 +4,7 @@
 // Two launches: h = A x, split over columns where rows are few, then y from the sums of h. A workgroup has the rows of one adapter
 // that stand together in a tile of the batch. Both products run on 16 x 16 x 32 bf16 matrix instructions whose fp32 operands are
 // taken apart into bf16 parts that hold all their bits (x and h: 3; adapters F32 3, F16 2, BF16 1), so that results are
-// those of fp32 products and sums; F32 adapters leave 3 of 9 products out, 2^-24 of the whole on average.
+// those of fp32 products and sums; F32 adapters leave 3 of 9 products out, up to 2^-21 of one, 2^-24 of the whole on average.
 //
 // Bound by memory where rows are many: 8192 tokens, 4096 -> 14336, rank 64, F16: 238 us for 1.08 GB, 4.5 TB/s; y alone at 5.0. By loads that wait for
 // each other where they are few: 64 tokens with 24 adapters 21 us (38 MB), one token 9.
@@ -368,8 +368,9 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraArgs a) {
 // at a time and 32 SB ranks of them, the next ones' values on their way during the products of some. ROWS (prompts): each wavefront has 16 rows and
 // all 64 outputs; else (few rows) 16 of the outputs and the same rows. Products: lane l has output l % 16 of a tile and row l % 16, ranks 8 (l / 16)
 // .. + 7, and gets outputs 4 (l / 16) .. + 3 of its row; through LDS they come to lie as y does, 16 lanes with 256 bytes of a row. KB: such blocks of
-// ranks, whose h stays in registers; 0: any number, which does not. ROWS: three workgroups a compute unit, since at four registers spill (2500
-// tokens, F32: 46.8 us, without 35.7).
+// ranks, whose h stays in registers; 0: any number (max_rank above 128), whose h is summed and taken apart for every turn (64 tokens, 24
+// adapters, BF16: rank 128 40 us, 136 87, 512 158; 8192 tokens, F16: 307, 513, 1309). ROWS: three workgroups a compute unit, since at
+// four registers spill (2500 tokens, F32: 46.8 us, without 35.7).
 template <int TYPE, int SB, int KB, bool ROWS>
 __global__ __launch_bounds__(256, KB != 1 ? 2 : ROWS ? 3 : 4) void lora_up_kernel(LoraArgs a) {
     using S = Stage<TYPE, SB>;
@@ -600,6 +601,8 @@ size_t lora_plan(LoraArgs &a, int num_cu) {
     // if there are tiles for the device; few rows, and many short prompts, are better in tiles of 16 (4096 -> 14336, F16, rank 64; one prompt of 512: 27 us,
     // 34 with 64; of 1024: 48 and 49; of 2048: 82 and 76; 64 of 63: 220 and 200. 4096 -> 6144, F32, rank 32; 128 of 16: 46 and 74; 256 of 4, which are
     // tiles of 64 again: 40, of 16: 69).
+    // One plan for all rows: prompts beside single tokens of many adapters are better in calls of their own (24 adapters, BF16, rank 64; 8192 + 63 single:
+    // 1009 us, in two calls 269; 2048 + 63: 286 and 94; 512 + 255: 356 and 79).
     const bool prompts = a.n_tok >= 16 * (int64_t)a.n_seq;
     a.whole = a.n_tok >= 32 * (int64_t)a.n_seq && a.n_tok >= 4 * num_cu;
     a.tile = a.whole || !prompts ? 64 : 16;

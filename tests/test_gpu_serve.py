@@ -683,6 +683,21 @@ def test_lora_mixed(backend, i, t):
     check_lora(backend, *lora_case(180 + i, t, n, max_rank, cols, rows, news, ids, ranks.tolist(), (i % 3, 5)), pad=i % 4, form=["apart", "in place", "alone"][i % 3])
 
 
+@pytest.mark.parametrize("news, few, rows", [([1] * 63 + [1500], 63, 70), ([3, 1, 0, 4] * 10 + [600, 70], 40, 130)])
+def test_lora_in_two_calls(backend, news, few, rows):
+    """Single tokens first, prompts behind them, a call for each over the same starts: together what one call gives."""
+    ad, tok, ids, x, y_in = lora_case(190, T_BF16, 6, 16, 136, rows, news, [s % 7 - 1 for s in range(len(news))], [16, 3, 0, 9, 16, 5], (0, 4))
+    want, tol, mine = R.lora(ad, tok, ids, x, y_in)
+    most = 4 * few  # rows that the first call may have
+    with Dev(backend) as d:
+        set_ = Lora(ad.type, d.put(ad.a), d.put(ad.b), n_adapter=ad.n, max_rank=ad.max_rank, cols=ad.cols, rows=ad.rows, rank=d.put(ad.rank), scale=d.put(ad.scale))
+        td, idd, xd, y = d.put(tok.astype(np.int32)), d.put(np.array(ids, np.int32)), d.put(x), d.put(y_in)
+        for at, n, n_tok in ((0, few, most), (few, len(ids) - few, len(x))):
+            backend.lora_dev(set_, td + 4 * at, idd + 4 * at, n, n_tok, xd, ad.cols, y, rows, y_in_dev=y, ldyi=rows)
+        got = d.get(y, y_in)
+    assert (np.abs(got - want) <= tol)[mine].all() and np.array_equal(got[~mine], y_in[~mine])
+
+
 @pytest.mark.parametrize("form", ["apart", "in place", "alone"])
 @pytest.mark.parametrize("pad", [0, 1, 4])
 def test_lora_forms(backend, form, pad):
