@@ -7,8 +7,8 @@
 // place and the sum of exp((x - largest) / T); whole rows, and the sums that a number has to be compared with, are joined
 // from those.
 //
-// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 46 to 49 us: the rows 26 (20 for reading alone, 25 for the
-// exponentials alone, in one kernel they overlap), the rejected rows' sums 15, the choice 7. Few rows are a matter of launches that wait for each
+// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 46 to 49 us: the rows 26 (each with the kernel's start: 20 for reading
+// alone, 25 for the exponentials alone, in one kernel they overlap), the rejected rows' sums 15, the choice 7. Few rows are a matter of launches that wait for each
 // other and, in the choice, of five loads that do: 8.1 us for one token of one row.
 #include "fgh_serve.h"
 
@@ -126,7 +126,8 @@ __device__ __forceinline__ Part join_lanes(Part p, double c, bool greedy) {
 }
 
 // Each row's largest value and sum, a workgroup to a part of its words, 4 NV words a thread at a time, all of whose loads are under way at
-// once. Bound by vector instructions, 76 % of the cycles: 17 a word, of which 13 are of 64 bits, and a third as many again around them. (The next
+// once. Bound by vector instructions, 76 % of the compute units' busy cycles: 17 a word, of which 13 are of 64 bits, and a third as many again around
+// them (64 sequences: 26 us, of which 21 busy and 16 of instructions at 4 cycles each; the rest is the start and the end). (The next
 // block's loads a block ahead, at 86 registers instead of 63, gained nothing.)
 template <int NV>
 __global__ __launch_bounds__(256) void verify_rows_kernel(VerifyArgs a) {
