@@ -5,6 +5,7 @@
 // that stand together in a tile of the batch. Both products run on 16 x 16 x 32 bf16 matrix instructions whose fp32 operands are
 // taken apart into bf16 parts that hold all their bits (x and h: 3; adapters F32 3, F16 2, BF16 1), so that results are
 // those of fp32 products and sums; F32 adapters leave 3 of 9 products out, up to 2^-21 of one, 2^-24 of the whole on average.
+// A part below 2^-126 is a bf16 subnormal: its bits end at 2^-133.
 //
 // Bound by memory where rows are many: 8192 tokens, 4096 -> 14336, rank 64, F16: 238 us for 1.08 GB, 4.5 TB/s; y alone at 5.0. By loads that wait for
 // each other where they are few: 64 tokens with 24 adapters 21 us (38 MB), one token 9.

@@ -426,7 +426,8 @@ FGH_API int fgh_draft_verify_dev(fgh_ctx *ctx, const fgh_drafts *drafts, int32_t
  * adapter id[s] of n_adapter: A [max_rank][cols] and B [rows][max_rank], of which the first rank[id] (0 .. max_rank; NULL: max_rank) count;
  * scale [n_adapter] (NULL: 1). id -1: y = y_in; any other id or rank: NaN rows. y_in NULL: 0. y_in may be y (ldyi == ldy); else
  * y overlaps no input. Rows before tok[0] and from tok[n_seq] on are left as they were. Results are those of fp32 sums,
- * whatever the type; with F32 adapters a product may lose 2^-21 of itself. Rows of one adapter among 64 neighbouring ones share its reads: order sequences by adapter. x that is not
+ * whatever the type; with F32 adapters a product may lose 2^-21 of itself, and bits of x, A x
+ * and F32 adapters below 2^-133 are cut. Rows of one adapter among 64 neighbouring ones share its reads: order sequences by adapter. x that is not
  * finite makes its own row anything, and no other. n_seq up to 65535. Kernels are chosen by n_seq, n_tok and max_rank: a recorded step of single
  * tokens is best recorded with an n_tok of its own, and where prompts and single tokens of several adapters meet in a batch, put the
  * single tokens first and give each kind a call of its own: tok, id, n_single and the n_tok that those have at most, then

@@ -732,6 +732,23 @@ def test_lora_ranges(backend, t):
     check_lora(backend, ad, tok, ids, x, y_in, form="alone")
 
 
+@pytest.mark.parametrize("t", R.TYPES)
+@pytest.mark.parametrize("news", [[3, 20], [1100, 40]])
+@pytest.mark.parametrize("e", [-100, -116, -124])
+def test_lora_smallest(backend, t, news, e):
+    """x near the smallest numbers: a value's bits below 2^-133 are cut, of x and of A x, and no more."""
+    ad, tok, ids, x, y_in = lora_case(69, t, 2, 16, 256, 64, news, [0, 1])
+    x, y_in = np.ldexp(x, e).astype(np.float32), np.zeros_like(y_in)
+    ad.scale[:] = 2.0**100
+    got, _ = run_lora(backend, ad, tok, ids, x, y_in, form="alone")
+    want, tol, _ = R.lora(ad, tok, ids, x, y_in)
+    for s, i in enumerate(ids):
+        a, b = (np.abs(w) for w in ad.of(i))
+        # every x and every h off by 2^-133; sums' own roundings, fewer than 2^10 of up to 2^-150 each, where they are subnormal
+        tol[tok[s]:tok[s + 1]] += 2.0**100 * (b @ (2.0**-133 * (a.sum(1) + 1) + 2.0**-140) + 2.0**-140)
+    assert (np.abs(got - want) <= tol).all()
+
+
 def test_lora_non_finite(backend):
     """A row with an infinity or a NaN, and NaN in an adapter that others do not use, stay with themselves."""
     ad, tok, ids, x, y_in = lora_case(64, T_F16, 3, 16, 128, 40, [1, 1, 20, 1], [0, 1, 1, 2])
