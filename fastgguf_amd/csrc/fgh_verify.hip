@@ -7,7 +7,7 @@
 // place and the sum of exp((x - largest) / T); whole rows, and the sums that a number has to be compared with, are joined
 // from those.
 //
-// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 46 to 49 us: the rows 26 (each with the kernel's start: 20 for reading
+// 64 sequences of 1 to 6 rows of 128256 words with the drafter's probabilities take 45 to 49 us: the rows 26 (each with the kernel's start: 20 for reading
 // alone, 25 for the exponentials alone, in one kernel they overlap), the rejected rows' sums 15, the choice 7. Few rows are a matter of launches that wait for each
 // other and, in the choice, of five loads that do: 8.1 us for one token of one row.
 #include "fgh_serve.h"
